@@ -1,5 +1,5 @@
 # SPDX-License-Identifier: MIT
-"""ctypes view of the engine's C ABI (include/dbs_cuda.h, include/dbs_cuda_b200.h).
+"""ctypes view of the engine's C ABI (include/dbs_cuda.h, dbs_cuda_b200.h, dbs_cuda_cache.h).
 
 The structs mirror the header field for field (tests/test_abi.py checks every
 size and offset against the C compiler's layout of both this header and the
@@ -199,6 +199,58 @@ class PoolGradients(C.Structure):
     ]
 
 
+class Cache(C.Structure):
+    """DBSCudaCache (include/dbs_cuda_cache.h)."""
+
+    _fields_ = [
+        ("batch_size", C.c_int32),
+        ("beam_size", C.c_int32),
+        ("max_pages", C.c_int32),
+        ("num_pages", C.c_int32),
+        ("num_layers", C.c_int32),
+        ("num_heads", C.c_int32),
+        ("head_dim", C.c_int32),
+        ("page_size", C.c_int32),
+        ("data_type", C.c_int32),
+        ("reserved0", C.c_int32),
+        ("pages", _p),
+        ("table", _p),
+        ("lengths", _p),
+        ("references", _p),
+        ("plan", _p),
+        ("plan_bytes", C.c_int64),
+        ("status", _p),
+    ]
+
+
+class AttendArgs(C.Structure):
+    """DBSCudaAttendArgs."""
+
+    _fields_ = [
+        ("layer", C.c_int32),
+        ("beams", C.c_int32),
+        ("new_tokens", C.c_int32),
+        ("query_heads", C.c_int32),
+        ("scale", C.c_float),
+        ("reserved0", C.c_int32),
+        ("q", _p),
+        ("k", _p),
+        ("v", _p),
+        ("q_strides", C.c_int64 * 4),
+        ("k_strides", C.c_int64 * 4),
+        ("v_strides", C.c_int64 * 4),
+        ("mask", _p),
+        ("counts", _p),
+        ("out", _p),
+        ("lse", _p),
+        ("workspace", _p),
+        ("workspace_bytes", C.c_int64),
+    ]
+
+
+CACHE_STATUS_POOL, CACHE_STATUS_CAPACITY, CACHE_STATUS_INDEX = 1, 2, 4
+CACHE_STATUS_SHARED, CACHE_STATUS_TIMEOUT = 8, 16
+
 MAX_POOL = 1024  # DBS_CUDA_B200_MAX_POOL
 
 VSHARD_MAX_WORLD = 8
@@ -281,13 +333,23 @@ SIGNATURES = {
     ),
     "dbs_cuda_backward_pool": (
         C.c_int, [C.POINTER(DecodeArgs), C.POINTER(BackwardInputs), C.POINTER(PoolGradients), _p, _p]),
+    # the paged beam cache (include/dbs_cuda_cache.h)
+    "dbs_cuda_cache_plan_bytes": (C.c_int64, [C.POINTER(Cache)]),
+    "dbs_cuda_cache_refresh": (C.c_int, [C.POINTER(Cache), C.c_int, _p]),
+    "dbs_cuda_cache_fork": (C.c_int, [C.POINTER(Cache), _p, _p, C.c_int32, _p, C.c_int32, _p]),
+    "dbs_cuda_cache_commit": (C.c_int, [C.POINTER(Cache), _p, C.c_int32, _p, C.c_int32, _p]),
+    "dbs_cuda_cache_compact": (C.c_int, [C.POINTER(Cache), _p]),
+    "dbs_cuda_cache_attend_workspace_size": (C.c_int64, [C.POINTER(Cache), C.POINTER(AttendArgs)]),
+    "dbs_cuda_cache_attend": (C.c_int, [C.POINTER(Cache), C.POINTER(AttendArgs), _p]),
 }
 
 VSHARD_SYMBOLS = ("dbs_cuda_vshard_plan", "dbs_cuda_vshard_scan", "dbs_cuda_vshard_lanes", "dbs_cuda_vshard_merge",
                   "dbs_cuda_vshard_select", "dbs_cuda_vshard_rescan")
+CACHE_SYMBOLS = ("dbs_cuda_cache_plan_bytes", "dbs_cuda_cache_refresh", "dbs_cuda_cache_fork", "dbs_cuda_cache_commit",
+                 "dbs_cuda_cache_compact", "dbs_cuda_cache_attend_workspace_size", "dbs_cuda_cache_attend")
 ADDED_SYMBOLS = ("dbs_cuda_b200_abi_version", "dbs_cuda_backtrack", "dbs_cuda_backward_dense", "dbs_cuda_advance_prefixes",
                  "dbs_cuda_selected_weights", "dbs_cuda_backward_selected", "dbs_cuda_b200_wait_selftest",
-                 "dbs_cuda_decode_no_alloc", "dbs_cuda_relaxed_pool", "dbs_cuda_backward_pool") + VSHARD_SYMBOLS
+                 "dbs_cuda_decode_no_alloc", "dbs_cuda_relaxed_pool", "dbs_cuda_backward_pool") + VSHARD_SYMBOLS + CACHE_SYMBOLS
 REFERENCE_SYMBOLS = [n for n in SIGNATURES if n not in ADDED_SYMBOLS]
 
 # Size of the fixed device array behind dbs_cuda_decode_no_alloc (DBS_CUDA_B200_NO_ALLOC_SCRATCH_BYTES).

@@ -1,0 +1,86 @@
+// SPDX-License-Identifier: MIT
+//
+// Attention over the paged beam cache, and the write of the new tokens before it
+// (include/dbs_cuda_cache.h gives the definition).
+#include "attend.cuh"
+
+namespace dbsb {
+
+namespace {
+
+constexpr int kAppendThreads = 256;
+constexpr int kRowThreads = 128;
+
+// Keys and values of the new tokens into their pages, 16 bytes a thread. A value that is not
+// finite raises the cache's second status word: the attention then keeps masked values out of its
+// sums element by element, where otherwise a weight of zero is enough.
+template <class T>
+__global__ void __launch_bounds__(kAppendThreads) append_kernel(CacheView c, AttendParams a) {
+    grid_wait();
+    grid_release();
+    const int vecs = c.D / Pack<T>::n;
+    const int64_t items = static_cast<int64_t>(c.B) * a.beams * a.N * c.H * vecs;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kAppendThreads + threadIdx.x; i < items;
+         i += static_cast<int64_t>(gridDim.x) * kAppendThreads) {
+        const int vec = static_cast<int>(i % vecs);
+        int64_t rest = i / vecs;
+        const int h = static_cast<int>(rest % c.H);
+        rest /= c.H;
+        const int j = static_cast<int>(rest % a.N);
+        const int64_t bk = rest / a.N;
+        const int64_t b = bk / a.beams, k = bk % a.beams;
+        if (j >= new_count(a, bk)) continue;
+        const int64_t slot = b * c.K + k, pos = static_cast<int64_t>(c.lengths[slot]) + j, col = pos >> c.page_log2;
+        if (col >= c.M) {
+            atomicOr(c.status, DBS_CUDA_CACHE_STATUS_CAPACITY);
+            continue;
+        }
+        const int p = c.table[slot * c.M + col];
+        if (p < 0) continue;
+        const int64_t block = static_cast<int64_t>(a.layer) * 2 * c.P + p;
+        const int64_t row = pos & (c.page - 1);
+        const T* ks = static_cast<const T*>(a.k) + b * a.ks[0] + k * a.ks[1] + j * a.ks[2] + h * a.ks[3];
+        const T* vs = static_cast<const T*>(a.v) + b * a.vs[0] + k * a.vs[1] + j * a.vs[2] + h * a.vs[3];
+        const uint4 kx = reinterpret_cast<const uint4*>(ks)[vec], vx = reinterpret_cast<const uint4*>(vs)[vec];
+        uint4* pages = static_cast<uint4*>(c.pages);
+        pages[((block * c.H + h) * c.page + row) * vecs + vec] = kx;
+        pages[(((block + c.P) * c.H + h) * c.page + row) * vecs + vec] = vx;
+        if (!(Pack<T>::finite(vx.x) && Pack<T>::finite(vx.y) && Pack<T>::finite(vx.z) && Pack<T>::finite(vx.w)))
+            c.status[1] = 1;
+    }
+}
+
+// One warp a query row.
+template <class T>
+__global__ void __launch_bounds__(kRowThreads) rows_kernel(CacheView c, AttendParams a) {
+    __shared__ float query[kRowThreads / 32 * DBS_CUDA_CACHE_MAX_HEAD_DIM];
+    grid_wait();
+    attend_all_rows<T>(c, a, query, threadIdx.x >> 5, kRowThreads / 32);
+}
+
+template <class T>
+cudaError_t launch_typed(const CacheView& c, const AttendParams& a, int sm_count, cudaStream_t stream) {
+    const int64_t cap = static_cast<int64_t>(sm_count) * 8;
+    if (a.k != nullptr) {
+        const int64_t items = static_cast<int64_t>(c.B) * a.beams * a.N * c.H * (c.D / Pack<T>::n);
+        const int64_t want = (items + kAppendThreads - 1) / kAppendThreads;
+        const cudaError_t e = launch_after(append_kernel<T>, static_cast<unsigned>(want < cap ? want : cap),
+                                           kAppendThreads, 0, stream, c, a);
+        if (e != cudaSuccess) return e;
+    }
+    const int64_t rows = static_cast<int64_t>(c.B) * a.beams * a.N * a.Hq;
+    return launch_after(rows_kernel<T>, static_cast<unsigned>((rows + kRowThreads / 32 - 1) / (kRowThreads / 32)),
+                        kRowThreads, 0, stream, c, a);
+}
+
+}  // namespace
+
+int64_t attend_workspace(const CacheView&, const AttendParams&, int) { return 256; }
+
+cudaError_t launch_attend(const CacheView& c, int dtype, const AttendParams& a, int sm_count, cudaStream_t stream) {
+    if (dtype == DBS_CUDA_DTYPE_F32) return launch_typed<float>(c, a, sm_count, stream);
+    if (dtype == DBS_CUDA_DTYPE_F16) return launch_typed<__half>(c, a, sm_count, stream);
+    return launch_typed<__nv_bfloat16>(c, a, sm_count, stream);
+}
+
+}  // namespace dbsb

@@ -1,0 +1,367 @@
+// SPDX-License-Identifier: MIT
+//
+// Pieces that the attention kernels share: element types, the row-at-a-time form, the split of
+// the work over the CTAs, and the copies and barriers of the tiled kernels.
+#pragma once
+
+#include <climits>
+
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "cache.cuh"
+
+namespace dbsb {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+template <class T> struct Pack;  // 16 bytes of elements
+template <> struct Pack<float> {
+    static constexpr int n = 4;
+    static __device__ __forceinline__ void widen(const uint4& v, float* f) {
+        f[0] = __uint_as_float(v.x), f[1] = __uint_as_float(v.y), f[2] = __uint_as_float(v.z), f[3] = __uint_as_float(v.w);
+    }
+    static __device__ __forceinline__ bool finite(uint32_t w) { return (w & 0x7f800000u) != 0x7f800000u; }
+};
+template <> struct Pack<__half> {
+    static constexpr int n = 8;
+    static __device__ __forceinline__ void widen(const uint4& v, float* f) {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+            f[2 * i] = t.x, f[2 * i + 1] = t.y;
+        }
+    }
+    static __device__ __forceinline__ bool finite(uint32_t w) {
+        return (w & 0x7c00u) != 0x7c00u && (w & 0x7c000000u) != 0x7c000000u;
+    }
+    static __device__ __forceinline__ uint32_t pair(float lo, float hi) {
+        uint32_t r;
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+        return r;
+    }
+};
+template <> struct Pack<__nv_bfloat16> {
+    static constexpr int n = 8;
+    static __device__ __forceinline__ void widen(const uint4& v, float* f) {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            f[2 * i] = __uint_as_float(w[i] << 16);
+            f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    }
+    static __device__ __forceinline__ bool finite(uint32_t w) {
+        return (w & 0x7f80u) != 0x7f80u && (w & 0x7f800000u) != 0x7f800000u;
+    }
+    static __device__ __forceinline__ uint32_t pair(float lo, float hi) {
+        uint32_t r;
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+        return r;
+    }
+};
+
+template <class T> __device__ __forceinline__ float to_float(T x) { return static_cast<float>(x); }
+template <class T> __device__ __forceinline__ T from_float(float x) { return static_cast<T>(x); }
+
+__device__ __forceinline__ float lanes_max(float v) {
+#pragma unroll
+    for (int m = 16; m > 0; m >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, m));
+    return v;
+}
+__device__ __forceinline__ float lanes_sum(float v) {
+#pragma unroll
+    for (int m = 16; m > 0; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
+    return v;
+}
+// 2^x, within 2 ulp: the weights are sums' terms of at most 1 in magnitude.
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// New tokens of (b, k): clamped into [0, N]. row: b * beams + k.
+__device__ __forceinline__ int new_count(const AttendParams& a, int64_t row) {
+    if (a.counts == nullptr) return a.N;
+    const int n = a.counts[row];
+    return n < 0 ? 0 : (n > a.N ? a.N : n);
+}
+
+// One query row by one warp: 32 positions a round, a lane each for the scores, the lanes over the
+// head's elements for the values, in which a value that the row does not see takes no part. Right
+// for every type and every value; the tiled kernels use it once the cache holds values that are
+// not finite, because there a weight of zero would not keep them out of a product.
+template <class T>
+__device__ __noinline__ void attend_row(const CacheView& c, const AttendParams& a, int64_t row, float* query) {
+    const int lane = threadIdx.x & 31;
+    const int hq = static_cast<int>(row % a.Hq);
+    const int64_t token = row / a.Hq;
+    const int i = static_cast<int>(token % a.N);
+    const int64_t bk = token / a.N, b = bk / a.beams, k = bk % a.beams;
+    const int64_t slot = b * c.K + k;
+    const int h = hq / a.G, count = new_count(a, bk), length = c.lengths[slot];
+    const T* q = static_cast<const T*>(a.q) + b * a.qs[0] + k * a.qs[1] + i * a.qs[2] + hq * a.qs[3];
+    __syncwarp();
+    for (int d = lane; d < c.D; d += 32) query[d] = to_float(q[d]) * a.scale;
+    __syncwarp();
+    constexpr int kEach = DBS_CUDA_CACHE_MAX_HEAD_DIM / 32;
+    float acc[kEach] = {};
+    float top = -INFINITY, total = 0.0f;
+    const int64_t end = i < count ? static_cast<int64_t>(length) + count : 0;
+    const uint8_t* mask = a.mask ? a.mask + (bk * a.N + i) * a.N : nullptr;
+    const T* pages = static_cast<const T*>(c.pages);
+    const int vecs = c.D / Pack<T>::n;
+    for (int64_t base = 0; base < end; base += 32) {
+        const int64_t pos = base + lane, col = pos >> c.page_log2;
+        int p = -1;
+        if (pos < end && col < c.M) p = c.table[slot * c.M + col];
+        if (pos >= length && p >= 0) {
+            const int j = static_cast<int>(pos - length);
+            if (mask ? mask[j] == 0 : j > i) p = -1;
+        }
+        const int64_t at = p < 0 ? 0
+            : (((static_cast<int64_t>(a.layer) * 2 * c.P + p) * c.H + h) * c.page + (pos & (c.page - 1))) * c.D;
+        float score = -INFINITY;
+        if (p >= 0) {
+            float sum = 0.0f;
+            for (int v = 0; v < vecs; ++v) {
+                float f[Pack<T>::n];
+                Pack<T>::widen(reinterpret_cast<const uint4*>(pages + at)[v], f);
+#pragma unroll
+                for (int e = 0; e < Pack<T>::n; ++e) sum = fmaf(query[v * Pack<T>::n + e], f[e], sum);
+            }
+            score = sum;
+        }
+        const unsigned seen = __ballot_sync(0xffffffffu, p >= 0);
+        if (seen == 0) continue;
+        const float now = fmaxf(top, lanes_max(score));
+        // A row whose scores are all -inf so far keeps weights of zero instead of NaN.
+        const float ref = now == -INFINITY ? 0.0f : now;
+        const float keep = expf(top - ref);
+        const float weight = p >= 0 ? expf(score - ref) : 0.0f;
+        total = total * keep + lanes_sum(weight);
+        top = now;
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) acc[e] *= keep;
+        for (unsigned rest = seen; rest != 0; rest &= rest - 1) {
+            const int from = __ffs(rest) - 1;
+            const float w = __shfl_sync(0xffffffffu, weight, from);
+            const T* v = pages + __shfl_sync(0xffffffffu, at, from) + static_cast<int64_t>(c.P) * c.H * c.page * c.D;
+#pragma unroll
+            for (int e = 0; e < kEach; ++e)
+                if (lane + 32 * e < c.D) acc[e] = fmaf(w, to_float(v[lane + 32 * e]), acc[e]);
+        }
+    }
+    T* out = static_cast<T*>(a.out) + row * c.D;
+    const float inverse = total > 0.0f ? 1.0f / total : total;  // 0: nothing seen; NaN stays
+#pragma unroll
+    for (int e = 0; e < kEach; ++e)
+        if (lane + 32 * e < c.D) out[lane + 32 * e] = from_float<T>(acc[e] * inverse);
+    if (a.lse != nullptr && lane == 0) a.lse[row] = total == 0.0f ? -INFINITY : top + logf(total);
+}
+
+template <class T>
+__device__ __forceinline__ void attend_all_rows(const CacheView& c, const AttendParams& a, float* query, int warp,
+                                                int warps) {
+    const int64_t rows = static_cast<int64_t>(c.B) * a.beams * a.N * a.Hq;
+    for (int64_t row = static_cast<int64_t>(blockIdx.x) * warps + warp; row < rows;
+         row += static_cast<int64_t>(gridDim.x) * warps)
+        attend_row<T>(c, a, row, query + warp * DBS_CUDA_CACHE_MAX_HEAD_DIM);
+}
+
+// ---------------------------------------------------------------------------
+// The split of the work. A segment is one group of beams, one block of kRows query rows of it
+// (rows in (beam, token, head of the key head's group) order) and one key head; its tiles are the
+// group's units, a few at a time. All tiles of all segments form one line that is cut into equal
+// parts, one a CTA, so that every SM reads the same amount whatever the lengths are. A segment
+// that a cut divides is joined by the CTA that finishes its part last.
+// ---------------------------------------------------------------------------
+struct WorkSplit {
+    int64_t total;   // tiles
+    int ctas;        // CTAs that take part
+    int64_t lo, hi;  // this CTA's tiles
+    int group;       // group that tile lo lies in
+    int64_t base;    // its first tile
+};
+
+struct GroupWork {
+    int units, tiles, blocks, rows;  // blocks: row blocks
+};
+
+template <int kRows>
+__device__ __forceinline__ GroupWork group_work(const CacheView& c, const AttendParams& a, int g, int tile_units) {
+    const int first = (g % c.groups) * kGroupBeams;
+    int beams = a.beams - first;
+    beams = beams < 0 ? 0 : (beams > kGroupBeams ? kGroupBeams : beams);
+    GroupWork w;
+    w.units = c.unit_count[g];
+    w.tiles = (w.units + tile_units - 1) / tile_units;
+    if (w.tiles < 1) w.tiles = 1;  // rows without a page are written too
+    w.rows = beams * a.N * a.G;
+    w.blocks = (w.rows + kRows - 1) / kRows;
+    return w;
+}
+
+// All threads of the block; sums: 33 ints, found: a WorkSplit in shared memory. The host has
+// checked that the tiles of all segments are counted in 31 bits.
+template <int kRows>
+__device__ WorkSplit split_work(const CacheView& c, const AttendParams& a, int tile_units, int min_tiles, int* sums,
+                                WorkSplit* found) {
+    const int groups = c.B * c.groups, tid = threadIdx.x, threads = blockDim.x;
+    int total = 0, segments = 0;
+    for (int base = 0; base < groups; base += threads) {
+        int n = 0, s = 0, sum;
+        if (base + tid < groups) {
+            const GroupWork w = group_work<kRows>(c, a, base + tid, tile_units);
+            s = w.blocks * c.H;
+            n = w.tiles * s;
+        }
+        block_scan(n, sums, &sum);
+        total += sum;
+        block_scan(s, sums, &sum);
+        segments += sum;
+    }
+    // A segment in more than 32 parts costs more to join than its parts save.
+    int64_t ctas = total / min_tiles;
+    if (ctas > static_cast<int64_t>(segments) * 32) ctas = static_cast<int64_t>(segments) * 32;
+    if (ctas > gridDim.x) ctas = gridDim.x;
+    if (ctas < 1) ctas = 1;
+    WorkSplit w;
+    w.total = total;
+    w.ctas = static_cast<int>(ctas);
+    w.lo = static_cast<int64_t>(total) * blockIdx.x / ctas;
+    w.hi = static_cast<int64_t>(total) * (blockIdx.x + 1) / ctas;
+    w.group = 0;
+    w.base = 0;
+    if (static_cast<int64_t>(blockIdx.x) >= ctas) {
+        w.lo = w.hi = 0;
+        return w;
+    }
+    int before = 0;
+    for (int base = 0; base < groups; base += threads) {
+        int n = 0, sum;
+        if (base + tid < groups) {
+            const GroupWork g = group_work<kRows>(c, a, base + tid, tile_units);
+            n = g.tiles * g.blocks * c.H;
+        }
+        const int at = before + block_scan(n, sums, &sum);
+        if (n > 0 && at <= w.lo && w.lo < at + n) {
+            w.group = base + tid;
+            w.base = at;
+            *found = w;
+        }
+        before += sum;
+        if (before > w.lo) break;
+    }
+    __syncthreads();
+    w.group = found->group;
+    w.base = found->base;
+    return w;
+}
+
+// The CTA whose part holds tile x.
+__device__ __forceinline__ int cta_of(const WorkSplit& w, int64_t x) {
+    return static_cast<int>(((x + 1) * w.ctas - 1) / w.total);
+}
+
+// A CTA's share of one segment.
+struct Piece {
+    int group, block, head;  // block: row block
+    int t0, t1;              // tiles
+    int tiles, units, rows;  // of the group
+    int c0, c1;              // CTAs that hold the segment's first and last tile
+};
+
+// The piece at tile `cur` of the line; advances group and base to it.
+template <int kRows>
+__device__ __forceinline__ Piece piece_at(const CacheView& c, const AttendParams& a, const WorkSplit& w, int64_t cur,
+                                          int& group, int64_t& base, int tile_units) {
+    GroupWork g = group_work<kRows>(c, a, group, tile_units);
+    while (cur >= base + static_cast<int64_t>(g.tiles) * g.blocks * c.H) {
+        base += static_cast<int64_t>(g.tiles) * g.blocks * c.H;
+        g = group_work<kRows>(c, a, ++group, tile_units);
+    }
+    const int off = static_cast<int>(cur - base), seg = off / g.tiles;
+    Piece p;
+    p.group = group;
+    p.block = seg / c.H;
+    p.head = seg - p.block * c.H;
+    p.t0 = off - seg * g.tiles;
+    const int64_t left = w.hi - cur;
+    p.t1 = left < g.tiles - p.t0 ? p.t0 + static_cast<int>(left) : g.tiles;
+    p.tiles = g.tiles;
+    p.units = g.units;
+    p.rows = g.rows;
+    const int64_t first = base + static_cast<int64_t>(seg) * g.tiles;
+    p.c0 = cta_of(w, first);
+    p.c1 = cta_of(w, first + g.tiles - 1);
+    return p;
+}
+
+// Row r of a group's block: its beam within the group, drafted token and query head.
+struct RowId {
+    int beam, token, head;
+};
+__device__ __forceinline__ RowId row_id(const AttendParams& a, int r) {
+    RowId id;
+    const int per = a.N * a.G;
+    id.beam = r / per;
+    r -= id.beam * per;
+    id.token = r / a.G;
+    id.head = r - id.token * a.G;
+    return id;
+}
+
+// ---------------------------------------------------------------------------
+// Barriers and copies. Every wait is bounded: it records a timeout in the cache's status word and
+// goes on, so that a kernel ends whatever happens.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t smem_address(const void* p) {
+    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+__device__ __forceinline__ void barrier_init(uint32_t bar, int count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void barrier_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void barrier_expect(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.release.cta.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool barrier_try(uint32_t bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(done)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return done != 0;
+}
+constexpr int kWaitLimit = 1 << 22;  // tries; each may sleep for the hardware's time limit
+__device__ __forceinline__ void barrier_wait(uint32_t bar, uint32_t parity, int32_t* status) {
+    for (int i = 0; i < kWaitLimit; ++i)
+        if (barrier_try(bar, parity)) return;
+    atomicOr(status, DBS_CUDA_CACHE_STATUS_TIMEOUT);
+}
+__device__ __forceinline__ void named_sync(int id, int threads) {
+    asm volatile("barrier.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+__device__ __forceinline__ void tma_load(uint32_t to, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(to),
+        "l"(map), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
+
+// The tensor map of the pages as [rows, head_dim], boxes of one page by 64 elements, swizzled so
+// that eight rows of 128 bytes cover all banks. False: the driver refused it.
+bool page_map(const CacheView& c, int dtype, CUtensorMap* map);
+
+int64_t attend_mma_workspace(const CacheView& c, const AttendParams& a, int sm_count);
+cudaError_t launch_attend_mma(const CacheView& c, int dtype, const AttendParams& a, int sm_count, cudaStream_t stream);
+
+}  // namespace dbsb

@@ -1,0 +1,572 @@
+// SPDX-License-Identifier: MIT
+//
+// State of the paged beam cache: forking beams by their parents, accepting a drafted path,
+// compacting the pool (include/dbs_cuda_cache.h gives the rules).
+//
+// References need no recount. Of the old entry (r, c), a complete page, every child of r keeps a
+// reference; of an incomplete or spare page only the first child does, if it needs the column. So
+// the entry's page changes by (holders - 1), known from three numbers a beam (children, first
+// child, columns the first child needs), and entries that all beams share cancel in the thread
+// before they reach an atomic. Integer sums, so the order of the atomics does not show.
+//
+// New pages are handed out by the last CTA to finish: one scan of the slots' wishes, one scan of
+// the references for zeros that stops as soon as there are enough. Nothing else is serial.
+#include <climits>
+
+#include "cache.cuh"
+
+namespace dbsb {
+
+namespace {
+
+constexpr int kMetaThreads = 512;
+constexpr int kStageInts = 8192;  // table entries of an example staged at a time
+constexpr int kCopyThreads = 256;
+
+struct ForkArgs {
+    const int32_t* parents;
+    const int32_t* written;
+    const int32_t* room;
+    int written_all, room_all;
+};
+
+__device__ __forceinline__ void raise(const CacheView& c, int bit) { atomicOr(c.status, bit); }
+
+// The last CTA of fork_meta_kernel: ranks of the wishes, free pages for them, the copy list.
+__device__ void hand_out(const CacheView& c, int* sums) {
+    const int S = c.B * c.K, tid = threadIdx.x;
+    int wanted = 0, copies = 0;
+    for (int base = 0; base < S; base += kMetaThreads) {
+        const int s = base + tid;
+        const int n = s < S ? __ldcg(c.want_count + s) : 0;
+        const int copy = s < S && __ldcg(c.copy_rows + s) > 0;
+        int total;
+        const int before = block_scan(n, sums, &total);
+        if (s < S) c.want_rank[s] = wanted + before;
+        wanted += total;
+        const int at = block_scan(copy, sums, &total);
+        if (copy) c.copy_list[copies + at] = s;
+        copies += total;
+    }
+    // Zeros of the references, 16 a thread and round.
+    int found = 0;
+    for (int base = 0; base < c.P && found < wanted; base += kMetaThreads * 16) {
+        const int at = base + tid * 16;
+        unsigned zero = 0;
+        if (at + 16 <= c.P) {
+            int4 v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = __ldcg(reinterpret_cast<const int4*>(c.references + at) + i);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                zero |= ((v[i].x == 0) | (v[i].y == 0) << 1 | (v[i].z == 0) << 2 | (v[i].w == 0) << 3) << (4 * i);
+        } else {
+            for (int i = 0; i < 16 && at + i < c.P; ++i) zero |= (__ldcg(c.references + at + i) == 0) << i;
+        }
+        int total;
+        int rank = found + block_scan(__popc(zero), sums, &total);
+        for (; zero != 0 && rank < wanted; zero &= zero - 1, ++rank) {
+            const int p = at + __ffs(zero) - 1;
+            c.free_list[rank] = p;
+            c.references[p] = 1;
+        }
+        found += total;
+    }
+    if (tid == 0) {
+        c.words[kWordCopies] = copies;
+        c.words[kWordFree] = found < wanted ? found : wanted;
+        c.words[kWordArrive] = 0;
+        if (found < wanted) raise(c, DBS_CUDA_CACHE_STATUS_POOL);
+    }
+}
+
+// One CTA an example. Entries that ask for a new page become -2 until cache_finish_kernel.
+__global__ void __launch_bounds__(kMetaThreads) fork_meta_kernel(CacheView c, ForkArgs a) {
+    extern __shared__ int32_t smem[];
+    __shared__ int sums[33];
+    __shared__ int last;
+    const int K = c.K, M = c.M, b = blockIdx.x, tid = threadIdx.x, log2 = c.page_log2;
+    int32_t* length = smem;         // [K] committed tokens of each beam, with the written ones
+    int32_t* children = length + K; // [K]
+    int32_t* first = children + K;  // [K] first child or INT_MAX
+    int32_t* src = first + K;       // [K] parent of each new beam or -1
+    int32_t* need = src + K;        // [K] columns of each new beam
+    int32_t* want = need + K;       // [K] new pages it asks for
+    int32_t* want_at = want + K;    // [K] the first such column
+    int32_t* stage = want_at + K;   // [K, width]
+    const int64_t slot0 = static_cast<int64_t>(b) * K;
+    grid_wait();   // what ran before may have written the parents
+    grid_release();
+    for (int k = tid; k < K; k += kMetaThreads) {
+        int64_t w = a.written ? a.written[slot0 + k] : a.written_all;
+        if (w < 0) {
+            raise(c, DBS_CUDA_CACHE_STATUS_INDEX);
+            w = 0;
+        }
+        int64_t n = c.lengths[slot0 + k] + w;
+        const int64_t most = static_cast<int64_t>(M) << log2;
+        if (n > most) {
+            raise(c, DBS_CUDA_CACHE_STATUS_CAPACITY);
+            n = most;
+        }
+        length[k] = static_cast<int32_t>(n < 0 ? 0 : n);
+        children[k] = 0;
+        first[k] = INT_MAX;
+        want[k] = 0;
+        want_at[k] = INT_MAX;
+    }
+    __syncthreads();
+    for (int k = tid; k < K; k += kMetaThreads) {
+        int p = a.parents ? a.parents[slot0 + k] : k;
+        if (p >= K) {
+            raise(c, DBS_CUDA_CACHE_STATUS_INDEX);
+            p = -1;
+        }
+        src[k] = p < 0 ? -1 : p;
+        int columns = 0;
+        if (p >= 0) {
+            atomicAdd(&children[p], 1);
+            atomicMin(&first[p], k);
+            int64_t m = a.room ? a.room[slot0 + k] : a.room_all;
+            if (m < 0) {
+                raise(c, DBS_CUDA_CACHE_STATUS_INDEX);
+                m = 0;
+            }
+            const int64_t n = (length[p] + m + c.page - 1) >> log2;
+            if (n > M) raise(c, DBS_CUDA_CACHE_STATUS_CAPACITY);
+            columns = static_cast<int>(n > M ? M : n);
+        }
+        need[k] = columns;
+        c.copy_from[slot0 + k] = -1;
+    }
+    __syncthreads();
+    const int width = K * M <= kStageInts ? M : (kStageInts / K > 1 ? kStageInts / K : 1);
+    int32_t* table = c.table + slot0 * M;
+    for (int base = 0; base < M; base += width) {
+        const int cols = M - base < width ? M - base : width;
+        for (int i = tid; i < K * cols; i += kMetaThreads) {
+            const int r = i / cols;
+            stage[r * width + i - r * cols] = table[static_cast<int64_t>(r) * M + base + i - r * cols];
+        }
+        __syncthreads();
+        for (int i = tid; i < cols; i += kMetaThreads) {
+            const int col = base + i;
+            int run = -1, delta = 0;
+            for (int r = 0; r < K; ++r) {
+                const int e = stage[r * width + i];
+                if (e < 0) continue;
+                const int heir = first[r];
+                const int holders = col < (length[r] >> log2) ? children[r] : (heir < K && col < need[heir]);
+                if (e != run) {
+                    if (delta != 0) atomicAdd(c.references + run, delta);
+                    run = e;
+                    delta = 0;
+                }
+                delta += holders - 1;
+            }
+            if (delta != 0) atomicAdd(c.references + run, delta);
+            for (int s = 0; s < K; ++s) {
+                const int p = src[s];
+                int e = -1;
+                if (p >= 0 && col < need[s]) {
+                    const int held = stage[p * width + i], full = length[p] >> log2;
+                    if (col < full || first[p] == s) e = held;
+                    if (col >= full && e < 0) {
+                        e = -2;
+                        atomicAdd(&want[s], 1);
+                        atomicMin(&want_at[s], col);
+                    }
+                    if (col == full && first[p] != s && (length[p] & (c.page - 1)) != 0) c.copy_from[slot0 + s] = held;
+                }
+                if (e != stage[s * width + i]) table[static_cast<int64_t>(s) * M + col] = e;
+            }
+        }
+        __syncthreads();
+    }
+    for (int s = tid; s < K; s += kMetaThreads) {
+        const int p = src[s];
+        c.lengths[slot0 + s] = p >= 0 ? length[p] : 0;
+        c.want_count[slot0 + s] = want[s];
+        c.want_first[slot0 + s] = want_at[s];
+        const bool copies = p >= 0 && first[p] != s && c.copy_from[slot0 + s] >= 0;
+        c.copy_rows[slot0 + s] = copies ? length[p] & (c.page - 1) : 0;
+    }
+    __threadfence();
+    __syncthreads();
+    if (tid == 0) last = atomicAdd(c.words + kWordArrive, 1) == c.B - 1;
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    hand_out(c, sums);
+}
+
+// The units of a group of beams, from its final table rows (column order, then first beam).
+// resolve: entries of -2 take their slot's new pages first.
+__device__ void write_plan(const CacheView& c, int group, bool resolve, int* sums, int32_t* shared) {
+    const int b = group / c.groups, k0 = (group - b * c.groups) * kGroupBeams;
+    const int n = c.K - k0 < kGroupBeams ? c.K - k0 : kGroupBeams;
+    const int64_t slot0 = static_cast<int64_t>(b) * c.K + k0;
+    int32_t* table = c.table + slot0 * c.M;
+    CacheUnit* units = c.units + static_cast<int64_t>(group) * c.unit_cap;
+    int32_t* length = shared;                   // [32]
+    int32_t* rank = shared + kGroupBeams;       // [32] rank of the first new page
+    int32_t* from = shared + 2 * kGroupBeams;   // [32] its column
+    int32_t* stage = shared + 3 * kGroupBeams;  // [n, blockDim.x]
+    const int tid = threadIdx.x, threads = blockDim.x;
+    if (tid < n) {
+        length[tid] = c.lengths[slot0 + tid];
+        rank[tid] = resolve ? c.want_rank[slot0 + tid] : 0;
+        from[tid] = resolve ? c.want_first[slot0 + tid] : 0;
+    }
+    const int handed = resolve ? c.words[kWordFree] : 0;
+    __syncthreads();
+    int count = 0;
+    for (int base = 0; base < c.M; base += threads) {
+        const int col = base + tid;
+        int mine = 0;
+        bool shared_tail = false;
+        if (col < c.M) {
+            const int end = (col + 1) << c.page_log2;
+            uint32_t seen = 0;
+            for (int k = 0; k < n; ++k) {
+                int e = table[static_cast<int64_t>(k) * c.M + col];
+                if (resolve && e == -2) {
+                    const int at = rank[k] + col - from[k];
+                    e = at < handed ? c.free_list[at] : -1;
+                    table[static_cast<int64_t>(k) * c.M + col] = e;
+                }
+                stage[k * threads + tid] = e;
+            }
+            for (int k = 0; k < n; ++k) {
+                const int e = stage[k * threads + tid];
+                if (e < 0 || (seen >> k & 1)) continue;
+                ++mine;
+                bool complete = true;
+                uint32_t holders = 0;
+                for (int j = k; j < n; ++j)
+                    if (stage[j * threads + tid] == e) {
+                        holders |= 1u << j;
+                        complete &= end <= length[j];
+                    }
+                seen |= holders;
+                shared_tail |= !complete && (holders & (holders - 1)) != 0;
+            }
+        }
+        int total;
+        int at = count + block_scan(mine, sums, &total);
+        if (mine > 0) {
+            const int end = (col + 1) << c.page_log2;
+            uint32_t seen = 0;
+            for (int k = 0; k < n; ++k) {
+                const int e = stage[k * threads + tid];
+                if (e < 0 || (seen >> k & 1)) continue;
+                bool complete = true;
+                uint32_t holders = 0;
+                for (int j = k; j < n; ++j)
+                    if (stage[j * threads + tid] == e) {
+                        holders |= 1u << j;
+                        complete &= end <= length[j];
+                    }
+                seen |= holders;
+                units[at++] = CacheUnit{e, col << c.page_log2, holders, complete ? -1 : length[k]};
+            }
+        }
+        if (shared_tail) raise(c, DBS_CUDA_CACHE_STATUS_SHARED);
+        count += total;
+    }
+    if (tid == 0) c.unit_count[group] = count;
+}
+
+constexpr size_t plan_smem() { return (3 * kGroupBeams + kGroupBeams * kCopyThreads) * sizeof(int32_t); }
+
+// After fork_meta_kernel: the plan and the new pages of the table (one CTA a group), and the
+// copies of incomplete pages (the other CTAs; a warp takes the rows of one layer, kind and head,
+// which are contiguous).
+__global__ void __launch_bounds__(kCopyThreads) cache_finish_kernel(CacheView c, int plan_blocks) {
+    extern __shared__ int32_t smem[];
+    __shared__ int sums[33];
+    grid_wait();
+    if (static_cast<int>(blockIdx.x) < plan_blocks) {
+        write_plan(c, blockIdx.x, true, sums, smem);
+        return;
+    }
+    const int copies = c.words[kWordCopies], handed = c.words[kWordFree];
+    const int per = c.L * 2 * c.H;
+    const int64_t items = static_cast<int64_t>(copies) * per;
+    const int lane = threadIdx.x & 31;
+    const int64_t warps = static_cast<int64_t>(gridDim.x - plan_blocks) * (kCopyThreads / 32);
+    const int row_vecs = c.D * c.elem / 16;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x - plan_blocks) * (kCopyThreads / 32) + (threadIdx.x >> 5);
+         i < items; i += warps) {
+        const int slot = c.copy_list[i / per], part = static_cast<int>(i % per);
+        const int from = c.copy_from[slot], at = c.want_rank[slot];
+        if (at >= handed) continue;  // the pool ran out
+        const int to = c.free_list[at];
+        const int64_t block = part / c.H, head = part % c.H;  // block: layer * 2 + kind
+        const int64_t vecs = static_cast<int64_t>(c.page) * row_vecs;
+        const uint4* x = static_cast<const uint4*>(c.pages) + ((block * c.P + from) * c.H + head) * vecs;
+        uint4* y = static_cast<uint4*>(c.pages) + ((block * c.P + to) * c.H + head) * vecs;
+        const int n = c.copy_rows[slot] * row_vecs;
+        int v = lane;
+        for (; v + 7 * 32 < n; v += 8 * 32) {
+            uint4 t[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) t[j] = x[v + 32 * j];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[v + 32 * j] = t[j];
+        }
+        for (; v < n; v += 32) y[v] = x[v];
+    }
+}
+
+// Rows of an accepted path to the front of the drafted area. A thread owns 16 bytes of every row
+// of one slot, layer, kind and head, and moves eight rows a round: row path[a] >= a lies at or
+// behind every row that earlier rounds wrote, and a round reads all its rows before it writes.
+__global__ void __launch_bounds__(kCopyThreads) commit_move_kernel(CacheView c, const int32_t* path, int path_stride,
+                                                                   const int32_t* counts) {
+    grid_wait();
+    grid_release();
+    const int row_vecs = c.D * c.elem / 16;
+    const int64_t per = static_cast<int64_t>(c.L) * 2 * c.H * row_vecs;
+    const int64_t items = static_cast<int64_t>(c.B) * c.K * per;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kCopyThreads + threadIdx.x; i < items;
+         i += static_cast<int64_t>(gridDim.x) * kCopyThreads) {
+        const int64_t slot = i / per;
+        int rest = static_cast<int>(i - slot * per);
+        const int vec = rest % row_vecs;
+        rest /= row_vecs;
+        const int64_t head = rest % c.H, block = rest / c.H;
+        int count = counts[slot];
+        if (count > path_stride) {
+            raise(c, DBS_CUDA_CACHE_STATUS_INDEX);
+            count = path_stride;
+        }
+        const int n = c.lengths[slot];
+        const int32_t* row = c.table + slot * c.M;
+        uint4* pages = static_cast<uint4*>(c.pages) + vec;
+        auto place = [&](int64_t pos) -> uint4* {
+            const int64_t col = pos >> c.page_log2;
+            if (col >= c.M) return nullptr;
+            const int p = row[col];
+            if (p < 0) return nullptr;
+            return pages + (((block * c.P + p) * c.H + head) * c.page + (pos & (c.page - 1))) * row_vecs;
+        };
+        int before = -1;
+        for (int a = 0; a < count; a += 8) {
+            uint4 t[8];
+            uint4* to[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                to[j] = nullptr;
+                if (a + j < count) {
+                    const int from = path[slot * path_stride + a + j];
+                    if (from <= before) {  // not increasing: leave the row
+                        raise(c, DBS_CUDA_CACHE_STATUS_INDEX);
+                    } else {
+                        before = from;
+                        const uint4* x = from != a + j ? place(static_cast<int64_t>(n) + from) : nullptr;
+                        uint4* y = place(static_cast<int64_t>(n) + a + j);
+                        if (x != nullptr && y != nullptr) {
+                            t[j] = *x;
+                            to[j] = y;
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (to[j] != nullptr) *to[j] = t[j];
+        }
+    }
+}
+
+// Ranks of holes and movers from one prefix count of the pages in use: with n in use, hole h < n
+// has rank h - live_before(h), mover m >= n rank live_before(m) - live_before(n).
+__global__ void __launch_bounds__(1024) compact_meta_kernel(CacheView c) {
+    __shared__ int sums[33];
+    __shared__ int below;
+    grid_wait();
+    grid_release();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int span = (c.P + 32 * 32 - 1) / (32 * 32) * 32;  // pages of a warp
+    const int lo = warp * span, hi = lo + span < c.P ? lo + span : c.P;
+    int mine = 0;
+    for (int p = lo + lane; p < hi; p += 32) mine += c.references[p] > 0;
+    for (int d = 16; d > 0; d >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, d);
+    int n;
+    const int scanned = block_scan(lane == 0 ? mine : 0, sums, &n);
+    const int before = __shfl_sync(0xffffffffu, scanned, 0);
+    if (tid == 0) below = n;  // when every live page is below n already
+    __syncthreads();
+    auto walk = [&](auto&& visit) {
+        int live = before;
+        for (int base = lo; base < hi; base += 32) {
+            const int p = base + lane;
+            const int refs = p < hi ? c.references[p] : 0;
+            const unsigned bits = __ballot_sync(0xffffffffu, refs > 0);
+            if (p < hi) visit(p, refs, live + __popc(bits & ((1u << lane) - 1)));
+            live += __popc(bits);
+        }
+    };
+    if (lo <= n && n < hi) walk([&](int p, int, int rank) {
+        if (p == n) below = rank;
+    });
+    __syncthreads();
+    walk([&](int p, int refs, int rank) {
+        if (p < n && refs <= 0) c.free_list[p - rank] = p;
+        if (p >= n && refs > 0) c.move_list[rank - below] = p;
+    });
+    __threadfence_block();
+    __syncthreads();
+    const int moves = n - below;
+    for (int i = tid; i < moves; i += 1024) {
+        const int from = c.move_list[i], to = c.free_list[i];
+        c.move_to[from] = to;
+        c.references[to] = c.references[from];
+        c.references[from] = 0;
+    }
+    if (tid == 0) {
+        c.words[kWordLive] = n;
+        c.words[kWordMoves] = moves;
+    }
+}
+
+// The moves (a CTA takes 16 KB of a page's block of one layer and kind at a time), and the new
+// page numbers in table and plan.
+__global__ void __launch_bounds__(kCopyThreads) compact_move_kernel(CacheView c) {
+    grid_wait();
+    const int n = c.words[kWordLive], moves = c.words[kWordMoves];
+    if (moves == 0) return;
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * kCopyThreads + threadIdx.x;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * kCopyThreads;
+    const int64_t entries = static_cast<int64_t>(c.B) * c.K * c.M;
+    for (int64_t i = first; i < entries; i += step) {
+        const int p = c.table[i];
+        if (p >= n) c.table[i] = c.move_to[p];
+    }
+    const int64_t units = static_cast<int64_t>(c.B) * c.groups * c.unit_cap;
+    for (int64_t i = first; i < units; i += step) {
+        const int64_t group = i / c.unit_cap;
+        if (i - group * c.unit_cap >= c.unit_count[group]) continue;
+        const int p = c.units[i].page;
+        if (p >= n) c.units[i].page = c.move_to[p];
+    }
+    const int64_t vecs = static_cast<int64_t>(c.H) * c.page * c.D * c.elem / 16;  // of a block
+    constexpr int kPiece = kCopyThreads * 4;
+    const int64_t pieces = (vecs + kPiece - 1) / kPiece;
+    const int64_t items = static_cast<int64_t>(moves) * c.L * 2 * pieces;
+    for (int64_t i = blockIdx.x; i < items; i += gridDim.x) {
+        const int64_t piece = i % pieces, rest = i / pieces;
+        const int64_t block = rest % (c.L * 2), move = rest / (c.L * 2);
+        const uint4* x = static_cast<const uint4*>(c.pages) + (block * c.P + c.move_list[move]) * vecs;
+        uint4* y = static_cast<uint4*>(c.pages) + (block * c.P + c.free_list[move]) * vecs;
+        const int64_t at = piece * kPiece + threadIdx.x;
+        uint4 t[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (at + j * kCopyThreads < vecs) t[j] = x[at + j * kCopyThreads];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (at + j * kCopyThreads < vecs) y[at + j * kCopyThreads] = t[j];
+    }
+}
+
+__global__ void refresh_count_kernel(CacheView c) {
+    const int64_t entries = static_cast<int64_t>(c.B) * c.K * c.M;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < entries;
+         i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+        const int p = c.table[i];
+        if (p >= c.P || p < -1) {
+            raise(c, DBS_CUDA_CACHE_STATUS_INDEX);
+            c.table[i] = -1;
+        } else if (p >= 0) {
+            atomicAdd(c.references + p, 1);
+        }
+    }
+}
+
+__global__ void __launch_bounds__(kCopyThreads) refresh_plan_kernel(CacheView c) {
+    extern __shared__ int32_t smem[];
+    __shared__ int sums[33];
+    write_plan(c, blockIdx.x, false, sums, smem);
+}
+
+// Whether the values of the pool hold one that is not finite (exponent bits all set).
+__global__ void refresh_values_kernel(CacheView c, uint32_t exponent_lo, uint32_t exponent_hi) {
+    const int64_t vecs = static_cast<int64_t>(c.P) * c.H * c.page * c.D * c.elem / 16;  // of a layer and kind
+    bool odd = false;
+    for (int layer = 0; layer < c.L; ++layer) {
+        const uint4* x = static_cast<const uint4*>(c.pages) + (2 * layer + 1) * vecs;
+        for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < vecs;
+             i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+            const uint4 v = x[i];
+            for (uint32_t w : {v.x, v.y, v.z, v.w})
+                odd |= (w & exponent_lo) == exponent_lo || (w & exponent_hi) == exponent_hi;
+        }
+    }
+    if (odd) c.status[1] = 1;
+}
+
+size_t meta_smem(const CacheView& c) {
+    const int64_t all = static_cast<int64_t>(c.K) * c.M;
+    const int64_t stage = all <= kStageInts ? all : (c.K > kStageInts ? c.K : kStageInts);
+    return (7 * static_cast<size_t>(c.K) + stage) * sizeof(int32_t);
+}
+
+unsigned copy_blocks(int64_t work, int sm_count) {
+    const int64_t cap = static_cast<int64_t>(sm_count) * 8;
+    return static_cast<unsigned>(work < 1 ? 1 : (work < cap ? work : cap));
+}
+
+}  // namespace
+
+cudaError_t launch_cache_fork(const CacheView& c, const int32_t* parents, const int32_t* written, int written_all,
+                              const int32_t* room, int room_all, int sm_count, cudaStream_t stream) {
+    const size_t smem = meta_smem(c);
+    cudaError_t e = cudaSuccess;
+    if (smem > 48 * 1024)
+        e = cudaFuncSetAttribute(fork_meta_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (e != cudaSuccess) return e;
+    const ForkArgs a{parents, written, room, written_all, room_all};
+    e = launch_after(fork_meta_kernel, c.B, kMetaThreads, smem, stream, c, a);
+    if (e != cudaSuccess) return e;
+    const int plan_blocks = c.B * c.groups;
+    // Without parents every beam is its own first child: nothing is copied.
+    const int64_t parts = parents ? static_cast<int64_t>(c.B) * c.K * c.L * 2 * c.H / (kCopyThreads / 32) : 0;
+    const unsigned blocks = plan_blocks + (parts > 0 || parents ? copy_blocks(parts, sm_count) : 0);
+    return launch_after(cache_finish_kernel, blocks, kCopyThreads, plan_smem(), stream, c, plan_blocks);
+}
+
+cudaError_t launch_cache_commit(const CacheView& c, const int32_t* path, int path_stride, const int32_t* counts,
+                                int room_all, int sm_count, cudaStream_t stream) {
+    const int64_t items = static_cast<int64_t>(c.B) * c.K * c.L * 2 * c.H * (c.D * c.elem / 16);
+    const cudaError_t e = launch_after(commit_move_kernel, copy_blocks((items + kCopyThreads - 1) / kCopyThreads, sm_count),
+                                       kCopyThreads, 0, stream, c, path, path_stride, counts);
+    if (e != cudaSuccess) return e;
+    return launch_cache_fork(c, nullptr, counts, 0, nullptr, room_all, sm_count, stream);
+}
+
+cudaError_t launch_cache_compact(const CacheView& c, int sm_count, cudaStream_t stream) {
+    const cudaError_t e = launch_after(compact_meta_kernel, 1, 1024, 0, stream, c);
+    if (e != cudaSuccess) return e;
+    const int64_t most = static_cast<int64_t>(c.P) * c.L * 2 * c.H * c.page * c.D * c.elem / 16 / (kCopyThreads * 4);
+    return launch_after(compact_move_kernel, copy_blocks(most, sm_count), kCopyThreads, 0, stream, c);
+}
+
+cudaError_t launch_cache_refresh(const CacheView& c, int dtype, bool values, int sm_count, cudaStream_t stream) {
+    cudaError_t e = cudaMemsetAsync(c.references, 0, static_cast<size_t>(c.P) * 4, stream);
+    if (e != cudaSuccess) return e;
+    const int64_t entries = static_cast<int64_t>(c.B) * c.K * c.M;
+    refresh_count_kernel<<<copy_blocks((entries + 255) / 256, sm_count), 256, 0, stream>>>(c);
+    refresh_plan_kernel<<<c.B * c.groups, kCopyThreads, plan_smem(), stream>>>(c);
+    if (values) {
+        e = cudaMemsetAsync(c.status + 1, 0, 4, stream);
+        if (e != cudaSuccess) return e;
+        const uint32_t exponent = dtype == DBS_CUDA_DTYPE_F16 ? 0x7c00u : 0x7f80u;
+        const uint32_t lo = dtype == DBS_CUDA_DTYPE_F32 ? exponent << 16 : exponent;
+        refresh_values_kernel<<<sm_count * 8, 256, 0, stream>>>(c, lo, exponent << 16);
+    }
+    return cudaGetLastError();
+}
+
+}  // namespace dbsb
