@@ -15,7 +15,7 @@ constexpr int kRowThreads = 128;
 // finite raises the cache's second status word: the attention then keeps masked values out of its
 // sums element by element, where otherwise a weight of zero is enough.
 template <class T>
-__global__ void __launch_bounds__(kAppendThreads) append_kernel(CacheView c, AttendParams a) {
+__global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_constant__ CacheView c, const __grid_constant__ AttendParams a) {
     grid_wait();
     grid_release();
     const int vecs = c.D / Pack<T>::n;
@@ -52,14 +52,14 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(CacheView c, Att
 
 // One warp a query row.
 template <class T>
-__global__ void __launch_bounds__(kRowThreads) rows_kernel(CacheView c, AttendParams a) {
+__global__ void __launch_bounds__(kRowThreads) rows_kernel(const __grid_constant__ CacheView c, const __grid_constant__ AttendParams a) {
     __shared__ float query[kRowThreads / 32 * DBS_CUDA_CACHE_MAX_HEAD_DIM];
     grid_wait();
     attend_all_rows<T>(c, a, query, threadIdx.x >> 5, kRowThreads / 32);
 }
 
 template <class T>
-cudaError_t launch_typed(const CacheView& c, const AttendParams& a, int sm_count, cudaStream_t stream) {
+cudaError_t launch_typed(const CacheView& c, int dtype, const AttendParams& a, int sm_count, cudaStream_t stream) {
     const int64_t cap = static_cast<int64_t>(sm_count) * 8;
     if (a.k != nullptr) {
         const int64_t items = static_cast<int64_t>(c.B) * a.beams * a.N * c.H * (c.D / Pack<T>::n);
@@ -68,6 +68,7 @@ cudaError_t launch_typed(const CacheView& c, const AttendParams& a, int sm_count
                                            kAppendThreads, 0, stream, c, a);
         if (e != cudaSuccess) return e;
     }
+    if constexpr (sizeof(T) == 2) return launch_attend_mma(c, dtype, a, sm_count, stream);
     const int64_t rows = static_cast<int64_t>(c.B) * a.beams * a.N * a.Hq;
     return launch_after(rows_kernel<T>, static_cast<unsigned>((rows + kRowThreads / 32 - 1) / (kRowThreads / 32)),
                         kRowThreads, 0, stream, c, a);
@@ -75,12 +76,14 @@ cudaError_t launch_typed(const CacheView& c, const AttendParams& a, int sm_count
 
 }  // namespace
 
-int64_t attend_workspace(const CacheView&, const AttendParams&, int) { return 256; }
+int64_t attend_workspace(const CacheView& c, const AttendParams& a, int sm_count) {
+    return c.elem == 2 ? attend_mma_workspace(c, a, sm_count) : 256;
+}
 
 cudaError_t launch_attend(const CacheView& c, int dtype, const AttendParams& a, int sm_count, cudaStream_t stream) {
-    if (dtype == DBS_CUDA_DTYPE_F32) return launch_typed<float>(c, a, sm_count, stream);
-    if (dtype == DBS_CUDA_DTYPE_F16) return launch_typed<__half>(c, a, sm_count, stream);
-    return launch_typed<__nv_bfloat16>(c, a, sm_count, stream);
+    if (dtype == DBS_CUDA_DTYPE_F32) return launch_typed<float>(c, dtype, a, sm_count, stream);
+    if (dtype == DBS_CUDA_DTYPE_F16) return launch_typed<__half>(c, dtype, a, sm_count, stream);
+    return launch_typed<__nv_bfloat16>(c, dtype, a, sm_count, stream);
 }
 
 }  // namespace dbsb

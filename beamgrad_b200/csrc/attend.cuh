@@ -341,11 +341,16 @@ __device__ __forceinline__ bool barrier_try(uint32_t bar, uint32_t parity) {
         : "memory");
     return done != 0;
 }
-constexpr int kWaitLimit = 1 << 22;  // tries; each may sleep for the hardware's time limit
-__device__ __forceinline__ void barrier_wait(uint32_t bar, uint32_t parity, int32_t* status) {
-    for (int i = 0; i < kWaitLimit; ++i)
+constexpr int kWaitLimit = 1 << 20;  // tries; each may sleep for the hardware's time limit
+__device__ __forceinline__ void barrier_wait_long(uint32_t bar, uint32_t parity, int32_t* status) {
+    for (int i = 0; i < kWaitLimit; ++i) {
         if (barrier_try(bar, parity)) return;
+        if ((i & 1023) == 1023 && (*static_cast<volatile int32_t*>(status) & DBS_CUDA_CACHE_STATUS_TIMEOUT) != 0) return;
+    }
     atomicOr(status, DBS_CUDA_CACHE_STATUS_TIMEOUT);
+}
+__device__ __forceinline__ void barrier_wait(uint32_t bar, uint32_t parity, int32_t* status) {
+    if (!barrier_try(bar, parity)) barrier_wait_long(bar, parity, status);
 }
 __device__ __forceinline__ void named_sync(int id, int threads) {
     asm volatile("barrier.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
