@@ -68,7 +68,8 @@ cudaError_t launch_typed(const CacheView& c, int dtype, const AttendParams& a, i
                                            kAppendThreads, 0, stream, c, a);
         if (e != cudaSuccess) return e;
     }
-    if constexpr (sizeof(T) == 2) return launch_attend_mma(c, dtype, a, sm_count, stream);
+    if constexpr (sizeof(T) == 2)
+        return c.D <= 128 ? launch_attend_tc(c, dtype, a, sm_count, stream) : launch_attend_mma(c, dtype, a, sm_count, stream);
     const int64_t rows = static_cast<int64_t>(c.B) * a.beams * a.N * a.Hq;
     return launch_after(rows_kernel<T>, static_cast<unsigned>((rows + kRowThreads / 32 - 1) / (kRowThreads / 32)),
                         kRowThreads, 0, stream, c, a);
@@ -77,7 +78,8 @@ cudaError_t launch_typed(const CacheView& c, int dtype, const AttendParams& a, i
 }  // namespace
 
 int64_t attend_workspace(const CacheView& c, const AttendParams& a, int sm_count) {
-    return c.elem == 2 ? attend_mma_workspace(c, a, sm_count) : 256;
+    if (c.elem == 4) return 256;
+    return c.D <= 128 ? attend_tc_workspace(c, a, sm_count) : attend_mma_workspace(c, a, sm_count);
 }
 
 cudaError_t launch_attend(const CacheView& c, int dtype, const AttendParams& a, int sm_count, cudaStream_t stream) {

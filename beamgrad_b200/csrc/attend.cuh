@@ -5,6 +5,7 @@
 #pragma once
 
 #include <climits>
+#include <type_traits>
 
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -366,6 +367,8 @@ __device__ __forceinline__ void tma_load(uint32_t to, const CUtensorMap* map, in
 // that eight rows of 128 bytes cover all banks. False: the driver refused it.
 bool page_map(const CacheView& c, int dtype, CUtensorMap* map);
 
+int64_t attend_tc_workspace(const CacheView& c, const AttendParams& a, int sm_count);
+cudaError_t launch_attend_tc(const CacheView& c, int dtype, const AttendParams& a, int sm_count, cudaStream_t stream);
 int64_t attend_mma_workspace(const CacheView& c, const AttendParams& a, int sm_count);
 cudaError_t launch_attend_mma(const CacheView& c, int dtype, const AttendParams& a, int sm_count, cudaStream_t stream);
 

@@ -89,7 +89,7 @@ attend_mma_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant
     float* join = reinterpret_cast<float*>(query + S::kQuery);  // 4 buffers of [kHalfRows][DP]
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int tile_units = kTileKeys >> c.page_log2;
-    const int blocks = (c.D + 63) / 64;
+    constexpr int blocks = S::kBlocks;  // all of them: past head_dim the copies fill in zeros
 
     if (tid == 0) {
         for (int s = 0; s < S::kStages; ++s) {
@@ -228,7 +228,6 @@ attend_mma_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant
                         for (int e = 0; e < 4; ++e) s[mt][n][e] = 0.0f;
 #pragma unroll
                 for (int k = 0; k < kSteps; ++k) {
-                    if (k * 16 >= c.D) break;
                     uint32_t kf[4];
                     const int row = key0 + (lane & 7) + ((lane & 16) >> 1), chunk = 2 * k + ((lane >> 3) & 1);
                     ldmatrix4(kf, keys + (chunk >> 3) * (kTileKeys * 128) + swizzled(row, chunk & 7));
@@ -305,7 +304,6 @@ attend_mma_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant
                 }
 #pragma unroll
                 for (int n = 0; n < kSteps; ++n) {
-                    if (n * 16 >= c.D) break;
                     uint32_t vf[4];
                     const int row = key0 + (lane & 15), chunk = 2 * n + (lane >> 4);
                     ldmatrix4_trans(vf, keys + S::kHalf + (chunk >> 3) * (kTileKeys * 128) + swizzled(row, chunk & 7));

@@ -1,0 +1,609 @@
+// SPDX-License-Identifier: MIT
+//
+// Attention of a group of beams over the paged cache on the fifth-generation tensor cores, for
+// float16 and bfloat16 and heads of up to 128.
+//
+// 128 query rows by 128 positions at a time: S = Q K^T into tensor memory, the weights P back to
+// tensor memory in the place of S, O += P V in tensor memory. One warp copies keys and values by
+// TMA through a ring of slots (a slot holds 128 rows of keys or of values), one thread issues the
+// products, and two warpgroups work on the scores, a thread a row: no maximum or sum crosses a
+// thread. The two warpgroups and their S and O are two streams, so that the products of one run
+// while the other takes exponentials. NQ = 2: each stream has query rows of its own (256 a block)
+// and takes every tile; NQ = 1: both have the same 128 rows, take alternate tiles and are joined
+// at the end of a segment.
+//
+// A row's reference for the exponentials is raised only when its maximum has grown by more than
+// 2^8: until then the weights stay below 2^8 and the sums within 32 bits, and O in tensor memory
+// is left alone. Weights are rounded to the input type, as the values are; their sum is taken
+// before. All statistics are 32 bits.
+#include "attend.cuh"
+
+namespace dbsb {
+
+namespace {
+
+constexpr int kTileKeys = 128;
+constexpr int kSoftThreads = 256;
+constexpr int kThreads = kSoftThreads + 128;  // and a warpgroup with the copying and the issuing warp
+constexpr int kCopyWarp = 8, kIssueWarp = 9;
+constexpr int kMaxSlots = 12;
+constexpr float kRaise = 8.0f;  // log2 of the growth that a reference tolerates
+
+template <int DP, int NQ>
+struct Shape {
+    static constexpr int kRows = 128 * NQ;
+    static constexpr int kBlocks = DP / 64;
+    static constexpr int kSlot = kTileKeys * DP * 2;
+    // The queries; at the end of a segment NQ = 1 joins its streams there, 2 x 128 x 32 floats.
+    static constexpr int kQuery = kRows * DP * 2 > 32768 ? kRows * DP * 2 : 32768;
+    static constexpr int kSlots = (224 * 1024 - kQuery) / kSlot < kMaxSlots ? (224 * 1024 - kQuery) / kSlot : kMaxSlots;
+    static constexpr int kOut = kRows * (DP + 2);  // floats of a partial result
+    static constexpr int kBytes = 1024 + kSlots * kSlot + kQuery;
+};
+
+struct Control {
+    uint64_t full[kMaxSlots], empty[kMaxSlots];
+    uint64_t scores[2], weights[2], output[2], queries;
+    float top[128], sum[128];
+    int sums[33];
+    WorkSplit split;
+    uint32_t tmem;
+    int last;
+};
+
+// ---- tcgen05 ----
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void product_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t kind, bool add) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(kind), "r"(static_cast<uint32_t>(add))
+        : "memory");
+}
+__device__ __forceinline__ void product_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t kind, bool add) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+        "r"(a), "l"(b), "r"(kind), "r"(static_cast<uint32_t>(add))
+        : "memory");
+}
+#define REGS8(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]), "=r"(r[i + 7])
+#define REGS32(r, i) REGS8(r, i), REGS8(r, i + 8), REGS8(r, i + 16), REGS8(r, i + 24)
+// 32 (128) columns of the warp's 32 lanes, with the wait for them: a use of a register cannot move
+// before it.
+__device__ __forceinline__ void tmem_load(uint32_t (&r)[32], uint32_t at) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+        "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n tcgen05.wait::ld.sync.aligned;"
+        : REGS32(r, 0)
+        : "r"(at)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_load(uint32_t (&r)[128], uint32_t at) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x128.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
+        "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
+        "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63,"
+        "%64,%65,%66,%67,%68,%69,%70,%71,%72,%73,%74,%75,%76,%77,%78,%79,"
+        "%80,%81,%82,%83,%84,%85,%86,%87,%88,%89,%90,%91,%92,%93,%94,%95,"
+        "%96,%97,%98,%99,%100,%101,%102,%103,%104,%105,%106,%107,%108,%109,%110,%111,"
+        "%112,%113,%114,%115,%116,%117,%118,%119,%120,%121,%122,%123,%124,%125,%126,%127}, [%128];\n tcgen05.wait::ld.sync.aligned;"
+        : REGS32(r, 0), REGS32(r, 32), REGS32(r, 64), REGS32(r, 96)
+        : "r"(at)
+        : "memory");
+}
+#undef REGS32
+#undef REGS8
+__device__ __forceinline__ void tmem_store(uint32_t at, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+        "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(at),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Shared-memory operand with 128-byte rows, swizzled: eight rows (1024 bytes) to the next eight
+// rows, and `blocks` bytes between 64-element blocks of an operand that runs along the row.
+__device__ __forceinline__ uint64_t operand(uint32_t at, uint32_t blocks) {
+    return static_cast<uint64_t>((at & 0x3ffffu) >> 4) | static_cast<uint64_t>(blocks >> 4) << 16 |
+           static_cast<uint64_t>(1024 >> 4) << 32 | uint64_t{1} << 46 | uint64_t{2} << 61;
+}
+// Instruction word: 32-bit sums, both operands of one 16-bit type, 128 rows, `columns` columns;
+// by_row: the second operand's columns run along its rows (values: positions by elements).
+template <class T>
+__device__ __forceinline__ constexpr uint32_t product_kind(int columns, bool by_row) {
+    constexpr uint32_t type = sizeof(T) == 2 && std::is_same_v<T, __nv_bfloat16> ? 1 : 0;
+    return 1u << 4 | type << 7 | type << 10 | (by_row ? 1u << 16 : 0u) | static_cast<uint32_t>(columns / 8) << 17 | 8u << 24;
+}
+
+template <class T, int DP, int NQ>
+__global__ void __launch_bounds__(kThreads, 1)
+attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ CacheView c,
+                 const __grid_constant__ AttendParams a) {
+    using S = Shape<DP, NQ>;
+    extern __shared__ uint8_t raw[];
+    __shared__ Control ctl;
+    uint8_t* smem = raw + (1024 - (smem_address(raw) & 1023)) % 1024;
+    const uint32_t slots = smem_address(smem);
+    uint8_t* query = smem + S::kSlots * S::kSlot;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int tile_units = kTileKeys >> c.page_log2;
+
+    if (tid == 0) {
+        for (int s = 0; s < S::kSlots; ++s) {
+            barrier_init(smem_address(&ctl.full[s]), 1);
+            barrier_init(smem_address(&ctl.empty[s]), 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            barrier_init(smem_address(&ctl.scores[i]), 1);
+            barrier_init(smem_address(&ctl.weights[i]), 4);
+            barrier_init(smem_address(&ctl.output[i]), 1);
+        }
+        barrier_init(smem_address(&ctl.queries), kSoftThreads / 32);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    // The plan was complete before the new tokens' copy began; only the pages have to be waited for.
+    const WorkSplit work = split_work<S::kRows>(c, a, tile_units, 1, ctl.sums, &ctl.split);
+    grid_wait();
+    grid_release();
+    if (__ldcg(c.status + 1) != 0) {
+        attend_all_rows<T>(c, a, reinterpret_cast<float*>(smem), warp, kThreads / 32);
+        return;
+    }
+    if (work.lo >= work.hi) return;
+    if (warp == kIssueWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_address(&ctl.tmem)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        fence_before();
+    }
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = ctl.tmem;  // S0, S1, O0, O1: 128 columns each
+    int group = work.group;
+    int64_t base = work.base;
+
+    // Registers: launched with 168 a thread; 2 x 128 x 224 + 128 x 56 = 384 x 168.
+    if (warp >= kCopyWarp) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp > kIssueWarp) return;
+        int used = 0;  // slots so far
+        if (warp == kCopyWarp) {
+            asm volatile("fence.proxy.async;" ::: "memory");
+            for (int64_t cur = work.lo; cur < work.hi;) {
+                const Piece p = piece_at<S::kRows>(c, a, work, cur, group, base, tile_units);
+                const CacheUnit* units = c.units + static_cast<int64_t>(p.group) * c.unit_cap;
+                const int n_tiles = p.t1 - p.t0;
+                // The page of this lane's copy; past the last unit, page 0: whatever finite values lie
+                // there meet weights of zero.
+                const int which = lane / S::kBlocks, block = lane % S::kBlocks;
+                auto page_of = [&](int t) {
+                    const int i = (p.t0 + t) * tile_units + which;
+                    return t < n_tiles && which < tile_units && i < p.units ? __ldg(&units[i].page) : 0;
+                };
+                auto copy = [&](int kind, int page) {
+                    const int slot = used % S::kSlots;
+                    const uint32_t full = smem_address(&ctl.full[slot]);
+                    if (used >= S::kSlots) barrier_wait(smem_address(&ctl.empty[slot]), (used / S::kSlots - 1) & 1, c.status);
+                    if (lane == 0) barrier_expect(full, S::kSlot);
+                    __syncwarp();
+                    if (which < tile_units) {
+                        const int64_t row = (((static_cast<int64_t>(a.layer) * 2 + kind) * c.P + page) * c.H + p.head) * c.page;
+                        tma_load(slots + slot * S::kSlot + block * (kTileKeys * 128) + which * c.page * 128, &map, block * 64,
+                                 static_cast<int>(row), full);
+                    }
+                    ++used;
+                };
+                // In the order in which the issuing thread takes them.
+                int page = page_of(0), next = page_of(1);
+                copy(0, page);
+                for (int t = 0; t < n_tiles; ++t) {
+                    const int after = page_of(t + 2);
+                    if (NQ == 1 && t + 1 < n_tiles) copy(0, next);
+                    copy(1, page);
+                    if (NQ == 2 && t + 1 < n_tiles) copy(0, next);
+                    page = next;
+                    next = after;
+                }
+                cur += n_tiles;
+            }
+            // No copy may be in flight when the CTA ends, even if a wait gave up.
+            for (int i = used > S::kSlots ? used - S::kSlots : 0; i < used; ++i)
+                barrier_wait(smem_address(&ctl.full[i % S::kSlots]), (i / S::kSlots) & 1, c.status);
+        } else {
+            if (lane == 0) {
+                constexpr uint32_t kScores = product_kind<T>(kTileKeys, false), kValues = product_kind<T>(DP, true);
+                uint32_t query_phase = 0, weight_phase[2] = {0, 0};
+                auto slot_of = [&](int i) { return i % S::kSlots; };
+                auto wait_slot = [&](int i) {
+                    barrier_wait(smem_address(&ctl.full[slot_of(i)]), (i / S::kSlots) & 1, c.status);
+                    fence_after();
+                };
+                auto free_slot = [&](int i) { commit(smem_address(&ctl.empty[slot_of(i)])); };
+                auto scores = [&](int stream, int i) {
+                    const uint32_t q = smem_address(query) + (NQ == 2 ? stream * 128 * DP * 2 : 0);
+                    const uint32_t k = slots + slot_of(i) * S::kSlot;
+#pragma unroll
+                    for (int s = 0; s < DP / 16; ++s)
+                        product_ss(tmem + stream * 128, operand(q + (s >> 2) * (128 * 128) + (s & 3) * 32, 16),
+                                   operand(k + (s >> 2) * (kTileKeys * 128) + (s & 3) * 32, 16), kScores, s > 0);
+                    commit(smem_address(&ctl.scores[stream]));
+                };
+                auto values = [&](int stream, int i, bool add) {
+                    barrier_wait(smem_address(&ctl.weights[stream]), weight_phase[stream], c.status);
+                    weight_phase[stream] ^= 1;
+                    fence_after();
+                    const uint32_t v = slots + slot_of(i) * S::kSlot;
+#pragma unroll
+                    for (int s = 0; s < kTileKeys / 16; ++s)
+                        product_ts(tmem + 256 + stream * 128, tmem + stream * 128 + s * 8,
+                                   operand(v + s * (16 * 128), kTileKeys * 128), kValues, add || s > 0);
+                };
+                for (int64_t cur = work.lo; cur < work.hi;) {
+                    const Piece p = piece_at<S::kRows>(c, a, work, cur, group, base, tile_units);
+                    const int n = p.t1 - p.t0;
+                    barrier_wait(smem_address(&ctl.queries), query_phase, c.status);
+                    query_phase ^= 1;
+                    fence_after();
+                    if (NQ == 2) {  // slots: K0 V0 K1 V1 ...
+                        const int streams = p.rows - p.block * S::kRows > 128 ? 2 : 1;
+                        wait_slot(used);
+                        for (int i = 0; i < streams; ++i) scores(i, used);
+                        free_slot(used);
+                        for (int t = 0; t < n; ++t) {
+                            const int v = used + 2 * t + 1;
+                            wait_slot(v);
+                            if (t + 1 < n) wait_slot(v + 1);
+                            for (int i = 0; i < streams; ++i) {
+                                values(i, v, t > 0);
+                                if (t + 1 < n) scores(i, v + 1);
+                                else commit(smem_address(&ctl.output[i]));
+                            }
+                            free_slot(v);
+                            if (t + 1 < n) free_slot(v + 1);
+                        }
+                    } else {  // slots: K0 K1 V0 K2 V1 ...
+                        auto key_slot = [&](int t) { return used + (t == 0 ? 0 : 2 * t - 1); };
+                        for (int t = 0; t < 2 && t < n; ++t) {
+                            wait_slot(key_slot(t));
+                            scores(t, key_slot(t));
+                            free_slot(key_slot(t));
+                        }
+                        for (int t = 0; t < n; ++t) {
+                            const int v = used + (t + 1 < n ? 2 * t + 2 : 2 * t + 1);
+                            wait_slot(v);
+                            values(t & 1, v, t > 1);
+                            free_slot(v);
+                            if (t + 2 < n) {
+                                wait_slot(key_slot(t + 2));
+                                scores(t & 1, key_slot(t + 2));
+                                free_slot(key_slot(t + 2));
+                            } else {
+                                commit(smem_address(&ctl.output[t & 1]));
+                            }
+                        }
+                    }
+                    used += 2 * n;
+                    cur += n;
+                }
+            }
+            __syncwarp();
+            named_sync(2, kSoftThreads + 32);  // every read of tensor memory is over
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+        }
+        return;
+    }
+
+    // Scores to weights.
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    const int stream = warp >> 2, row = tid & 127;  // row of the stream's 128
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t s_at = tmem + lanes + stream * 128, o_at = tmem + lanes + 256 + stream * 128;
+    const uint32_t scores_bar = smem_address(&ctl.scores[stream]), weights_bar = smem_address(&ctl.weights[stream]);
+    // Not 0, which would make a masked score's -inf a NaN.
+    const float scale = fmaxf(fabsf(a.scale) * kLog2e, 1.2e-38f);
+    const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;  // a negative scale turns the queries' signs
+    uint32_t score_phase = 0, output_phase = 0;
+    for (int64_t cur = work.lo; cur < work.hi;) {
+        const Piece p = piece_at<S::kRows>(c, a, work, cur, group, base, tile_units);
+        const int n_tiles = p.t1 - p.t0;
+        cur += n_tiles;
+        const int b = p.group / c.groups, beam0 = (p.group - b * c.groups) * kGroupBeams;
+        const int row0 = p.block * S::kRows;
+        const int rows = p.rows - row0 < S::kRows ? p.rows - row0 : S::kRows;
+        // Both streams are done with the last segment's products, and so with its queries.
+        named_sync(1, kSoftThreads);
+        for (int i = tid; i < S::kRows * (DP / 8); i += kSoftThreads) {
+            const int r = i / (DP / 8), chunk = i - r * (DP / 8);
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (r < rows && chunk * 8 < c.D) {
+                const RowId id = row_id(a, row0 + r);
+                const T* q = static_cast<const T*>(a.q) + b * a.qs[0] + (beam0 + id.beam) * a.qs[1] + id.token * a.qs[2] +
+                             (p.head * a.G + id.head) * a.qs[3];
+                v = __ldg(reinterpret_cast<const uint4*>(q) + chunk);
+                v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
+            }
+            const int in = r & 127;
+            *reinterpret_cast<uint4*>(query + (r >> 7) * (128 * DP * 2) + (chunk >> 3) * (128 * 128) + in * 128 +
+                                      (((chunk & 7) ^ (in & 7)) << 4)) = v;
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) barrier_arrive(smem_address(&ctl.queries));
+
+        const int my_row = NQ == 2 ? stream * 128 + row : row;
+        const bool mine = my_row < rows;
+        RowId id{0, 0, 0};
+        if (mine) id = row_id(a, row0 + my_row);
+        const int64_t bk = static_cast<int64_t>(b) * a.beams + beam0 + id.beam;
+        const int count = mine ? new_count(a, bk) : 0;
+        const uint32_t bit = mine && id.token < count ? 1u << id.beam : 0u;
+        const uint32_t need = __reduce_or_sync(0xffffffffu, bit);
+        const uint8_t* fresh = a.mask ? a.mask + (bk * a.N + id.token) * a.N : nullptr;
+        const CacheUnit* units = c.units + static_cast<int64_t>(p.group) * c.unit_cap;
+
+        float top = -INFINITY, sum = 0.0f;  // the reference (a score) and the weights' sum
+        const bool active = NQ == 1 || rows > stream * 128;
+        const int first = NQ == 2 ? 0 : stream, step = NQ == 2 ? 1 : 2;
+        bool began = false;
+        if (active) {
+            for (int t = first; t < n_tiles; t += step) {
+                CacheUnit u{-1, 0, 0, -1};
+                const int unit = (p.t0 + t) * tile_units + lane;
+                if (lane < tile_units && unit < p.units) {
+                    const int4 v = __ldg(reinterpret_cast<const int4*>(units + unit));
+                    u = CacheUnit{v.x, v.y, static_cast<uint32_t>(v.z), v.w};
+                }
+                const bool none = __all_sync(0xffffffffu, (u.mask & need) == 0);
+                const bool plain = __all_sync(0xffffffffu, lane >= tile_units || (u.limit < 0 && (u.mask & need) == need));
+                barrier_wait(scores_bar, score_phase, c.status);
+                score_phase ^= 1;
+                fence_after();
+                if (none) {
+                    // No row of the warp sees any of it.
+                    if (need != 0) {
+                        uint32_t zero[32] = {};
+                        tmem_store(s_at, zero);
+                        tmem_store(s_at + 32, zero);
+                        tmem_stored();
+                    }
+                } else {
+                    uint32_t s[128];
+                    tmem_load(s, s_at);
+                    if (!plain) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {  // 16 positions lie in one unit
+                            const int from = (i * 16) >> c.page_log2;
+                            const uint32_t holders = __shfl_sync(0xffffffffu, u.mask, from);
+                            const int limit = __shfl_sync(0xffffffffu, u.limit, from);
+                            const int start = __shfl_sync(0xffffffffu, u.start, from) + ((i * 16) & (c.page - 1));
+                            const bool holds = (holders & bit) != 0;
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) {
+                                bool sees = holds;
+                                const int j = start + e - limit;
+                                if (holds && limit >= 0 && j >= 0) sees = j < count && (fresh ? fresh[j] != 0 : j <= id.token);
+                                if (!sees) s[i * 16 + e] = 0xff800000u;
+                            }
+                        }
+                    }
+                    float now = -INFINITY;
+#pragma unroll
+                    for (int e = 0; e < 128; ++e) now = fmaxf(now, __uint_as_float(s[e]));
+                    float keep = 1.0f;
+                    if ((now - top) * scale > kRaise || (top == -INFINITY && now > top)) {
+                        keep = exp2_fast((top - now) * scale);
+                        top = now;
+                    }
+                    // (inf - inf is not a growth, and a reference of -inf, nothing seen yet, keeps 1.)
+                    if (began && __any_sync(0xffffffffu, keep != 1.0f)) {
+#pragma unroll
+                        for (int i = 0; i < DP / 32; ++i) {
+                            uint32_t o[32];
+                            tmem_load(o, o_at + 32 * i);
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+                            tmem_store(o_at + 32 * i, o);
+                        }
+                    }
+                    const float ref = top == -INFINITY ? 0.0f : top * scale;
+                    float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t w[32];
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) {
+                            const float x = exp2_fast(fmaf(__uint_as_float(s[64 * h + 2 * e]), scale, -ref));
+                            const float y = exp2_fast(fmaf(__uint_as_float(s[64 * h + 2 * e + 1]), scale, -ref));
+                            part[(e & 1) * 2] += x;
+                            part[(e & 1) * 2 + 1] += y;
+                            w[e] = Pack<T>::pair(x, y);
+                        }
+                        tmem_store(s_at + 32 * h, w);
+                    }
+                    sum = sum * keep + ((part[0] + part[1]) + (part[2] + part[3]));
+                    tmem_stored();
+                }
+                began = true;
+                fence_before();
+                __syncwarp();
+                if (lane == 0) barrier_arrive(weights_bar);
+            }
+            if (began) {
+                barrier_wait(smem_address(&ctl.output[stream]), output_phase, c.status);
+                output_phase ^= 1;
+                fence_after();
+            }
+        }
+
+        // The streams' rows, joined where they are the same, to the output or to this CTA's part.
+        const bool whole = p.t0 == 0 && p.t1 == p.tiles;
+        float* parts = static_cast<float*>(a.workspace) + 2048;
+        int32_t* counters = static_cast<int32_t*>(a.workspace);
+        float* part = parts + static_cast<int64_t>(2 * blockIdx.x + (p.t0 == 0)) * S::kOut;
+        float m = top == -INFINITY ? top : top * scale, l = sum, factor = 1.0f;  // base-2 maximum, sum
+        if constexpr (NQ == 1) {
+            if (stream == 1) ctl.top[row] = m, ctl.sum[row] = l;
+            named_sync(1, kSoftThreads);
+            const float m1 = ctl.top[row], l1 = ctl.sum[row];
+            named_sync(1, kSoftThreads);
+            if (stream == 0) ctl.top[row] = m, ctl.sum[row] = l;
+            named_sync(1, kSoftThreads);
+            const float m0 = ctl.top[row], l0 = ctl.sum[row];
+            const float both = fmaxf(m0, m1), ref = both == -INFINITY ? 0.0f : both;
+            factor = exp2_fast(m - ref);
+            l = l0 * exp2_fast(m0 - ref) + l1 * exp2_fast(m1 - ref);
+            m = both;
+        }
+        const bool live = mine && id.token < count;
+        const float inverse = live ? (l > 0.0f ? 1.0f / l : l) : 0.0f;
+        T* out = static_cast<T*>(a.out) + ((bk * a.N + id.token) * a.Hq + p.head * a.G + id.head) * c.D;
+        const int warp_row = my_row & ~31;
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i) {
+            uint32_t o[32];
+            if (began && warp_row < rows) {
+                tmem_load(o, o_at + 32 * i);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] = 0;
+            }
+            if constexpr (NQ == 1) {
+                // Stream 1 hands its columns over where the queries were (their products are done).
+                float4* at = reinterpret_cast<float4*>(query) + (i & 1) * 1024 + row * 8;
+                if (stream == 1 && warp_row < rows) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        at[e ^ (row & 7)] = make_float4(__uint_as_float(o[4 * e]) * factor, __uint_as_float(o[4 * e + 1]) * factor,
+                                                        __uint_as_float(o[4 * e + 2]) * factor, __uint_as_float(o[4 * e + 3]) * factor);
+                }
+                named_sync(1, kSoftThreads);
+                if (stream == 0 && warp_row < rows) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float4 x = at[e ^ (row & 7)];
+                        o[4 * e] = __float_as_uint(fmaf(__uint_as_float(o[4 * e]), factor, x.x));
+                        o[4 * e + 1] = __float_as_uint(fmaf(__uint_as_float(o[4 * e + 1]), factor, x.y));
+                        o[4 * e + 2] = __float_as_uint(fmaf(__uint_as_float(o[4 * e + 2]), factor, x.z));
+                        o[4 * e + 3] = __float_as_uint(fmaf(__uint_as_float(o[4 * e + 3]), factor, x.w));
+                    }
+                }
+            }
+            if ((NQ == 1 && stream == 1) || !mine) continue;
+            if (whole) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (i * 32 + e * 8 >= c.D) break;
+                    uint4 v = make_uint4(0, 0, 0, 0);
+                    if (live) {
+                        auto y = [&](int x) { return __uint_as_float(o[8 * e + x]) * inverse; };
+                        v = make_uint4(Pack<T>::pair(y(0), y(1)), Pack<T>::pair(y(2), y(3)), Pack<T>::pair(y(4), y(5)),
+                                       Pack<T>::pair(y(6), y(7)));
+                    }
+                    reinterpret_cast<uint4*>(out)[i * 4 + e] = v;
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    *reinterpret_cast<uint4*>(part + my_row * DP + i * 32 + e * 4) =
+                        make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+            }
+        }
+        if (mine && !(NQ == 1 && stream == 1)) {
+            if (whole) {
+                if (a.lse != nullptr)
+                    a.lse[(bk * a.N + id.token) * a.Hq + p.head * a.G + id.head] =
+                        live && l != 0.0f ? (m + log2f(l)) * kLn2 : -INFINITY;
+            } else {
+                part[S::kRows * DP + my_row] = m;
+                part[S::kRows * DP + S::kRows + my_row] = l;
+            }
+        }
+        if (whole) continue;
+        __threadfence();
+        named_sync(1, kSoftThreads);
+        const int n_parts = p.c1 - p.c0 + 1;
+        if (tid == 0) {
+            const int before = atomicAdd(counters + p.c0, 1);
+            ctl.last = before == n_parts - 1;
+            if (ctl.last) counters[p.c0] = 0;
+        }
+        named_sync(1, kSoftThreads);
+        if (!ctl.last) continue;
+        __threadfence();
+        // The last of the segment's CTAs adds the parts in their order: the result does not depend on
+        // which one that is.
+        auto part_of = [&](int i) { return parts + static_cast<int64_t>(2 * (p.c0 + i) + (i == 0)) * S::kOut; };
+        const int vecs = c.D / 4;
+        for (int i = tid; i < rows * vecs; i += kSoftThreads) {
+            const int r = i / vecs, vec = i - r * vecs;
+            float pm = -INFINITY;
+            for (int j = 0; j < n_parts; ++j) pm = fmaxf(pm, __ldcg(part_of(j) + S::kRows * DP + r));
+            const float ref = pm == -INFINITY ? 0.0f : pm;
+            float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            float pl = 0.0f;
+#pragma unroll 4
+            for (int j = 0; j < n_parts; ++j) {
+                const float* x = part_of(j);
+                const float w = exp2_fast(__ldcg(x + S::kRows * DP + r) - ref);
+                const float4 v = __ldcg(reinterpret_cast<const float4*>(x + r * DP + vec * 4));
+                pl = fmaf(__ldcg(x + S::kRows * DP + S::kRows + r), w, pl);
+                o.x = fmaf(v.x, w, o.x), o.y = fmaf(v.y, w, o.y);
+                o.z = fmaf(v.z, w, o.z), o.w = fmaf(v.w, w, o.w);
+            }
+            const RowId rid = row_id(a, row0 + r);
+            const int64_t rbk = static_cast<int64_t>(b) * a.beams + beam0 + rid.beam;
+            const int64_t at = (rbk * a.N + rid.token) * a.Hq + p.head * a.G + rid.head;
+            const bool shown = rid.token < new_count(a, rbk);
+            const float inv = pl > 0.0f ? 1.0f / pl : pl;
+            uint2 packed = make_uint2(0, 0);
+            if (shown) packed = make_uint2(Pack<T>::pair(o.x * inv, o.y * inv), Pack<T>::pair(o.z * inv, o.w * inv));
+            reinterpret_cast<uint2*>(static_cast<T*>(a.out) + at * c.D)[vec] = packed;
+            if (vec == 0 && a.lse != nullptr) a.lse[at] = shown && pl != 0.0f ? (pm + log2f(pl)) * kLn2 : -INFINITY;
+        }
+    }
+    fence_before();
+    named_sync(2, kSoftThreads + 32);
+}
+
+template <class T, int DP, int NQ>
+cudaError_t launch_shape(const CacheView& c, const CUtensorMap& map, const AttendParams& a, int sm_count,
+                         cudaStream_t stream) {
+    using S = Shape<DP, NQ>;
+    auto* kernel = attend_tc_kernel<T, DP, NQ>;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes);
+    if (e != cudaSuccess) return e;
+    return launch_after(kernel, sm_count, kThreads, S::kBytes, stream, map, c, a);
+}
+
+template <class T>
+cudaError_t launch_typed(const CacheView& c, const CUtensorMap& map, const AttendParams& a, int sm_count,
+                         cudaStream_t stream) {
+    const int beams = a.beams < kGroupBeams ? a.beams : kGroupBeams;
+    const bool one = static_cast<int64_t>(beams) * a.N * a.G <= 128;
+    if (c.D <= 64)
+        return one ? launch_shape<T, 64, 1>(c, map, a, sm_count, stream) : launch_shape<T, 64, 2>(c, map, a, sm_count, stream);
+    return one ? launch_shape<T, 128, 1>(c, map, a, sm_count, stream) : launch_shape<T, 128, 2>(c, map, a, sm_count, stream);
+}
+
+}  // namespace
+
+int64_t attend_tc_workspace(const CacheView&, const AttendParams&, int sm_count) {
+    // A counter for each CTA (8192 bytes), then two partial results for each.
+    return 8192 + static_cast<int64_t>(2) * sm_count * Shape<128, 2>::kOut * 4;
+}
+
+cudaError_t launch_attend_tc(const CacheView& c, int dtype, const AttendParams& a, int sm_count, cudaStream_t stream) {
+    CUtensorMap map;
+    if (!page_map(c, dtype, &map)) return cudaErrorInvalidValue;
+    if (dtype == DBS_CUDA_DTYPE_F16) return launch_typed<__half>(c, map, a, sm_count, stream);
+    return launch_typed<__nv_bfloat16>(c, map, a, sm_count, stream);
+}
+
+}  // namespace dbsb
