@@ -66,7 +66,7 @@ __device__ __forceinline__ void mma<__nv_bfloat16>(float (&d)[4], const uint32_t
 struct Control {
     uint64_t full[kMaxStages], empty[kMaxStages];
     CacheUnit unit[kMaxStages][4];
-    int sums[33];
+    int sums[34];
     WorkSplit split;
     float top[kComputeWarps][32], sum[kComputeWarps][32];  // each compute warp's row statistics
     float row_top[64], row_sum[64];
@@ -170,17 +170,10 @@ attend_mma_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant
         const int row0 = p.block * S::kRows;
         // The queries: [row][DP], 128-byte blocks swizzled by row.
         named_sync(1, kComputeThreads);
-        for (int i = tid; i < S::kRows * (DP / 8); i += kComputeThreads) {
-            const int r = i / (DP / 8), chunk = i - r * (DP / 8);
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (row0 + r < p.rows && chunk * 8 < c.D) {
-                const RowId id = row_id(a, row0 + r);
-                const T* q = static_cast<const T*>(a.q) + b * a.qs[0] + (beam0 + id.beam) * a.qs[1] + id.token * a.qs[2] +
-                             (p.head * a.G + id.head) * a.qs[3];
-                v = __ldg(reinterpret_cast<const uint4*>(q) + chunk);
-            }
+        const int rows = p.rows - row0 < S::kRows ? p.rows - row0 : S::kRows;
+        load_queries<T, S::kRows, DP, kComputeThreads>(c, a, p, b, beam0, row0, rows, tid, [&](int r, int chunk, uint4 v) {
             *reinterpret_cast<uint4*>(query + (chunk >> 3) * (S::kRows * 128) + swizzled(r, chunk & 7)) = v;
-        }
+        });
         named_sync(1, kComputeThreads);
         // Which beams the warp's rows belong to; rows past the count or the end see nothing.
         const int warp_row0 = WR == 2 ? half * kHalfRows : 0;
@@ -390,7 +383,6 @@ attend_mma_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant
         named_sync(1, kComputeThreads);
         // Four values at a time: to the output, or to this CTA's part of a divided segment.
         const bool whole = p.t0 == 0 && p.t1 == p.tiles;
-        const int rows = p.rows - row0 < S::kRows ? p.rows - row0 : S::kRows;
         const int vecs = c.D / 4;
         auto put = [&](int r, int vec, float4 o, float m, float l) {
             const RowId id = row_id(a, row0 + r);
@@ -430,36 +422,15 @@ attend_mma_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant
         if (whole) continue;
         __threadfence();
         named_sync(1, kComputeThreads);
-        const int n_parts = p.c1 - p.c0 + 1;
         if (tid == 0) {
             const int before = atomicAdd(counters + p.c0, 1);
-            ctl.last = before == n_parts - 1;
+            ctl.last = before == p.c1 - p.c0;
             if (ctl.last) counters[p.c0] = 0;
         }
         named_sync(1, kComputeThreads);
         if (!ctl.last) continue;
         __threadfence();
-        // The last of the segment's CTAs adds the parts in their order: the result does not depend on
-        // which one that is.
-        auto part_of = [&](int i) { return parts + static_cast<int64_t>(2 * (p.c0 + i) + (i == 0)) * S::kOut; };
-        for (int i = tid; i < rows * vecs; i += kComputeThreads) {
-            const int r = i / vecs, vec = i - r * vecs;
-            float m = -INFINITY;
-            for (int j = 0; j < n_parts; ++j) m = fmaxf(m, __ldcg(part_of(j) + S::kRows * DP + r));
-            const float ref = m == -INFINITY ? 0.0f : m;
-            float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            float l = 0.0f;
-#pragma unroll 4
-            for (int j = 0; j < n_parts; ++j) {
-                const float* x = part_of(j);
-                const float factor = exp2_fast(__ldcg(x + S::kRows * DP + r) - ref);
-                const float4 v = __ldcg(reinterpret_cast<const float4*>(x + r * DP + vec * 4));
-                l = fmaf(__ldcg(x + S::kRows * DP + S::kRows + r), factor, l);
-                o.x = fmaf(v.x, factor, o.x), o.y = fmaf(v.y, factor, o.y);
-                o.z = fmaf(v.z, factor, o.z), o.w = fmaf(v.w, factor, o.w);
-            }
-            put(r, vec, o, m, l);
-        }
+        join_parts<T, S::kRows, DP, kComputeThreads>(c, a, p, b, beam0, row0, rows, parts, join, tid);
     }
 }
 

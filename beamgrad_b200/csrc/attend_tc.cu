@@ -45,7 +45,7 @@ struct Control {
     uint64_t full[kMaxSlots], empty[kMaxSlots];
     uint64_t scores[2], weights[2], output[2], queries;
     float top[128], sum[128];
-    int sums[33];
+    int sums[34];
     WorkSplit split;
     uint32_t tmem;
     int last;
@@ -169,9 +169,9 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
     int group = work.group;
     int64_t base = work.base;
 
-    // Registers: launched with 168 a thread; 2 x 128 x 224 + 128 x 56 = 384 x 168.
+    // Registers: launched with 168 a thread; 2 x 128 x 216 + 128 x 72 = 384 x 168.
     if (warp >= kCopyWarp) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         if (warp > kIssueWarp) return;
         int used = 0;  // slots so far
         if (warp == kCopyWarp) {
@@ -219,7 +219,7 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
         } else {
             if (lane == 0) {
                 constexpr uint32_t kScores = product_kind<T>(kTileKeys, false), kValues = product_kind<T>(DP, true);
-                uint32_t query_phase = 0, weight_phase[2] = {0, 0};
+                uint32_t query_phase = 0, weight_phase = 0;  // weight_phase: a bit a stream
                 auto slot_of = [&](int i) { return i % S::kSlots; };
                 auto wait_slot = [&](int i) {
                     barrier_wait(smem_address(&ctl.full[slot_of(i)]), (i / S::kSlots) & 1, c.status);
@@ -227,23 +227,24 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
                 };
                 auto free_slot = [&](int i) { commit(smem_address(&ctl.empty[slot_of(i)])); };
                 auto scores = [&](int stream, int i) {
-                    const uint32_t q = smem_address(query) + (NQ == 2 ? stream * 128 * DP * 2 : 0);
-                    const uint32_t k = slots + slot_of(i) * S::kSlot;
+                    const uint64_t q = operand(smem_address(query) + (NQ == 2 ? stream * 128 * DP * 2 : 0), 16);
+                    const uint64_t k = operand(slots + slot_of(i) * S::kSlot, 16);
 #pragma unroll
-                    for (int s = 0; s < DP / 16; ++s)
-                        product_ss(tmem + stream * 128, operand(q + (s >> 2) * (128 * 128) + (s & 3) * 32, 16),
-                                   operand(k + (s >> 2) * (kTileKeys * 128) + (s & 3) * 32, 16), kScores, s > 0);
+                    for (int s = 0; s < DP / 16; ++s) {
+                        const uint64_t at = ((s >> 2) * (128 * 128) + (s & 3) * 32) >> 4;
+                        product_ss(tmem + stream * 128, q + at, k + at, kScores, s > 0);
+                    }
                     commit(smem_address(&ctl.scores[stream]));
                 };
                 auto values = [&](int stream, int i, bool add) {
-                    barrier_wait(smem_address(&ctl.weights[stream]), weight_phase[stream], c.status);
-                    weight_phase[stream] ^= 1;
+                    barrier_wait(smem_address(&ctl.weights[stream]), weight_phase >> stream & 1, c.status);
+                    weight_phase ^= 1u << stream;
                     fence_after();
-                    const uint32_t v = slots + slot_of(i) * S::kSlot;
+                    const uint64_t v = operand(slots + slot_of(i) * S::kSlot, kTileKeys * 128);
 #pragma unroll
                     for (int s = 0; s < kTileKeys / 16; ++s)
-                        product_ts(tmem + 256 + stream * 128, tmem + stream * 128 + s * 8,
-                                   operand(v + s * (16 * 128), kTileKeys * 128), kValues, add || s > 0);
+                        product_ts(tmem + 256 + stream * 128, tmem + stream * 128 + s * 8, v + s * ((16 * 128) >> 4), kValues,
+                                   add || s > 0);
                 };
                 for (int64_t cur = work.lo; cur < work.hi;) {
                     const Piece p = piece_at<S::kRows>(c, a, work, cur, group, base, tile_units);
@@ -254,12 +255,14 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
                     if (NQ == 2) {  // slots: K0 V0 K1 V1 ...
                         const int streams = p.rows - p.block * S::kRows > 128 ? 2 : 1;
                         wait_slot(used);
+#pragma unroll 1
                         for (int i = 0; i < streams; ++i) scores(i, used);
                         free_slot(used);
                         for (int t = 0; t < n; ++t) {
                             const int v = used + 2 * t + 1;
                             wait_slot(v);
                             if (t + 1 < n) wait_slot(v + 1);
+#pragma unroll 1
                             for (int i = 0; i < streams; ++i) {
                                 values(i, v, t > 0);
                                 if (t + 1 < n) scores(i, v + 1);
@@ -270,6 +273,7 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
                         }
                     } else {  // slots: K0 K1 V0 K2 V1 ...
                         auto key_slot = [&](int t) { return used + (t == 0 ? 0 : 2 * t - 1); };
+#pragma unroll 1
                         for (int t = 0; t < 2 && t < n; ++t) {
                             wait_slot(key_slot(t));
                             scores(t, key_slot(t));
@@ -301,7 +305,7 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
     }
 
     // Scores to weights.
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     const int stream = warp >> 2, row = tid & 127;  // row of the stream's 128
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t s_at = tmem + lanes + stream * 128, o_at = tmem + lanes + 256 + stream * 128;
@@ -319,20 +323,12 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
         const int rows = p.rows - row0 < S::kRows ? p.rows - row0 : S::kRows;
         // Both streams are done with the last segment's products, and so with its queries.
         named_sync(1, kSoftThreads);
-        for (int i = tid; i < S::kRows * (DP / 8); i += kSoftThreads) {
-            const int r = i / (DP / 8), chunk = i - r * (DP / 8);
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (r < rows && chunk * 8 < c.D) {
-                const RowId id = row_id(a, row0 + r);
-                const T* q = static_cast<const T*>(a.q) + b * a.qs[0] + (beam0 + id.beam) * a.qs[1] + id.token * a.qs[2] +
-                             (p.head * a.G + id.head) * a.qs[3];
-                v = __ldg(reinterpret_cast<const uint4*>(q) + chunk);
-                v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
-            }
+        load_queries<T, S::kRows, DP, kSoftThreads>(c, a, p, b, beam0, row0, rows, tid, [&](int r, int chunk, uint4 v) {
+            v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
             const int in = r & 127;
             *reinterpret_cast<uint4*>(query + (r >> 7) * (128 * DP * 2) + (chunk >> 3) * (128 * 128) + in * 128 +
                                       (((chunk & 7) ^ (in & 7)) << 4)) = v;
-        }
+        });
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) barrier_arrive(smem_address(&ctl.queries));
@@ -353,13 +349,19 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
         const int first = NQ == 2 ? 0 : stream, step = NQ == 2 ? 1 : 2;
         bool began = false;
         if (active) {
-            for (int t = first; t < n_tiles; t += step) {
+            auto unit_of = [&](int t) {  // a lane each
                 CacheUnit u{-1, 0, 0, -1};
-                const int unit = (p.t0 + t) * tile_units + lane;
-                if (lane < tile_units && unit < p.units) {
-                    const int4 v = __ldg(reinterpret_cast<const int4*>(units + unit));
+                const int i = (p.t0 + t) * tile_units + lane;
+                if (t < n_tiles && lane < tile_units && i < p.units) {
+                    const int4 v = __ldg(reinterpret_cast<const int4*>(units + i));
                     u = CacheUnit{v.x, v.y, static_cast<uint32_t>(v.z), v.w};
                 }
+                return u;
+            };
+            CacheUnit next = unit_of(first);
+            for (int t = first; t < n_tiles; t += step) {
+                const CacheUnit u = next;
+                next = unit_of(t + step);
                 const bool none = __all_sync(0xffffffffu, (u.mask & need) == 0);
                 const bool plain = __all_sync(0xffffffffu, lane >= tile_units || (u.limit < 0 && (u.mask & need) == need));
                 barrier_wait(scores_bar, score_phase, c.status);
@@ -384,18 +386,31 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
                             const int limit = __shfl_sync(0xffffffffu, u.limit, from);
                             const int start = __shfl_sync(0xffffffffu, u.start, from) + ((i * 16) & (c.page - 1));
                             const bool holds = (holders & bit) != 0;
+                            uint32_t sees = holds ? 0xffffu : 0u;
+                            if (limit >= 0) {
+                                // The holder's committed tokens end in this page: of the new ones behind them a
+                                // chain shows the first, a mask those that it names.
+                                const int old = limit - start;
+                                const int upto = old + (fresh ? 0 : (id.token < count ? id.token + 1 : count));
+                                if (upto < 16) sees &= upto > 0 ? (1u << upto) - 1 : 0u;
+                                if (fresh != nullptr && holds && old < 16 && old + count > 0) {
 #pragma unroll
-                            for (int e = 0; e < 16; ++e) {
-                                bool sees = holds;
-                                const int j = start + e - limit;
-                                if (holds && limit >= 0 && j >= 0) sees = j < count && (fresh ? fresh[j] != 0 : j <= id.token);
-                                if (!sees) s[i * 16 + e] = 0xff800000u;
+                                    for (int e = 0; e < 16; ++e)
+                                        if (e >= old && e - old < count) sees |= (fresh[e - old] != 0 ? 1u : 0u) << e;
+                                }
                             }
+#pragma unroll
+                            for (int e = 0; e < 16; ++e)
+                                if ((sees >> e & 1) == 0) s[i * 16 + e] = 0xff800000u;
                         }
                     }
-                    float now = -INFINITY;
+                    float most[8];
 #pragma unroll
-                    for (int e = 0; e < 128; ++e) now = fmaxf(now, __uint_as_float(s[e]));
+                    for (int e = 0; e < 8; ++e) most[e] = __uint_as_float(s[e]);
+#pragma unroll
+                    for (int e = 8; e < 128; ++e) most[e & 7] = fmaxf(most[e & 7], __uint_as_float(s[e]));
+                    const float now = fmaxf(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])),
+                                            fmaxf(fmaxf(most[4], most[5]), fmaxf(most[6], most[7])));
                     float keep = 1.0f;
                     if ((now - top) * scale > kRaise || (top == -INFINITY && now > top)) {
                         keep = exp2_fast((top - now) * scale);
@@ -528,45 +543,15 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
         if (whole) continue;
         __threadfence();
         named_sync(1, kSoftThreads);
-        const int n_parts = p.c1 - p.c0 + 1;
         if (tid == 0) {
             const int before = atomicAdd(counters + p.c0, 1);
-            ctl.last = before == n_parts - 1;
+            ctl.last = before == p.c1 - p.c0;
             if (ctl.last) counters[p.c0] = 0;
         }
         named_sync(1, kSoftThreads);
         if (!ctl.last) continue;
         __threadfence();
-        // The last of the segment's CTAs adds the parts in their order: the result does not depend on
-        // which one that is.
-        auto part_of = [&](int i) { return parts + static_cast<int64_t>(2 * (p.c0 + i) + (i == 0)) * S::kOut; };
-        const int vecs = c.D / 4;
-        for (int i = tid; i < rows * vecs; i += kSoftThreads) {
-            const int r = i / vecs, vec = i - r * vecs;
-            float pm = -INFINITY;
-            for (int j = 0; j < n_parts; ++j) pm = fmaxf(pm, __ldcg(part_of(j) + S::kRows * DP + r));
-            const float ref = pm == -INFINITY ? 0.0f : pm;
-            float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            float pl = 0.0f;
-#pragma unroll 4
-            for (int j = 0; j < n_parts; ++j) {
-                const float* x = part_of(j);
-                const float w = exp2_fast(__ldcg(x + S::kRows * DP + r) - ref);
-                const float4 v = __ldcg(reinterpret_cast<const float4*>(x + r * DP + vec * 4));
-                pl = fmaf(__ldcg(x + S::kRows * DP + S::kRows + r), w, pl);
-                o.x = fmaf(v.x, w, o.x), o.y = fmaf(v.y, w, o.y);
-                o.z = fmaf(v.z, w, o.z), o.w = fmaf(v.w, w, o.w);
-            }
-            const RowId rid = row_id(a, row0 + r);
-            const int64_t rbk = static_cast<int64_t>(b) * a.beams + beam0 + rid.beam;
-            const int64_t at = (rbk * a.N + rid.token) * a.Hq + p.head * a.G + rid.head;
-            const bool shown = rid.token < new_count(a, rbk);
-            const float inv = pl > 0.0f ? 1.0f / pl : pl;
-            uint2 packed = make_uint2(0, 0);
-            if (shown) packed = make_uint2(Pack<T>::pair(o.x * inv, o.y * inv), Pack<T>::pair(o.z * inv, o.w * inv));
-            reinterpret_cast<uint2*>(static_cast<T*>(a.out) + at * c.D)[vec] = packed;
-            if (vec == 0 && a.lse != nullptr) a.lse[at] = shown && pl != 0.0f ? (pm + log2f(pl)) * kLn2 : -INFINITY;
-        }
+        join_parts<T, S::kRows, DP, kSoftThreads>(c, a, p, b, beam0, row0, rows, parts, reinterpret_cast<float*>(query), tid);
     }
     fence_before();
     named_sync(2, kSoftThreads + 32);
