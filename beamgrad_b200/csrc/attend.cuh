@@ -328,15 +328,16 @@ __device__ __forceinline__ RowId row_id(const AttendParams& a, int r) {
     return id;
 }
 
-// Rows of queries to a thread: kEach loads in flight. put(row, chunk, value) gets 16 bytes of every
-// row of the block, zeros past its end and past the head.
+// The queries of a row block by kThreads threads, eight loads in flight each. at: the rows' places
+// in q, in shared memory; put(row, chunk, value) gets 16 bytes of every row of the block, zeros past
+// its end and past the head.
 template <class T, int kRows, int DP, int kThreads, class Put>
-__device__ __forceinline__ void load_queries(const CacheView& c, const AttendParams& a, const Piece& p, int b, int beam0,
-                                             int row0, int rows, int tid, Put&& put) {
+__device__ __forceinline__ void load_queries(const CacheView& c, const AttendParams& a, const int64_t* at, int rows, int tid,
+                                             Put&& put) {
     constexpr int kChunks = DP / 8, kStride = kThreads / kChunks, kTotal = (kRows + kStride - 1) / kStride;
     constexpr int kEach = kTotal < 8 ? kTotal : 8;
     const int chunk = tid % kChunks, first = tid / kChunks;
-    const T* q = static_cast<const T*>(a.q) + b * a.qs[0] + beam0 * a.qs[1] + (p.head * a.G) * a.qs[3] + chunk * 8;
+    const T* q = static_cast<const T*>(a.q) + chunk * 8;
 #pragma unroll 1
     for (int i = 0; i < kTotal; i += kEach) {
         uint4 v[kEach];
@@ -344,10 +345,7 @@ __device__ __forceinline__ void load_queries(const CacheView& c, const AttendPar
         for (int j = 0; j < kEach; ++j) {
             const int r = first + (i + j) * kStride;
             v[j] = make_uint4(0, 0, 0, 0);
-            if (r < rows && chunk * 8 < c.D) {
-                const RowId id = row_id(a, row0 + r);
-                v[j] = __ldg(reinterpret_cast<const uint4*>(q + id.beam * a.qs[1] + id.token * a.qs[2] + id.head * a.qs[3]));
-            }
+            if (r < rows && chunk * 8 < c.D) v[j] = __ldg(reinterpret_cast<const uint4*>(q + at[r]));
         }
 #pragma unroll
         for (int j = 0; j < kEach; ++j) {
@@ -359,32 +357,31 @@ __device__ __forceinline__ void load_queries(const CacheView& c, const AttendPar
 
 // The parts of a divided segment to the output, in their order, so that the result does not depend
 // on which CTA comes last. A part: kRows x DP sums, the rows' references (base 2), their weights'
-// sums. scratch: 2 * kRows floats of shared memory. All kThreads threads of named barrier 1.
+// sums. scratch: 16 * kRows bytes of shared memory. All kThreads threads of named barrier 1.
 template <class T, int kRows, int DP, int kThreads>
 __device__ __forceinline__ void join_parts(const CacheView& c, const AttendParams& a, const Piece& p, int b, int beam0,
-                                           int row0, int rows, const float* parts, float* scratch, int tid) {
-    constexpr int kOut = kRows * (DP + 2);
+                                           int row0, int rows, const float* parts, void* scratch, int tid) {
+    constexpr int kOut = kRows * (DP + 2), kVecs = DP / 4;
     const int n_parts = p.c1 - p.c0 + 1;
     // A CTA's second part is the one that begins a segment.
     auto part_of = [&](int i) { return parts + static_cast<int64_t>(2 * (p.c0 + i) + (i == 0)) * kOut; };
-    auto place_of = [&](int r, bool* shown) {
-        const RowId id = row_id(a, row0 + r);
-        const int64_t bk = static_cast<int64_t>(b) * a.beams + beam0 + id.beam;
-        if (shown != nullptr) *shown = id.token < new_count(a, bk);
-        return (bk * a.N + id.token) * a.Hq + p.head * a.G + id.head;
-    };
-    float* refs = scratch;
-    float* factors = scratch + kRows;  // 1 / sum; -1 for rows that are not shown
+    int64_t* places = static_cast<int64_t*>(scratch);
+    float* refs = reinterpret_cast<float*>(places + kRows);
+    float* factors = refs + kRows;  // 1 / sum; -1 for rows that are not shown
+#pragma unroll 1
     for (int r = tid; r < rows; r += kThreads) {
         float m = -INFINITY, l = 0.0f;
-#pragma unroll 8
+#pragma unroll 4
         for (int j = 0; j < n_parts; ++j) m = fmaxf(m, __ldcg(part_of(j) + kRows * DP + r));
         const float ref = m == -INFINITY ? 0.0f : m;
-#pragma unroll 8
+#pragma unroll 4
         for (int j = 0; j < n_parts; ++j)
             l = fmaf(__ldcg(part_of(j) + kRows * DP + kRows + r), exp2_fast(__ldcg(part_of(j) + kRows * DP + r) - ref), l);
-        bool shown;
-        const int64_t at = place_of(r, &shown);
+        const RowId id = row_id(a, row0 + r);
+        const int64_t bk = static_cast<int64_t>(b) * a.beams + beam0 + id.beam;
+        const bool shown = id.token < new_count(a, bk);
+        const int64_t at = (bk * a.N + id.token) * a.Hq + p.head * a.G + id.head;
+        places[r] = at;
         refs[r] = ref;
         factors[r] = shown ? (l > 0.0f ? 1.0f / l : l) : -1.0f;
         if (a.lse != nullptr) a.lse[at] = shown && l != 0.0f ? (m + log2f(l)) * kLn2 : -INFINITY;
@@ -392,41 +389,39 @@ __device__ __forceinline__ void join_parts(const CacheView& c, const AttendParam
     __syncwarp();
     asm volatile("barrier.sync 1, %0;" ::"r"(kThreads) : "memory");
     constexpr int kEach = 8;
-    const int vecs = c.D / 4, items = rows * vecs;
+    const int items = rows * kVecs;
+#pragma unroll 1
     for (int i0 = tid; i0 < items; i0 += kEach * kThreads) {
         float4 o[kEach];
-        int r[kEach], vec[kEach];
 #pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-            const int i = i0 + e * kThreads < items ? i0 + e * kThreads : i0;
-            r[e] = i / vecs;
-            vec[e] = i - r[e] * vecs;
-            o[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        }
-#pragma unroll 2
+        for (int e = 0; e < kEach; ++e) o[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 1
         for (int j = 0; j < n_parts; ++j) {
             const float* x = part_of(j);
             float4 v[kEach];
             float w[kEach];
 #pragma unroll
             for (int e = 0; e < kEach; ++e) {
-                v[e] = __ldcg(reinterpret_cast<const float4*>(x + r[e] * DP + vec[e] * 4));
-                w[e] = __ldcg(x + kRows * DP + r[e]);
+                const int i = i0 + e * kThreads < items ? i0 + e * kThreads : i0, r = i / kVecs;
+                v[e] = __ldcg(reinterpret_cast<const float4*>(x + i * 4));
+                w[e] = __ldcg(x + kRows * DP + r) - refs[r];
             }
 #pragma unroll
             for (int e = 0; e < kEach; ++e) {
-                const float f = exp2_fast(w[e] - refs[r[e]]);
+                const float f = exp2_fast(w[e]);
                 o[e].x = fmaf(v[e].x, f, o[e].x), o[e].y = fmaf(v[e].y, f, o[e].y);
                 o[e].z = fmaf(v[e].z, f, o[e].z), o[e].w = fmaf(v[e].w, f, o[e].w);
             }
         }
 #pragma unroll
         for (int e = 0; e < kEach; ++e) {
-            if (i0 + e * kThreads >= items) break;
-            const float f = factors[r[e]];
+            const int i = i0 + e * kThreads, r = i / kVecs, vec = i % kVecs;
+            if (i >= items) break;
+            if (vec * 4 >= c.D) continue;
+            const float f = factors[r];
             uint2 packed = make_uint2(Pack<T>::pair(o[e].x * f, o[e].y * f), Pack<T>::pair(o[e].z * f, o[e].w * f));
             if (f == -1.0f) packed = make_uint2(0, 0);
-            reinterpret_cast<uint2*>(static_cast<T*>(a.out) + place_of(r[e], nullptr) * c.D)[vec[e]] = packed;
+            reinterpret_cast<uint2*>(static_cast<T*>(a.out) + places[r] * c.D)[vec] = packed;
         }
     }
 }

@@ -71,6 +71,7 @@ struct Control {
     float top[kComputeWarps][32], sum[kComputeWarps][32];  // each compute warp's row statistics
     float row_top[64], row_sum[64];
     int last;
+    int64_t query_at[64];
 };
 
 // MT: 16-row tiles a warp; WR: 1, the two halves of the compute warps take alternate tiles; 2,
@@ -169,9 +170,14 @@ attend_mma_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant
         const int b = p.group / c.groups, beam0 = (p.group - b * c.groups) * kGroupBeams;
         const int row0 = p.block * S::kRows;
         // The queries: [row][DP], 128-byte blocks swizzled by row.
-        named_sync(1, kComputeThreads);
         const int rows = p.rows - row0 < S::kRows ? p.rows - row0 : S::kRows;
-        load_queries<T, S::kRows, DP, kComputeThreads>(c, a, p, b, beam0, row0, rows, tid, [&](int r, int chunk, uint4 v) {
+        named_sync(1, kComputeThreads);
+        if (tid < rows) {
+            const RowId id = row_id(a, row0 + tid);
+            ctl.query_at[tid] = b * a.qs[0] + (beam0 + id.beam) * a.qs[1] + id.token * a.qs[2] + (p.head * a.G + id.head) * a.qs[3];
+        }
+        named_sync(1, kComputeThreads);
+        load_queries<T, S::kRows, DP, kComputeThreads>(c, a, ctl.query_at, rows, tid, [&](int r, int chunk, uint4 v) {
             *reinterpret_cast<uint4*>(query + (chunk >> 3) * (S::kRows * 128) + swizzled(r, chunk & 7)) = v;
         });
         named_sync(1, kComputeThreads);

@@ -4,13 +4,19 @@
 // float16 and bfloat16 and heads of up to 128.
 //
 // 128 query rows by 128 positions at a time: S = Q K^T into tensor memory, the weights P back to
-// tensor memory in the place of S, O += P V in tensor memory. One warp copies keys and values by
-// TMA through a ring of slots (a slot holds 128 rows of keys or of values), one thread issues the
-// products, and two warpgroups work on the scores, a thread a row: no maximum or sum crosses a
-// thread. The two warpgroups and their S and O are two streams, so that the products of one run
-// while the other takes exponentials. NQ = 2: each stream has query rows of its own (256 a block)
-// and takes every tile; NQ = 1: both have the same 128 rows, take alternate tiles and are joined
-// at the end of a segment.
+// tensor memory, O += P V in tensor memory. One warp copies keys and values by TMA through a ring
+// of slots (a slot holds 128 rows of keys or of values), one thread issues the products, and two
+// warpgroups turn scores into weights, a thread a row: no maximum or sum crosses a thread. The
+// warpgroups and their P and O are two streams: the products of one run while the other takes
+// exponentials. S is one buffer for both. A warpgroup moves its scores to registers as soon as they
+// are there, and the next product may begin.
+//
+// NQ = 2 (more than 128 rows): each stream has query rows of its own, 256 a block, and takes every
+// tile, so that keys and values cross from L2 once for 256 rows. NQ = 1: both have the same rows and
+// take alternate tiles. With at most 64 (32) rows these lie in tensor memory 2 (4) times and each
+// copy weighs a half (a quarter) of the positions, with zeros for the others: the product costs the
+// same, and the chain from scores to weights is a half (a quarter) as long. Copies and streams are
+// joined at the end of a segment.
 //
 // A row's reference for the exponentials is raised only when its maximum has grown by more than
 // 2^8: until then the weights stay below 2^8 and the sums within 32 bits, and O in tensor memory
@@ -27,28 +33,36 @@ constexpr int kSoftThreads = 256;
 constexpr int kThreads = kSoftThreads + 128;  // and a warpgroup with the copying and the issuing warp
 constexpr int kCopyWarp = 8, kIssueWarp = 9;
 constexpr int kMaxSlots = 12;
+constexpr int kMinTiles = 1;     // tiles of a CTA at least
 constexpr float kRaise = 8.0f;  // log2 of the growth that a reference tolerates
-
-template <int DP, int NQ>
-struct Shape {
-    static constexpr int kRows = 128 * NQ;
-    static constexpr int kBlocks = DP / 64;
-    static constexpr int kSlot = kTileKeys * DP * 2;
-    // The queries; at the end of a segment NQ = 1 joins its streams there, 2 x 128 x 32 floats.
-    static constexpr int kQuery = kRows * DP * 2 > 32768 ? kRows * DP * 2 : 32768;
-    static constexpr int kSlots = (224 * 1024 - kQuery) / kSlot < kMaxSlots ? (224 * 1024 - kQuery) / kSlot : kMaxSlots;
-    static constexpr int kOut = kRows * (DP + 2);  // floats of a partial result
-    static constexpr int kBytes = 1024 + kSlots * kSlot + kQuery;
-};
 
 struct Control {
     uint64_t full[kMaxSlots], empty[kMaxSlots];
-    uint64_t scores[2], weights[2], output[2], queries;
-    float top[128], sum[128];
-    int sums[34];
+    uint64_t queries, scores[2], loaded[2], weights[2], done[2];
     WorkSplit split;
+    int sums[34];
     uint32_t tmem;
     int last;
+    union {
+        int64_t query_at[256];              // while queries are loaded: the rows' places
+        struct {
+            float top[256], sum[256];       // at the end of a segment: [copy][row]
+        };
+    };
+};
+
+template <int DP, int NQ, int COPIES>
+struct Shape {
+    static constexpr int kRows = NQ == 2 ? 256 : 128 / COPIES;
+    static constexpr int kCols = 128 / COPIES;  // positions of a tile that a thread weighs
+    static constexpr int kBlocks = DP / 64;
+    static constexpr int kSlot = kTileKeys * DP * 2;
+    // The queries; at the end of a segment NQ = 1 joins its copies there, 256 x 32 floats.
+    static constexpr int kQuery = NQ * 128 * DP * 2 > 32768 ? NQ * 128 * DP * 2 : 32768;
+    static constexpr int kFit = (227 * 1024 - static_cast<int>(sizeof(Control)) - kQuery) / kSlot;
+    static constexpr int kSlots = kFit < kMaxSlots ? kFit : kMaxSlots;
+    static constexpr int kOut = kRows * (DP + 2);  // floats of a partial result
+    static constexpr int kBytes = kSlots * kSlot + kQuery + sizeof(Control);
 };
 
 // ---- tcgen05 ----
@@ -81,6 +95,16 @@ __device__ __forceinline__ void tmem_load(uint32_t (&r)[32], uint32_t at) {
         : "r"(at)
         : "memory");
 }
+__device__ __forceinline__ void tmem_load(uint32_t (&r)[64], uint32_t at) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
+        "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
+        "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];\n tcgen05.wait::ld.sync.aligned;"
+        : REGS32(r, 0), REGS32(r, 32)
+        : "r"(at)
+        : "memory");
+}
 __device__ __forceinline__ void tmem_load(uint32_t (&r)[128], uint32_t at) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x128.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
@@ -107,6 +131,13 @@ __device__ __forceinline__ void tmem_store(uint32_t at, const uint32_t (&r)[32])
         "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
 }
+__device__ __forceinline__ void tmem_store(uint32_t at, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
 __device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // Shared-memory operand with 128-byte rows, swizzled: eight rows (1024 bytes) to the next eight
@@ -123,16 +154,15 @@ __device__ __forceinline__ constexpr uint32_t product_kind(int columns, bool by_
     return 1u << 4 | type << 7 | type << 10 | (by_row ? 1u << 16 : 0u) | static_cast<uint32_t>(columns / 8) << 17 | 8u << 24;
 }
 
-template <class T, int DP, int NQ>
+template <class T, int DP, int NQ, int COPIES>
 __global__ void __launch_bounds__(kThreads, 1)
 attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ CacheView c,
                  const __grid_constant__ AttendParams a) {
-    using S = Shape<DP, NQ>;
-    extern __shared__ uint8_t raw[];
-    __shared__ Control ctl;
-    uint8_t* smem = raw + (1024 - (smem_address(raw) & 1023)) % 1024;
-    const uint32_t slots = smem_address(smem);
+    using S = Shape<DP, NQ, COPIES>;
+    extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* query = smem + S::kSlots * S::kSlot;
+    Control& ctl = *reinterpret_cast<Control*>(query + S::kQuery);
+    const uint32_t slots = smem_address(smem);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int tile_units = kTileKeys >> c.page_log2;
 
@@ -143,14 +173,15 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
         }
         for (int i = 0; i < 2; ++i) {
             barrier_init(smem_address(&ctl.scores[i]), 1);
+            barrier_init(smem_address(&ctl.loaded[i]), 4);
             barrier_init(smem_address(&ctl.weights[i]), 4);
-            barrier_init(smem_address(&ctl.output[i]), 1);
+            barrier_init(smem_address(&ctl.done[i]), 1);
         }
         barrier_init(smem_address(&ctl.queries), kSoftThreads / 32);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     // The plan was complete before the new tokens' copy began; only the pages have to be waited for.
-    const WorkSplit work = split_work<S::kRows>(c, a, tile_units, 1, ctl.sums, &ctl.split);
+    const WorkSplit work = split_work<S::kRows>(c, a, tile_units, kMinTiles, ctl.sums, &ctl.split);
     grid_wait();
     grid_release();
     if (__ldcg(c.status + 1) != 0) {
@@ -165,7 +196,7 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
     }
     __syncthreads();
     fence_after();
-    const uint32_t tmem = ctl.tmem;  // S0, S1, O0, O1: 128 columns each
+    const uint32_t tmem = ctl.tmem;  // columns: S 0..127, P of the streams 128.. and 192.., O 256.. and 384..
     int group = work.group;
     int64_t base = work.base;
 
@@ -173,7 +204,7 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
     if (warp >= kCopyWarp) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         if (warp > kIssueWarp) return;
-        int used = 0;  // slots so far
+        int used = 0;  // slots so far: K0 V0 K1 V1 ...
         if (warp == kCopyWarp) {
             asm volatile("fence.proxy.async;" ::: "memory");
             for (int64_t cur = work.lo; cur < work.hi;) {
@@ -187,29 +218,25 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
                     const int i = (p.t0 + t) * tile_units + which;
                     return t < n_tiles && which < tile_units && i < p.units ? __ldg(&units[i].page) : 0;
                 };
-                auto copy = [&](int kind, int page) {
-                    const int slot = used % S::kSlots;
-                    const uint32_t full = smem_address(&ctl.full[slot]);
-                    if (used >= S::kSlots) barrier_wait(smem_address(&ctl.empty[slot]), (used / S::kSlots - 1) & 1, c.status);
-                    if (lane == 0) barrier_expect(full, S::kSlot);
-                    __syncwarp();
-                    if (which < tile_units) {
-                        const int64_t row = (((static_cast<int64_t>(a.layer) * 2 + kind) * c.P + page) * c.H + p.head) * c.page;
-                        tma_load(slots + slot * S::kSlot + block * (kTileKeys * 128) + which * c.page * 128, &map, block * 64,
-                                 static_cast<int>(row), full);
-                    }
-                    ++used;
-                };
-                // In the order in which the issuing thread takes them.
-                int page = page_of(0), next = page_of(1);
-                copy(0, page);
+                int page = page_of(0);
+#pragma unroll 1
                 for (int t = 0; t < n_tiles; ++t) {
-                    const int after = page_of(t + 2);
-                    if (NQ == 1 && t + 1 < n_tiles) copy(0, next);
-                    copy(1, page);
-                    if (NQ == 2 && t + 1 < n_tiles) copy(0, next);
+                    const int next = page_of(t + 1);
+#pragma unroll 1
+                    for (int kind = 0; kind < 2; ++kind, ++used) {
+                        const int slot = used % S::kSlots;
+                        const uint32_t full = smem_address(&ctl.full[slot]);
+                        if (used >= S::kSlots)
+                            barrier_wait(smem_address(&ctl.empty[slot]), (used / S::kSlots - 1) & 1, c.status);
+                        if (lane == 0) barrier_expect(full, S::kSlot);
+                        __syncwarp();
+                        if (which < tile_units) {
+                            const int64_t row = (((static_cast<int64_t>(a.layer) * 2 + kind) * c.P + page) * c.H + p.head) * c.page;
+                            tma_load(slots + slot * S::kSlot + block * (kTileKeys * 128) + which * c.page * 128, &map, block * 64,
+                                     static_cast<int>(row), full);
+                        }
+                    }
                     page = next;
-                    next = after;
                 }
                 cur += n_tiles;
             }
@@ -219,32 +246,10 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
         } else {
             if (lane == 0) {
                 constexpr uint32_t kScores = product_kind<T>(kTileKeys, false), kValues = product_kind<T>(DP, true);
-                uint32_t query_phase = 0, weight_phase = 0;  // weight_phase: a bit a stream
-                auto slot_of = [&](int i) { return i % S::kSlots; };
+                uint32_t query_phase = 0, loaded_phase = 0, weight_phase = 0;  // a bit a stream
                 auto wait_slot = [&](int i) {
-                    barrier_wait(smem_address(&ctl.full[slot_of(i)]), (i / S::kSlots) & 1, c.status);
+                    barrier_wait(smem_address(&ctl.full[i % S::kSlots]), (i / S::kSlots) & 1, c.status);
                     fence_after();
-                };
-                auto free_slot = [&](int i) { commit(smem_address(&ctl.empty[slot_of(i)])); };
-                auto scores = [&](int stream, int i) {
-                    const uint64_t q = operand(smem_address(query) + (NQ == 2 ? stream * 128 * DP * 2 : 0), 16);
-                    const uint64_t k = operand(slots + slot_of(i) * S::kSlot, 16);
-#pragma unroll
-                    for (int s = 0; s < DP / 16; ++s) {
-                        const uint64_t at = ((s >> 2) * (128 * 128) + (s & 3) * 32) >> 4;
-                        product_ss(tmem + stream * 128, q + at, k + at, kScores, s > 0);
-                    }
-                    commit(smem_address(&ctl.scores[stream]));
-                };
-                auto values = [&](int stream, int i, bool add) {
-                    barrier_wait(smem_address(&ctl.weights[stream]), weight_phase >> stream & 1, c.status);
-                    weight_phase ^= 1u << stream;
-                    fence_after();
-                    const uint64_t v = operand(slots + slot_of(i) * S::kSlot, kTileKeys * 128);
-#pragma unroll
-                    for (int s = 0; s < kTileKeys / 16; ++s)
-                        product_ts(tmem + 256 + stream * 128, tmem + stream * 128 + s * 8, v + s * ((16 * 128) >> 4), kValues,
-                                   add || s > 0);
                 };
                 for (int64_t cur = work.lo; cur < work.hi;) {
                     const Piece p = piece_at<S::kRows>(c, a, work, cur, group, base, tile_units);
@@ -252,46 +257,48 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
                     barrier_wait(smem_address(&ctl.queries), query_phase, c.status);
                     query_phase ^= 1;
                     fence_after();
-                    if (NQ == 2) {  // slots: K0 V0 K1 V1 ...
-                        const int streams = p.rows - p.block * S::kRows > 128 ? 2 : 1;
-                        wait_slot(used);
-#pragma unroll 1
-                        for (int i = 0; i < streams; ++i) scores(i, used);
-                        free_slot(used);
-                        for (int t = 0; t < n; ++t) {
-                            const int v = used + 2 * t + 1;
-                            wait_slot(v);
-                            if (t + 1 < n) wait_slot(v + 1);
-#pragma unroll 1
-                            for (int i = 0; i < streams; ++i) {
-                                values(i, v, t > 0);
-                                if (t + 1 < n) scores(i, v + 1);
-                                else commit(smem_address(&ctl.output[i]));
-                            }
-                            free_slot(v);
-                            if (t + 1 < n) free_slot(v + 1);
+                    // Jobs: a stream and a tile. Two streams on every tile, or one stream a tile, in turn or
+                    // always the first. The scores of job j + 1 are issued before the values of job j.
+                    const int per_tile = NQ == 2 && p.rows - p.block * S::kRows > 128 ? 2 : 1;
+                    const int jobs = n * per_tile;
+                    auto stream_of = [&](int j) { return NQ == 1 || per_tile == 2 ? j & 1 : 0; };
+                    auto tile_of = [&](int j) { return per_tile == 2 ? j >> 1 : j; };
+                    auto scores = [&](int j) {
+                        const int stream = stream_of(j), slot = used + 2 * tile_of(j);
+                        if (per_tile == 1 || stream == 0) wait_slot(slot);
+                        const uint64_t q = operand(smem_address(query) + (NQ == 2 ? stream * 128 * DP * 2 : 0), 16);
+                        const uint64_t k = operand(slots + slot % S::kSlots * S::kSlot, 16);
+#pragma unroll
+                        for (int s = 0; s < DP / 16; ++s) {
+                            const uint64_t at = ((s >> 2) * (128 * 128) + (s & 3) * 32) >> 4;
+                            product_ss(tmem, q + at, k + at, kScores, s > 0);
                         }
-                    } else {  // slots: K0 K1 V0 K2 V1 ...
-                        auto key_slot = [&](int t) { return used + (t == 0 ? 0 : 2 * t - 1); };
+                        commit(smem_address(&ctl.scores[stream]));
+                        if (per_tile == 1 || stream == 1) commit(smem_address(&ctl.empty[slot % S::kSlots]));
+                    };
+                    scores(0);
 #pragma unroll 1
-                        for (int t = 0; t < 2 && t < n; ++t) {
-                            wait_slot(key_slot(t));
-                            scores(t, key_slot(t));
-                            free_slot(key_slot(t));
+                    for (int j = 0; j < jobs; ++j) {
+                        const int stream = stream_of(j);
+                        if (j + 1 < jobs) {
+                            barrier_wait(smem_address(&ctl.loaded[stream]), loaded_phase >> stream & 1, c.status);
+                            fence_after();
+                            scores(j + 1);
                         }
-                        for (int t = 0; t < n; ++t) {
-                            const int v = used + (t + 1 < n ? 2 * t + 2 : 2 * t + 1);
-                            wait_slot(v);
-                            values(t & 1, v, t > 1);
-                            free_slot(v);
-                            if (t + 2 < n) {
-                                wait_slot(key_slot(t + 2));
-                                scores(t & 1, key_slot(t + 2));
-                                free_slot(key_slot(t + 2));
-                            } else {
-                                commit(smem_address(&ctl.output[t & 1]));
-                            }
-                        }
+                        loaded_phase ^= 1u << stream;
+                        const int slot = used + 2 * tile_of(j) + 1;
+                        if (per_tile == 1 || stream == 0) wait_slot(slot);
+                        barrier_wait(smem_address(&ctl.weights[stream]), weight_phase >> stream & 1, c.status);
+                        weight_phase ^= 1u << stream;
+                        fence_after();
+                        const bool add = j >= (NQ == 1 ? 2 : per_tile);  // the stream's first job begins the sum
+                        const uint64_t v = operand(slots + slot % S::kSlots * S::kSlot, kTileKeys * 128);
+#pragma unroll
+                        for (int s = 0; s < kTileKeys / 16; ++s)
+                            product_ts(tmem + 256 + stream * 128, tmem + 128 + stream * 64 + s * 8, v + s * ((16 * 128) >> 4),
+                                       kValues, add || s > 0);
+                        commit(smem_address(&ctl.done[stream]));
+                        if (per_tile == 1 || stream == 1) commit(smem_address(&ctl.empty[slot % S::kSlots]));
                     }
                     used += 2 * n;
                     cur += n;
@@ -307,13 +314,23 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
     // Scores to weights.
     asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     const int stream = warp >> 2, row = tid & 127;  // row of the stream's 128
+    const int my_row = NQ == 2 ? tid : row % S::kRows, copy = NQ == 2 ? 0 : row / S::kRows;
+    const int col0 = copy * S::kCols;  // the first position of a tile that the thread weighs
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t s_at = tmem + lanes + stream * 128, o_at = tmem + lanes + 256 + stream * 128;
-    const uint32_t scores_bar = smem_address(&ctl.scores[stream]), weights_bar = smem_address(&ctl.weights[stream]);
+    const uint32_t s_at = tmem + lanes + col0, p_at = tmem + lanes + 128 + stream * 64 + col0 / 2;
+    const uint32_t o_at = tmem + lanes + 256 + stream * 128;
+    const uint32_t scores_bar = smem_address(&ctl.scores[stream]), loaded_bar = smem_address(&ctl.loaded[stream]);
+    const uint32_t weights_bar = smem_address(&ctl.weights[stream]), done_bar = smem_address(&ctl.done[stream]);
     // Not 0, which would make a masked score's -inf a NaN.
     const float scale = fmaxf(fabsf(a.scale) * kLog2e, 1.2e-38f);
     const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;  // a negative scale turns the queries' signs
-    uint32_t score_phase = 0, output_phase = 0;
+    uint32_t score_phase = 0, done_phase = 0;
+    if constexpr (COPIES > 1) {  // the weights of other copies' positions stay zero
+        const uint32_t zero[32] = {};
+        tmem_store(tmem + lanes + 128 + stream * 64, zero);
+        tmem_store(tmem + lanes + 160 + stream * 64, zero);
+        tmem_stored();
+    }
     for (int64_t cur = work.lo; cur < work.hi;) {
         const Piece p = piece_at<S::kRows>(c, a, work, cur, group, base, tile_units);
         const int n_tiles = p.t1 - p.t0;
@@ -321,25 +338,31 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
         const int b = p.group / c.groups, beam0 = (p.group - b * c.groups) * kGroupBeams;
         const int row0 = p.block * S::kRows;
         const int rows = p.rows - row0 < S::kRows ? p.rows - row0 : S::kRows;
+        const bool mine = my_row < rows;
+        RowId id{0, 0, 0};
+        if (mine) id = row_id(a, row0 + my_row);
         // Both streams are done with the last segment's products, and so with its queries.
         named_sync(1, kSoftThreads);
-        load_queries<T, S::kRows, DP, kSoftThreads>(c, a, p, b, beam0, row0, rows, tid, [&](int r, int chunk, uint4 v) {
+        if (NQ == 2 || (stream == 0 && copy == 0))
+            ctl.query_at[my_row] = b * a.qs[0] + (beam0 + id.beam) * a.qs[1] + id.token * a.qs[2] + (p.head * a.G + id.head) * a.qs[3];
+        named_sync(1, kSoftThreads);
+        load_queries<T, S::kRows, DP, kSoftThreads>(c, a, ctl.query_at, rows, tid, [&](int r, int chunk, uint4 v) {
             v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
-            const int in = r & 127;
-            *reinterpret_cast<uint4*>(query + (r >> 7) * (128 * DP * 2) + (chunk >> 3) * (128 * 128) + in * 128 +
-                                      (((chunk & 7) ^ (in & 7)) << 4)) = v;
+#pragma unroll
+            for (int i = 0; i < (NQ == 2 ? 1 : COPIES); ++i) {
+                const int in = (r & 127) + i * S::kRows;
+                *reinterpret_cast<uint4*>(query + (r >> 7) * (128 * DP * 2) + (chunk >> 3) * (128 * 128) + in * 128 +
+                                          (((chunk & 7) ^ (in & 7)) << 4)) = v;
+            }
         });
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) barrier_arrive(smem_address(&ctl.queries));
 
-        const int my_row = NQ == 2 ? stream * 128 + row : row;
-        const bool mine = my_row < rows;
-        RowId id{0, 0, 0};
-        if (mine) id = row_id(a, row0 + my_row);
         const int64_t bk = static_cast<int64_t>(b) * a.beams + beam0 + id.beam;
         const int count = mine ? new_count(a, bk) : 0;
-        const uint32_t bit = mine && id.token < count ? 1u << id.beam : 0u;
+        const bool live = mine && id.token < count;
+        const uint32_t bit = live ? 1u << id.beam : 0u;
         const uint32_t need = __reduce_or_sync(0xffffffffu, bit);
         const uint8_t* fresh = a.mask ? a.mask + (bk * a.N + id.token) * a.N : nullptr;
         const CacheUnit* units = c.units + static_cast<int64_t>(p.group) * c.unit_cap;
@@ -349,7 +372,9 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
         const int first = NQ == 2 ? 0 : stream, step = NQ == 2 ? 1 : 2;
         bool began = false;
         if (active) {
-            auto unit_of = [&](int t) {  // a lane each
+            // A lane each; `other`: the unit has no position among the warp's.
+            const bool other = (lane << c.page_log2) >= col0 + S::kCols || ((lane + 1) << c.page_log2) <= col0;
+            auto unit_of = [&](int t) {
                 CacheUnit u{-1, 0, 0, -1};
                 const int i = (p.t0 + t) * tile_units + lane;
                 if (t < n_tiles && lane < tile_units && i < p.units) {
@@ -359,32 +384,29 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
                 return u;
             };
             CacheUnit next = unit_of(first);
+#pragma unroll 1
             for (int t = first; t < n_tiles; t += step) {
                 const CacheUnit u = next;
                 next = unit_of(t + step);
-                const bool none = __all_sync(0xffffffffu, (u.mask & need) == 0);
-                const bool plain = __all_sync(0xffffffffu, lane >= tile_units || (u.limit < 0 && (u.mask & need) == need));
+                const bool none = __all_sync(0xffffffffu, other || (u.mask & need) == 0);
+                const bool plain = __all_sync(0xffffffffu, other || (u.limit < 0 && (u.mask & need) == need));
                 barrier_wait(scores_bar, score_phase, c.status);
                 score_phase ^= 1;
                 fence_after();
-                if (none) {
-                    // No row of the warp sees any of it.
-                    if (need != 0) {
-                        uint32_t zero[32] = {};
-                        tmem_store(s_at, zero);
-                        tmem_store(s_at + 32, zero);
-                        tmem_stored();
-                    }
-                } else {
-                    uint32_t s[128];
-                    tmem_load(s, s_at);
+                uint32_t s[S::kCols];
+                if (!none) tmem_load(s, s_at);
+                fence_before();
+                __syncwarp();
+                if (lane == 0) barrier_arrive(loaded_bar);
+                float keep = 1.0f;
+                if (!none) {
                     if (!plain) {
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) {  // 16 positions lie in one unit
-                            const int from = (i * 16) >> c.page_log2;
+                        for (int i = 0; i < S::kCols / 16; ++i) {  // 16 positions lie in one unit
+                            const int from = (col0 + i * 16) >> c.page_log2;
                             const uint32_t holders = __shfl_sync(0xffffffffu, u.mask, from);
                             const int limit = __shfl_sync(0xffffffffu, u.limit, from);
-                            const int start = __shfl_sync(0xffffffffu, u.start, from) + ((i * 16) & (c.page - 1));
+                            const int start = __shfl_sync(0xffffffffu, u.start, from) + ((col0 + i * 16) & (c.page - 1));
                             const bool holds = (holders & bit) != 0;
                             uint32_t sees = holds ? 0xffffu : 0u;
                             if (limit >= 0) {
@@ -408,17 +430,21 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
 #pragma unroll
                     for (int e = 0; e < 8; ++e) most[e] = __uint_as_float(s[e]);
 #pragma unroll
-                    for (int e = 8; e < 128; ++e) most[e & 7] = fmaxf(most[e & 7], __uint_as_float(s[e]));
+                    for (int e = 8; e < S::kCols; ++e) most[e & 7] = fmaxf(most[e & 7], __uint_as_float(s[e]));
                     const float now = fmaxf(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])),
                                             fmaxf(fmaxf(most[4], most[5]), fmaxf(most[6], most[7])));
-                    float keep = 1.0f;
+                    // (inf - inf is not a growth, and a reference of -inf, nothing seen yet, keeps 1.)
                     if ((now - top) * scale > kRaise || (top == -INFINITY && now > top)) {
                         keep = exp2_fast((top - now) * scale);
                         top = now;
                     }
-                    // (inf - inf is not a growth, and a reference of -inf, nothing seen yet, keeps 1.)
-                    if (began && __any_sync(0xffffffffu, keep != 1.0f)) {
-#pragma unroll
+                }
+                if (began) {  // P and O are this thread's again once the last weights' product is done
+                    barrier_wait(done_bar, done_phase, c.status);
+                    done_phase ^= 1;
+                    fence_after();
+                    if (__any_sync(0xffffffffu, keep != 1.0f)) {
+#pragma unroll 1
                         for (int i = 0; i < DP / 32; ++i) {
                             uint32_t o[32];
                             tmem_load(o, o_at + 32 * i);
@@ -427,117 +453,166 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
                             tmem_store(o_at + 32 * i, o);
                         }
                     }
+                }
+                constexpr int kWords = S::kCols / 2 < 32 ? S::kCols / 2 : 32;  // pairs of weights stored at a time
+                if (none) {
+                    // No row of the warp sees any of it.
+                    uint32_t w[kWords];
+#pragma unroll
+                    for (int e = 0; e < kWords; ++e) w[e] = 0;
+#pragma unroll
+                    for (int i = 0; i < S::kCols / 2; i += kWords) tmem_store(p_at + i, w);
+                } else {
                     const float ref = top == -INFINITY ? 0.0f : top * scale;
                     float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        uint32_t w[32];
+                    for (int i = 0; i < S::kCols / 2; i += kWords) {
+                        uint32_t w[kWords];
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) {
-                            const float x = exp2_fast(fmaf(__uint_as_float(s[64 * h + 2 * e]), scale, -ref));
-                            const float y = exp2_fast(fmaf(__uint_as_float(s[64 * h + 2 * e + 1]), scale, -ref));
+                        for (int e = 0; e < kWords; ++e) {
+                            const float x = exp2_fast(fmaf(__uint_as_float(s[2 * (i + e)]), scale, -ref));
+                            const float y = exp2_fast(fmaf(__uint_as_float(s[2 * (i + e) + 1]), scale, -ref));
                             part[(e & 1) * 2] += x;
                             part[(e & 1) * 2 + 1] += y;
                             w[e] = Pack<T>::pair(x, y);
                         }
-                        tmem_store(s_at + 32 * h, w);
+                        tmem_store(p_at + i, w);
                     }
                     sum = sum * keep + ((part[0] + part[1]) + (part[2] + part[3]));
-                    tmem_stored();
                 }
+                tmem_stored();
                 began = true;
                 fence_before();
                 __syncwarp();
                 if (lane == 0) barrier_arrive(weights_bar);
             }
             if (began) {
-                barrier_wait(smem_address(&ctl.output[stream]), output_phase, c.status);
-                output_phase ^= 1;
+                barrier_wait(done_bar, done_phase, c.status);
+                done_phase ^= 1;
                 fence_after();
             }
         }
 
-        // The streams' rows, joined where they are the same, to the output or to this CTA's part.
+        // To the output, or to this CTA's part of a divided segment.
         const bool whole = p.t0 == 0 && p.t1 == p.tiles;
         float* parts = static_cast<float*>(a.workspace) + 2048;
         int32_t* counters = static_cast<int32_t*>(a.workspace);
         float* part = parts + static_cast<int64_t>(2 * blockIdx.x + (p.t0 == 0)) * S::kOut;
-        float m = top == -INFINITY ? top : top * scale, l = sum, factor = 1.0f;  // base-2 maximum, sum
-        if constexpr (NQ == 1) {
-            if (stream == 1) ctl.top[row] = m, ctl.sum[row] = l;
-            named_sync(1, kSoftThreads);
-            const float m1 = ctl.top[row], l1 = ctl.sum[row];
-            named_sync(1, kSoftThreads);
-            if (stream == 0) ctl.top[row] = m, ctl.sum[row] = l;
-            named_sync(1, kSoftThreads);
-            const float m0 = ctl.top[row], l0 = ctl.sum[row];
-            const float both = fmaxf(m0, m1), ref = both == -INFINITY ? 0.0f : both;
-            factor = exp2_fast(m - ref);
-            l = l0 * exp2_fast(m0 - ref) + l1 * exp2_fast(m1 - ref);
-            m = both;
-        }
-        const bool live = mine && id.token < count;
-        const float inverse = live ? (l > 0.0f ? 1.0f / l : l) : 0.0f;
-        T* out = static_cast<T*>(a.out) + ((bk * a.N + id.token) * a.Hq + p.head * a.G + id.head) * c.D;
-        const int warp_row = my_row & ~31;
+        float m = top == -INFINITY ? top : top * scale, l = sum;  // base-2 maximum, sum
+        const bool holds_rows = began && (my_row & ~31) < rows;   // of the warp
+        if constexpr (NQ == 2) {
+            const float inverse = l > 0.0f ? 1.0f / l : l;
+            const int64_t place = (bk * a.N + id.token) * a.Hq + p.head * a.G + id.head;
+            T* out = static_cast<T*>(a.out) + place * c.D;
+#pragma unroll 1
+            for (int i = 0; i < DP / 32; ++i) {
+                uint32_t o[32];
+                if (holds_rows) tmem_load(o, o_at + 32 * i);
+                if (!mine) continue;
+                if (whole) {
 #pragma unroll
-        for (int i = 0; i < DP / 32; ++i) {
-            uint32_t o[32];
-            if (began && warp_row < rows) {
-                tmem_load(o, o_at + 32 * i);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] = 0;
-            }
-            if constexpr (NQ == 1) {
-                // Stream 1 hands its columns over where the queries were (their products are done).
-                float4* at = reinterpret_cast<float4*>(query) + (i & 1) * 1024 + row * 8;
-                if (stream == 1 && warp_row < rows) {
+                    for (int e = 0; e < 4; ++e) {
+                        if (i * 32 + e * 8 >= c.D) break;
+                        uint4 v = make_uint4(0, 0, 0, 0);
+                        if (live) {
+                            auto y = [&](int x) { return __uint_as_float(o[8 * e + x]) * inverse; };
+                            v = make_uint4(Pack<T>::pair(y(0), y(1)), Pack<T>::pair(y(2), y(3)), Pack<T>::pair(y(4), y(5)),
+                                           Pack<T>::pair(y(6), y(7)));
+                        }
+                        reinterpret_cast<uint4*>(out)[i * 4 + e] = v;
+                    }
+                } else {
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
-                        at[e ^ (row & 7)] = make_float4(__uint_as_float(o[4 * e]) * factor, __uint_as_float(o[4 * e + 1]) * factor,
-                                                        __uint_as_float(o[4 * e + 2]) * factor, __uint_as_float(o[4 * e + 3]) * factor);
+                        *reinterpret_cast<uint4*>(part + my_row * DP + i * 32 + e * 4) =
+                            make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                }
+            }
+            if (mine) {
+                if (whole) {
+                    if (a.lse != nullptr) a.lse[place] = live && l != 0.0f ? (m + log2f(l)) * kLn2 : -INFINITY;
+                } else {
+                    part[S::kRows * DP + my_row] = m;
+                    part[S::kRows * DP + S::kRows + my_row] = l;
+                }
+            }
+        } else {
+            // The rows' 2 * COPIES partial results, 32 columns at a time through shared memory.
+            constexpr int kParts = 2 * COPIES;
+            const int which = stream * COPIES + copy;
+            named_sync(1, kSoftThreads);  // (query_at shares the space)
+            ctl.top[which * S::kRows + my_row] = m;
+            ctl.sum[which * S::kRows + my_row] = l;
+            named_sync(1, kSoftThreads);
+            auto row_stats = [&](int r, float* ref, float* total) {
+                float top_all = -INFINITY, l_all = 0.0f;
+#pragma unroll
+                for (int i = 0; i < kParts; ++i) top_all = fmaxf(top_all, ctl.top[i * S::kRows + r]);
+                *ref = top_all == -INFINITY ? 0.0f : top_all;
+#pragma unroll
+                for (int i = 0; i < kParts; ++i) l_all = fmaf(ctl.sum[i * S::kRows + r], exp2_fast(ctl.top[i * S::kRows + r] - *ref), l_all);
+                *total = l_all;
+                return top_all;
+            };
+            float ref, total;
+            row_stats(my_row, &ref, &total);
+            const float factor = exp2_fast(m - ref);
+            float4* stage = reinterpret_cast<float4*>(query);  // [which][row][8], swizzled
+#pragma unroll 1
+            for (int i = 0; i < DP / 32; ++i) {
+                if (holds_rows) {
+                    uint32_t o[32];
+                    tmem_load(o, o_at + 32 * i);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        stage[(which * S::kRows + my_row) * 8 + (e ^ (my_row & 7))] =
+                            make_float4(__uint_as_float(o[4 * e]) * factor, __uint_as_float(o[4 * e + 1]) * factor,
+                                        __uint_as_float(o[4 * e + 2]) * factor, __uint_as_float(o[4 * e + 3]) * factor);
                 }
                 named_sync(1, kSoftThreads);
-                if (stream == 0 && warp_row < rows) {
+                const int vec = tid & 7, streams = n_tiles > 1 ? 2 : 1;  // a segment of one tile has no second stream
+#pragma unroll 1
+                for (int r = tid >> 3; r < rows; r += kSoftThreads / 8) {
+                    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const float4 x = at[e ^ (row & 7)];
-                        o[4 * e] = __float_as_uint(fmaf(__uint_as_float(o[4 * e]), factor, x.x));
-                        o[4 * e + 1] = __float_as_uint(fmaf(__uint_as_float(o[4 * e + 1]), factor, x.y));
-                        o[4 * e + 2] = __float_as_uint(fmaf(__uint_as_float(o[4 * e + 2]), factor, x.z));
-                        o[4 * e + 3] = __float_as_uint(fmaf(__uint_as_float(o[4 * e + 3]), factor, x.w));
+                    for (int j = 0; j < kParts; ++j) {
+                        if (j / COPIES >= streams) break;
+                        const float4 x = stage[(j * S::kRows + r) * 8 + (vec ^ (r & 7))];
+                        o.x += x.x, o.y += x.y, o.z += x.z, o.w += x.w;
+                    }
+                    const float l_row = [&] {
+                        float f, t;
+                        row_stats(r, &f, &t);
+                        return t;
+                    }();
+                    if (i * 32 + vec * 4 < c.D) {
+                        if (whole) {
+                            const RowId rid = row_id(a, row0 + r);
+                            const int64_t rbk = static_cast<int64_t>(b) * a.beams + beam0 + rid.beam;
+                            const int64_t place = (rbk * a.N + rid.token) * a.Hq + p.head * a.G + rid.head;
+                            const bool shown = rid.token < new_count(a, rbk);
+                            const float inverse = l_row > 0.0f ? 1.0f / l_row : l_row;
+                            uint2 v = make_uint2(0, 0);
+                            if (shown)
+                                v = make_uint2(Pack<T>::pair(o.x * inverse, o.y * inverse), Pack<T>::pair(o.z * inverse, o.w * inverse));
+                            *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + place * c.D + i * 32 + vec * 4) = v;
+                        } else {
+                            *reinterpret_cast<float4*>(part + r * DP + i * 32 + vec * 4) = o;
+                        }
                     }
                 }
+                named_sync(1, kSoftThreads);
             }
-            if ((NQ == 1 && stream == 1) || !mine) continue;
-            if (whole) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    if (i * 32 + e * 8 >= c.D) break;
-                    uint4 v = make_uint4(0, 0, 0, 0);
-                    if (live) {
-                        auto y = [&](int x) { return __uint_as_float(o[8 * e + x]) * inverse; };
-                        v = make_uint4(Pack<T>::pair(y(0), y(1)), Pack<T>::pair(y(2), y(3)), Pack<T>::pair(y(4), y(5)),
-                                       Pack<T>::pair(y(6), y(7)));
-                    }
-                    reinterpret_cast<uint4*>(out)[i * 4 + e] = v;
+            if (mine && which == 0) {
+                const float top_all = row_stats(my_row, &ref, &total);
+                if (whole) {
+                    if (a.lse != nullptr)
+                        a.lse[(bk * a.N + id.token) * a.Hq + p.head * a.G + id.head] =
+                            live && total != 0.0f ? (top_all + log2f(total)) * kLn2 : -INFINITY;
+                } else {
+                    part[S::kRows * DP + my_row] = top_all;
+                    part[S::kRows * DP + S::kRows + my_row] = total;
                 }
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    *reinterpret_cast<uint4*>(part + my_row * DP + i * 32 + e * 4) =
-                        make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-            }
-        }
-        if (mine && !(NQ == 1 && stream == 1)) {
-            if (whole) {
-                if (a.lse != nullptr)
-                    a.lse[(bk * a.N + id.token) * a.Hq + p.head * a.G + id.head] =
-                        live && l != 0.0f ? (m + log2f(l)) * kLn2 : -INFINITY;
-            } else {
-                part[S::kRows * DP + my_row] = m;
-                part[S::kRows * DP + S::kRows + my_row] = l;
             }
         }
         if (whole) continue;
@@ -551,37 +626,45 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
         named_sync(1, kSoftThreads);
         if (!ctl.last) continue;
         __threadfence();
-        join_parts<T, S::kRows, DP, kSoftThreads>(c, a, p, b, beam0, row0, rows, parts, reinterpret_cast<float*>(query), tid);
+        join_parts<T, S::kRows, DP, kSoftThreads>(c, a, p, b, beam0, row0, rows, parts, query, tid);
     }
     fence_before();
     named_sync(2, kSoftThreads + 32);
 }
 
-template <class T, int DP, int NQ>
+template <class T, int DP, int NQ, int COPIES>
 cudaError_t launch_shape(const CacheView& c, const CUtensorMap& map, const AttendParams& a, int sm_count,
                          cudaStream_t stream) {
-    using S = Shape<DP, NQ>;
-    auto* kernel = attend_tc_kernel<T, DP, NQ>;
+    using S = Shape<DP, NQ, COPIES>;
+    static_assert(S::kBytes <= 227 * 1024 && S::kSlots >= 4);
+    auto* kernel = attend_tc_kernel<T, DP, NQ, COPIES>;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes);
     if (e != cudaSuccess) return e;
     return launch_after(kernel, sm_count, kThreads, S::kBytes, stream, map, c, a);
 }
 
+template <class T, int DP>
+cudaError_t launch_width(const CacheView& c, const CUtensorMap& map, const AttendParams& a, int sm_count,
+                         cudaStream_t stream) {
+    const int beams = a.beams < kGroupBeams ? a.beams : kGroupBeams;
+    const int64_t rows = static_cast<int64_t>(beams) * a.N * a.G;
+    if (rows <= 32) return launch_shape<T, DP, 1, 4>(c, map, a, sm_count, stream);
+    if (rows <= 64) return launch_shape<T, DP, 1, 2>(c, map, a, sm_count, stream);
+    if (rows <= 128) return launch_shape<T, DP, 1, 1>(c, map, a, sm_count, stream);
+    return launch_shape<T, DP, 2, 1>(c, map, a, sm_count, stream);
+}
+
 template <class T>
 cudaError_t launch_typed(const CacheView& c, const CUtensorMap& map, const AttendParams& a, int sm_count,
                          cudaStream_t stream) {
-    const int beams = a.beams < kGroupBeams ? a.beams : kGroupBeams;
-    const bool one = static_cast<int64_t>(beams) * a.N * a.G <= 128;
-    if (c.D <= 64)
-        return one ? launch_shape<T, 64, 1>(c, map, a, sm_count, stream) : launch_shape<T, 64, 2>(c, map, a, sm_count, stream);
-    return one ? launch_shape<T, 128, 1>(c, map, a, sm_count, stream) : launch_shape<T, 128, 2>(c, map, a, sm_count, stream);
+    return c.D <= 64 ? launch_width<T, 64>(c, map, a, sm_count, stream) : launch_width<T, 128>(c, map, a, sm_count, stream);
 }
 
 }  // namespace
 
 int64_t attend_tc_workspace(const CacheView&, const AttendParams&, int sm_count) {
     // A counter for each CTA (8192 bytes), then two partial results for each.
-    return 8192 + static_cast<int64_t>(2) * sm_count * Shape<128, 2>::kOut * 4;
+    return 8192 + static_cast<int64_t>(2) * sm_count * Shape<128, 2, 1>::kOut * 4;
 }
 
 cudaError_t launch_attend_tc(const CacheView& c, int dtype, const AttendParams& a, int sm_count, cudaStream_t stream) {
