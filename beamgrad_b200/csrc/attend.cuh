@@ -81,7 +81,7 @@ __device__ __forceinline__ float lanes_sum(float v) {
 // 2^x, within 2 ulp: the weights are sums' terms of at most 1 in magnitude.
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 
@@ -285,8 +285,19 @@ struct Piece {
     int group, block, head;  // block: row block
     int t0, t1;              // tiles
     int tiles, units, rows;  // of the group
-    int c0, c1;              // CTAs that hold the segment's first and last tile
+    int64_t first;           // the segment's first tile on the line
 };
+
+// The CTAs that hold a divided segment's first and last tile.
+struct Span {
+    int c0, c1;
+};
+__device__ __forceinline__ Span span_of(const WorkSplit& w, const Piece& p) {
+    Span s;
+    s.c0 = p.t0 == 0 ? static_cast<int>(blockIdx.x) : cta_of(w, p.first);
+    s.c1 = p.t1 == p.tiles ? static_cast<int>(blockIdx.x) : cta_of(w, p.first + p.tiles - 1);
+    return s;
+}
 
 // The piece at tile `cur` of the line; advances group and base to it.
 template <int kRows>
@@ -308,9 +319,7 @@ __device__ __forceinline__ Piece piece_at(const CacheView& c, const AttendParams
     p.tiles = g.tiles;
     p.units = g.units;
     p.rows = g.rows;
-    const int64_t first = base + static_cast<int64_t>(seg) * g.tiles;
-    p.c0 = cta_of(w, first);
-    p.c1 = cta_of(w, first + g.tiles - 1);
+    p.first = base + static_cast<int64_t>(seg) * g.tiles;
     return p;
 }
 
@@ -359,12 +368,12 @@ __device__ __forceinline__ void load_queries(const CacheView& c, const AttendPar
 // on which CTA comes last. A part: kRows x DP sums, the rows' references (base 2), their weights'
 // sums. scratch: 16 * kRows bytes of shared memory. All kThreads threads of named barrier 1.
 template <class T, int kRows, int DP, int kThreads>
-__device__ __forceinline__ void join_parts(const CacheView& c, const AttendParams& a, const Piece& p, int b, int beam0,
-                                           int row0, int rows, const float* parts, void* scratch, int tid) {
+__device__ __forceinline__ void join_parts(const CacheView& c, const AttendParams& a, const Piece& p, Span span, int b,
+                                           int beam0, int row0, int rows, const float* parts, void* scratch, int tid) {
     constexpr int kOut = kRows * (DP + 2), kVecs = DP / 4;
-    const int n_parts = p.c1 - p.c0 + 1;
+    const int n_parts = span.c1 - span.c0 + 1;
     // A CTA's second part is the one that begins a segment.
-    auto part_of = [&](int i) { return parts + static_cast<int64_t>(2 * (p.c0 + i) + (i == 0)) * kOut; };
+    auto part_of = [&](int i) { return parts + static_cast<int64_t>(2 * (span.c0 + i) + (i == 0)) * kOut; };
     int64_t* places = static_cast<int64_t*>(scratch);
     float* refs = reinterpret_cast<float*>(places + kRows);
     float* factors = refs + kRows;  // 1 / sum; -1 for rows that are not shown

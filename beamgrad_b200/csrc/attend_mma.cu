@@ -428,15 +428,16 @@ attend_mma_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant
         if (whole) continue;
         __threadfence();
         named_sync(1, kComputeThreads);
+        const Span span = span_of(work, p);
         if (tid == 0) {
-            const int before = atomicAdd(counters + p.c0, 1);
-            ctl.last = before == p.c1 - p.c0;
-            if (ctl.last) counters[p.c0] = 0;
+            const int before = atomicAdd(counters + span.c0, 1);
+            ctl.last = before == span.c1 - span.c0;
+            if (ctl.last) counters[span.c0] = 0;
         }
         named_sync(1, kComputeThreads);
         if (!ctl.last) continue;
         __threadfence();
-        join_parts<T, S::kRows, DP, kComputeThreads>(c, a, p, b, beam0, row0, rows, parts, join, tid);
+        join_parts<T, S::kRows, DP, kComputeThreads>(c, a, p, span, b, beam0, row0, rows, parts, join, tid);
     }
 }
 

@@ -68,6 +68,14 @@ struct Shape {
 // ---- tcgen05 ----
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+// One lane of the (converged) warp. Products are issued by the elected lane of a warp that runs its
+// loop as a whole: with a loop for one lane alone, every operand of every product takes a detour to
+// the warp's uniform registers (8 products took 750 cycles to issue instead of 512).
+__device__ __forceinline__ bool elected() {
+    uint32_t yes;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(yes));
+    return yes != 0;
+}
 __device__ __forceinline__ void commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
@@ -152,6 +160,57 @@ template <class T>
 __device__ __forceinline__ constexpr uint32_t product_kind(int columns, bool by_row) {
     constexpr uint32_t type = sizeof(T) == 2 && std::is_same_v<T, __nv_bfloat16> ? 1 : 0;
     return 1u << 4 | type << 7 | type << 10 | (by_row ? 1u << 16 : 0u) | static_cast<uint32_t>(columns / 8) << 17 | 8u << 24;
+}
+
+// ---- exponentials ----
+// Pairs of 32-bit numbers, one instruction for both.
+using Pair = uint64_t;
+__device__ __forceinline__ Pair pair_of(float x, float y) {
+    Pair p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(x), "f"(y));
+    return p;
+}
+__device__ __forceinline__ void unpair(Pair p, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(p)); }
+__device__ __forceinline__ Pair pair_fma(Pair a, Pair b, Pair c) {
+    Pair d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ Pair pair_add(Pair a, Pair b) {
+    Pair d;
+    asm("add.rn.ftz.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {  // NaN if one is
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// 2^x of a pair on the multiply-add pipe, which has room while the special-function unit (16 a cycle
+// and SM) is what the weights of 128 x 128 scores wait for. x = n + f with n = floor(x): 2^f by a
+// polynomial of degree 5 (least relative error on [0, 1], 1.6e-7 as evaluated), n added to its
+// exponent. x is at most kRaise; at -126 and below the result is a denormal (the polynomial is just
+// below 1 at 0), which the sum takes as 0.
+__device__ __forceinline__ void exp2_pair(Pair x2, float& a, float& b) {
+    float x, y;
+    unpair(x2, x, y);
+    x2 = pair_of(fmaxf(x, -126.0f), fmaxf(y, -126.0f));
+    const Pair shift = pair_of(12582912.0f, 12582912.0f);  // 1.5 * 2^23: n in the low bits
+    Pair t, n, f;
+    asm("add.rm.f32x2 %0, %1, %2;" : "=l"(t) : "l"(x2), "l"(shift));
+    asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(n) : "l"(t), "l"(shift));
+    asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(f) : "l"(x2), "l"(n));
+    auto both = [](float c) { return pair_of(c, c); };
+    Pair r = pair_fma(both(0.0018775766948238015f), f, both(0.00898933969438076f));
+    r = pair_fma(r, f, both(0.05582631751894951f));
+    r = pair_fma(r, f, both(0.24015361070632935f));
+    r = pair_fma(r, f, both(0.6931530833244324f));
+    r = pair_fma(r, f, both(0.9999999403953552f));
+    float p, q, u, v;
+    unpair(r, p, q);
+    unpair(t, u, v);
+    a = __uint_as_float(__float_as_uint(p) + (__float_as_uint(u) << 23));
+    b = __uint_as_float(__float_as_uint(q) + (__float_as_uint(v) << 23));
 }
 
 template <class T, int DP, int NQ, int COPIES>
@@ -244,30 +303,31 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
             for (int i = used > S::kSlots ? used - S::kSlots : 0; i < used; ++i)
                 barrier_wait(smem_address(&ctl.full[i % S::kSlots]), (i / S::kSlots) & 1, c.status);
         } else {
-            if (lane == 0) {
-                constexpr uint32_t kScores = product_kind<T>(kTileKeys, false), kValues = product_kind<T>(DP, true);
-                uint32_t query_phase = 0, loaded_phase = 0, weight_phase = 0;  // a bit a stream
-                auto wait_slot = [&](int i) {
-                    barrier_wait(smem_address(&ctl.full[i % S::kSlots]), (i / S::kSlots) & 1, c.status);
-                    fence_after();
-                };
-                for (int64_t cur = work.lo; cur < work.hi;) {
-                    const Piece p = piece_at<S::kRows>(c, a, work, cur, group, base, tile_units);
-                    const int n = p.t1 - p.t0;
-                    barrier_wait(smem_address(&ctl.queries), query_phase, c.status);
-                    query_phase ^= 1;
-                    fence_after();
-                    // Jobs: a stream and a tile. Two streams on every tile, or one stream a tile, in turn or
-                    // always the first. The scores of job j + 1 are issued before the values of job j.
-                    const int per_tile = NQ == 2 && p.rows - p.block * S::kRows > 128 ? 2 : 1;
-                    const int jobs = n * per_tile;
-                    auto stream_of = [&](int j) { return NQ == 1 || per_tile == 2 ? j & 1 : 0; };
-                    auto tile_of = [&](int j) { return per_tile == 2 ? j >> 1 : j; };
-                    auto scores = [&](int j) {
-                        const int stream = stream_of(j), slot = used + 2 * tile_of(j);
-                        if (per_tile == 1 || stream == 0) wait_slot(slot);
-                        const uint64_t q = operand(smem_address(query) + (NQ == 2 ? stream * 128 * DP * 2 : 0), 16);
-                        const uint64_t k = operand(slots + slot % S::kSlots * S::kSlot, 16);
+            constexpr uint32_t kScores = product_kind<T>(kTileKeys, false), kValues = product_kind<T>(DP, true);
+            uint32_t query_phase = 0, loaded_phase = 0, weight_phase = 0;  // a bit a stream
+            auto wait_slot = [&](int i) {
+                barrier_wait(smem_address(&ctl.full[i % S::kSlots]), (i / S::kSlots) & 1, c.status);
+                fence_after();
+            };
+            for (int64_t cur = work.lo; cur < work.hi;) {
+                const Piece p = piece_at<S::kRows>(c, a, work, cur, group, base, tile_units);
+                const int n = p.t1 - p.t0;
+                barrier_wait(smem_address(&ctl.queries), query_phase, c.status);
+                query_phase ^= 1;
+                fence_after();
+                // Jobs: a stream and a tile. Two streams on every tile, or one stream a tile, in turn or
+                // always the first. The scores of job j + 2 are issued before the values of job j, so that
+                // they are there when job j's warpgroup is done with its weights.
+                const int per_tile = NQ == 2 && p.rows - p.block * S::kRows > 128 ? 2 : 1;
+                const int jobs = n * per_tile;
+                auto stream_of = [&](int j) { return NQ == 1 || per_tile == 2 ? j & 1 : 0; };
+                auto tile_of = [&](int j) { return per_tile == 2 ? j >> 1 : j; };
+                auto scores = [&](int j) {
+                    const int stream = stream_of(j), slot = used + 2 * tile_of(j);
+                    if (per_tile == 1 || stream == 0) wait_slot(slot);
+                    const uint64_t q = operand(smem_address(query) + (NQ == 2 ? stream * 128 * DP * 2 : 0), 16);
+                    const uint64_t k = operand(slots + slot % S::kSlots * S::kSlot, 16);
+                    if (elected()) {
 #pragma unroll
                         for (int s = 0; s < DP / 16; ++s) {
                             const uint64_t at = ((s >> 2) * (128 * 128) + (s & 3) * 32) >> 4;
@@ -275,24 +335,32 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
                         }
                         commit(smem_address(&ctl.scores[stream]));
                         if (per_tile == 1 || stream == 1) commit(smem_address(&ctl.empty[slot % S::kSlots]));
-                    };
-                    scores(0);
-#pragma unroll 1
-                    for (int j = 0; j < jobs; ++j) {
-                        const int stream = stream_of(j);
-                        if (j + 1 < jobs) {
-                            barrier_wait(smem_address(&ctl.loaded[stream]), loaded_phase >> stream & 1, c.status);
-                            fence_after();
-                            scores(j + 1);
-                        }
-                        loaded_phase ^= 1u << stream;
-                        const int slot = used + 2 * tile_of(j) + 1;
-                        if (per_tile == 1 || stream == 0) wait_slot(slot);
-                        barrier_wait(smem_address(&ctl.weights[stream]), weight_phase >> stream & 1, c.status);
-                        weight_phase ^= 1u << stream;
+                    }
+                    __syncwarp();
+                };
+                auto next_scores = [&](int j) {  // once job j - 1's scores are in registers
+                    const int before = stream_of(j - 1);
+                    if (j < jobs) {
+                        barrier_wait(smem_address(&ctl.loaded[before]), loaded_phase >> before & 1, c.status);
                         fence_after();
-                        const bool add = j >= (NQ == 1 ? 2 : per_tile);  // the stream's first job begins the sum
-                        const uint64_t v = operand(slots + slot % S::kSlots * S::kSlot, kTileKeys * 128);
+                        scores(j);
+                    }
+                    if (j <= jobs) loaded_phase ^= 1u << before;
+                };
+                scores(0);
+                next_scores(1);
+#pragma unroll 1
+                for (int j = 0; j < jobs; ++j) {
+                    const int stream = stream_of(j);
+                    next_scores(j + 2);
+                    const int slot = used + 2 * tile_of(j) + 1;
+                    if (per_tile == 1 || stream == 0) wait_slot(slot);
+                    barrier_wait(smem_address(&ctl.weights[stream]), weight_phase >> stream & 1, c.status);
+                    weight_phase ^= 1u << stream;
+                    fence_after();
+                    const bool add = j >= (NQ == 1 ? 2 : per_tile);  // the stream's first job begins the sum
+                    const uint64_t v = operand(slots + slot % S::kSlots * S::kSlot, kTileKeys * 128);
+                    if (elected()) {
 #pragma unroll
                         for (int s = 0; s < kTileKeys / 16; ++s)
                             product_ts(tmem + 256 + stream * 128, tmem + 128 + stream * 64 + s * 8, v + s * ((16 * 128) >> 4),
@@ -300,11 +368,11 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
                         commit(smem_address(&ctl.done[stream]));
                         if (per_tile == 1 || stream == 1) commit(smem_address(&ctl.empty[slot % S::kSlots]));
                     }
-                    used += 2 * n;
-                    cur += n;
+                    __syncwarp();
                 }
+                used += 2 * n;
+                cur += n;
             }
-            __syncwarp();
             named_sync(2, kSoftThreads + 32);  // every read of tensor memory is over
             asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
         }
@@ -426,15 +494,15 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
                                 if ((sees >> e & 1) == 0) s[i * 16 + e] = 0xff800000u;
                         }
                     }
-                    float most[8];
+                    // A NaN among the scores stays in the maximum.
+                    float most[4];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) most[e] = __uint_as_float(s[e]);
+                    for (int e = 0; e < 4; ++e) most[e] = __uint_as_float(s[e]);
 #pragma unroll
-                    for (int e = 8; e < S::kCols; ++e) most[e & 7] = fmaxf(most[e & 7], __uint_as_float(s[e]));
-                    const float now = fmaxf(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])),
-                                            fmaxf(fmaxf(most[4], most[5]), fmaxf(most[6], most[7])));
-                    // (inf - inf is not a growth, and a reference of -inf, nothing seen yet, keeps 1.)
-                    if ((now - top) * scale > kRaise || (top == -INFINITY && now > top)) {
+                    for (int e = 4; e + 1 < S::kCols; e += 2)
+                        most[(e >> 1) & 3] = max3(most[(e >> 1) & 3], __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
+                    const float now = max3(max3(most[0], most[1], most[2]), most[3], most[3]);
+                    if (now != -INFINITY && !((now - top) * scale <= kRaise)) {
                         keep = exp2_fast((top - now) * scale);
                         top = now;
                     }
@@ -454,7 +522,7 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
                         }
                     }
                 }
-                constexpr int kWords = S::kCols / 2 < 32 ? S::kCols / 2 : 32;  // pairs of weights stored at a time
+                constexpr int kWords = 16;  // pairs of weights stored at a time
                 if (none) {
                     // No row of the warp sees any of it.
                     uint32_t w[kWords];
@@ -463,22 +531,41 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
 #pragma unroll
                     for (int i = 0; i < S::kCols / 2; i += kWords) tmem_store(p_at + i, w);
                 } else {
-                    const float ref = top == -INFINITY ? 0.0f : top * scale;
-                    float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    // Nothing seen yet: any reference gives weights of 0. A maximum that is inf or NaN gives NaN.
+                    const float ref = top == -INFINITY ? 0.0f : (top < INFINITY ? top * scale : NAN);
+                    const Pair scale2 = pair_of(scale, scale), ref2 = pair_of(-ref, -ref);
+                    Pair part[2] = {pair_of(0.0f, 0.0f), pair_of(0.0f, 0.0f)};
 #pragma unroll
                     for (int i = 0; i < S::kCols / 2; i += kWords) {
+                        // In stages over 16 pairs: a result is not used before its latency is over.
+                        Pair x[kWords];
+                        float u[kWords], v[kWords];
+#pragma unroll
+                        for (int e = 0; e < kWords; ++e)
+                            x[e] = pair_fma(pair_of(__uint_as_float(s[2 * (i + e)]), __uint_as_float(s[2 * (i + e) + 1])), scale2,
+                                            ref2);
+#pragma unroll
+                        for (int e = 0; e < kWords; ++e) {
+                            if (S::kCols == 128 && e % 4 == 3) continue;
+                            unpair(x[e], u[e], v[e]);
+                            u[e] = exp2_fast(u[e]);
+                            v[e] = exp2_fast(v[e]);
+                        }
+                        if constexpr (S::kCols == 128) {
+#pragma unroll
+                            for (int e = 3; e < kWords; e += 4) exp2_pair(x[e], u[e], v[e]);
+                        }
                         uint32_t w[kWords];
 #pragma unroll
                         for (int e = 0; e < kWords; ++e) {
-                            const float x = exp2_fast(fmaf(__uint_as_float(s[2 * (i + e)]), scale, -ref));
-                            const float y = exp2_fast(fmaf(__uint_as_float(s[2 * (i + e) + 1]), scale, -ref));
-                            part[(e & 1) * 2] += x;
-                            part[(e & 1) * 2 + 1] += y;
-                            w[e] = Pack<T>::pair(x, y);
+                            part[e & 1] = pair_add(part[e & 1], pair_of(u[e], v[e]));
+                            w[e] = Pack<T>::pair(u[e], v[e]);
                         }
                         tmem_store(p_at + i, w);
                     }
-                    sum = sum * keep + ((part[0] + part[1]) + (part[2] + part[3]));
+                    float x0, x1;
+                    unpair(pair_add(part[0], part[1]), x0, x1);
+                    sum = fmaf(sum, keep, x0 + x1);
                 }
                 tmem_stored();
                 began = true;
@@ -555,8 +642,24 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
                 return top_all;
             };
             float ref, total;
-            row_stats(my_row, &ref, &total);
+            const float top_all = row_stats(my_row, &ref, &total);
             const float factor = exp2_fast(m - ref);
+            // The rows that this thread puts together, four columns of each at a time.
+            constexpr int kEach = S::kRows / 32;
+            const int vec = tid & 7, streams = n_tiles > 1 ? 2 : 1;  // a segment of one tile has no second stream
+            int64_t to[kEach];
+            float inverse[kEach];  // -1: rows that are not shown
+#pragma unroll
+            for (int k = 0; k < kEach; ++k) {
+                const int r = (tid >> 3) + 32 * k;
+                if (r >= rows) break;
+                const RowId rid = row_id(a, row0 + r);
+                const int64_t rbk = static_cast<int64_t>(b) * a.beams + beam0 + rid.beam;
+                to[k] = ((rbk * a.N + rid.token) * a.Hq + p.head * a.G + rid.head) * c.D + vec * 4;
+                float unused, l_row;
+                row_stats(r, &unused, &l_row);
+                inverse[k] = rid.token < new_count(a, rbk) ? (l_row > 0.0f ? 1.0f / l_row : l_row) : -1.0f;
+            }
             float4* stage = reinterpret_cast<float4*>(query);  // [which][row][8], swizzled
 #pragma unroll 1
             for (int i = 0; i < DP / 32; ++i) {
@@ -570,9 +673,10 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
                                         __uint_as_float(o[4 * e + 2]) * factor, __uint_as_float(o[4 * e + 3]) * factor);
                 }
                 named_sync(1, kSoftThreads);
-                const int vec = tid & 7, streams = n_tiles > 1 ? 2 : 1;  // a segment of one tile has no second stream
-#pragma unroll 1
-                for (int r = tid >> 3; r < rows; r += kSoftThreads / 8) {
+#pragma unroll
+                for (int k = 0; k < kEach; ++k) {
+                    const int r = (tid >> 3) + 32 * k;
+                    if (r >= rows) break;
                     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
                     for (int j = 0; j < kParts; ++j) {
@@ -580,31 +684,19 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
                         const float4 x = stage[(j * S::kRows + r) * 8 + (vec ^ (r & 7))];
                         o.x += x.x, o.y += x.y, o.z += x.z, o.w += x.w;
                     }
-                    const float l_row = [&] {
-                        float f, t;
-                        row_stats(r, &f, &t);
-                        return t;
-                    }();
-                    if (i * 32 + vec * 4 < c.D) {
-                        if (whole) {
-                            const RowId rid = row_id(a, row0 + r);
-                            const int64_t rbk = static_cast<int64_t>(b) * a.beams + beam0 + rid.beam;
-                            const int64_t place = (rbk * a.N + rid.token) * a.Hq + p.head * a.G + rid.head;
-                            const bool shown = rid.token < new_count(a, rbk);
-                            const float inverse = l_row > 0.0f ? 1.0f / l_row : l_row;
-                            uint2 v = make_uint2(0, 0);
-                            if (shown)
-                                v = make_uint2(Pack<T>::pair(o.x * inverse, o.y * inverse), Pack<T>::pair(o.z * inverse, o.w * inverse));
-                            *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + place * c.D + i * 32 + vec * 4) = v;
-                        } else {
-                            *reinterpret_cast<float4*>(part + r * DP + i * 32 + vec * 4) = o;
-                        }
+                    if (i * 32 + vec * 4 >= c.D) continue;
+                    if (whole) {
+                        const float f = inverse[k];
+                        uint2 v = make_uint2(Pack<T>::pair(o.x * f, o.y * f), Pack<T>::pair(o.z * f, o.w * f));
+                        if (f == -1.0f) v = make_uint2(0, 0);
+                        *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + to[k] + i * 32) = v;
+                    } else {
+                        *reinterpret_cast<float4*>(part + r * DP + i * 32 + vec * 4) = o;
                     }
                 }
                 named_sync(1, kSoftThreads);
             }
             if (mine && which == 0) {
-                const float top_all = row_stats(my_row, &ref, &total);
                 if (whole) {
                     if (a.lse != nullptr)
                         a.lse[(bk * a.N + id.token) * a.Hq + p.head * a.G + id.head] =
@@ -618,15 +710,16 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
         if (whole) continue;
         __threadfence();
         named_sync(1, kSoftThreads);
+        const Span span = span_of(work, p);
         if (tid == 0) {
-            const int before = atomicAdd(counters + p.c0, 1);
-            ctl.last = before == p.c1 - p.c0;
-            if (ctl.last) counters[p.c0] = 0;
+            const int before = atomicAdd(counters + span.c0, 1);
+            ctl.last = before == span.c1 - span.c0;
+            if (ctl.last) counters[span.c0] = 0;
         }
         named_sync(1, kSoftThreads);
         if (!ctl.last) continue;
         __threadfence();
-        join_parts<T, S::kRows, DP, kSoftThreads>(c, a, p, b, beam0, row0, rows, parts, query, tid);
+        join_parts<T, S::kRows, DP, kSoftThreads>(c, a, p, span, b, beam0, row0, rows, parts, query, tid);
     }
     fence_before();
     named_sync(2, kSoftThreads + 32);
