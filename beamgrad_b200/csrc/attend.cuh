@@ -397,7 +397,7 @@ __device__ __forceinline__ void join_parts(const CacheView& c, const AttendParam
     }
     __syncwarp();
     asm volatile("barrier.sync 1, %0;" ::"r"(kThreads) : "memory");
-    constexpr int kEach = 8;
+    constexpr int kEach = kThreads > 256 ? 4 : 8;
     const int items = rows * kVecs;
 #pragma unroll 1
     for (int i0 = tid; i0 < items; i0 += kEach * kThreads) {

@@ -4,19 +4,18 @@
 // float16 and bfloat16 and heads of up to 128.
 //
 // 128 query rows by 128 positions at a time: S = Q K^T into tensor memory, the weights P back to
-// tensor memory, O += P V in tensor memory. One warp copies keys and values by TMA through a ring
-// of slots (a slot holds 128 rows of keys or of values), one thread issues the products, and two
-// warpgroups turn scores into weights, a thread a row: no maximum or sum crosses a thread. The
-// warpgroups and their P and O are two streams: the products of one run while the other takes
-// exponentials. S is one buffer for both. A warpgroup moves its scores to registers as soon as they
-// are there, and the next product may begin.
+// tensor memory in the place of S, O += P V in tensor memory. One warp copies keys and values by
+// TMA through a ring of slots (a slot holds 128 rows of keys or of values), one warp issues the
+// products, and the others turn scores into weights. S, P and O are two streams: the products of one
+// run while the other takes exponentials.
 //
 // NQ = 2 (more than 128 rows): each stream has query rows of its own, 256 a block, and takes every
 // tile, so that keys and values cross from L2 once for 256 rows. NQ = 1: both have the same rows and
-// take alternate tiles. With at most 64 (32) rows these lie in tensor memory 2 (4) times and each
-// copy weighs a half (a quarter) of the positions, with zeros for the others: the product costs the
-// same, and the chain from scores to weights is a half (a quarter) as long. Copies and streams are
-// joined at the end of a segment.
+// take alternate tiles. A stream of 128 rows has two warpgroups, each for a half of the positions (four
+// warps a scheduler; with two, the exponentials wait for their own latency). With at most 64 (32)
+// rows these lie in tensor memory 2 (4) times and each copy weighs a half (a quarter) of the
+// positions, with zeros for the others: the product costs the same, and the chain from scores to
+// weights is a half (a quarter) as long. Copies and streams are joined at the end of a segment.
 //
 // A row's reference for the exponentials is raised only when its maximum has grown by more than
 // 2^8: until then the weights stay below 2^8 and the sums within 32 bits, and O in tensor memory
@@ -29,16 +28,13 @@ namespace dbsb {
 namespace {
 
 constexpr int kTileKeys = 128;
-constexpr int kSoftThreads = 256;
-constexpr int kThreads = kSoftThreads + 128;  // and a warpgroup with the copying and the issuing warp
-constexpr int kCopyWarp = 8, kIssueWarp = 9;
 constexpr int kMaxSlots = 12;
 constexpr int kMinTiles = 1;     // tiles of a CTA at least
 constexpr float kRaise = 8.0f;  // log2 of the growth that a reference tolerates
 
 struct Control {
     uint64_t full[kMaxSlots], empty[kMaxSlots];
-    uint64_t queries, scores[2], loaded[2], weights[2], done[2];
+    uint64_t queries, scores[2], weights[2], output[2];
     WorkSplit split;
     int sums[34];
     uint32_t tmem;
@@ -48,13 +44,18 @@ struct Control {
         struct {
             float top[256], sum[256];       // at the end of a segment: [copy][row]
         };
+        float half[2][2][128];              // between a stream's warpgroups: [stream][half][row]
     };
 };
 
 template <int DP, int NQ, int COPIES>
 struct Shape {
     static constexpr int kRows = NQ == 2 ? 256 : 128 / COPIES;
-    static constexpr int kCols = 128 / COPIES;  // positions of a tile that a thread weighs
+    static constexpr int kHalves = COPIES == 1 ? 2 : 1;   // warpgroups of a stream
+    static constexpr int kCols = 128 / (COPIES * kHalves);  // positions of a tile that a thread weighs
+    static constexpr int kSoftThreads = 256 * kHalves;
+    static constexpr int kThreads = kSoftThreads + 128;   // and a warpgroup with the copying and the issuing warp
+    static constexpr int kCopyWarp = kSoftThreads / 32, kIssueWarp = kCopyWarp + 1;
     static constexpr int kBlocks = DP / 64;
     static constexpr int kSlot = kTileKeys * DP * 2;
     // The queries; at the end of a segment NQ = 1 joins its copies there, 256 x 32 floats.
@@ -93,37 +94,13 @@ __device__ __forceinline__ void product_ts(uint32_t d, uint32_t a, uint64_t b, u
 }
 #define REGS8(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]), "=r"(r[i + 7])
 #define REGS32(r, i) REGS8(r, i), REGS8(r, i + 8), REGS8(r, i + 16), REGS8(r, i + 24)
-// 32 (128) columns of the warp's 32 lanes, with the wait for them: a use of a register cannot move
+// 32 columns of the warp's 32 lanes, with the wait for them: a use of a register cannot move
 // before it.
 __device__ __forceinline__ void tmem_load(uint32_t (&r)[32], uint32_t at) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
         "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n tcgen05.wait::ld.sync.aligned;"
         : REGS32(r, 0)
-        : "r"(at)
-        : "memory");
-}
-__device__ __forceinline__ void tmem_load(uint32_t (&r)[64], uint32_t at) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
-        "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
-        "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];\n tcgen05.wait::ld.sync.aligned;"
-        : REGS32(r, 0), REGS32(r, 32)
-        : "r"(at)
-        : "memory");
-}
-__device__ __forceinline__ void tmem_load(uint32_t (&r)[128], uint32_t at) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x128.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
-        "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
-        "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63,"
-        "%64,%65,%66,%67,%68,%69,%70,%71,%72,%73,%74,%75,%76,%77,%78,%79,"
-        "%80,%81,%82,%83,%84,%85,%86,%87,%88,%89,%90,%91,%92,%93,%94,%95,"
-        "%96,%97,%98,%99,%100,%101,%102,%103,%104,%105,%106,%107,%108,%109,%110,%111,"
-        "%112,%113,%114,%115,%116,%117,%118,%119,%120,%121,%122,%123,%124,%125,%126,%127}, [%128];\n tcgen05.wait::ld.sync.aligned;"
-        : REGS32(r, 0), REGS32(r, 32), REGS32(r, 64), REGS32(r, 96)
         : "r"(at)
         : "memory");
 }
@@ -147,6 +124,17 @@ __device__ __forceinline__ void tmem_store(uint32_t at, const uint32_t (&r)[16])
         : "memory");
 }
 __device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Whether any thread of the named barrier says so.
+__device__ __forceinline__ bool named_any(int id, int threads, bool yes) {
+    uint32_t any;
+    asm volatile(
+        "{\n .reg .pred p, q;\n setp.ne.u32 p, %3, 0;\n barrier.red.or.pred q, %1, %2, p;\n selp.u32 %0, 1, 0, q;\n}\n"
+        : "=r"(any)
+        : "r"(id), "r"(threads), "r"(static_cast<uint32_t>(yes))
+        : "memory");
+    return any != 0;
+}
 
 // Shared-memory operand with 128-byte rows, swizzled: eight rows (1024 bytes) to the next eight
 // rows, and `blocks` bytes between 64-element blocks of an operand that runs along the row.
@@ -214,10 +202,12 @@ __device__ __forceinline__ void exp2_pair(Pair x2, float& a, float& b) {
 }
 
 template <class T, int DP, int NQ, int COPIES>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Shape<DP, NQ, COPIES>::kThreads, 1)
 attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ CacheView c,
                  const __grid_constant__ AttendParams a) {
     using S = Shape<DP, NQ, COPIES>;
+    constexpr int kHalves = S::kHalves, kSoftThreads = S::kSoftThreads, kThreads = S::kThreads;
+    constexpr int kCopyWarp = S::kCopyWarp, kIssueWarp = S::kIssueWarp;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* query = smem + S::kSlots * S::kSlot;
     Control& ctl = *reinterpret_cast<Control*>(query + S::kQuery);
@@ -232,9 +222,8 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
         }
         for (int i = 0; i < 2; ++i) {
             barrier_init(smem_address(&ctl.scores[i]), 1);
-            barrier_init(smem_address(&ctl.loaded[i]), 4);
-            barrier_init(smem_address(&ctl.weights[i]), 4);
-            barrier_init(smem_address(&ctl.done[i]), 1);
+            barrier_init(smem_address(&ctl.weights[i]), 4 * kHalves);
+            barrier_init(smem_address(&ctl.output[i]), 1);
         }
         barrier_init(smem_address(&ctl.queries), kSoftThreads / 32);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -255,13 +244,14 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
     }
     __syncthreads();
     fence_after();
-    const uint32_t tmem = ctl.tmem;  // columns: S 0..127, P of the streams 128.. and 192.., O 256.. and 384..
+    const uint32_t tmem = ctl.tmem;  // S of the streams, then O: 128 columns each
     int group = work.group;
     int64_t base = work.base;
 
-    // Registers: launched with 168 a thread; 2 x 128 x 216 + 128 x 72 = 384 x 168.
+    // Registers: 640 threads are launched with 96 each, 512 x 104 + 128 x 64 (384 have 168 each, which
+    // is enough for all roles).
     if (warp >= kCopyWarp) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if constexpr (kHalves == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
         if (warp > kIssueWarp) return;
         int used = 0;  // slots so far: K0 V0 K1 V1 ...
         if (warp == kCopyWarp) {
@@ -304,7 +294,7 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
                 barrier_wait(smem_address(&ctl.full[i % S::kSlots]), (i / S::kSlots) & 1, c.status);
         } else {
             constexpr uint32_t kScores = product_kind<T>(kTileKeys, false), kValues = product_kind<T>(DP, true);
-            uint32_t query_phase = 0, loaded_phase = 0, weight_phase = 0;  // a bit a stream
+            uint32_t query_phase = 0, weight_phase = 0;  // a bit a stream
             auto wait_slot = [&](int i) {
                 barrier_wait(smem_address(&ctl.full[i % S::kSlots]), (i / S::kSlots) & 1, c.status);
                 fence_after();
@@ -316,14 +306,11 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
                 query_phase ^= 1;
                 fence_after();
                 // Jobs: a stream and a tile. Two streams on every tile, or one stream a tile, in turn or
-                // always the first. The scores of job j + 2 are issued before the values of job j, so that
-                // they are there when job j's warpgroup is done with its weights.
+                // always the first.
                 const int per_tile = NQ == 2 && p.rows - p.block * S::kRows > 128 ? 2 : 1;
-                const int jobs = n * per_tile;
-                auto stream_of = [&](int j) { return NQ == 1 || per_tile == 2 ? j & 1 : 0; };
-                auto tile_of = [&](int j) { return per_tile == 2 ? j >> 1 : j; };
+                const int jobs = n * per_tile, streams = NQ == 1 ? 2 : per_tile;
                 auto scores = [&](int j) {
-                    const int stream = stream_of(j), slot = used + 2 * tile_of(j);
+                    const int stream = streams == 2 ? j & 1 : 0, slot = used + 2 * (per_tile == 2 ? j >> 1 : j);
                     if (per_tile == 1 || stream == 0) wait_slot(slot);
                     const uint64_t q = operand(smem_address(query) + (NQ == 2 ? stream * 128 * DP * 2 : 0), 16);
                     const uint64_t k = operand(slots + slot % S::kSlots * S::kSlot, 16);
@@ -331,44 +318,36 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
 #pragma unroll
                         for (int s = 0; s < DP / 16; ++s) {
                             const uint64_t at = ((s >> 2) * (128 * 128) + (s & 3) * 32) >> 4;
-                            product_ss(tmem, q + at, k + at, kScores, s > 0);
+                            product_ss(tmem + stream * 128, q + at, k + at, kScores, s > 0);
                         }
                         commit(smem_address(&ctl.scores[stream]));
                         if (per_tile == 1 || stream == 1) commit(smem_address(&ctl.empty[slot % S::kSlots]));
                     }
                     __syncwarp();
                 };
-                auto next_scores = [&](int j) {  // once job j - 1's scores are in registers
-                    const int before = stream_of(j - 1);
-                    if (j < jobs) {
-                        barrier_wait(smem_address(&ctl.loaded[before]), loaded_phase >> before & 1, c.status);
-                        fence_after();
-                        scores(j);
-                    }
-                    if (j <= jobs) loaded_phase ^= 1u << before;
-                };
                 scores(0);
-                next_scores(1);
+                if (streams == 2 && jobs > 1) scores(1);
 #pragma unroll 1
                 for (int j = 0; j < jobs; ++j) {
-                    const int stream = stream_of(j);
-                    next_scores(j + 2);
-                    const int slot = used + 2 * tile_of(j) + 1;
+                    const int stream = streams == 2 ? j & 1 : 0, slot = used + 2 * (per_tile == 2 ? j >> 1 : j) + 1;
                     if (per_tile == 1 || stream == 0) wait_slot(slot);
                     barrier_wait(smem_address(&ctl.weights[stream]), weight_phase >> stream & 1, c.status);
                     weight_phase ^= 1u << stream;
                     fence_after();
-                    const bool add = j >= (NQ == 1 ? 2 : per_tile);  // the stream's first job begins the sum
+                    const bool add = j >= streams;  // the stream's first job begins the sum
                     const uint64_t v = operand(slots + slot % S::kSlots * S::kSlot, kTileKeys * 128);
                     if (elected()) {
+                        // The weights of kCols positions lie at the front of those positions' scores.
 #pragma unroll
                         for (int s = 0; s < kTileKeys / 16; ++s)
-                            product_ts(tmem + 256 + stream * 128, tmem + 128 + stream * 64 + s * 8, v + s * ((16 * 128) >> 4),
-                                       kValues, add || s > 0);
-                        commit(smem_address(&ctl.done[stream]));
+                            product_ts(tmem + 256 + stream * 128,
+                                       tmem + stream * 128 + s * 16 / S::kCols * S::kCols + s * 16 % S::kCols / 2,
+                                       v + s * ((16 * 128) >> 4), kValues, add || s > 0);
                         if (per_tile == 1 || stream == 1) commit(smem_address(&ctl.empty[slot % S::kSlots]));
+                        if (j + streams >= jobs) commit(smem_address(&ctl.output[stream]));
                     }
                     __syncwarp();
+                    if (j + streams < jobs) scores(j + streams);
                 }
                 used += 2 * n;
                 cur += n;
@@ -380,25 +359,17 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
     }
 
     // Scores to weights.
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-    const int stream = warp >> 2, row = tid & 127;  // row of the stream's 128
-    const int my_row = NQ == 2 ? tid : row % S::kRows, copy = NQ == 2 ? 0 : row / S::kRows;
-    const int col0 = copy * S::kCols;  // the first position of a tile that the thread weighs
+    if constexpr (kHalves == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+    const int stream = warp / (4 * kHalves), half = kHalves == 2 ? (warp >> 2) & 1 : 0, row = tid & 127;  // of the stream's 128
+    const int my_row = NQ == 2 ? stream * 128 + row : row % S::kRows, copy = NQ == 2 ? 0 : row / S::kRows;
+    const int col0 = (kHalves == 2 ? half : copy) * S::kCols;  // the first position of a tile that the thread weighs
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t s_at = tmem + lanes + col0, p_at = tmem + lanes + 128 + stream * 64 + col0 / 2;
-    const uint32_t o_at = tmem + lanes + 256 + stream * 128;
-    const uint32_t scores_bar = smem_address(&ctl.scores[stream]), loaded_bar = smem_address(&ctl.loaded[stream]);
-    const uint32_t weights_bar = smem_address(&ctl.weights[stream]), done_bar = smem_address(&ctl.done[stream]);
+    const uint32_t s_at = tmem + lanes + stream * 128 + col0, o_at = tmem + lanes + 256 + stream * 128;
+    const uint32_t scores_bar = smem_address(&ctl.scores[stream]), weights_bar = smem_address(&ctl.weights[stream]);
     // Not 0, which would make a masked score's -inf a NaN.
     const float scale = fmaxf(fabsf(a.scale) * kLog2e, 1.2e-38f);
     const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;  // a negative scale turns the queries' signs
-    uint32_t score_phase = 0, done_phase = 0;
-    if constexpr (COPIES > 1) {  // the weights of other copies' positions stay zero
-        const uint32_t zero[32] = {};
-        tmem_store(tmem + lanes + 128 + stream * 64, zero);
-        tmem_store(tmem + lanes + 160 + stream * 64, zero);
-        tmem_stored();
-    }
+    uint32_t score_phase = 0, output_phase = 0;
     for (int64_t cur = work.lo; cur < work.hi;) {
         const Piece p = piece_at<S::kRows>(c, a, work, cur, group, base, tile_units);
         const int n_tiles = p.t1 - p.t0;
@@ -411,7 +382,7 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
         if (mine) id = row_id(a, row0 + my_row);
         // Both streams are done with the last segment's products, and so with its queries.
         named_sync(1, kSoftThreads);
-        if (NQ == 2 || (stream == 0 && copy == 0))
+        if (half == 0 && (NQ == 2 || (stream == 0 && copy == 0)))
             ctl.query_at[my_row] = b * a.qs[0] + (beam0 + id.beam) * a.qs[1] + id.token * a.qs[2] + (p.head * a.G + id.head) * a.qs[3];
         named_sync(1, kSoftThreads);
         load_queries<T, S::kRows, DP, kSoftThreads>(c, a, ctl.query_at, rows, tid, [&](int r, int chunk, uint4 v) {
@@ -440,6 +411,26 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
         const int first = NQ == 2 ? 0 : stream, step = NQ == 2 ? 1 : 2;
         bool began = false;
         if (active) {
+            // Tiles from the first on whose units are all complete and held by every row of the warp.
+            int plain_tiles = 0;
+            {
+                const int from = p.t0 * tile_units, to = p.t1 * tile_units < p.units ? p.t1 * tile_units : p.units;
+                int leading = 0;
+#pragma unroll 1
+                for (int i = from; i < to && leading == i - from; i += 128) {
+                    int4 v[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        v[k] = i + 32 * k + lane < to ? __ldg(reinterpret_cast<const int4*>(units + i + 32 * k + lane)) : make_int4(0, 0, 0, 0);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const bool whole = i + 32 * k + lane < to && v[k].w < 0 && (static_cast<uint32_t>(v[k].z) & need) == need;
+                        const uint32_t gaps = ~__ballot_sync(0xffffffffu, whole);
+                        if (leading == i - from + 32 * k) leading += gaps == 0 ? 32 : __ffs(gaps) - 1;
+                    }
+                }
+                plain_tiles = leading / tile_units;
+            }
             // A lane each; `other`: the unit has no position among the warp's.
             const bool other = (lane << c.page_log2) >= col0 + S::kCols || ((lane + 1) << c.page_log2) <= col0;
             auto unit_of = [&](int t) {
@@ -451,122 +442,153 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
                 }
                 return u;
             };
-            CacheUnit next = unit_of(first);
 #pragma unroll 1
             for (int t = first; t < n_tiles; t += step) {
-                const CacheUnit u = next;
-                next = unit_of(t + step);
-                const bool none = __all_sync(0xffffffffu, other || (u.mask & need) == 0);
-                const bool plain = __all_sync(0xffffffffu, other || (u.limit < 0 && (u.mask & need) == need));
+                CacheUnit u{-1, 0, 0, -1};
+                bool none = need == 0, plain = true;
+                if (t >= plain_tiles) {
+                    u = unit_of(t);
+                    none = __all_sync(0xffffffffu, other || (u.mask & need) == 0);
+                    plain = __all_sync(0xffffffffu, other || (u.limit < 0 && (u.mask & need) == need));
+                }
                 barrier_wait(scores_bar, score_phase, c.status);
                 score_phase ^= 1;
                 fence_after();
-                uint32_t s[S::kCols];
-                if (!none) tmem_load(s, s_at);
-                fence_before();
-                __syncwarp();
-                if (lane == 0) barrier_arrive(loaded_bar);
-                float keep = 1.0f;
+                constexpr int kChunks = S::kCols / 32;
+                uint32_t s[32], sees[kChunks];
+                float peak = -INFINITY;
                 if (!none) {
-                    if (!plain) {
+                    // The row's maximum. A NaN among the scores stays in it.
 #pragma unroll
-                        for (int i = 0; i < S::kCols / 16; ++i) {  // 16 positions lie in one unit
-                            const int from = (col0 + i * 16) >> c.page_log2;
-                            const uint32_t holders = __shfl_sync(0xffffffffu, u.mask, from);
-                            const int limit = __shfl_sync(0xffffffffu, u.limit, from);
-                            const int start = __shfl_sync(0xffffffffu, u.start, from) + ((col0 + i * 16) & (c.page - 1));
-                            const bool holds = (holders & bit) != 0;
-                            uint32_t sees = holds ? 0xffffu : 0u;
-                            if (limit >= 0) {
-                                // The holder's committed tokens end in this page: of the new ones behind them a
-                                // chain shows the first, a mask those that it names.
-                                const int old = limit - start;
-                                const int upto = old + (fresh ? 0 : (id.token < count ? id.token + 1 : count));
-                                if (upto < 16) sees &= upto > 0 ? (1u << upto) - 1 : 0u;
-                                if (fresh != nullptr && holds && old < 16 && old + count > 0) {
+                    for (int i = 0; i < kChunks; ++i) {
+                        tmem_load(s, s_at + 32 * i);
+                        if (!plain) {
+                            sees[i] = 0;
 #pragma unroll
-                                    for (int e = 0; e < 16; ++e)
-                                        if (e >= old && e - old < count) sees |= (fresh[e - old] != 0 ? 1u : 0u) << e;
+                            for (int h = 0; h < 2; ++h) {  // 16 positions lie in one unit
+                                const int col = col0 + 32 * i + 16 * h, from = col >> c.page_log2;
+                                const uint32_t holders = __shfl_sync(0xffffffffu, u.mask, from);
+                                const int limit = __shfl_sync(0xffffffffu, u.limit, from);
+                                const int start = __shfl_sync(0xffffffffu, u.start, from) + (col & (c.page - 1));
+                                const bool holds = (holders & bit) != 0;
+                                uint32_t bits = holds ? 0xffffu : 0u;
+                                if (limit >= 0) {
+                                    // The holder's committed tokens end in this page: of the new ones behind them
+                                    // a chain shows the first, a mask those that it names.
+                                    const int old = limit - start;
+                                    const int upto = old + (fresh ? 0 : (id.token < count ? id.token + 1 : count));
+                                    if (upto < 16) bits &= upto > 0 ? (1u << upto) - 1 : 0u;
+                                    if (fresh != nullptr && holds && old < 16 && old + count > 0) {
+#pragma unroll
+                                        for (int e = 0; e < 16; ++e)
+                                            if (e >= old && e - old < count) bits |= (fresh[e - old] != 0 ? 1u : 0u) << e;
+                                    }
                                 }
+                                sees[i] |= bits << (16 * h);
                             }
 #pragma unroll
-                            for (int e = 0; e < 16; ++e)
-                                if ((sees >> e & 1) == 0) s[i * 16 + e] = 0xff800000u;
+                            for (int e = 0; e < 32; ++e)
+                                if ((sees[i] >> e & 1) == 0) s[e] = 0xff800000u;
                         }
-                    }
-                    // A NaN among the scores stays in the maximum.
-                    float most[4];
+                        float most[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) most[e] = __uint_as_float(s[e]);
+                        for (int e = 0; e < 4; ++e) most[e] = __uint_as_float(s[e]);
 #pragma unroll
-                    for (int e = 4; e + 1 < S::kCols; e += 2)
-                        most[(e >> 1) & 3] = max3(most[(e >> 1) & 3], __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
-                    const float now = max3(max3(most[0], most[1], most[2]), most[3], most[3]);
-                    if (now != -INFINITY && !((now - top) * scale <= kRaise)) {
-                        keep = exp2_fast((top - now) * scale);
-                        top = now;
+                        for (int e = 4; e + 1 < 32; e += 2)
+                            most[(e >> 1) & 3] = max3(most[(e >> 1) & 3], __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
+                        peak = max3(peak, max3(most[0], most[1], most[2]), most[3]);
                     }
                 }
-                if (began) {  // P and O are this thread's again once the last weights' product is done
-                    barrier_wait(done_bar, done_phase, c.status);
-                    done_phase ^= 1;
-                    fence_after();
-                    if (__any_sync(0xffffffffu, keep != 1.0f)) {
-#pragma unroll 1
-                        for (int i = 0; i < DP / 32; ++i) {
-                            uint32_t o[32];
-                            tmem_load(o, o_at + 32 * i);
-#pragma unroll
-                            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
-                            tmem_store(o_at + 32 * i, o);
-                        }
+                // Whether the row's reference is to be raised, and for the halves of a stream to what.
+                bool raise_it = peak != -INFINITY && !((peak - top) * scale <= kRaise);
+                bool any_raised;
+                if constexpr (kHalves == 2) {
+                    any_raised = named_any(3 + stream, 256, raise_it);
+                    if (any_raised) {
+                        ctl.half[stream][half][row] = peak;
+                        named_sync(3 + stream, 256);
+                        const float its = ctl.half[stream][half ^ 1][row];
+                        peak = max3(peak, its, its);
+                        raise_it = peak != -INFINITY && !((peak - top) * scale <= kRaise);
+                        named_sync(3 + stream, 256);
                     }
-                }
-                constexpr int kWords = 16;  // pairs of weights stored at a time
-                if (none) {
-                    // No row of the warp sees any of it.
-                    uint32_t w[kWords];
-#pragma unroll
-                    for (int e = 0; e < kWords; ++e) w[e] = 0;
-#pragma unroll
-                    for (int i = 0; i < S::kCols / 2; i += kWords) tmem_store(p_at + i, w);
                 } else {
-                    // Nothing seen yet: any reference gives weights of 0. A maximum that is inf or NaN gives NaN.
-                    const float ref = top == -INFINITY ? 0.0f : (top < INFINITY ? top * scale : NAN);
-                    const Pair scale2 = pair_of(scale, scale), ref2 = pair_of(-ref, -ref);
-                    Pair part[2] = {pair_of(0.0f, 0.0f), pair_of(0.0f, 0.0f)};
+                    any_raised = __any_sync(0xffffffffu, raise_it);
+                }
+                if (any_raised) {
+                    float keep = 1.0f;
+                    if (raise_it) {
+                        keep = exp2_fast((top - peak) * scale);
+                        top = peak;
+                        sum *= keep;
+                    }
+                    // (The products so far are done: these scores were issued behind them.)
+#pragma unroll 1
+                    for (int i = half * (DP / 32 / kHalves); began && i < (half + 1) * (DP / 32 / kHalves); ++i) {
+                        uint32_t o[32];
+                        tmem_load(o, o_at + 32 * i);
 #pragma unroll
-                    for (int i = 0; i < S::kCols / 2; i += kWords) {
-                        // In stages over 16 pairs: a result is not used before its latency is over.
-                        Pair x[kWords];
-                        float u[kWords], v[kWords];
+                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+                        tmem_store(o_at + 32 * i, o);
+                    }
+                }
+                // Nothing seen yet: any reference gives weights of 0. A maximum that is inf or NaN gives NaN.
+                const float ref = top == -INFINITY ? 0.0f : (top < INFINITY ? top * scale : NAN);
+                const Pair scale2 = pair_of(scale, scale), ref2 = pair_of(-ref, -ref);
+                Pair part[2] = {pair_of(0.0f, 0.0f), pair_of(0.0f, 0.0f)};
 #pragma unroll
-                        for (int e = 0; e < kWords; ++e)
-                            x[e] = pair_fma(pair_of(__uint_as_float(s[2 * (i + e)]), __uint_as_float(s[2 * (i + e) + 1])), scale2,
-                                            ref2);
+                for (int i = 0; i < kChunks; ++i) {
+                    uint32_t w[16];
+                    if (none) {
+                        // No row of the warp sees any of it.
 #pragma unroll
-                        for (int e = 0; e < kWords; ++e) {
-                            if (S::kCols == 128 && e % 4 == 3) continue;
+                        for (int e = 0; e < 16; ++e) w[e] = 0;
+                    } else {
+                        if (kChunks > 1) {
+                            tmem_load(s, s_at + 32 * i);
+                            if (!plain) {
+#pragma unroll
+                                for (int e = 0; e < 32; ++e)
+                                    if ((sees[i] >> e & 1) == 0) s[e] = 0xff800000u;
+                            }
+                        }
+                        // In stages: a result is not used before its latency is over.
+                        Pair x[16];
+                        float u[16], v[16];
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            x[e] = pair_fma(pair_of(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), scale2, ref2);
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            if (COPIES == 1 && e % 4 == 3) continue;
                             unpair(x[e], u[e], v[e]);
                             u[e] = exp2_fast(u[e]);
                             v[e] = exp2_fast(v[e]);
                         }
-                        if constexpr (S::kCols == 128) {
+                        if constexpr (COPIES == 1) {
 #pragma unroll
-                            for (int e = 3; e < kWords; e += 4) exp2_pair(x[e], u[e], v[e]);
+                            for (int e = 3; e < 16; e += 4) exp2_pair(x[e], u[e], v[e]);
                         }
-                        uint32_t w[kWords];
 #pragma unroll
-                        for (int e = 0; e < kWords; ++e) {
+                        for (int e = 0; e < 16; ++e) {
                             part[e & 1] = pair_add(part[e & 1], pair_of(u[e], v[e]));
                             w[e] = Pack<T>::pair(u[e], v[e]);
                         }
-                        tmem_store(p_at + i, w);
                     }
-                    float x0, x1;
-                    unpair(pair_add(part[0], part[1]), x0, x1);
-                    sum = fmaf(sum, keep, x0 + x1);
+                    tmem_store(s_at + 16 * i, w);
                 }
+                if constexpr (COPIES > 1) {  // the weights of the other copies' positions
+                    const uint32_t zero[16] = {};
+#pragma unroll 1
+                    for (int g = 0; g < COPIES; ++g) {
+                        if (g == copy) continue;
+#pragma unroll
+                        for (int i = 0; i < kChunks; ++i) tmem_store(tmem + lanes + stream * 128 + g * S::kCols + 16 * i, zero);
+                    }
+                }
+                float x0, x1;
+                unpair(pair_add(part[0], part[1]), x0, x1);
+                sum += x0 + x1;
                 tmem_stored();
                 began = true;
                 fence_before();
@@ -574,8 +596,8 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
                 if (lane == 0) barrier_arrive(weights_bar);
             }
             if (began) {
-                barrier_wait(done_bar, done_phase, c.status);
-                done_phase ^= 1;
+                barrier_wait(smem_address(&ctl.output[stream]), output_phase, c.status);
+                output_phase ^= 1;
                 fence_after();
             }
         }
@@ -587,12 +609,18 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
         float* part = parts + static_cast<int64_t>(2 * blockIdx.x + (p.t0 == 0)) * S::kOut;
         float m = top == -INFINITY ? top : top * scale, l = sum;  // base-2 maximum, sum
         const bool holds_rows = began && (my_row & ~31) < rows;   // of the warp
+        if constexpr (kHalves == 2) {
+            named_sync(1, kSoftThreads);  // (query_at shares the space)
+            ctl.half[stream][half][row] = l;
+            named_sync(1, kSoftThreads);
+            l += ctl.half[stream][half ^ 1][row];
+        }
         if constexpr (NQ == 2) {
             const float inverse = l > 0.0f ? 1.0f / l : l;
             const int64_t place = (bk * a.N + id.token) * a.Hq + p.head * a.G + id.head;
             T* out = static_cast<T*>(a.out) + place * c.D;
 #pragma unroll 1
-            for (int i = 0; i < DP / 32; ++i) {
+            for (int i = half * (DP / 64); i < (half + 1) * (DP / 64); ++i) {
                 uint32_t o[32];
                 if (holds_rows) tmem_load(o, o_at + 32 * i);
                 if (!mine) continue;
@@ -615,7 +643,7 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
                             make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
                 }
             }
-            if (mine) {
+            if (mine && half == 0) {
                 if (whole) {
                     if (a.lse != nullptr) a.lse[place] = live && l != 0.0f ? (m + log2f(l)) * kLn2 : -INFINITY;
                 } else {
@@ -645,13 +673,13 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
             const float top_all = row_stats(my_row, &ref, &total);
             const float factor = exp2_fast(m - ref);
             // The rows that this thread puts together, four columns of each at a time.
-            constexpr int kEach = S::kRows / 32;
+            constexpr int kEach = S::kRows * 8 / kSoftThreads;
             const int vec = tid & 7, streams = n_tiles > 1 ? 2 : 1;  // a segment of one tile has no second stream
             int64_t to[kEach];
             float inverse[kEach];  // -1: rows that are not shown
 #pragma unroll
             for (int k = 0; k < kEach; ++k) {
-                const int r = (tid >> 3) + 32 * k;
+                const int r = (tid >> 3) + kSoftThreads / 8 * k;
                 if (r >= rows) break;
                 const RowId rid = row_id(a, row0 + r);
                 const int64_t rbk = static_cast<int64_t>(b) * a.beams + beam0 + rid.beam;
@@ -663,7 +691,7 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
             float4* stage = reinterpret_cast<float4*>(query);  // [which][row][8], swizzled
 #pragma unroll 1
             for (int i = 0; i < DP / 32; ++i) {
-                if (holds_rows) {
+                if (holds_rows && (kHalves == 1 || half == (i & 1))) {
                     uint32_t o[32];
                     tmem_load(o, o_at + 32 * i);
 #pragma unroll
@@ -675,7 +703,7 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
                 named_sync(1, kSoftThreads);
 #pragma unroll
                 for (int k = 0; k < kEach; ++k) {
-                    const int r = (tid >> 3) + 32 * k;
+                    const int r = (tid >> 3) + kSoftThreads / 8 * k;
                     if (r >= rows) break;
                     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
@@ -696,7 +724,7 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
                 }
                 named_sync(1, kSoftThreads);
             }
-            if (mine && which == 0) {
+            if (mine && which == 0 && half == 0) {
                 if (whole) {
                     if (a.lse != nullptr)
                         a.lse[(bk * a.N + id.token) * a.Hq + p.head * a.G + id.head] =
@@ -733,7 +761,7 @@ cudaError_t launch_shape(const CacheView& c, const CUtensorMap& map, const Atten
     auto* kernel = attend_tc_kernel<T, DP, NQ, COPIES>;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes);
     if (e != cudaSuccess) return e;
-    return launch_after(kernel, sm_count, kThreads, S::kBytes, stream, map, c, a);
+    return launch_after(kernel, sm_count, S::kThreads, S::kBytes, stream, map, c, a);
 }
 
 template <class T, int DP>
