@@ -9,7 +9,6 @@ namespace dbsb {
 namespace {
 
 constexpr int kAppendThreads = 256;
-constexpr int kRowThreads = 128;
 
 // Keys and values of the new tokens into their pages, 16 bytes a thread. A value that is not
 // finite raises the cache's second status word: the attention then keeps masked values out of its
@@ -50,42 +49,28 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
     }
 }
 
-// One warp a query row.
 template <class T>
-__global__ void __launch_bounds__(kRowThreads) rows_kernel(const __grid_constant__ CacheView c, const __grid_constant__ AttendParams a) {
-    __shared__ float query[kRowThreads / 32 * DBS_CUDA_CACHE_MAX_HEAD_DIM];
-    grid_wait();
-    attend_all_rows<T>(c, a, query, threadIdx.x >> 5, kRowThreads / 32);
-}
-
-template <class T>
-cudaError_t launch_typed(const CacheView& c, int dtype, const AttendParams& a, int sm_count, cudaStream_t stream) {
-    const int64_t cap = static_cast<int64_t>(sm_count) * 8;
-    if (a.k != nullptr) {
-        const int64_t items = static_cast<int64_t>(c.B) * a.beams * a.N * c.H * (c.D / Pack<T>::n);
-        const int64_t want = (items + kAppendThreads - 1) / kAppendThreads;
-        const cudaError_t e = launch_after(append_kernel<T>, static_cast<unsigned>(want < cap ? want : cap),
-                                           kAppendThreads, 0, stream, c, a);
-        if (e != cudaSuccess) return e;
-    }
-    if constexpr (sizeof(T) == 2)
-        return c.D <= 128 ? launch_attend_tc(c, dtype, a, sm_count, stream) : launch_attend_mma(c, dtype, a, sm_count, stream);
-    const int64_t rows = static_cast<int64_t>(c.B) * a.beams * a.N * a.Hq;
-    return launch_after(rows_kernel<T>, static_cast<unsigned>((rows + kRowThreads / 32 - 1) / (kRowThreads / 32)),
-                        kRowThreads, 0, stream, c, a);
+cudaError_t launch_append(const CacheView& c, const AttendParams& a, int sm_count, cudaStream_t stream) {
+    if (a.k == nullptr) return cudaSuccess;
+    const int64_t items = static_cast<int64_t>(c.B) * a.beams * a.N * c.H * (c.D / Pack<T>::n);
+    const int64_t want = (items + kAppendThreads - 1) / kAppendThreads, cap = static_cast<int64_t>(sm_count) * 8;
+    return launch_after(append_kernel<T>, static_cast<unsigned>(want < cap ? want : cap), kAppendThreads, 0, stream, c, a);
 }
 
 }  // namespace
 
 int64_t attend_workspace(const CacheView& c, const AttendParams& a, int sm_count) {
-    if (c.elem == 4) return 256;
+    if (c.elem == 4) return attend_f32_workspace(c, a, sm_count);
     return c.D <= 128 ? attend_tc_workspace(c, a, sm_count) : attend_mma_workspace(c, a, sm_count);
 }
 
 cudaError_t launch_attend(const CacheView& c, int dtype, const AttendParams& a, int sm_count, cudaStream_t stream) {
-    if (dtype == DBS_CUDA_DTYPE_F32) return launch_typed<float>(c, dtype, a, sm_count, stream);
-    if (dtype == DBS_CUDA_DTYPE_F16) return launch_typed<__half>(c, dtype, a, sm_count, stream);
-    return launch_typed<__nv_bfloat16>(c, dtype, a, sm_count, stream);
+    const cudaError_t e = dtype == DBS_CUDA_DTYPE_F32 ? launch_append<float>(c, a, sm_count, stream)
+                          : dtype == DBS_CUDA_DTYPE_F16 ? launch_append<__half>(c, a, sm_count, stream)
+                                                        : launch_append<__nv_bfloat16>(c, a, sm_count, stream);
+    if (e != cudaSuccess) return e;
+    if (dtype == DBS_CUDA_DTYPE_F32) return launch_attend_f32(c, a, sm_count, stream);
+    return c.D <= 128 ? launch_attend_tc(c, dtype, a, sm_count, stream) : launch_attend_mma(c, dtype, a, sm_count, stream);
 }
 
 }  // namespace dbsb

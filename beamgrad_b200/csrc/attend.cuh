@@ -65,6 +65,11 @@ template <> struct Pack<__nv_bfloat16> {
     }
 };
 
+// Four consecutive elements.
+__device__ __forceinline__ void store4(float* to, float4 v) { *reinterpret_cast<float4*>(to) = v; }
+template <class T> __device__ __forceinline__ void store4(T* to, float4 v) {
+    *reinterpret_cast<uint2*>(to) = make_uint2(Pack<T>::pair(v.x, v.y), Pack<T>::pair(v.z, v.w));
+}
 template <class T> __device__ __forceinline__ float to_float(T x) { return static_cast<float>(x); }
 template <class T> __device__ __forceinline__ T from_float(float x) { return static_cast<T>(x); }
 
@@ -428,9 +433,9 @@ __device__ __forceinline__ void join_parts(const CacheView& c, const AttendParam
             if (i >= items) break;
             if (vec * 4 >= c.D) continue;
             const float f = factors[r];
-            uint2 packed = make_uint2(Pack<T>::pair(o[e].x * f, o[e].y * f), Pack<T>::pair(o[e].z * f, o[e].w * f));
-            if (f == -1.0f) packed = make_uint2(0, 0);
-            reinterpret_cast<uint2*>(static_cast<T*>(a.out) + places[r] * c.D)[vec] = packed;
+            float4 y = make_float4(o[e].x * f, o[e].y * f, o[e].z * f, o[e].w * f);
+            if (f == -1.0f) y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            store4(static_cast<T*>(a.out) + places[r] * c.D + vec * 4, y);
         }
     }
 }
@@ -485,6 +490,8 @@ __device__ __forceinline__ void tma_load(uint32_t to, const CUtensorMap* map, in
 // that eight rows of 128 bytes cover all banks. False: the driver refused it.
 bool page_map(const CacheView& c, int dtype, CUtensorMap* map);
 
+int64_t attend_f32_workspace(const CacheView& c, const AttendParams& a, int sm_count);
+cudaError_t launch_attend_f32(const CacheView& c, const AttendParams& a, int sm_count, cudaStream_t stream);
 int64_t attend_tc_workspace(const CacheView& c, const AttendParams& a, int sm_count);
 cudaError_t launch_attend_tc(const CacheView& c, int dtype, const AttendParams& a, int sm_count, cudaStream_t stream);
 int64_t attend_mma_workspace(const CacheView& c, const AttendParams& a, int sm_count);

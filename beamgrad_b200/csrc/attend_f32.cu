@@ -1,0 +1,325 @@
+// SPDX-License-Identifier: MIT
+//
+// Attention over the paged cache in float32, on the multiply-add pipe: the tensor cores would round
+// the operands to 11 bits.
+//
+// Blocks of 8, 16 or 32 query rows by tiles of 64 positions (32 for heads above 128), copied by
+// cp.async, the next tile while this one is worked on. Both products run on register tiles of up to
+// 4 x 4, for which a warp's eight shared-memory reads of 16 bytes an element group (each one pass of
+// the banks: rows are padded by 16 bytes) feed 64 multiply-adds. At 32 rows of 128 that is 4096
+// cycles a tile and SM, at 12 rows (2048) the bytes bound it (2800 cycles).
+#include "attend.cuh"
+
+namespace dbsb {
+
+namespace {
+
+constexpr int kThreads = 256;
+
+template <int DP, int RT>
+struct Shape {
+    static constexpr int kRows = 8 * RT;
+    static constexpr int kKeys = DP > 128 ? 32 : 64;
+    static constexpr int kPitch = DP + 4;           // floats of a staged row
+    static constexpr int kSplit = 128 / kKeys;      // parts of the head that the scores' sums are taken in
+    static constexpr int kScorePitch = kKeys + 4;
+    static constexpr int kStage = 2 * kKeys * kPitch;  // floats: keys, values
+    static constexpr int kScores = kRows * kScorePitch;
+    static constexpr int kCols = (DP + 127) / 128;  // groups of four columns that a thread has of the output
+    static constexpr int kBytes = (2 * kStage + kSplit * kScores + kRows * kPitch) * 4;
+    static constexpr int kOut = kRows * (DP + 2);
+};
+
+struct Control {
+    int sums[34];
+    WorkSplit split;
+    CacheUnit unit[2][4];
+    int64_t query_at[32];
+    float factor[32], top[32], sum[32];
+    int last;
+};
+
+__device__ __forceinline__ void copy16(float* to, const float* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_address(to)), "l"(from) : "memory");
+}
+
+template <int DP, int RT>
+__global__ void __launch_bounds__(kThreads, 1)
+attend_f32_kernel(const __grid_constant__ CacheView c, const __grid_constant__ AttendParams a) {
+    using S = Shape<DP, RT>;
+    extern __shared__ __align__(16) float smem[];
+    __shared__ Control ctl;
+    float* stages = smem;
+    float* scores = stages + 2 * S::kStage;          // [kSplit][kRows][kScorePitch]; the weights in the first
+    float* query = scores + S::kSplit * S::kScores;  // [kRows][kPitch]
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int tile_units = S::kKeys >> c.page_log2 > 0 ? S::kKeys >> c.page_log2 : 1;
+    const int page_tiles = c.page > S::kKeys ? c.page / S::kKeys : 1;  // tiles of a page (64 by tiles of 32)
+
+    const WorkSplit work = split_work<S::kRows>(c, a, tile_units, 1, ctl.sums, &ctl.split);
+    grid_wait();
+    grid_release();
+    if (__ldcg(c.status + 1) != 0) {
+        attend_all_rows<float>(c, a, smem, warp, kThreads / 32);
+        return;
+    }
+    int group = work.group;
+    int64_t base = work.base;
+    const float scale = a.scale * kLog2e;
+    const int vecs = c.D / 4;
+    // Scores: a warp has 4 * RT rows by 32 positions (a thread RT rows, 4 positions 8 apart) of one part
+    // of the head.
+    const int row_half = warp & 1, key_half = S::kKeys == 64 ? (warp >> 1) & 1 : 0;
+    const int part = S::kKeys == 64 ? warp >> 2 : warp >> 1;
+    const int s_row = row_half * 4 * RT + (lane >> 3) * RT, s_key = key_half * 32 + (lane & 7);
+    // Weights: kThreads / kRows threads a row. Output: RT rows, four columns (and four more 128 on).
+    constexpr int kPerRow = kThreads / S::kRows, kEach = S::kKeys / kPerRow;
+    const int w_row = tid / kPerRow, w_key = tid % kPerRow;
+    const int o_row = warp * RT;
+
+    for (int64_t cur = work.lo; cur < work.hi;) {
+        const Piece p = piece_at<S::kRows>(c, a, work, cur, group, base, tile_units);
+        const int n_tiles = (p.t1 - p.t0) * page_tiles;
+        cur += p.t1 - p.t0;
+        const int b = p.group / c.groups, beam0 = (p.group - b * c.groups) * kGroupBeams;
+        const int row0 = p.block * S::kRows;
+        const int rows = p.rows - row0 < S::kRows ? p.rows - row0 : S::kRows;
+        const CacheUnit* units = c.units + static_cast<int64_t>(p.group) * c.unit_cap;
+        __syncthreads();
+        if (tid < rows) {
+            const RowId id = row_id(a, row0 + tid);
+            ctl.query_at[tid] = b * a.qs[0] + (beam0 + id.beam) * a.qs[1] + id.token * a.qs[2] + (p.head * a.G + id.head) * a.qs[3];
+        }
+        __syncthreads();
+        for (int i = tid; i < S::kRows * (DP / 4); i += kThreads) {
+            const int r = i / (DP / 4), v = i % (DP / 4);
+            float4 q = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (r < rows && v < vecs) q = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + ctl.query_at[r]) + v);
+            *reinterpret_cast<float4*>(query + r * S::kPitch + v * 4) = q;
+        }
+        // Tile t: kKeys positions of its units' pages; past the last unit page 0, whatever finite values
+        // lie there meet weights of zero.
+        auto fetch = [&](int t) {
+            float* stage = stages + (t & 1) * S::kStage;
+            const int first = (p.t0 + t / page_tiles) * tile_units, offset = t % page_tiles * S::kKeys;
+            if (tid < tile_units) {
+                CacheUnit u{-1, 0, 0, -1};
+                if (first + tid < p.units) {
+                    const int4 v = __ldg(reinterpret_cast<const int4*>(units + first + tid));
+                    u = CacheUnit{v.x, v.y + offset, static_cast<uint32_t>(v.z), v.w};
+                }
+                ctl.unit[t & 1][tid] = u;
+            }
+            for (int i = tid; i < 2 * S::kKeys * (DP / 4); i += kThreads) {
+                const int v = i % (DP / 4), key = i / (DP / 4) % S::kKeys, kind = i / (DP / 4 * S::kKeys);
+                if (v >= vecs) continue;
+                const int unit = first + (key >> c.page_log2), at = (key + offset) & (c.page - 1);
+                const int page = unit < p.units ? __ldg(&units[unit].page) : 0;
+                const int64_t row = ((((static_cast<int64_t>(a.layer) * 2 + kind) * c.P + page) * c.H + p.head) << c.page_log2) + at;
+                copy16(stage + (kind * S::kKeys + key) * S::kPitch + v * 4, static_cast<const float*>(c.pages) + row * c.D + v * 4);
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        // The row that this thread weighs.
+        RowId id{0, 0, 0};
+        if (w_row < rows) id = row_id(a, row0 + w_row);
+        const int64_t bk = static_cast<int64_t>(b) * a.beams + beam0 + id.beam;
+        const int count = w_row < rows ? new_count(a, bk) : 0;
+        const bool live = w_row < rows && id.token < count;
+        const uint32_t bit = live ? 1u << id.beam : 0u;
+        const uint8_t* fresh = a.mask ? a.mask + (bk * a.N + id.token) * a.N : nullptr;
+        float top = -INFINITY, sum = 0.0f;
+        float4 acc[S::kCols][RT];
+#pragma unroll
+        for (int j = 0; j < S::kCols; ++j)
+#pragma unroll
+            for (int r = 0; r < RT; ++r) acc[j][r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+
+        fetch(0);
+        for (int t = 0; t < n_tiles; ++t) {
+            if (t + 1 < n_tiles) {
+                fetch(t + 1);
+                asm volatile("cp.async.wait_group 1;" ::: "memory");
+            } else {
+                asm volatile("cp.async.wait_group 0;" ::: "memory");
+            }
+            __syncthreads();
+            const float* keys = stages + (t & 1) * S::kStage;
+            const float* values = keys + S::kKeys * S::kPitch;
+            {
+                float s[RT][4];
+#pragma unroll
+                for (int r = 0; r < RT; ++r)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) s[r][k] = 0.0f;
+#pragma unroll 2
+                for (int v = part; v < vecs; v += S::kSplit) {
+                    float4 q[RT], x[4];
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) q[r] = *reinterpret_cast<const float4*>(query + (s_row + r) * S::kPitch + v * 4);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) x[k] = *reinterpret_cast<const float4*>(keys + (s_key + 8 * k) * S::kPitch + v * 4);
+#pragma unroll
+                    for (int r = 0; r < RT; ++r)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            s[r][k] = fmaf(q[r].w, x[k].w, fmaf(q[r].z, x[k].z, fmaf(q[r].y, x[k].y, fmaf(q[r].x, x[k].x, s[r][k]))));
+                }
+#pragma unroll
+                for (int r = 0; r < RT; ++r)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) scores[part * S::kScores + (s_row + r) * S::kScorePitch + s_key + 8 * k] = s[r][k];
+            }
+            __syncthreads();
+            {
+                float x[kEach];
+                float now = -INFINITY;
+#pragma unroll
+                for (int e = 0; e < kEach; ++e) {
+                    const int key = w_key + kPerRow * e;
+                    float v = scores[w_row * S::kScorePitch + key];
+#pragma unroll
+                    for (int i = 1; i < S::kSplit; ++i) v += scores[i * S::kScores + w_row * S::kScorePitch + key];
+                    const CacheUnit u = ctl.unit[t & 1][key >> c.page_log2];
+                    bool sees = (u.mask & bit) != 0;
+                    const int j = u.start + (key & (c.page - 1)) - u.limit;
+                    if (sees && u.limit >= 0 && j >= 0) sees = j < count && (fresh ? fresh[j] != 0 : j <= id.token);
+                    x[e] = sees ? v * scale : -INFINITY;
+                    now = fmaxf(now, x[e]);
+                }
+#pragma unroll
+                for (int m = kPerRow / 2; m > 0; m >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, m));
+                now = fmaxf(now, top);
+                const float ref = now == -INFINITY ? 0.0f : now;
+                const float keep = exp2_fast(top - ref);
+                top = now;
+                sum *= keep;
+#pragma unroll
+                for (int e = 0; e < kEach; ++e) {
+                    const float w = exp2_fast(x[e] - ref);
+                    sum += w;
+                    scores[w_row * S::kScorePitch + w_key + kPerRow * e] = w;
+                }
+                if (w_key == 0) ctl.factor[w_row] = keep;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                const float f = ctl.factor[o_row + r];
+#pragma unroll
+                for (int j = 0; j < S::kCols; ++j) acc[j][r].x *= f, acc[j][r].y *= f, acc[j][r].z *= f, acc[j][r].w *= f;
+            }
+#pragma unroll
+            for (int j = 0; j < S::kCols; ++j) {
+                const int col = lane + 32 * j;
+                if (col >= vecs) break;
+#pragma unroll 2
+                for (int k = 0; k < S::kKeys; k += 4) {
+                    float4 w[RT], x[4];
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) w[r] = *reinterpret_cast<const float4*>(scores + (o_row + r) * S::kScorePitch + k);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const float4*>(values + (k + i) * S::kPitch + col * 4);
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) {
+                        const float y[4] = {w[r].x, w[r].y, w[r].z, w[r].w};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            acc[j][r].x = fmaf(y[i], x[i].x, acc[j][r].x), acc[j][r].y = fmaf(y[i], x[i].y, acc[j][r].y);
+                            acc[j][r].z = fmaf(y[i], x[i].z, acc[j][r].z), acc[j][r].w = fmaf(y[i], x[i].w, acc[j][r].w);
+                        }
+                    }
+                }
+            }
+            __syncthreads();
+        }
+        // To the output, or to this CTA's part of a divided segment.
+#pragma unroll
+        for (int m = kPerRow / 2; m > 0; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
+        if (w_key == 0) {
+            ctl.top[w_row] = top;
+            ctl.sum[w_row] = sum;
+        }
+        __syncthreads();
+        const bool whole = p.t0 == 0 && p.t1 == p.tiles;
+        float* parts = static_cast<float*>(a.workspace) + 2048;
+        int32_t* counters = static_cast<int32_t*>(a.workspace);
+        float* out_part = parts + static_cast<int64_t>(2 * blockIdx.x + (p.t0 == 0)) * S::kOut;
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            if (o_row + r >= rows) break;
+            const RowId rid = row_id(a, row0 + o_row + r);
+            const int64_t rbk = static_cast<int64_t>(b) * a.beams + beam0 + rid.beam;
+            const int64_t place = (rbk * a.N + rid.token) * a.Hq + p.head * a.G + rid.head;
+            const bool shown = rid.token < new_count(a, rbk);
+            const float m = ctl.top[o_row + r], l = ctl.sum[o_row + r];
+            const float inverse = l > 0.0f ? 1.0f / l : l;
+#pragma unroll
+            for (int j = 0; j < S::kCols; ++j) {
+                const int col = lane + 32 * j;
+                if (col >= vecs) break;
+                const float4 o = acc[j][r];
+                if (!whole) {
+                    *reinterpret_cast<float4*>(out_part + (o_row + r) * DP + col * 4) = o;
+                } else {
+                    reinterpret_cast<float4*>(static_cast<float*>(a.out) + place * c.D)[col] =
+                        shown ? make_float4(o.x * inverse, o.y * inverse, o.z * inverse, o.w * inverse)
+                              : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                }
+            }
+            if (lane == 0) {
+                if (!whole) {
+                    out_part[S::kRows * DP + o_row + r] = m;
+                    out_part[S::kRows * DP + S::kRows + o_row + r] = l;
+                } else if (a.lse != nullptr) {
+                    a.lse[place] = shown && l != 0.0f ? (m + log2f(l)) * kLn2 : -INFINITY;
+                }
+            }
+        }
+        if (whole) continue;
+        __threadfence();
+        __syncthreads();
+        const Span span = span_of(work, p);
+        if (tid == 0) {
+            const int before = atomicAdd(counters + span.c0, 1);
+            ctl.last = before == span.c1 - span.c0;
+            if (ctl.last) counters[span.c0] = 0;
+        }
+        __syncthreads();
+        if (!ctl.last) continue;
+        __threadfence();
+        join_parts<float, S::kRows, DP, kThreads>(c, a, p, span, b, beam0, row0, rows, parts, query, tid);
+    }
+}
+
+template <int DP, int RT>
+cudaError_t launch_shape(const CacheView& c, const AttendParams& a, int sm_count, cudaStream_t stream) {
+    using S = Shape<DP, RT>;
+    auto* kernel = attend_f32_kernel<DP, RT>;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes);
+    if (e != cudaSuccess) return e;
+    return launch_after(kernel, sm_count, kThreads, S::kBytes, stream, c, a);
+}
+
+template <int DP>
+cudaError_t launch_width(const CacheView& c, const AttendParams& a, int sm_count, cudaStream_t stream) {
+    const int beams = a.beams < kGroupBeams ? a.beams : kGroupBeams;
+    const int64_t rows = static_cast<int64_t>(beams) * a.N * a.G;
+    if (rows <= 8) return launch_shape<DP, 1>(c, a, sm_count, stream);
+    if (rows <= 16) return launch_shape<DP, 2>(c, a, sm_count, stream);
+    return launch_shape<DP, 4>(c, a, sm_count, stream);
+}
+
+}  // namespace
+
+int64_t attend_f32_workspace(const CacheView&, const AttendParams&, int sm_count) {
+    // A counter for each CTA (8192 bytes), then two partial results for each.
+    return 8192 + static_cast<int64_t>(2) * sm_count * Shape<256, 4>::kOut * 4;
+}
+
+cudaError_t launch_attend_f32(const CacheView& c, const AttendParams& a, int sm_count, cudaStream_t stream) {
+    if (c.D <= 128) return launch_width<128>(c, a, sm_count, stream);
+    return launch_width<256>(c, a, sm_count, stream);
+}
+
+}  // namespace dbsb
