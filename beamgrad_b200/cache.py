@@ -29,6 +29,9 @@ import torch
 from beamgrad_b200 import _abi as A
 
 _DTYPES = {torch.float32: A.DTYPE_F32, torch.float16: A.DTYPE_F16, torch.bfloat16: A.DTYPE_BF16}
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
 _STATUS = (
     (A.CACHE_STATUS_POOL, "the pool ran out of pages"),
     (A.CACHE_STATUS_CAPACITY, "a beam outgrew the table (max_length)"),
@@ -111,7 +114,7 @@ class PagedCache:
 
     def _adopt(self, pages, table, lengths, references) -> None:
         self.pages, self.table, self.lengths, self.references = pages, table, lengths, references
-        self.device, self.dtype = pages.device, pages.dtype
+        self.device, self.dtype = pages.device, pages.dtype  # the device with its index
         self.num_layers, _, self.num_pages, self.num_kv_heads, self.page_size, self.head_dim = pages.shape
         self.batch_size, self.beam_size, columns = table.shape
         self.max_length = columns * self.page_size
@@ -121,10 +124,9 @@ class PagedCache:
         c.pages, c.table, c.lengths = pages.data_ptr(), table.data_ptr(), lengths.data_ptr()
         c.references, c.plan, c.status = references.data_ptr(), self._plan.data_ptr(), self._status.data_ptr()
         self._ref = C.byref(c)
-        self._args = A.AttendArgs()
-        self._args_ref = C.byref(self._args)
         self._workspaces = {}  # stream -> zero-initialised workspace
-        self._sizes = {}       # (beams, new tokens, query heads) -> its bytes
+        self._calls = {}       # shapes and layouts of attend's arguments -> _Call
+        self._float = torch.empty(0, dtype=torch.float32, device=self.device)
 
     # -- state ----------------------------------------------------------------------------
     def reset(self) -> None:
@@ -214,7 +216,61 @@ class PagedCache:
         Returns out [B, beams, N, query heads, head_dim], and with ``return_lse`` also the
         logsumexp of the scaled scores, [B, beams, N, query heads] float32.
         """
-        a = self._args
+        if (k is None) != (v is None):
+            raise ValueError("k and v are given together or not at all")
+        if torch.is_grad_enabled() and (q.requires_grad or k is not None and (k.requires_grad or v.requires_grad)):
+            raise RuntimeError("attend has no backward pass: call it under torch.no_grad()")
+        # Arguments of one shape and layout are checked and written down once.
+        key = (q.shape, q.stride(), q.dtype, q.device, mask is None) if k is None else (
+            q.shape, q.stride(), q.dtype, q.device, mask is None, k.shape, k.stride(), k.dtype, k.device,
+            v.shape, v.stride(), v.dtype, v.device)
+        call = self._calls.get(key)
+        if call is None:
+            call = self._calls[key] = self._check_shapes(q, k, v)
+        if not 0 <= layer < self.num_layers:
+            raise ValueError(f"layer {layer} is not one of {self.num_layers}")
+        a, shape = call.args, call.shape
+        if call.copies or (q.data_ptr() | (0 if k is None else k.data_ptr() | v.data_ptr())) % 16:
+            q, k, v = self._rows(q), None if k is None else self._rows(k), None if v is None else self._rows(v)
+            call = self._check_shapes(q, k, v)
+            a = call.args
+        a.q = q.data_ptr()
+        if k is not None:
+            a.k, a.v = k.data_ptr(), v.data_ptr()
+        if mask is not None:
+            if mask.shape != call.mask_shape or mask.dtype != torch.bool or mask.device != self.device:
+                raise ValueError(f"mask must be a bool {call.mask_shape} tensor on {self.device}")
+            mask = mask.contiguous()
+            a.mask = mask.data_ptr()
+        if counts is not None:
+            counts = self._int32(counts, "counts", shape[:2])
+            a.counts = counts.data_ptr()
+        else:
+            a.counts = None
+        if out is None:
+            out = self.pages.new_empty(shape)
+        elif out.shape != shape or out.dtype != self.dtype or out.device != self.device or not out.is_contiguous():
+            raise ValueError(f"out must be a contiguous {self.dtype} {tuple(shape)} tensor on {self.device}")
+        a.out = out.data_ptr()
+        if return_lse:
+            lse = self._float.new_empty(shape[:4])
+            a.lse = lse.data_ptr()
+        else:
+            a.lse = None
+        a.layer = layer
+        a.scale = call.scale if scale is None else scale
+        with _on(self.device):
+            stream = self._stream()
+            workspace = self._workspaces.get(stream)
+            if workspace is None or workspace.numel() < call.workspace:
+                workspace = self._workspaces[stream] = torch.zeros(call.workspace, dtype=torch.uint8, device=self.device)
+            a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel()
+            status = self.lib.dbs_cuda_cache_attend(self._ref, call.ref, stream)
+        if status:
+            A.check(status, "cache_attend")
+        return (out, lse) if return_lse else out
+
+    def _check_shapes(self, q, k, v) -> "_Call":
         if q.dim() != 5:
             raise ValueError(f"q must be [B, beams, N, query heads, head_dim], got {tuple(q.shape)}")
         B, beams, N, heads, D = shape = q.shape
@@ -222,84 +278,49 @@ class PagedCache:
                 or heads % self.num_kv_heads or heads < 1):
             raise ValueError(f"q {tuple(shape)} does not fit a cache of {self.batch_size} x {self.beam_size} beams with "
                              f"{self.num_kv_heads} heads of {self.head_dim}")
-        if not 0 <= layer < self.num_layers:
-            raise ValueError(f"layer {layer} is not one of {self.num_layers}")
-        if (k is None) != (v is None):
-            raise ValueError("k and v are given together or not at all")
-        if torch.is_grad_enabled() and (q.requires_grad or k is not None and (k.requires_grad or v.requires_grad)):
-            raise RuntimeError("attend has no backward pass: call it under torch.no_grad()")
-        q = self._rows(q, "q")
-        a.q = q.data_ptr()
+        for name, x in (("q", q), ("k", k), ("v", v)):
+            if x is None:
+                continue
+            if x.dtype != self.dtype or x.device != self.device:
+                raise ValueError(f"{name} must be a {self.dtype} tensor on {self.device}, got {x.dtype} on {x.device}")
+            if x is not q and tuple(x.shape) != (B, beams, N, self.num_kv_heads, D):
+                raise ValueError(f"{name} must be {(B, beams, N, self.num_kv_heads, D)}, got {tuple(x.shape)}")
+        call = _Call()
+        a = call.args = A.AttendArgs()
+        call.ref = C.byref(a)
+        call.shape, call.mask_shape, call.scale = shape, (B, beams, N, N), 1.0 / math.sqrt(D)
+        step = 16 // q.element_size()
+        call.copies = any(x is not None and (x.stride(4) != 1 or any(n % step for n in x.stride()[:4])) for x in (q, k, v))
         a.q_strides[:] = q.stride()[:4]
         if k is not None:
-            if tuple(k.shape) != (B, beams, N, self.num_kv_heads, D) or k.shape != v.shape:
-                raise ValueError(f"k and v must be {(B, beams, N, self.num_kv_heads, D)}, got {tuple(k.shape)} and "
-                                 f"{tuple(v.shape)}")
-            k, v = self._rows(k, "k"), self._rows(v, "v")
-            a.k, a.v = k.data_ptr(), v.data_ptr()
             a.k_strides[:] = k.stride()[:4]
             a.v_strides[:] = v.stride()[:4]
-        else:
-            a.k = a.v = None
-        if mask is not None:
-            if tuple(mask.shape) != (B, beams, N, N) or mask.dtype != torch.bool or mask.device != self.device:
-                raise ValueError(f"mask must be a bool {(B, beams, N, N)} tensor on {self.device}")
-            mask = mask.contiguous()
-        a.mask = None if mask is None else mask.data_ptr()
-        if counts is not None:
-            counts = self._int32(counts, "counts", (B, beams))
-        a.counts = None if counts is None else counts.data_ptr()
-        if out is None:
-            out = torch.empty(shape, dtype=self.dtype, device=self.device)
-        elif out.shape != shape or out.dtype != self.dtype or out.device != self.device or not out.is_contiguous():
-            raise ValueError(f"out must be a contiguous {self.dtype} {tuple(shape)} tensor on {self.device}")
-        lse = torch.empty(shape[:4], dtype=torch.float32, device=self.device) if return_lse else None
-        a.out, a.lse = out.data_ptr(), None if lse is None else lse.data_ptr()
-        a.layer, a.beams, a.new_tokens, a.query_heads = layer, beams, N, heads
-        a.scale = 1.0 / math.sqrt(D) if scale is None else scale
-        with _on(self.device):
-            stream = self._stream()
-            workspace = self._workspace(stream, (beams, N, heads))
-            a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel()
-            status = self.lib.dbs_cuda_cache_attend(self._ref, self._args_ref, stream)
-        if status:
-            A.check(status, "cache_attend")
-        return (out, lse) if return_lse else out
+        a.beams, a.new_tokens, a.query_heads, a.scale = beams, N, heads, 1.0
+        call.workspace = self.lib.dbs_cuda_cache_attend_workspace_size(self._ref, call.ref)
+        if call.workspace < 0:
+            raise ValueError("the engine rejects these attention sizes")
+        return call
 
     # -- helpers --------------------------------------------------------------------------
     def _stream(self) -> int:
-        return torch.cuda.current_stream(self.device).cuda_stream
+        return _raw_stream(self.device.index)
 
-    def _workspace(self, stream: int, sizes: tuple) -> torch.Tensor:
-        """The stream's workspace, grown to what a call of these sizes needs."""
-        need = self._sizes.get(sizes)
-        if need is None:
-            need = self.lib.dbs_cuda_cache_attend_workspace_size(self._ref, self._args_ref)
-            if need < 0:
-                raise ValueError("the engine rejects these attention sizes")
-            self._sizes[sizes] = need
-        have = self._workspaces.get(stream)
-        if have is None or have.numel() < need:
-            have = self._workspaces[stream] = torch.zeros(need, dtype=torch.uint8, device=self.device)
-        return have
-
-    def _rows(self, x: torch.Tensor, name: str) -> torch.Tensor:
-        if x.dtype != self.dtype or x.device != self.device:
-            raise ValueError(f"{name} must be a {self.dtype} tensor on {self.device}, got {x.dtype} on {x.device}")
+    @staticmethod
+    def _rows(x: torch.Tensor) -> torch.Tensor:
+        """x with rows on 16-byte boundaries (a copy where it is not laid out so)."""
         step = 16 // x.element_size()
-        s0, s1, s2, s3, s4 = x.stride()
-        if s4 != 1 or (s0 | s1 | s2 | s3) % step or x.data_ptr() % 16:
-            return x.contiguous() if not x.is_contiguous() else x.clone()
-        return x
+        if x.stride(4) == 1 and not any(n % step for n in x.stride()[:4]) and x.data_ptr() % 16 == 0:
+            return x
+        return x.clone(memory_format=torch.contiguous_format)
 
     def _int32(self, x: torch.Tensor | None, name: str, shape: tuple | None = ()) -> torch.Tensor | None:
         if x is None:
             return None
         if shape == ():
-            shape = (self.batch_size, self.beam_size)
-        if x.device != self.device or x.dtype not in (torch.int32, torch.int64) or shape and tuple(x.shape) != shape:
-            raise ValueError(f"{name} must be an integer {shape or ''} tensor on {self.device}")
-        return x.to(torch.int32).contiguous()
+            shape = self.lengths.shape
+        if x.device != self.device or x.dtype not in (torch.int32, torch.int64) or shape and x.shape != shape:
+            raise ValueError(f"{name} must be an integer {tuple(shape or ())} tensor on {self.device}")
+        return x if x.dtype == torch.int32 and x.is_contiguous() else x.to(torch.int32).contiguous()
 
     def _per_beam(self, x: int | torch.Tensor, name: str) -> tuple:
         return (self._int32(x, name), 0) if isinstance(x, torch.Tensor) else (None, _number(x, name))
@@ -315,6 +336,12 @@ def _ptr(x: torch.Tensor | None) -> int | None:
     return None if x is None else x.data_ptr()
 
 
+class _Call:
+    """What attend keeps of arguments of one shape and layout."""
+
+    __slots__ = ("args", "ref", "shape", "mask_shape", "scale", "copies", "workspace")
+
+
 class _Here:
     def __enter__(self):
         return None
@@ -328,4 +355,4 @@ _HERE = _Here()
 
 def _on(device: torch.device):
     """The device as the current one; nothing to do where it is already."""
-    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return _HERE if _current_device() == device.index else torch.cuda.device(device)

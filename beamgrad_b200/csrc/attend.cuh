@@ -4,6 +4,7 @@
 // the work over the CTAs, and the copies and barriers of the tiled kernels.
 #pragma once
 
+#include <atomic>
 #include <climits>
 #include <type_traits>
 
@@ -484,6 +485,19 @@ __device__ __forceinline__ void tma_load(uint32_t to, const CUtensorMap* map, in
         "cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(to),
         "l"(map), "r"(x), "r"(y), "r"(bar)
         : "memory");
+}
+
+// Lets a kernel have that much shared memory, once a device. ready: a bit for each that has it.
+template <class Kernel>
+cudaError_t allow_shared(Kernel* kernel, int bytes, std::atomic<uint64_t>& ready) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = uint64_t{1} << (dev & 63);
+    if (dev < 64 && (ready.load(std::memory_order_acquire) & bit) != 0) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && dev < 64) ready.fetch_or(bit, std::memory_order_release);
+    return e;
 }
 
 // The tensor map of the pages as [rows, head_dim], boxes of one page by 64 elements, swizzled so

@@ -296,7 +296,8 @@ template <int DP, int RT>
 cudaError_t launch_shape(const CacheView& c, const AttendParams& a, int sm_count, cudaStream_t stream) {
     using S = Shape<DP, RT>;
     auto* kernel = attend_f32_kernel<DP, RT>;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes);
+    static std::atomic<uint64_t> ready{0};  // a bit a device
+    const cudaError_t e = allow_shared(kernel, S::kBytes, ready);
     if (e != cudaSuccess) return e;
     return launch_after(kernel, sm_count, kThreads, S::kBytes, stream, c, a);
 }

@@ -446,7 +446,8 @@ cudaError_t launch_shape(const CacheView& c, const CUtensorMap& map, const Atten
                          cudaStream_t stream) {
     using S = Shape<T, DP, MT, WR>;
     auto* kernel = attend_mma_kernel<T, DP, MT, WR>;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes);
+    static std::atomic<uint64_t> ready{0};  // a bit a device
+    const cudaError_t e = allow_shared(kernel, S::kBytes, ready);
     if (e != cudaSuccess) return e;
     return launch_after(kernel, sm_count, kThreads, S::kBytes, stream, map, c, a);
 }

@@ -759,7 +759,8 @@ cudaError_t launch_shape(const CacheView& c, const CUtensorMap& map, const Atten
     using S = Shape<DP, NQ, COPIES>;
     static_assert(S::kBytes <= 227 * 1024 && S::kSlots >= 4);
     auto* kernel = attend_tc_kernel<T, DP, NQ, COPIES>;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes);
+    static std::atomic<uint64_t> ready{0};  // a bit a device
+    const cudaError_t e = allow_shared(kernel, S::kBytes, ready);
     if (e != cudaSuccess) return e;
     return launch_after(kernel, sm_count, S::kThreads, S::kBytes, stream, map, c, a);
 }
