@@ -29,7 +29,7 @@ namespace {
 
 constexpr int kTileKeys = 128;
 constexpr int kMaxSlots = 12;
-constexpr int kMinTiles = 1;     // tiles of a CTA at least
+constexpr int kMinTiles = 2;     // tiles of a CTA at least: a join costs about as much as two
 constexpr float kRaise = 8.0f;  // log2 of the growth that a reference tolerates
 
 struct Control {

@@ -6,8 +6,8 @@
 // References need no recount. Of the old entry (r, c), a complete page, every child of r keeps a
 // reference; of an incomplete or spare page only the first child does, if it needs the column. So
 // the entry's page changes by (holders - 1), known from three numbers a beam (children, first
-// child, columns the first child needs), and entries that all beams share cancel in the thread
-// before they reach an atomic. Integer sums, so the order of the atomics does not show.
+// child, columns the first child needs): one atomic an entry at the most, of integers, so their order
+// does not show.
 //
 // New pages are handed out by the last CTA to finish: one scan of the slots' wishes, one scan of
 // the references for zeros that stops as soon as there are enough. Nothing else is serial.
@@ -35,18 +35,14 @@ __device__ __forceinline__ void raise(const CacheView& c, int bit) { atomicOr(c.
 // The last CTA of fork_meta_kernel: ranks of the wishes, free pages for them, the copy list.
 __device__ void hand_out(const CacheView& c, int* sums) {
     const int S = c.B * c.K, tid = threadIdx.x;
-    int wanted = 0, copies = 0;
+    int wanted = 0;
     for (int base = 0; base < S; base += kMetaThreads) {
         const int s = base + tid;
         const int n = s < S ? __ldcg(c.want_count + s) : 0;
-        const int copy = s < S && __ldcg(c.copy_rows + s) > 0;
         int total;
         const int before = block_scan(n, sums, &total);
         if (s < S) c.want_rank[s] = wanted + before;
         wanted += total;
-        const int at = block_scan(copy, sums, &total);
-        if (copy) c.copy_list[copies + at] = s;
-        copies += total;
     }
     // Zeros of the references, 16 a thread and round.
     int found = 0;
@@ -72,9 +68,23 @@ __device__ void hand_out(const CacheView& c, int* sums) {
         }
         found += total;
     }
+    const int handed = found < wanted ? found : wanted;
+    __syncthreads();
+    // A slot that copies takes its first new page for the rows.
+    int copies = 0;
+    for (int base = 0; base < S; base += kMetaThreads) {
+        const int s = base + tid;
+        const int rows = s < S ? __ldcg(c.copy_rows + s) : 0;
+        const int rank = rows > 0 ? c.want_rank[s] : 0;
+        const bool copy = rows > 0 && rank < handed;
+        int total;
+        const int at = copies + block_scan(copy, sums, &total);
+        if (copy) c.copies[at] = make_int4(__ldcg(c.copy_from + s), c.free_list[rank], rows, s);
+        copies += total;
+    }
     if (tid == 0) {
         c.words[kWordCopies] = copies;
-        c.words[kWordFree] = found < wanted ? found : wanted;
+        c.words[kWordFree] = handed;
         c.words[kWordArrive] = 0;
         if (found < wanted) raise(c, DBS_CUDA_CACHE_STATUS_POOL);
     }
@@ -93,7 +103,8 @@ __global__ void __launch_bounds__(kMetaThreads) fork_meta_kernel(CacheView c, Fo
     int32_t* need = src + K;        // [K] columns of each new beam
     int32_t* want = need + K;       // [K] new pages it asks for
     int32_t* want_at = want + K;    // [K] the first such column
-    int32_t* stage = want_at + K;   // [K, width]
+    int32_t* copied = want_at + K;  // [K] page whose rows it copies or -1
+    int32_t* stage = copied + K;    // [K, width]
     const int64_t slot0 = static_cast<int64_t>(b) * K;
     grid_wait();   // what ran before may have written the parents
     grid_release();
@@ -137,7 +148,7 @@ __global__ void __launch_bounds__(kMetaThreads) fork_meta_kernel(CacheView c, Fo
             columns = static_cast<int>(n > M ? M : n);
         }
         need[k] = columns;
-        c.copy_from[slot0 + k] = -1;
+        copied[k] = -1;
     }
     __syncthreads();
     const int width = K * M <= kStageInts ? M : (kStageInts / K > 1 ? kStageInts / K : 1);
@@ -149,37 +160,27 @@ __global__ void __launch_bounds__(kMetaThreads) fork_meta_kernel(CacheView c, Fo
             stage[r * width + i - r * cols] = table[static_cast<int64_t>(r) * M + base + i - r * cols];
         }
         __syncthreads();
-        for (int i = tid; i < cols; i += kMetaThreads) {
-            const int col = base + i;
-            int run = -1, delta = 0;
-            for (int r = 0; r < K; ++r) {
-                const int e = stage[r * width + i];
-                if (e < 0) continue;
+        for (int i = tid; i < K * cols; i += kMetaThreads) {
+            const int r = i / cols, at = i - r * cols, col = base + at;
+            const int old = stage[r * width + at];
+            if (old >= 0) {  // as the entry of the old beam r
                 const int heir = first[r];
                 const int holders = col < (length[r] >> log2) ? children[r] : (heir < K && col < need[heir]);
-                if (e != run) {
-                    if (delta != 0) atomicAdd(c.references + run, delta);
-                    run = e;
-                    delta = 0;
-                }
-                delta += holders - 1;
+                if (holders != 1) atomicAdd(c.references + old, holders - 1);
             }
-            if (delta != 0) atomicAdd(c.references + run, delta);
-            for (int s = 0; s < K; ++s) {
-                const int p = src[s];
-                int e = -1;
-                if (p >= 0 && col < need[s]) {
-                    const int held = stage[p * width + i], full = length[p] >> log2;
-                    if (col < full || first[p] == s) e = held;
-                    if (col >= full && e < 0) {
-                        e = -2;
-                        atomicAdd(&want[s], 1);
-                        atomicMin(&want_at[s], col);
-                    }
-                    if (col == full && first[p] != s && (length[p] & (c.page - 1)) != 0) c.copy_from[slot0 + s] = held;
+            const int p = src[r];  // as the entry of the new beam r
+            int e = -1;
+            if (p >= 0 && col < need[r]) {
+                const int held = stage[p * width + at], full = length[p] >> log2;
+                if (col < full || first[p] == r) e = held;
+                if (col >= full && e < 0) {
+                    e = -2;
+                    atomicAdd(&want[r], 1);
+                    atomicMin(&want_at[r], col);
                 }
-                if (e != stage[s * width + i]) table[static_cast<int64_t>(s) * M + col] = e;
+                if (col == full && first[p] != r && (length[p] & (c.page - 1)) != 0) copied[r] = held;
             }
+            if (e != old) table[static_cast<int64_t>(r) * M + col] = e;
         }
         __syncthreads();
     }
@@ -188,8 +189,8 @@ __global__ void __launch_bounds__(kMetaThreads) fork_meta_kernel(CacheView c, Fo
         c.lengths[slot0 + s] = p >= 0 ? length[p] : 0;
         c.want_count[slot0 + s] = want[s];
         c.want_first[slot0 + s] = want_at[s];
-        const bool copies = p >= 0 && first[p] != s && c.copy_from[slot0 + s] >= 0;
-        c.copy_rows[slot0 + s] = copies ? length[p] & (c.page - 1) : 0;
+        c.copy_from[slot0 + s] = copied[s];
+        c.copy_rows[slot0 + s] = copied[s] >= 0 ? length[p] & (c.page - 1) : 0;
     }
     __threadfence();
     __syncthreads();
@@ -290,7 +291,7 @@ __global__ void __launch_bounds__(kCopyThreads) cache_finish_kernel(CacheView c,
         write_plan(c, blockIdx.x, true, sums, smem);
         return;
     }
-    const int copies = c.words[kWordCopies], handed = c.words[kWordFree];
+    const int copies = c.words[kWordCopies];
     const int per = c.L * 2 * c.H;
     const int64_t items = static_cast<int64_t>(copies) * per;
     const int lane = threadIdx.x & 31;
@@ -298,15 +299,13 @@ __global__ void __launch_bounds__(kCopyThreads) cache_finish_kernel(CacheView c,
     const int row_vecs = c.D * c.elem / 16;
     for (int64_t i = static_cast<int64_t>(blockIdx.x - plan_blocks) * (kCopyThreads / 32) + (threadIdx.x >> 5);
          i < items; i += warps) {
-        const int slot = c.copy_list[i / per], part = static_cast<int>(i % per);
-        const int from = c.copy_from[slot], at = c.want_rank[slot];
-        if (at >= handed) continue;  // the pool ran out
-        const int to = c.free_list[at];
-        const int64_t block = part / c.H, head = part % c.H;  // block: layer * 2 + kind
+        const int which = static_cast<int>(i / per), part = static_cast<int>(i - static_cast<int64_t>(which) * per);
+        const int4 copy = __ldg(c.copies + which);
+        const int64_t block = part / c.H, head = part - block * c.H;  // block: layer * 2 + kind
         const int64_t vecs = static_cast<int64_t>(c.page) * row_vecs;
-        const uint4* x = static_cast<const uint4*>(c.pages) + ((block * c.P + from) * c.H + head) * vecs;
-        uint4* y = static_cast<uint4*>(c.pages) + ((block * c.P + to) * c.H + head) * vecs;
-        const int n = c.copy_rows[slot] * row_vecs;
+        const uint4* x = static_cast<const uint4*>(c.pages) + ((block * c.P + copy.x) * c.H + head) * vecs;
+        uint4* y = static_cast<uint4*>(c.pages) + ((block * c.P + copy.y) * c.H + head) * vecs;
+        const int n = copy.z * row_vecs;
         int v = lane;
         for (; v + 7 * 32 < n; v += 8 * 32) {
             uint4 t[8];
@@ -319,63 +318,67 @@ __global__ void __launch_bounds__(kCopyThreads) cache_finish_kernel(CacheView c,
     }
 }
 
-// Rows of an accepted path to the front of the drafted area. A thread owns 16 bytes of every row
-// of one slot, layer, kind and head, and moves eight rows a round: row path[a] >= a lies at or
-// behind every row that earlier rounds wrote, and a round reads all its rows before it writes.
+// Rows of an accepted path to the front of the drafted area. A CTA takes one slot and a part of its
+// layers, kinds and heads; it looks the rows' places up once. A thread owns 16 bytes of every row of
+// one layer, kind and head, and moves eight rows a round: row path[a] >= a lies at or behind every row
+// that earlier rounds wrote, and a round reads all its rows before it writes.
+constexpr int kMoveRows = 256;  // accepted rows whose places are looked up at a time
+
 __global__ void __launch_bounds__(kCopyThreads) commit_move_kernel(CacheView c, const int32_t* path, int path_stride,
-                                                                   const int32_t* counts) {
+                                                                   const int32_t* counts, int parts) {
+    __shared__ int2 moves[kMoveRows];  // row numbers of a layer, kind and head (page * H * page_size + row), -1: none
+    __shared__ int bad;
     grid_wait();
     grid_release();
+    const int slot = blockIdx.x / parts, piece = blockIdx.x - slot * parts, tid = threadIdx.x;
     const int row_vecs = c.D * c.elem / 16;
-    const int64_t per = static_cast<int64_t>(c.L) * 2 * c.H * row_vecs;
-    const int64_t items = static_cast<int64_t>(c.B) * c.K * per;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kCopyThreads + threadIdx.x; i < items;
-         i += static_cast<int64_t>(gridDim.x) * kCopyThreads) {
-        const int64_t slot = i / per;
-        int rest = static_cast<int>(i - slot * per);
-        const int vec = rest % row_vecs;
-        rest /= row_vecs;
-        const int64_t head = rest % c.H, block = rest / c.H;
-        int count = counts[slot];
-        if (count > path_stride) {
-            raise(c, DBS_CUDA_CACHE_STATUS_INDEX);
-            count = path_stride;
-        }
-        const int n = c.lengths[slot];
-        const int32_t* row = c.table + slot * c.M;
-        uint4* pages = static_cast<uint4*>(c.pages) + vec;
-        auto place = [&](int64_t pos) -> uint4* {
-            const int64_t col = pos >> c.page_log2;
-            if (col >= c.M) return nullptr;
-            const int p = row[col];
-            if (p < 0) return nullptr;
-            return pages + (((block * c.P + p) * c.H + head) * c.page + (pos & (c.page - 1))) * row_vecs;
-        };
-        int before = -1;
-        for (int a = 0; a < count; a += 8) {
-            uint4 t[8];
-            uint4* to[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                to[j] = nullptr;
-                if (a + j < count) {
-                    const int from = path[slot * path_stride + a + j];
-                    if (from <= before) {  // not increasing: leave the row
-                        raise(c, DBS_CUDA_CACHE_STATUS_INDEX);
-                    } else {
-                        before = from;
-                        const uint4* x = from != a + j ? place(static_cast<int64_t>(n) + from) : nullptr;
-                        uint4* y = place(static_cast<int64_t>(n) + a + j);
-                        if (x != nullptr && y != nullptr) {
-                            t[j] = *x;
-                            to[j] = y;
-                        }
-                    }
+    int count = counts[slot];
+    const int n = c.lengths[slot];
+    const int32_t* row = c.table + static_cast<int64_t>(slot) * c.M;
+    const int32_t* steps = path + static_cast<int64_t>(slot) * path_stride;
+    if (tid == 0) {
+        bad = 0;
+        if (count > path_stride && piece == 0) raise(c, DBS_CUDA_CACHE_STATUS_INDEX);
+    }
+    if (count > path_stride) count = path_stride;
+    const int items = c.L * 2 * c.H * row_vecs;
+    for (int base = 0; base < count; base += kMoveRows) {
+        __syncthreads();
+        const int a = base + tid;
+        if (a < count) {
+            const int from = steps[a];
+            const bool rises = from > (a > 0 ? steps[a - 1] : -1);
+            if (!rises) bad = 1;  // (all such threads store 1)
+            int2 m = make_int2(-1, -1);
+            const int64_t at = static_cast<int64_t>(n) + from, to = static_cast<int64_t>(n) + a;
+            if (rises && from != a && (at >> c.page_log2) < c.M && (to >> c.page_log2) < c.M) {
+                const int p = row[at >> c.page_log2], q = row[to >> c.page_log2];
+                if (p >= 0 && q >= 0) {
+                    m.x = p * c.H * c.page + static_cast<int>(at & (c.page - 1));
+                    m.y = q * c.H * c.page + static_cast<int>(to & (c.page - 1));
                 }
             }
+            moves[tid] = m;
+        }
+        __syncthreads();
+        if (bad) {  // not increasing: the rows are left as they are
+            if (tid == 0 && piece == 0) raise(c, DBS_CUDA_CACHE_STATUS_INDEX);
+            return;
+        }
+        const int rows = count - base < kMoveRows ? count - base : kMoveRows;
+        for (int i = piece * kCopyThreads + tid; i < items; i += parts * kCopyThreads) {
+            const int part = i / row_vecs, vec = i - part * row_vecs, block = part / c.H, head = part - block * c.H;
+            uint4* pages = static_cast<uint4*>(c.pages) + vec +
+                           (static_cast<int64_t>(block) * c.P * c.H + head) * c.page * row_vecs;
+            for (int a0 = 0; a0 < rows; a0 += 8) {
+                uint4 t[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (to[j] != nullptr) *to[j] = t[j];
+                for (int j = 0; j < 8; ++j)
+                    if (a0 + j < rows && moves[a0 + j].x >= 0) t[j] = pages[static_cast<int64_t>(moves[a0 + j].x) * row_vecs];
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (a0 + j < rows && moves[a0 + j].x >= 0) pages[static_cast<int64_t>(moves[a0 + j].y) * row_vecs] = t[j];
+            }
         }
     }
 }
@@ -510,7 +513,7 @@ __global__ void refresh_values_kernel(CacheView c, uint32_t exponent_lo, uint32_
 size_t meta_smem(const CacheView& c) {
     const int64_t all = static_cast<int64_t>(c.K) * c.M;
     const int64_t stage = all <= kStageInts ? all : (c.K > kStageInts ? c.K : kStageInts);
-    return (7 * static_cast<size_t>(c.K) + stage) * sizeof(int32_t);
+    return (8 * static_cast<size_t>(c.K) + stage) * sizeof(int32_t);
 }
 
 unsigned copy_blocks(int64_t work, int sm_count) {
@@ -524,7 +527,7 @@ cudaError_t launch_cache_fork(const CacheView& c, const int32_t* parents, const 
                               const int32_t* room, int room_all, int sm_count, cudaStream_t stream) {
     const size_t smem = meta_smem(c);
     cudaError_t e = cudaSuccess;
-    if (smem > 48 * 1024)
+    if (smem > 47 * 1024)  // (and some static shared memory)
         e = cudaFuncSetAttribute(fork_meta_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) return e;
     const ForkArgs a{parents, written, room, written_all, room_all};
@@ -539,9 +542,13 @@ cudaError_t launch_cache_fork(const CacheView& c, const int32_t* parents, const 
 
 cudaError_t launch_cache_commit(const CacheView& c, const int32_t* path, int path_stride, const int32_t* counts,
                                 int room_all, int sm_count, cudaStream_t stream) {
-    const int64_t items = static_cast<int64_t>(c.B) * c.K * c.L * 2 * c.H * (c.D * c.elem / 16);
-    const cudaError_t e = launch_after(commit_move_kernel, copy_blocks((items + kCopyThreads - 1) / kCopyThreads, sm_count),
-                                       kCopyThreads, 0, stream, c, path, path_stride, counts);
+    // Two rounds of a CTA's threads, or so many CTAs that all SMs have some.
+    const int64_t slots = static_cast<int64_t>(c.B) * c.K, items = static_cast<int64_t>(c.L) * 2 * c.H * (c.D * c.elem / 16);
+    int64_t parts = (items + 2 * kCopyThreads - 1) / (2 * kCopyThreads);
+    const int64_t cap = slots * 2 > sm_count * 8 ? 2 : sm_count * 8 / slots;
+    if (parts > cap) parts = cap;
+    const cudaError_t e = launch_after(commit_move_kernel, static_cast<unsigned>(slots * parts), kCopyThreads, 0, stream, c,
+                                       path, path_stride, counts, static_cast<int>(parts));
     if (e != cudaSuccess) return e;
     return launch_cache_fork(c, nullptr, counts, 0, nullptr, room_all, sm_count, stream);
 }
