@@ -5,9 +5,10 @@
 //
 // Blocks of 8, 16 or 32 query rows by tiles of 64 positions (32 for heads above 128), copied by
 // cp.async, the next tile while this one is worked on. Both products run on register tiles of up to
-// 4 x 4, for which a warp's eight shared-memory reads of 16 bytes an element group (each one pass of
-// the banks: rows are padded by 16 bytes) feed 64 multiply-adds. At 32 rows of 128 that is 4096
-// cycles a tile and SM, at 12 rows (2048) the bytes bound it (2800 cycles).
+// 4 x 4 (of float4 in one direction), so laid over a warp that its eight shared-memory reads of 16
+// bytes take 8 (scores) or 12 (values) passes of the banks for 64 multiply-adds: rows are padded by
+// 16 bytes, rows of one read lie next to each other. At 32 rows of 128 that is 4096 cycles a tile and
+// SM, at 8 rows the bytes bound it (2800 cycles).
 #include "attend.cuh"
 
 namespace dbsb {
@@ -25,7 +26,11 @@ struct Shape {
     static constexpr int kScorePitch = kKeys + 4;
     static constexpr int kStage = 2 * kKeys * kPitch;  // floats: keys, values
     static constexpr int kScores = kRows * kScorePitch;
-    static constexpr int kCols = (DP + 127) / 128;  // groups of four columns that a thread has of the output
+    // Output: warps are kRowWarps by 8 / kRowWarps; a lane has RT rows and, of every 16 groups of four
+    // columns of its warp, one.
+    static constexpr int kRowWarps = 4;
+    static constexpr int kColWarps = 8 / kRowWarps;
+    static constexpr int kCols = DP / 4 / 16 / kColWarps;
     static constexpr int kBytes = (2 * kStage + kSplit * kScores + kRows * kPitch) * 4;
     static constexpr int kOut = kRows * (DP + 2);
 };
@@ -34,6 +39,7 @@ struct Control {
     int sums[34];
     WorkSplit split;
     CacheUnit unit[2][4];
+    int64_t row_at[2][64];  // of the tile's positions: the row's element among the pages of a layer's keys
     int64_t query_at[32];
     float factor[32], top[32], sum[32];
     int last;
@@ -67,15 +73,18 @@ attend_f32_kernel(const __grid_constant__ CacheView c, const __grid_constant__ A
     int64_t base = work.base;
     const float scale = a.scale * kLog2e;
     const int vecs = c.D / 4;
-    // Scores: a warp has 4 * RT rows by 32 positions (a thread RT rows, 4 positions 8 apart) of one part
-    // of the head.
+    // Scores: a warp has 4 * RT rows by 32 positions (a thread RT rows 4 apart, 4 positions 8 apart) of
+    // one part of the head.
     const int row_half = warp & 1, key_half = S::kKeys == 64 ? (warp >> 1) & 1 : 0;
     const int part = S::kKeys == 64 ? warp >> 2 : warp >> 1;
-    const int s_row = row_half * 4 * RT + (lane >> 3) * RT, s_key = key_half * 32 + (lane & 7);
-    // Weights: kThreads / kRows threads a row. Output: RT rows, four columns (and four more 128 on).
+    const int s_row = row_half * 4 * RT + (lane >> 3), s_key = key_half * 32 + (lane & 7);
+    // Weights: kThreads / kRows threads a row. Output: RT rows 2 apart by groups of four columns.
     constexpr int kPerRow = kThreads / S::kRows, kEach = S::kKeys / kPerRow;
     const int w_row = tid / kPerRow, w_key = tid % kPerRow;
-    const int o_row = warp * RT;
+    const int o_row = (warp % S::kRowWarps) * 2 * RT + (lane >> 4), o_col = (warp / S::kRowWarps) * 16 + (lane & 15);
+    constexpr int kColStep = 16 * S::kColWarps;
+    const int64_t kind_step = static_cast<int64_t>(c.P) * c.H * c.page * c.D;
+    const float* pages = static_cast<const float*>(c.pages) + static_cast<int64_t>(a.layer) * 2 * kind_step;
 
     for (int64_t cur = work.lo; cur < work.hi;) {
         const Piece p = piece_at<S::kRows>(c, a, work, cur, group, base, tile_units);
@@ -97,26 +106,30 @@ attend_f32_kernel(const __grid_constant__ CacheView c, const __grid_constant__ A
             if (r < rows && v < vecs) q = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + ctl.query_at[r]) + v);
             *reinterpret_cast<float4*>(query + r * S::kPitch + v * 4) = q;
         }
-        // Tile t: kKeys positions of its units' pages; past the last unit page 0, whatever finite values
-        // lie there meet weights of zero.
-        auto fetch = [&](int t) {
-            float* stage = stages + (t & 1) * S::kStage;
+        // Where the rows of tile t lie: kKeys positions of its units' pages; past the last unit page 0,
+        // whatever finite values lie there meet weights of zero.
+        auto find = [&](int t) {
+            if (tid >= S::kKeys || t >= n_tiles) return;
             const int first = (p.t0 + t / page_tiles) * tile_units, offset = t % page_tiles * S::kKeys;
-            if (tid < tile_units) {
-                CacheUnit u{-1, 0, 0, -1};
-                if (first + tid < p.units) {
-                    const int4 v = __ldg(reinterpret_cast<const int4*>(units + first + tid));
-                    u = CacheUnit{v.x, v.y + offset, static_cast<uint32_t>(v.z), v.w};
+            const int unit = first + (tid >> c.page_log2);
+            int4 v = make_int4(0, 0, 0, -1);  // no beam holds it
+            if (unit < p.units) v = __ldg(reinterpret_cast<const int4*>(units + unit));
+            ctl.row_at[t & 1][tid] = (((static_cast<int64_t>(v.x) * c.H + p.head) << c.page_log2) + ((tid + offset) & (c.page - 1))) * c.D;
+            if ((tid & (c.page - 1)) == 0)
+                ctl.unit[t & 1][tid >> c.page_log2] = CacheUnit{v.x, v.y + offset, static_cast<uint32_t>(v.z), v.w};
+        };
+        auto fetch = [&](int t) {
+            constexpr int kChunks = DP / 4, kAtOnce = kThreads / kChunks;
+            float* stage = stages + (t & 1) * S::kStage;
+            const int v = tid % kChunks, first = tid / kChunks;
+            if (v < vecs) {
+#pragma unroll
+                for (int j = 0; j < S::kKeys / kAtOnce; ++j) {
+                    const int key = first + j * kAtOnce;
+                    const float* from = pages + ctl.row_at[t & 1][key] + v * 4;
+                    copy16(stage + key * S::kPitch + v * 4, from);
+                    copy16(stage + (S::kKeys + key) * S::kPitch + v * 4, from + kind_step);
                 }
-                ctl.unit[t & 1][tid] = u;
-            }
-            for (int i = tid; i < 2 * S::kKeys * (DP / 4); i += kThreads) {
-                const int v = i % (DP / 4), key = i / (DP / 4) % S::kKeys, kind = i / (DP / 4 * S::kKeys);
-                if (v >= vecs) continue;
-                const int unit = first + (key >> c.page_log2), at = (key + offset) & (c.page - 1);
-                const int page = unit < p.units ? __ldg(&units[unit].page) : 0;
-                const int64_t row = ((((static_cast<int64_t>(a.layer) * 2 + kind) * c.P + page) * c.H + p.head) << c.page_log2) + at;
-                copy16(stage + (kind * S::kKeys + key) * S::kPitch + v * 4, static_cast<const float*>(c.pages) + row * c.D + v * 4);
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
@@ -135,7 +148,11 @@ attend_f32_kernel(const __grid_constant__ CacheView c, const __grid_constant__ A
 #pragma unroll
             for (int r = 0; r < RT; ++r) acc[j][r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 
+        find(0);
+        __syncthreads();
         fetch(0);
+        find(1);
+        __syncthreads();
         for (int t = 0; t < n_tiles; ++t) {
             if (t + 1 < n_tiles) {
                 fetch(t + 1);
@@ -152,11 +169,11 @@ attend_f32_kernel(const __grid_constant__ CacheView c, const __grid_constant__ A
                 for (int r = 0; r < RT; ++r)
 #pragma unroll
                     for (int k = 0; k < 4; ++k) s[r][k] = 0.0f;
-#pragma unroll 2
+#pragma unroll 4
                 for (int v = part; v < vecs; v += S::kSplit) {
                     float4 q[RT], x[4];
 #pragma unroll
-                    for (int r = 0; r < RT; ++r) q[r] = *reinterpret_cast<const float4*>(query + (s_row + r) * S::kPitch + v * 4);
+                    for (int r = 0; r < RT; ++r) q[r] = *reinterpret_cast<const float4*>(query + (s_row + 4 * r) * S::kPitch + v * 4);
 #pragma unroll
                     for (int k = 0; k < 4; ++k) x[k] = *reinterpret_cast<const float4*>(keys + (s_key + 8 * k) * S::kPitch + v * 4);
 #pragma unroll
@@ -168,7 +185,7 @@ attend_f32_kernel(const __grid_constant__ CacheView c, const __grid_constant__ A
 #pragma unroll
                 for (int r = 0; r < RT; ++r)
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) scores[part * S::kScores + (s_row + r) * S::kScorePitch + s_key + 8 * k] = s[r][k];
+                    for (int k = 0; k < 4; ++k) scores[part * S::kScores + (s_row + 4 * r) * S::kScorePitch + s_key + 8 * k] = s[r][k];
             }
             __syncthreads();
             {
@@ -205,19 +222,19 @@ attend_f32_kernel(const __grid_constant__ CacheView c, const __grid_constant__ A
             __syncthreads();
 #pragma unroll
             for (int r = 0; r < RT; ++r) {
-                const float f = ctl.factor[o_row + r];
+                const float f = ctl.factor[o_row + 2 * r];
 #pragma unroll
                 for (int j = 0; j < S::kCols; ++j) acc[j][r].x *= f, acc[j][r].y *= f, acc[j][r].z *= f, acc[j][r].w *= f;
             }
 #pragma unroll
             for (int j = 0; j < S::kCols; ++j) {
-                const int col = lane + 32 * j;
+                const int col = o_col + kColStep * j;
                 if (col >= vecs) break;
-#pragma unroll 2
+#pragma unroll 4
                 for (int k = 0; k < S::kKeys; k += 4) {
                     float4 w[RT], x[4];
 #pragma unroll
-                    for (int r = 0; r < RT; ++r) w[r] = *reinterpret_cast<const float4*>(scores + (o_row + r) * S::kScorePitch + k);
+                    for (int r = 0; r < RT; ++r) w[r] = *reinterpret_cast<const float4*>(scores + (o_row + 2 * r) * S::kScorePitch + k);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const float4*>(values + (k + i) * S::kPitch + col * 4);
 #pragma unroll
@@ -231,6 +248,7 @@ attend_f32_kernel(const __grid_constant__ CacheView c, const __grid_constant__ A
                     }
                 }
             }
+            find(t + 2);  // (tile t's places and units were last read before the last barrier but one)
             __syncthreads();
         }
         // To the output, or to this CTA's part of a divided segment.
@@ -247,30 +265,30 @@ attend_f32_kernel(const __grid_constant__ CacheView c, const __grid_constant__ A
         float* out_part = parts + static_cast<int64_t>(2 * blockIdx.x + (p.t0 == 0)) * S::kOut;
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
-            if (o_row + r >= rows) break;
-            const RowId rid = row_id(a, row0 + o_row + r);
+            if (o_row + 2 * r >= rows) break;
+            const RowId rid = row_id(a, row0 + o_row + 2 * r);
             const int64_t rbk = static_cast<int64_t>(b) * a.beams + beam0 + rid.beam;
             const int64_t place = (rbk * a.N + rid.token) * a.Hq + p.head * a.G + rid.head;
             const bool shown = rid.token < new_count(a, rbk);
-            const float m = ctl.top[o_row + r], l = ctl.sum[o_row + r];
+            const float m = ctl.top[o_row + 2 * r], l = ctl.sum[o_row + 2 * r];
             const float inverse = l > 0.0f ? 1.0f / l : l;
 #pragma unroll
             for (int j = 0; j < S::kCols; ++j) {
-                const int col = lane + 32 * j;
+                const int col = o_col + kColStep * j;
                 if (col >= vecs) break;
                 const float4 o = acc[j][r];
                 if (!whole) {
-                    *reinterpret_cast<float4*>(out_part + (o_row + r) * DP + col * 4) = o;
+                    *reinterpret_cast<float4*>(out_part + (o_row + 2 * r) * DP + col * 4) = o;
                 } else {
                     reinterpret_cast<float4*>(static_cast<float*>(a.out) + place * c.D)[col] =
                         shown ? make_float4(o.x * inverse, o.y * inverse, o.z * inverse, o.w * inverse)
                               : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                 }
             }
-            if (lane == 0) {
+            if (o_col == 0) {
                 if (!whole) {
-                    out_part[S::kRows * DP + o_row + r] = m;
-                    out_part[S::kRows * DP + S::kRows + o_row + r] = l;
+                    out_part[S::kRows * DP + o_row + 2 * r] = m;
+                    out_part[S::kRows * DP + S::kRows + o_row + 2 * r] = l;
                 } else if (a.lse != nullptr) {
                     a.lse[place] = shown && l != 0.0f ? (m + log2f(l)) * kLn2 : -INFINITY;
                 }
