@@ -3,34 +3,36 @@
 // Attention over the paged cache in float32, on the multiply-add pipe: the tensor cores would round
 // the operands to 11 bits.
 //
-// Blocks of 8, 16 or 32 query rows by tiles of 64 positions (32 for heads above 128), copied by
-// cp.async, the next tile while this one is worked on. Both products run on register tiles of up to
-// 4 x 4 (of float4 in one direction), so laid over a warp that its eight shared-memory reads of 16
-// bytes take 8 (scores) or 12 (values) passes of the banks for 64 multiply-adds: rows are padded by
-// 16 bytes, rows of one read lie next to each other. At 32 rows of 128 that is 4096 cycles a tile and
-// SM, at 8 rows the bytes bound it (2800 cycles).
+// Blocks of 16, 32 or 64 query rows by tiles of 64 positions (32 for heads above 128), copied by
+// cp.async, the next tile while this one is worked on. Scores run on register tiles of 4 x 4 (of
+// float4 along the head), outputs on 1, 2 or 4 rows by a float4: laid over a warp so that the eight
+// shared-memory reads of 16 bytes for 64 multiply-adds take 8 (12) passes of the banks: rows are
+// padded by 16 bytes, and rows of one read lie next to each other. At 32 rows of 128 the multiply-adds
+// take 4096 cycles a tile and SM, at 16 rows the bytes bound it (2800 cycles). 64 rows have 16 warps,
+// which hide each other's reads (165 rows over 14421: 335 us, with blocks of 32 and 8 warps 373); with
+// fewer rows 8 warps of larger tiles do better (32 rows over 16000: 184 us against 214).
 #include "attend.cuh"
 
 namespace dbsb {
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int threads_of(int rows) { return rows > 32 ? 512 : 256; }
 
-template <int DP, int RT>
+template <int DP, int ROWS>
 struct Shape {
-    static constexpr int kRows = 8 * RT;
+    static constexpr int kRows = ROWS, kThreads = threads_of(ROWS), kWarps = kThreads / 32;
     static constexpr int kKeys = DP > 128 ? 32 : 64;
-    static constexpr int kPitch = DP + 4;           // floats of a staged row
-    static constexpr int kSplit = 128 / kKeys;      // parts of the head that the scores' sums are taken in
-    static constexpr int kScorePitch = kKeys + 4;
+    static constexpr int kPitch = DP + 4;              // floats of a staged row
     static constexpr int kStage = 2 * kKeys * kPitch;  // floats: keys, values
+    // Scores: a warp has 16 rows by 32 positions of one part of the head.
+    static constexpr int kRowWarps = kRows / 16, kKeyWarps = kKeys / 32;
+    static constexpr int kSplit = kWarps / (kRowWarps * kKeyWarps);
+    static constexpr int kScorePitch = kKeys + 4;
     static constexpr int kScores = kRows * kScorePitch;
-    // Output: warps are kRowWarps by 8 / kRowWarps; a lane has RT rows and, of every 16 groups of four
-    // columns of its warp, one.
-    static constexpr int kRowWarps = 4;
-    static constexpr int kColWarps = 8 / kRowWarps;
-    static constexpr int kCols = DP / 4 / 16 / kColWarps;
+    // Output: half the warps by 2; a thread has kOwn rows and, of every 32 groups of four columns, one.
+    static constexpr int kOwn = kRows / kWarps;
+    static constexpr int kCols = DP / 128;
     static constexpr int kBytes = (2 * kStage + kSplit * kScores + kRows * kPitch) * 4;
     static constexpr int kOut = kRows * (DP + 2);
 };
@@ -40,8 +42,8 @@ struct Control {
     WorkSplit split;
     CacheUnit unit[2][4];
     int64_t row_at[2][64];  // of the tile's positions: the row's element among the pages of a layer's keys
-    int64_t query_at[32];
-    float factor[32], top[32], sum[32];
+    int64_t query_at[64];
+    float factor[64], top[64], sum[64];
     int last;
 };
 
@@ -49,10 +51,11 @@ __device__ __forceinline__ void copy16(float* to, const float* from) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_address(to)), "l"(from) : "memory");
 }
 
-template <int DP, int RT>
-__global__ void __launch_bounds__(kThreads, 1)
+template <int DP, int ROWS>
+__global__ void __launch_bounds__(threads_of(ROWS), 1)
 attend_f32_kernel(const __grid_constant__ CacheView c, const __grid_constant__ AttendParams a) {
-    using S = Shape<DP, RT>;
+    using S = Shape<DP, ROWS>;
+    constexpr int kThreads = S::kThreads;
     extern __shared__ __align__(16) float smem[];
     __shared__ Control ctl;
     float* stages = smem;
@@ -73,16 +76,14 @@ attend_f32_kernel(const __grid_constant__ CacheView c, const __grid_constant__ A
     int64_t base = work.base;
     const float scale = a.scale * kLog2e;
     const int vecs = c.D / 4;
-    // Scores: a warp has 4 * RT rows by 32 positions (a thread RT rows 4 apart, 4 positions 8 apart) of
-    // one part of the head.
-    const int row_half = warp & 1, key_half = S::kKeys == 64 ? (warp >> 1) & 1 : 0;
-    const int part = S::kKeys == 64 ? warp >> 2 : warp >> 1;
-    const int s_row = row_half * 4 * RT + (lane >> 3), s_key = key_half * 32 + (lane & 7);
-    // Weights: kThreads / kRows threads a row. Output: RT rows 2 apart by groups of four columns.
-    constexpr int kPerRow = kThreads / S::kRows, kEach = S::kKeys / kPerRow;
+    // Scores: a thread has rows 4 apart and positions 8 apart.
+    const int part = warp / (S::kRowWarps * S::kKeyWarps);
+    const int s_row = warp % S::kRowWarps * 16 + (lane >> 3), s_key = warp / S::kRowWarps % S::kKeyWarps * 32 + (lane & 7);
+    // Weights: kPerRow threads a row. Output: rows 2 apart.
+    constexpr int kPerRow = kThreads / S::kRows, kEach = S::kKeys / kPerRow, kOwn = S::kOwn;
     const int w_row = tid / kPerRow, w_key = tid % kPerRow;
-    const int o_row = (warp % S::kRowWarps) * 2 * RT + (lane >> 4), o_col = (warp / S::kRowWarps) * 16 + (lane & 15);
-    constexpr int kColStep = 16 * S::kColWarps;
+    const int o_row = warp % (S::kWarps / 2) * 2 * kOwn + (lane >> 4), o_col = warp / (S::kWarps / 2) * 16 + (lane & 15);
+    constexpr int kColStep = 32;
     const int64_t kind_step = static_cast<int64_t>(c.P) * c.H * c.page * c.D;
     const float* pages = static_cast<const float*>(c.pages) + static_cast<int64_t>(a.layer) * 2 * kind_step;
 
@@ -142,11 +143,11 @@ attend_f32_kernel(const __grid_constant__ CacheView c, const __grid_constant__ A
         const uint32_t bit = live ? 1u << id.beam : 0u;
         const uint8_t* fresh = a.mask ? a.mask + (bk * a.N + id.token) * a.N : nullptr;
         float top = -INFINITY, sum = 0.0f;
-        float4 acc[S::kCols][RT];
+        float4 acc[S::kCols][kOwn];
 #pragma unroll
         for (int j = 0; j < S::kCols; ++j)
 #pragma unroll
-            for (int r = 0; r < RT; ++r) acc[j][r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (int r = 0; r < kOwn; ++r) acc[j][r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 
         find(0);
         __syncthreads();
@@ -164,26 +165,26 @@ attend_f32_kernel(const __grid_constant__ CacheView c, const __grid_constant__ A
             const float* keys = stages + (t & 1) * S::kStage;
             const float* values = keys + S::kKeys * S::kPitch;
             {
-                float s[RT][4];
+                float s[4][4];
 #pragma unroll
-                for (int r = 0; r < RT; ++r)
+                for (int r = 0; r < 4; ++r)
 #pragma unroll
                     for (int k = 0; k < 4; ++k) s[r][k] = 0.0f;
 #pragma unroll 4
                 for (int v = part; v < vecs; v += S::kSplit) {
-                    float4 q[RT], x[4];
+                    float4 q[4], x[4];
 #pragma unroll
-                    for (int r = 0; r < RT; ++r) q[r] = *reinterpret_cast<const float4*>(query + (s_row + 4 * r) * S::kPitch + v * 4);
+                    for (int r = 0; r < 4; ++r) q[r] = *reinterpret_cast<const float4*>(query + (s_row + 4 * r) * S::kPitch + v * 4);
 #pragma unroll
                     for (int k = 0; k < 4; ++k) x[k] = *reinterpret_cast<const float4*>(keys + (s_key + 8 * k) * S::kPitch + v * 4);
 #pragma unroll
-                    for (int r = 0; r < RT; ++r)
+                    for (int r = 0; r < 4; ++r)
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
                             s[r][k] = fmaf(q[r].w, x[k].w, fmaf(q[r].z, x[k].z, fmaf(q[r].y, x[k].y, fmaf(q[r].x, x[k].x, s[r][k]))));
                 }
 #pragma unroll
-                for (int r = 0; r < RT; ++r)
+                for (int r = 0; r < 4; ++r)
 #pragma unroll
                     for (int k = 0; k < 4; ++k) scores[part * S::kScores + (s_row + 4 * r) * S::kScorePitch + s_key + 8 * k] = s[r][k];
             }
@@ -221,7 +222,7 @@ attend_f32_kernel(const __grid_constant__ CacheView c, const __grid_constant__ A
             }
             __syncthreads();
 #pragma unroll
-            for (int r = 0; r < RT; ++r) {
+            for (int r = 0; r < kOwn; ++r) {
                 const float f = ctl.factor[o_row + 2 * r];
 #pragma unroll
                 for (int j = 0; j < S::kCols; ++j) acc[j][r].x *= f, acc[j][r].y *= f, acc[j][r].z *= f, acc[j][r].w *= f;
@@ -232,13 +233,13 @@ attend_f32_kernel(const __grid_constant__ CacheView c, const __grid_constant__ A
                 if (col >= vecs) break;
 #pragma unroll 4
                 for (int k = 0; k < S::kKeys; k += 4) {
-                    float4 w[RT], x[4];
+                    float4 w[kOwn], x[4];
 #pragma unroll
-                    for (int r = 0; r < RT; ++r) w[r] = *reinterpret_cast<const float4*>(scores + (o_row + 2 * r) * S::kScorePitch + k);
+                    for (int r = 0; r < kOwn; ++r) w[r] = *reinterpret_cast<const float4*>(scores + (o_row + 2 * r) * S::kScorePitch + k);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const float4*>(values + (k + i) * S::kPitch + col * 4);
 #pragma unroll
-                    for (int r = 0; r < RT; ++r) {
+                    for (int r = 0; r < kOwn; ++r) {
                         const float y[4] = {w[r].x, w[r].y, w[r].z, w[r].w};
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
@@ -264,7 +265,7 @@ attend_f32_kernel(const __grid_constant__ CacheView c, const __grid_constant__ A
         int32_t* counters = static_cast<int32_t*>(a.workspace);
         float* out_part = parts + static_cast<int64_t>(2 * blockIdx.x + (p.t0 == 0)) * S::kOut;
 #pragma unroll
-        for (int r = 0; r < RT; ++r) {
+        for (int r = 0; r < kOwn; ++r) {
             if (o_row + 2 * r >= rows) break;
             const RowId rid = row_id(a, row0 + o_row + 2 * r);
             const int64_t rbk = static_cast<int64_t>(b) * a.beams + beam0 + rid.beam;
@@ -310,30 +311,34 @@ attend_f32_kernel(const __grid_constant__ CacheView c, const __grid_constant__ A
     }
 }
 
-template <int DP, int RT>
+template <int DP, int ROWS>
 cudaError_t launch_shape(const CacheView& c, const AttendParams& a, int sm_count, cudaStream_t stream) {
-    using S = Shape<DP, RT>;
-    auto* kernel = attend_f32_kernel<DP, RT>;
+    using S = Shape<DP, ROWS>;
+    static_assert(S::kBytes <= 224 * 1024);
+    auto* kernel = attend_f32_kernel<DP, ROWS>;
     static std::atomic<uint64_t> ready{0};  // a bit a device
     const cudaError_t e = allow_shared(kernel, S::kBytes, ready);
     if (e != cudaSuccess) return e;
-    return launch_after(kernel, sm_count, kThreads, S::kBytes, stream, c, a);
+    return launch_after(kernel, sm_count, S::kThreads, S::kBytes, stream, c, a);
 }
 
+// Rows of a block: as many as a group has, up to 64 (32 for heads above 128, which leave no room for
+// more). Rows past the group's cost multiply-adds with zeros.
 template <int DP>
 cudaError_t launch_width(const CacheView& c, const AttendParams& a, int sm_count, cudaStream_t stream) {
     const int beams = a.beams < kGroupBeams ? a.beams : kGroupBeams;
     const int64_t rows = static_cast<int64_t>(beams) * a.N * a.G;
-    if (rows <= 8) return launch_shape<DP, 1>(c, a, sm_count, stream);
-    if (rows <= 16) return launch_shape<DP, 2>(c, a, sm_count, stream);
-    return launch_shape<DP, 4>(c, a, sm_count, stream);
+    if (rows <= 16) return launch_shape<DP, 16>(c, a, sm_count, stream);
+    if constexpr (DP <= 128)
+        if (rows > 32) return launch_shape<DP, 64>(c, a, sm_count, stream);
+    return launch_shape<DP, 32>(c, a, sm_count, stream);
 }
 
 }  // namespace
 
 int64_t attend_f32_workspace(const CacheView&, const AttendParams&, int sm_count) {
     // A counter for each CTA (8192 bytes), then two partial results for each.
-    return 8192 + static_cast<int64_t>(2) * sm_count * Shape<256, 4>::kOut * 4;
+    return 8192 + static_cast<int64_t>(2) * sm_count * Shape<256, 32>::kOut * 4;
 }
 
 cudaError_t launch_attend_f32(const CacheView& c, const AttendParams& a, int sm_count, cudaStream_t stream) {
