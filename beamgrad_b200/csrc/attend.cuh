@@ -371,9 +371,9 @@ __device__ __forceinline__ void load_queries(const CacheView& c, const AttendPar
 }
 
 // The parts of a divided segment to the output, in their order, so that the result does not depend
-// on which CTA comes last. A part: kRows x DP sums, the rows' references (base 2), their weights'
-// sums. scratch: 16 * kRows bytes of shared memory. All kThreads threads of named barrier 1.
-template <class T, int kRows, int DP, int kThreads>
+// on which CTA comes last. A part: kRows x DP sums (kByColumn: four columns of all rows together, else
+// row by row), the rows' references (base 2), their weights' sums. scratch: 16 * kRows bytes of shared memory. All kThreads threads of named barrier 1.
+template <class T, int kRows, int DP, int kThreads, bool kByColumn>
 __device__ __forceinline__ void join_parts(const CacheView& c, const AttendParams& a, const Piece& p, Span span, int b,
                                            int beam0, int row0, int rows, const float* parts, void* scratch, int tid) {
     constexpr int kOut = kRows * (DP + 2), kVecs = DP / 4;
@@ -403,8 +403,9 @@ __device__ __forceinline__ void join_parts(const CacheView& c, const AttendParam
     }
     __syncwarp();
     asm volatile("barrier.sync 1, %0;" ::"r"(kThreads) : "memory");
-    constexpr int kEach = kThreads > 256 ? 4 : 8;
-    const int items = rows * kVecs;
+    constexpr int kEach = 8;
+    const int items = (kByColumn ? kRows : rows) * kVecs;
+    auto row_of = [](int i) { return kByColumn ? i % kRows : i / kVecs; };
 #pragma unroll 1
     for (int i0 = tid; i0 < items; i0 += kEach * kThreads) {
         float4 o[kEach];
@@ -417,9 +418,10 @@ __device__ __forceinline__ void join_parts(const CacheView& c, const AttendParam
             float w[kEach];
 #pragma unroll
             for (int e = 0; e < kEach; ++e) {
-                const int i = i0 + e * kThreads < items ? i0 + e * kThreads : i0, r = i / kVecs;
-                v[e] = __ldcg(reinterpret_cast<const float4*>(x + i * 4));
-                w[e] = __ldcg(x + kRows * DP + r) - refs[r];
+                const int i = i0 + e * kThreads, r = row_of(i);
+                const bool there = i < items && r < rows;
+                v[e] = there ? __ldcg(reinterpret_cast<const float4*>(x + i * 4)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                w[e] = there ? __ldcg(x + kRows * DP + r) - refs[r] : 0.0f;
             }
 #pragma unroll
             for (int e = 0; e < kEach; ++e) {
@@ -430,9 +432,8 @@ __device__ __forceinline__ void join_parts(const CacheView& c, const AttendParam
         }
 #pragma unroll
         for (int e = 0; e < kEach; ++e) {
-            const int i = i0 + e * kThreads, r = i / kVecs, vec = i % kVecs;
-            if (i >= items) break;
-            if (vec * 4 >= c.D) continue;
+            const int i = i0 + e * kThreads, r = row_of(i), vec = kByColumn ? i / kRows : i % kVecs;
+            if (i >= items || r >= rows || vec * 4 >= c.D) continue;
             const float f = factors[r];
             float4 y = make_float4(o[e].x * f, o[e].y * f, o[e].z * f, o[e].w * f);
             if (f == -1.0f) y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);

@@ -307,7 +307,7 @@ attend_f32_kernel(const __grid_constant__ CacheView c, const __grid_constant__ A
         __syncthreads();
         if (!ctl.last) continue;
         __threadfence();
-        join_parts<float, S::kRows, DP, kThreads>(c, a, p, span, b, beam0, row0, rows, parts, query, tid);
+        join_parts<float, S::kRows, DP, kThreads, false>(c, a, p, span, b, beam0, row0, rows, parts, query, tid);
     }
 }
 

@@ -437,7 +437,7 @@ attend_mma_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant
         named_sync(1, kComputeThreads);
         if (!ctl.last) continue;
         __threadfence();
-        join_parts<T, S::kRows, DP, kComputeThreads>(c, a, p, span, b, beam0, row0, rows, parts, join, tid);
+        join_parts<T, S::kRows, DP, kComputeThreads, false>(c, a, p, span, b, beam0, row0, rows, parts, join, tid);
     }
 }
 

@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(Shape<DP, NQ, COPIES>::kThreads, 1)
 attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ CacheView c,
                  const __grid_constant__ AttendParams a) {
     using S = Shape<DP, NQ, COPIES>;
-    constexpr int kHalves = S::kHalves, kSoftThreads = S::kSoftThreads, kThreads = S::kThreads;
+    constexpr int kHalves = S::kHalves, kSoftThreads = S::kSoftThreads;
     constexpr int kCopyWarp = S::kCopyWarp, kIssueWarp = S::kIssueWarp;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* query = smem + S::kSlots * S::kSlot;
@@ -228,15 +228,18 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
         barrier_init(smem_address(&ctl.queries), kSoftThreads / 32);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    // The plan was complete before the new tokens' copy began; only the pages have to be waited for.
-    const WorkSplit work = split_work<S::kRows>(c, a, tile_units, kMinTiles, ctl.sums, &ctl.split);
-    grid_wait();
+    // This kernel may run while the new tokens are still being written. Plan, lengths, queries and
+    // complete pages were there before that began; the copying warp waits for it at the first page
+    // that is not complete, the others before they look whether a value was not finite.
+    if (a.k == nullptr) grid_wait();
     grid_release();
-    if (__ldcg(c.status + 1) != 0) {
-        attend_all_rows<T>(c, a, reinterpret_cast<float*>(smem), warp, kThreads / 32);
+    const WorkSplit work = split_work<S::kRows>(c, a, tile_units, kMinTiles, ctl.sums, &ctl.split);
+    if (work.lo >= work.hi) {
+        grid_wait();
+        if (__ldcg(c.status + 1) != 0 && warp < kSoftThreads / 32)
+            attend_all_rows<T>(c, a, reinterpret_cast<float*>(smem), warp, kSoftThreads / 32);
         return;
     }
-    if (work.lo >= work.hi) return;
     if (warp == kIssueWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_address(&ctl.tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -255,7 +258,7 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
         if (warp > kIssueWarp) return;
         int used = 0;  // slots so far: K0 V0 K1 V1 ...
         if (warp == kCopyWarp) {
-            asm volatile("fence.proxy.async;" ::: "memory");
+            bool waited = false;
             for (int64_t cur = work.lo; cur < work.hi;) {
                 const Piece p = piece_at<S::kRows>(c, a, work, cur, group, base, tile_units);
                 const CacheUnit* units = c.units + static_cast<int64_t>(p.group) * c.unit_cap;
@@ -263,14 +266,21 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
                 // The page of this lane's copy; past the last unit, page 0: whatever finite values lie
                 // there meet weights of zero.
                 const int which = lane / S::kBlocks, block = lane % S::kBlocks;
-                auto page_of = [&](int t) {
+                auto unit_of = [&](int t) {
                     const int i = (p.t0 + t) * tile_units + which;
-                    return t < n_tiles && which < tile_units && i < p.units ? __ldg(&units[i].page) : 0;
+                    return t < n_tiles && which < tile_units && i < p.units ? __ldg(reinterpret_cast<const int4*>(units + i))
+                                                                            : make_int4(0, 0, 0, -1);
                 };
-                int page = page_of(0);
+                int4 next = unit_of(0);
 #pragma unroll 1
                 for (int t = 0; t < n_tiles; ++t) {
-                    const int next = page_of(t + 1);
+                    const int page = next.x;
+                    if (!waited && __any_sync(0xffffffffu, next.w >= 0)) {
+                        grid_wait();
+                        asm volatile("fence.proxy.async;" ::: "memory");
+                        waited = true;
+                    }
+                    next = unit_of(t + 1);
 #pragma unroll 1
                     for (int kind = 0; kind < 2; ++kind, ++used) {
                         const int slot = used % S::kSlots;
@@ -285,7 +295,6 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
                                      static_cast<int>(row), full);
                         }
                     }
-                    page = next;
                 }
                 cur += n_tiles;
             }
@@ -602,7 +611,12 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
             }
         }
 
-        // To the output, or to this CTA's part of a divided segment.
+        // A value that is not finite was met, in this call or before: weights of zero did not keep it out
+        // of the products. All CTAs see that and leave these outputs alone.
+        grid_wait();
+        if (__ldcg(c.status + 1) != 0) continue;
+        // To the output, or to this CTA's part of a divided segment (of which four columns of all rows lie
+        // together).
         const bool whole = p.t0 == 0 && p.t1 == p.tiles;
         float* parts = static_cast<float*>(a.workspace) + 2048;
         int32_t* counters = static_cast<int32_t*>(a.workspace);
@@ -639,7 +653,7 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
                 } else {
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
-                        *reinterpret_cast<uint4*>(part + my_row * DP + i * 32 + e * 4) =
+                        *reinterpret_cast<uint4*>(part + ((i * 8 + e) * S::kRows + my_row) * 4) =
                             make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
                 }
             }
@@ -719,7 +733,7 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
                         if (f == -1.0f) v = make_uint2(0, 0);
                         *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + to[k] + i * 32) = v;
                     } else {
-                        *reinterpret_cast<float4*>(part + r * DP + i * 32 + vec * 4) = o;
+                        *reinterpret_cast<float4*>(part + ((i * 8 + vec) * S::kRows + r) * 4) = o;
                     }
                 }
                 named_sync(1, kSoftThreads);
@@ -747,10 +761,11 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
         named_sync(1, kSoftThreads);
         if (!ctl.last) continue;
         __threadfence();
-        join_parts<T, S::kRows, DP, kSoftThreads>(c, a, p, span, b, beam0, row0, rows, parts, query, tid);
+        join_parts<T, S::kRows, DP, kSoftThreads, true>(c, a, p, span, b, beam0, row0, rows, parts, query, tid);
     }
     fence_before();
     named_sync(2, kSoftThreads + 32);
+    if (__ldcg(c.status + 1) != 0) attend_all_rows<T>(c, a, reinterpret_cast<float*>(query), warp, kSoftThreads / 32);
 }
 
 template <class T, int DP, int NQ, int COPIES>
