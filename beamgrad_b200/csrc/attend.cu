@@ -8,7 +8,7 @@ namespace dbsb {
 
 namespace {
 
-constexpr int kAppendThreads = 256;
+constexpr int kAppendThreads = 128;
 
 // Keys and values of the new tokens into their pages, 16 bytes a thread. A value that is not
 // finite raises the cache's second status word: the attention then keeps masked values out of its
@@ -28,8 +28,12 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
         const int j = static_cast<int>(rest % a.N);
         const int64_t bk = rest / a.N;
         const int64_t b = bk / a.beams, k = bk % a.beams;
-        if (j >= new_count(a, bk)) continue;
+        // The rows are on their way while their place is looked up.
+        const T* ks = static_cast<const T*>(a.k) + b * a.ks[0] + k * a.ks[1] + j * a.ks[2] + h * a.ks[3];
+        const T* vs = static_cast<const T*>(a.v) + b * a.vs[0] + k * a.vs[1] + j * a.vs[2] + h * a.vs[3];
+        const uint4 kx = __ldg(reinterpret_cast<const uint4*>(ks) + vec), vx = __ldg(reinterpret_cast<const uint4*>(vs) + vec);
         const int64_t slot = b * c.K + k, pos = static_cast<int64_t>(c.lengths[slot]) + j, col = pos >> c.page_log2;
+        if (j >= new_count(a, bk)) continue;
         if (col >= c.M) {
             atomicOr(c.status, DBS_CUDA_CACHE_STATUS_CAPACITY);
             continue;
@@ -38,9 +42,6 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
         if (p < 0) continue;
         const int64_t block = static_cast<int64_t>(a.layer) * 2 * c.P + p;
         const int64_t row = pos & (c.page - 1);
-        const T* ks = static_cast<const T*>(a.k) + b * a.ks[0] + k * a.ks[1] + j * a.ks[2] + h * a.ks[3];
-        const T* vs = static_cast<const T*>(a.v) + b * a.vs[0] + k * a.vs[1] + j * a.vs[2] + h * a.vs[3];
-        const uint4 kx = reinterpret_cast<const uint4*>(ks)[vec], vx = reinterpret_cast<const uint4*>(vs)[vec];
         uint4* pages = static_cast<uint4*>(c.pages);
         pages[((block * c.H + h) * c.page + row) * vecs + vec] = kx;
         pages[(((block + c.P) * c.H + h) * c.page + row) * vecs + vec] = vx;
@@ -53,7 +54,13 @@ template <class T>
 cudaError_t launch_append(const CacheView& c, const AttendParams& a, int sm_count, cudaStream_t stream) {
     if (a.k == nullptr) return cudaSuccess;
     const int64_t items = static_cast<int64_t>(c.B) * a.beams * a.N * c.H * (c.D / Pack<T>::n);
-    const int64_t want = (items + kAppendThreads - 1) / kAppendThreads, cap = static_cast<int64_t>(sm_count) * 8;
+    // Two small CTAs an SM at the most: their registers fit beside those of the attention's CTA, which
+    // else waits for a place (4 us of 100 on the SMs that this kernel has).
+    const int64_t want = (items + kAppendThreads - 1) / kAppendThreads, cap = 2 * sm_count;
+    // The same split of the SM's memory as the attention's: it would wait for the SM to change it.
+    static std::atomic<uint64_t> ready{0};
+    const cudaError_t e = prefer_shared(append_kernel<T>, ready);
+    if (e != cudaSuccess) return e;
     return launch_after(append_kernel<T>, static_cast<unsigned>(want < cap ? want : cap), kAppendThreads, 0, stream, c, a);
 }
 

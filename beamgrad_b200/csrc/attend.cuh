@@ -383,27 +383,48 @@ __device__ __forceinline__ void join_parts(const CacheView& c, const AttendParam
     int64_t* places = static_cast<int64_t*>(scratch);
     float* refs = reinterpret_cast<float*>(places + kRows);
     float* factors = refs + kRows;  // 1 / sum; -1 for rows that are not shown
+    // The rows' common references and sums: eight lanes a row, each for every eighth part.
 #pragma unroll 1
-    for (int r = tid; r < rows; r += kThreads) {
+    for (int r0 = 0; r0 < rows; r0 += kThreads / 8) {
+        const int r = r0 + tid / 8, lane = tid % 8;
         float m = -INFINITY, l = 0.0f;
-#pragma unroll 4
-        for (int j = 0; j < n_parts; ++j) m = fmaxf(m, __ldcg(part_of(j) + kRows * DP + r));
-        const float ref = m == -INFINITY ? 0.0f : m;
-#pragma unroll 4
-        for (int j = 0; j < n_parts; ++j)
-            l = fmaf(__ldcg(part_of(j) + kRows * DP + kRows + r), exp2_fast(__ldcg(part_of(j) + kRows * DP + r) - ref), l);
-        const RowId id = row_id(a, row0 + r);
-        const int64_t bk = static_cast<int64_t>(b) * a.beams + beam0 + id.beam;
-        const bool shown = id.token < new_count(a, bk);
-        const int64_t at = (bk * a.N + id.token) * a.Hq + p.head * a.G + id.head;
-        places[r] = at;
-        refs[r] = ref;
-        factors[r] = shown ? (l > 0.0f ? 1.0f / l : l) : -1.0f;
-        if (a.lse != nullptr) a.lse[at] = shown && l != 0.0f ? (m + log2f(l)) * kLn2 : -INFINITY;
+#pragma unroll 1
+        for (int j0 = 0; j0 < n_parts; j0 += 32) {
+            float pm[4], pl[4], now = m;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int j = j0 + lane + 8 * k;
+                const bool there = j < n_parts && r < rows;
+                pm[k] = there ? __ldcg(part_of(j) + kRows * DP + r) : -INFINITY;
+                pl[k] = there ? __ldcg(part_of(j) + kRows * DP + kRows + r) : 0.0f;
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) now = fmaxf(now, pm[k]);
+#pragma unroll
+            for (int d = 4; d > 0; d >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, d));
+            const float ref = now == -INFINITY ? 0.0f : now;
+            l *= exp2_fast(m - ref);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) l = fmaf(pl[k], exp2_fast(pm[k] - ref), l);
+            m = now;
+        }
+#pragma unroll
+        for (int d = 4; d > 0; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+        if (r < rows && lane == 0) {
+            const RowId id = row_id(a, row0 + r);
+            const int64_t bk = static_cast<int64_t>(b) * a.beams + beam0 + id.beam;
+            const bool shown = id.token < new_count(a, bk);
+            const int64_t at = (bk * a.N + id.token) * a.Hq + p.head * a.G + id.head;
+            places[r] = at;
+            refs[r] = m == -INFINITY ? 0.0f : m;
+            factors[r] = shown ? (l > 0.0f ? 1.0f / l : l) : -1.0f;
+            if (a.lse != nullptr) a.lse[at] = shown && l != 0.0f ? (m + log2f(l)) * kLn2 : -INFINITY;
+        }
     }
     __syncwarp();
     asm volatile("barrier.sync 1, %0;" ::"r"(kThreads) : "memory");
-    constexpr int kEach = 8;
+    // Four values of four items from four parts (two, with 512 threads' registers) in flight.
+    constexpr int kEach = 4, kPartsAtOnce = kThreads > 256 ? 2 : 4;
     const int items = (kByColumn ? kRows : rows) * kVecs;
     auto row_of = [](int i) { return kByColumn ? i % kRows : i / kVecs; };
 #pragma unroll 1
@@ -412,23 +433,28 @@ __device__ __forceinline__ void join_parts(const CacheView& c, const AttendParam
 #pragma unroll
         for (int e = 0; e < kEach; ++e) o[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 1
-        for (int j = 0; j < n_parts; ++j) {
-            const float* x = part_of(j);
-            float4 v[kEach];
-            float w[kEach];
+        for (int j0 = 0; j0 < n_parts; j0 += kPartsAtOnce) {
+            float4 v[kPartsAtOnce][kEach];
+            float w[kPartsAtOnce][kEach];
 #pragma unroll
-            for (int e = 0; e < kEach; ++e) {
-                const int i = i0 + e * kThreads, r = row_of(i);
-                const bool there = i < items && r < rows;
-                v[e] = there ? __ldcg(reinterpret_cast<const float4*>(x + i * 4)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                w[e] = there ? __ldcg(x + kRows * DP + r) - refs[r] : 0.0f;
+            for (int k = 0; k < kPartsAtOnce; ++k) {
+                const float* x = part_of(j0 + k < n_parts ? j0 + k : j0);
+#pragma unroll
+                for (int e = 0; e < kEach; ++e) {
+                    const int i = i0 + e * kThreads, r = row_of(i);
+                    const bool there = i < items && r < rows && j0 + k < n_parts;
+                    v[k][e] = there ? __ldcg(reinterpret_cast<const float4*>(x + i * 4)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    w[k][e] = there ? __ldcg(x + kRows * DP + r) - refs[r] : 0.0f;
+                }
             }
 #pragma unroll
-            for (int e = 0; e < kEach; ++e) {
-                const float f = exp2_fast(w[e]);
-                o[e].x = fmaf(v[e].x, f, o[e].x), o[e].y = fmaf(v[e].y, f, o[e].y);
-                o[e].z = fmaf(v[e].z, f, o[e].z), o[e].w = fmaf(v[e].w, f, o[e].w);
-            }
+            for (int k = 0; k < kPartsAtOnce; ++k)
+#pragma unroll
+                for (int e = 0; e < kEach; ++e) {
+                    const float f = exp2_fast(w[k][e]);
+                    o[e].x = fmaf(v[k][e].x, f, o[e].x), o[e].y = fmaf(v[k][e].y, f, o[e].y);
+                    o[e].z = fmaf(v[k][e].z, f, o[e].z), o[e].w = fmaf(v[k][e].w, f, o[e].w);
+                }
         }
 #pragma unroll
         for (int e = 0; e < kEach; ++e) {
@@ -488,17 +514,25 @@ __device__ __forceinline__ void tma_load(uint32_t to, const CUtensorMap* map, in
         : "memory");
 }
 
-// Lets a kernel have that much shared memory, once a device. ready: a bit for each that has it.
+// Sets a kernel's attribute once a device. ready: a bit for each that has it.
 template <class Kernel>
-cudaError_t allow_shared(Kernel* kernel, int bytes, std::atomic<uint64_t>& ready) {
+cudaError_t set_once(Kernel* kernel, cudaFuncAttribute attribute, int value, std::atomic<uint64_t>& ready) {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     const uint64_t bit = uint64_t{1} << (dev & 63);
     if (dev < 64 && (ready.load(std::memory_order_acquire) & bit) != 0) return cudaSuccess;
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    e = cudaFuncSetAttribute(kernel, attribute, value);
     if (e == cudaSuccess && dev < 64) ready.fetch_or(bit, std::memory_order_release);
     return e;
+}
+template <class Kernel>
+cudaError_t allow_shared(Kernel* kernel, int bytes, std::atomic<uint64_t>& ready) {
+    return set_once(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes, ready);
+}
+template <class Kernel>
+cudaError_t prefer_shared(Kernel* kernel, std::atomic<uint64_t>& ready) {
+    return set_once(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared, ready);
 }
 
 // The tensor map of the pages as [rows, head_dim], boxes of one page by 64 elements, swizzled so

@@ -54,7 +54,8 @@ struct Shape {
     static constexpr int kHalves = COPIES == 1 ? 2 : 1;   // warpgroups of a stream
     static constexpr int kCols = 128 / (COPIES * kHalves);  // positions of a tile that a thread weighs
     static constexpr int kSoftThreads = 256 * kHalves;
-    static constexpr int kThreads = kSoftThreads + 128;   // and a warpgroup with the copying and the issuing warp
+    // And the copying and the issuing warp, in a warpgroup where registers change hands.
+    static constexpr int kThreads = kSoftThreads + (kHalves == 2 ? 128 : 64);
     static constexpr int kCopyWarp = kSoftThreads / 32, kIssueWarp = kCopyWarp + 1;
     static constexpr int kBlocks = DP / 64;
     static constexpr int kSlot = kTileKeys * DP * 2;
@@ -251,7 +252,7 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
     int group = work.group;
     int64_t base = work.base;
 
-    // Registers: 640 threads are launched with 96 each, 512 x 104 + 128 x 64 (384 have 168 each, which
+    // Registers: 640 threads are launched with 96 each, 512 x 104 + 128 x 64 (320 have 168 each, which
     // is enough for all roles).
     if (warp >= kCopyWarp) {
         if constexpr (kHalves == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
@@ -379,8 +380,37 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
     const float scale = fmaxf(fabsf(a.scale) * kLog2e, 1.2e-38f);
     const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;  // a negative scale turns the queries' signs
     uint32_t score_phase = 0, output_phase = 0;
-    for (int64_t cur = work.lo; cur < work.hi;) {
-        const Piece p = piece_at<S::kRows>(c, a, work, cur, group, base, tile_units);
+    bool odd = false, odd_known = false;  // whether a value that is not finite was met, in this call or before
+    // The next segment's place, and with few rows its queries, are fetched before this one's output.
+    constexpr int kChunks8 = DP / 8, kAhead = COPIES > 1 ? S::kRows * kChunks8 / kSoftThreads : 1;
+    uint4 ahead[kAhead];
+    auto fetch_ahead = [&](const Piece& p) {
+        if constexpr (COPIES > 1) {
+            const int b = p.group / c.groups, beam0 = (p.group - b * c.groups) * kGroupBeams, chunk = tid % kChunks8;
+            const T* q = static_cast<const T*>(a.q) + b * a.qs[0] + beam0 * a.qs[1] + p.head * a.G * a.qs[3] + chunk * 8;
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                const int r = p.block * S::kRows + tid / kChunks8 + k * (kSoftThreads / kChunks8);
+                ahead[k] = make_uint4(0, 0, 0, 0);
+                if (r < p.rows && chunk * 8 < c.D) {
+                    const RowId id = row_id(a, r);
+                    ahead[k] = __ldg(reinterpret_cast<const uint4*>(q + id.beam * a.qs[1] + id.token * a.qs[2] + id.head * a.qs[3]));
+                }
+            }
+        }
+    };
+    auto put_query = [&](int r, int chunk, uint4 v) {
+        v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
+#pragma unroll
+        for (int i = 0; i < (NQ == 2 ? 1 : COPIES); ++i) {
+            const int in = (r & 127) + i * S::kRows;
+            *reinterpret_cast<uint4*>(query + (r >> 7) * (128 * DP * 2) + (chunk >> 3) * (128 * 128) + in * 128 +
+                                      (((chunk & 7) ^ (in & 7)) << 4)) = v;
+        }
+    };
+    Piece p = piece_at<S::kRows>(c, a, work, work.lo, group, base, tile_units), next_piece = p;
+    fetch_ahead(p);
+    for (int64_t cur = work.lo; cur < work.hi; p = next_piece) {
         const int n_tiles = p.t1 - p.t0;
         cur += n_tiles;
         const int b = p.group / c.groups, beam0 = (p.group - b * c.groups) * kGroupBeams;
@@ -391,18 +421,15 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
         if (mine) id = row_id(a, row0 + my_row);
         // Both streams are done with the last segment's products, and so with its queries.
         named_sync(1, kSoftThreads);
-        if (half == 0 && (NQ == 2 || (stream == 0 && copy == 0)))
-            ctl.query_at[my_row] = b * a.qs[0] + (beam0 + id.beam) * a.qs[1] + id.token * a.qs[2] + (p.head * a.G + id.head) * a.qs[3];
-        named_sync(1, kSoftThreads);
-        load_queries<T, S::kRows, DP, kSoftThreads>(c, a, ctl.query_at, rows, tid, [&](int r, int chunk, uint4 v) {
-            v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
+        if constexpr (COPIES > 1) {
 #pragma unroll
-            for (int i = 0; i < (NQ == 2 ? 1 : COPIES); ++i) {
-                const int in = (r & 127) + i * S::kRows;
-                *reinterpret_cast<uint4*>(query + (r >> 7) * (128 * DP * 2) + (chunk >> 3) * (128 * 128) + in * 128 +
-                                          (((chunk & 7) ^ (in & 7)) << 4)) = v;
-            }
-        });
+            for (int k = 0; k < kAhead; ++k) put_query(tid / kChunks8 + k * (kSoftThreads / kChunks8), tid % kChunks8, ahead[k]);
+        } else {
+            if (half == 0 && (NQ == 2 || stream == 0))
+                ctl.query_at[my_row] = b * a.qs[0] + (beam0 + id.beam) * a.qs[1] + id.token * a.qs[2] + (p.head * a.G + id.head) * a.qs[3];
+            named_sync(1, kSoftThreads);
+            load_queries<T, S::kRows, DP, kSoftThreads>(c, a, ctl.query_at, rows, tid, put_query);
+        }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) barrier_arrive(smem_address(&ctl.queries));
@@ -604,17 +631,25 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
                 __syncwarp();
                 if (lane == 0) barrier_arrive(weights_bar);
             }
-            if (began) {
-                barrier_wait(smem_address(&ctl.output[stream]), output_phase, c.status);
-                output_phase ^= 1;
-                fence_after();
-            }
         }
+        if (cur < work.hi) {
+            next_piece = piece_at<S::kRows>(c, a, work, cur, group, base, tile_units);
+            fetch_ahead(next_piece);
+        }
+        if (!odd_known) {
+            grid_wait();
+            odd = __ldcg(c.status + 1) != 0;
+            odd_known = true;
+        }
+        if (began) {
+            barrier_wait(smem_address(&ctl.output[stream]), output_phase, c.status);
+            output_phase ^= 1;
+            fence_after();
+        }
+        // Weights of zero did not keep a value that is not finite out of the products. All CTAs see that
+        // and leave these outputs alone.
+        if (odd) continue;
 
-        // A value that is not finite was met, in this call or before: weights of zero did not keep it out
-        // of the products. All CTAs see that and leave these outputs alone.
-        grid_wait();
-        if (__ldcg(c.status + 1) != 0) continue;
         // To the output, or to this CTA's part of a divided segment (of which four columns of all rows lie
         // together).
         const bool whole = p.t0 == 0 && p.t1 == p.tiles;
@@ -622,21 +657,65 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
         int32_t* counters = static_cast<int32_t*>(a.workspace);
         float* part = parts + static_cast<int64_t>(2 * blockIdx.x + (p.t0 == 0)) * S::kOut;
         float m = top == -INFINITY ? top : top * scale, l = sum;  // base-2 maximum, sum
-        const bool holds_rows = began && (my_row & ~31) < rows;   // of the warp
+        const bool holds_rows = (my_row & ~31) < rows && (NQ == 1 || began);  // of the warp
         if constexpr (kHalves == 2) {
             named_sync(1, kSoftThreads);  // (query_at shares the space)
             ctl.half[stream][half][row] = l;
             named_sync(1, kSoftThreads);
             l += ctl.half[stream][half ^ 1][row];
         }
-        if constexpr (NQ == 2) {
-            const float inverse = l > 0.0f ? 1.0f / l : l;
-            const int64_t place = (bk * a.N + id.token) * a.Hq + p.head * a.G + id.head;
+        // NQ = 1: the row's 2 * COPIES results, stream by stream. A warpgroup of either stream reads the
+        // outputs of both, for 32 columns of its own at a time.
+        constexpr int kParts = NQ == 2 ? 1 : 2 * COPIES;
+        const int streams = n_tiles > 1 ? 2 : 1;  // a segment of one tile has no second stream
+        auto row_stats = [&](int r, float* ref, float* total) {
+            float top_all = -INFINITY, l_all = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kParts; ++i) top_all = fmaxf(top_all, ctl.top[i * S::kRows + r]);
+            *ref = top_all == -INFINITY ? 0.0f : top_all;
+#pragma unroll
+            for (int i = 0; i < kParts; ++i) l_all = fmaf(ctl.sum[i * S::kRows + r], exp2_fast(ctl.top[i * S::kRows + r] - *ref), l_all);
+            *total = l_all;
+            return top_all;
+        };
+        float factor0 = 1.0f, factor1 = 0.0f;
+        if constexpr (NQ == 1) {
+            if constexpr (COPIES == 1) named_sync(1, kSoftThreads);  // (half shares the space)
+            ctl.top[(stream * COPIES + copy) * S::kRows + my_row] = m;
+            ctl.sum[(stream * COPIES + copy) * S::kRows + my_row] = l;
+            fence_before();
+            named_sync(1, kSoftThreads);
+            fence_after();
+            float ref;
+            m = row_stats(my_row, &ref, &l);
+            factor0 = exp2_fast(ctl.top[copy * S::kRows + my_row] - ref);
+            factor1 = exp2_fast(ctl.top[(COPIES + copy) * S::kRows + my_row] - ref);
+        }
+        const uint32_t from = NQ == 2 ? o_at : tmem + lanes + 256;
+        auto columns = [&](uint32_t (&o)[32], int i) {
+            tmem_load(o, from + 32 * i);
+            if constexpr (NQ == 1) {
+                uint32_t x[32];
+                if (streams > 1) {
+                    tmem_load(x, from + 128 + 32 * i);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) x[e] = 0;
+                }
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                    o[e] = __float_as_uint(fmaf(__uint_as_float(o[e]), factor0, __uint_as_float(x[e]) * factor1));
+            }
+        };
+        const int64_t place = (bk * a.N + id.token) * a.Hq + p.head * a.G + id.head;
+        const float inverse = l > 0.0f ? 1.0f / l : l;
+        const int groups = NQ == 2 ? kHalves : 2 * kHalves, my_group = NQ == 2 ? half : stream * kHalves + half;
+        if constexpr (COPIES == 1) {
             T* out = static_cast<T*>(a.out) + place * c.D;
 #pragma unroll 1
-            for (int i = half * (DP / 64); i < (half + 1) * (DP / 64); ++i) {
+            for (int i = my_group; i < DP / 32; i += groups) {
                 uint32_t o[32];
-                if (holds_rows) tmem_load(o, o_at + 32 * i);
+                if (holds_rows) columns(o, i);
                 if (!mine) continue;
                 if (whole) {
 #pragma unroll
@@ -657,78 +736,48 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
                             make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
                 }
             }
-            if (mine && half == 0) {
-                if (whole) {
-                    if (a.lse != nullptr) a.lse[place] = live && l != 0.0f ? (m + log2f(l)) * kLn2 : -INFINITY;
-                } else {
-                    part[S::kRows * DP + my_row] = m;
-                    part[S::kRows * DP + S::kRows + my_row] = l;
-                }
-            }
         } else {
-            // The rows' 2 * COPIES partial results, 32 columns at a time through shared memory.
-            constexpr int kParts = 2 * COPIES;
-            const int which = stream * COPIES + copy;
-            named_sync(1, kSoftThreads);  // (query_at shares the space)
-            ctl.top[which * S::kRows + my_row] = m;
-            ctl.sum[which * S::kRows + my_row] = l;
-            named_sync(1, kSoftThreads);
-            auto row_stats = [&](int r, float* ref, float* total) {
-                float top_all = -INFINITY, l_all = 0.0f;
-#pragma unroll
-                for (int i = 0; i < kParts; ++i) top_all = fmaxf(top_all, ctl.top[i * S::kRows + r]);
-                *ref = top_all == -INFINITY ? 0.0f : top_all;
-#pragma unroll
-                for (int i = 0; i < kParts; ++i) l_all = fmaf(ctl.sum[i * S::kRows + r], exp2_fast(ctl.top[i * S::kRows + r] - *ref), l_all);
-                *total = l_all;
-                return top_all;
-            };
-            float ref, total;
-            const float top_all = row_stats(my_row, &ref, &total);
-            const float factor = exp2_fast(m - ref);
-            // The rows that this thread puts together, four columns of each at a time.
-            constexpr int kEach = S::kRows * 8 / kSoftThreads;
-            const int vec = tid & 7, streams = n_tiles > 1 ? 2 : 1;  // a segment of one tile has no second stream
+            // The copies, through shared memory: a warpgroup's [copy][row][8], swizzled.
+            constexpr int kEach = S::kRows / 16;  // rows that a thread puts together, four columns of each
+            const int t = tid & 127, vec = t & 7;
             int64_t to[kEach];
-            float inverse[kEach];  // -1: rows that are not shown
+            float scales[kEach];  // -1: rows that are not shown
 #pragma unroll
             for (int k = 0; k < kEach; ++k) {
-                const int r = (tid >> 3) + kSoftThreads / 8 * k;
+                const int r = (t >> 3) + 16 * k;
                 if (r >= rows) break;
                 const RowId rid = row_id(a, row0 + r);
                 const int64_t rbk = static_cast<int64_t>(b) * a.beams + beam0 + rid.beam;
                 to[k] = ((rbk * a.N + rid.token) * a.Hq + p.head * a.G + rid.head) * c.D + vec * 4;
                 float unused, l_row;
                 row_stats(r, &unused, &l_row);
-                inverse[k] = rid.token < new_count(a, rbk) ? (l_row > 0.0f ? 1.0f / l_row : l_row) : -1.0f;
+                scales[k] = rid.token < new_count(a, rbk) ? (l_row > 0.0f ? 1.0f / l_row : l_row) : -1.0f;
             }
-            float4* stage = reinterpret_cast<float4*>(query);  // [which][row][8], swizzled
+            float4* stage = reinterpret_cast<float4*>(query) + stream * 1024;
 #pragma unroll 1
-            for (int i = 0; i < DP / 32; ++i) {
-                if (holds_rows && (kHalves == 1 || half == (i & 1))) {
+            for (int i = my_group; i < DP / 32; i += groups) {
+                if (holds_rows) {
                     uint32_t o[32];
-                    tmem_load(o, o_at + 32 * i);
+                    columns(o, i);
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
-                        stage[(which * S::kRows + my_row) * 8 + (e ^ (my_row & 7))] =
-                            make_float4(__uint_as_float(o[4 * e]) * factor, __uint_as_float(o[4 * e + 1]) * factor,
-                                        __uint_as_float(o[4 * e + 2]) * factor, __uint_as_float(o[4 * e + 3]) * factor);
+                        stage[row * 8 + (e ^ (row & 7))] = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]),
+                                                                        __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
                 }
-                named_sync(1, kSoftThreads);
+                named_sync(3 + stream, 128);
 #pragma unroll
                 for (int k = 0; k < kEach; ++k) {
-                    const int r = (tid >> 3) + kSoftThreads / 8 * k;
+                    const int r = (t >> 3) + 16 * k;
                     if (r >= rows) break;
                     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-                    for (int j = 0; j < kParts; ++j) {
-                        if (j / COPIES >= streams) break;
+                    for (int j = 0; j < COPIES; ++j) {
                         const float4 x = stage[(j * S::kRows + r) * 8 + (vec ^ (r & 7))];
                         o.x += x.x, o.y += x.y, o.z += x.z, o.w += x.w;
                     }
                     if (i * 32 + vec * 4 >= c.D) continue;
                     if (whole) {
-                        const float f = inverse[k];
+                        const float f = scales[k];
                         uint2 v = make_uint2(Pack<T>::pair(o.x * f, o.y * f), Pack<T>::pair(o.z * f, o.w * f));
                         if (f == -1.0f) v = make_uint2(0, 0);
                         *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + to[k] + i * 32) = v;
@@ -736,17 +785,15 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
                         *reinterpret_cast<float4*>(part + ((i * 8 + vec) * S::kRows + r) * 4) = o;
                     }
                 }
-                named_sync(1, kSoftThreads);
+                named_sync(3 + stream, 128);
             }
-            if (mine && which == 0 && half == 0) {
-                if (whole) {
-                    if (a.lse != nullptr)
-                        a.lse[(bk * a.N + id.token) * a.Hq + p.head * a.G + id.head] =
-                            live && total != 0.0f ? (top_all + log2f(total)) * kLn2 : -INFINITY;
-                } else {
-                    part[S::kRows * DP + my_row] = top_all;
-                    part[S::kRows * DP + S::kRows + my_row] = total;
-                }
+        }
+        if (mine && half == 0 && copy == 0 && (NQ == 2 || stream == 0)) {
+            if (whole) {
+                if (a.lse != nullptr) a.lse[place] = live && l != 0.0f ? (m + log2f(l)) * kLn2 : -INFINITY;
+            } else {
+                part[S::kRows * DP + my_row] = m;
+                part[S::kRows * DP + S::kRows + my_row] = l;
             }
         }
         if (whole) continue;
@@ -765,7 +812,7 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
     }
     fence_before();
     named_sync(2, kSoftThreads + 32);
-    if (__ldcg(c.status + 1) != 0) attend_all_rows<T>(c, a, reinterpret_cast<float*>(query), warp, kSoftThreads / 32);
+    if (odd) attend_all_rows<T>(c, a, reinterpret_cast<float*>(query), warp, kSoftThreads / 32);
 }
 
 template <class T, int DP, int NQ, int COPIES>
