@@ -1,14 +1,15 @@
 // SPDX-License-Identifier: MIT
 //
-// Attention of few query rows a key head (a token or a short draft a beam) over the paged cache,
-// for float16 and bfloat16.
+// Attention over the paged cache for float16 and bfloat16 heads of 136 to 256, on mma.sync: 128 rows
+// of such an output do not leave tensor memory room for two streams of scores (attend_tc.cu), and with
+// 16 or 32 rows a block the bytes decide.
 //
 // Bound by the bytes of keys and values: each is read once for all rows of a group of beams, and
 // every SM reads an equal share (attend.cuh). A producer warp copies tiles of 64 positions
 // through a ring of stages by TMA; eight warps compute, each on 16 positions of a tile and all
 // rows: with positions instead of rows divided among the warps, a key or value is taken from
 // shared memory once, by one warp, and no warp waits for another inside the loop. Each warp keeps
-// the running maximum, sum and output of its positions (in 32 bits); the eight are joined once, at
+// the running maximum, sum and output of its positions (in 32 bits); the warps are joined once, at
 // the end of a segment.
 //
 // Scores are taken in base 2: scale * log2(e) is applied to the 32-bit product. Weights are
@@ -19,20 +20,21 @@ namespace dbsb {
 
 namespace {
 
+constexpr int DP = 256;  // the head, padded
 constexpr int kTileKeys = 64;
 constexpr int kComputeWarps = 8;
 constexpr int kComputeThreads = kComputeWarps * 32;
 constexpr int kThreads = kComputeThreads + 128;  // and the producer's warpgroup, of which one warp works
 constexpr int kMaxStages = 8;
 
-template <class T, int DP, int MT, int WR>
+template <int WR>
 struct Shape {
-    static constexpr int kRows = 16 * MT * WR;
+    static constexpr int kRows = 16 * WR;
     static constexpr int kBlocks = DP / 64;
     static constexpr int kHalf = kBlocks * kTileKeys * 128;  // bytes of a tile's keys
     static constexpr int kStages = 128 * 1024 / (2 * kHalf);
     static constexpr int kQuery = kRows * DP * 2;
-    static constexpr int kJoin = 4 * 16 * MT * DP * 4;
+    static constexpr int kJoin = 4 * 16 * DP * 4;
     static constexpr int kOut = kRows * (DP + 2);  // floats of a partial result
     static constexpr int kBytes = 1024 + kStages * 2 * kHalf + kQuery + kJoin;
 };
@@ -68,20 +70,20 @@ struct Control {
     CacheUnit unit[kMaxStages][4];
     int sums[34];
     WorkSplit split;
-    float top[kComputeWarps][32], sum[kComputeWarps][32];  // each compute warp's row statistics
-    float row_top[64], row_sum[64];
+    float top[kComputeWarps][16], sum[kComputeWarps][16];  // each compute warp's row statistics
+    float row_top[32], row_sum[32];
     int last;
-    int64_t query_at[64];
+    int64_t query_at[32];
 };
 
-// MT: 16-row tiles a warp; WR: 1, the two halves of the compute warps take alternate tiles; 2,
-// they take alternate halves of the rows and every tile.
-template <class T, int DP, int MT, int WR>
+// WR = 1: the two halves of the compute warps take alternate tiles; 2: they take halves of the rows
+// and every tile.
+template <class T, int WR>
 __global__ void __launch_bounds__(kThreads, 1)
 attend_mma_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ CacheView c,
                   const __grid_constant__ AttendParams a) {
-    using S = Shape<T, DP, MT, WR>;
-    constexpr int kSteps = DP / 16, kHalfRows = 16 * MT;
+    using S = Shape<WR>;
+    constexpr int kSteps = DP / 16, kHalfRows = 16;
     extern __shared__ uint8_t raw[];
     __shared__ Control ctl;
     uint8_t* smem = raw + (1024 - (smem_address(raw) & 1023)) % 1024;
@@ -183,33 +185,28 @@ attend_mma_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant
         named_sync(1, kComputeThreads);
         // Which beams the warp's rows belong to; rows past the count or the end see nothing.
         const int warp_row0 = WR == 2 ? half * kHalfRows : 0;
-        uint32_t bit[MT][2];
+        uint32_t bit[2];
         uint32_t need = 0;
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int r = row0 + warp_row0 + mt * 16 + row_in_tile + 8 * e;
-                bit[mt][e] = 0;
-                if (r < p.rows) {
-                    const RowId id = row_id(a, r);
-                    const bool live = a.counts == nullptr || id.token < new_count(a, static_cast<int64_t>(b) * a.beams + beam0 + id.beam);
-                    if (live) bit[mt][e] = 1u << id.beam;
-                }
-                need |= bit[mt][e];
+        for (int e = 0; e < 2; ++e) {
+            const int r = row0 + warp_row0 + row_in_tile + 8 * e;
+            bit[e] = 0;
+            if (r < p.rows) {
+                const RowId id = row_id(a, r);
+                const bool live = a.counts == nullptr || id.token < new_count(a, static_cast<int64_t>(b) * a.beams + beam0 + id.beam);
+                if (live) bit[e] = 1u << id.beam;
             }
+            need |= bit[e];
+        }
         need = __reduce_or_sync(0xffffffffu, need);
 
-        float top[MT][2], sum[MT][2], acc[MT][kSteps * 2][4];
+        float top[2], sum[2], acc[kSteps * 2][4];
+        top[0] = top[1] = -INFINITY;
+        sum[0] = sum[1] = 0.0f;
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-            top[mt][0] = top[mt][1] = -INFINITY;
-            sum[mt][0] = sum[mt][1] = 0.0f;
+        for (int n = 0; n < kSteps * 2; ++n)
 #pragma unroll
-            for (int n = 0; n < kSteps * 2; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[mt][n][e] = 0.0f;
-        }
+            for (int e = 0; e < 4; ++e) acc[n][e] = 0.0f;
         for (int t = p.t0; t < p.t1; ++t, ++it) {
             if (WR == 1 && (it & 1) != half) continue;
             const int stage = it % S::kStages;
@@ -218,99 +215,88 @@ attend_mma_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant
             const CacheUnit u = ctl.unit[stage][key0 >> c.page_log2];
             if (u.page >= 0 && (u.mask & need) != 0) {
                 const uint32_t keys = stages + stage * 2 * S::kHalf;
-                float s[MT][2][4];
+                float s[2][4];
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
+                for (int n = 0; n < 2; ++n)
 #pragma unroll
-                    for (int n = 0; n < 2; ++n)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) s[mt][n][e] = 0.0f;
+                    for (int e = 0; e < 4; ++e) s[n][e] = 0.0f;
 #pragma unroll
                 for (int k = 0; k < kSteps; ++k) {
                     uint32_t kf[4];
                     const int row = key0 + (lane & 7) + ((lane & 16) >> 1), chunk = 2 * k + ((lane >> 3) & 1);
                     ldmatrix4(kf, keys + (chunk >> 3) * (kTileKeys * 128) + swizzled(row, chunk & 7));
-#pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) {
-                        uint32_t qf[4];
-                        const int qrow = warp_row0 + mt * 16 + (lane & 15), qchunk = 2 * k + (lane >> 4);
-                        ldmatrix4(qf, smem_address(query) + (qchunk >> 3) * (S::kRows * 128) + swizzled(qrow, qchunk & 7));
-                        mma<T>(s[mt][0], qf, kf[0], kf[1]);
-                        mma<T>(s[mt][1], qf, kf[2], kf[3]);
-                    }
+                    uint32_t qf[4];
+                    const int qrow = warp_row0 + (lane & 15), qchunk = 2 * k + (lane >> 4);
+                    ldmatrix4(qf, smem_address(query) + (qchunk >> 3) * (S::kRows * 128) + swizzled(qrow, qchunk & 7));
+                    mma<T>(s[0], qf, kf[0], kf[1]);
+                    mma<T>(s[1], qf, kf[2], kf[3]);
                 }
                 const bool plain = u.limit < 0 && (u.mask & need) == need;
-                uint32_t weights[MT][4];
+                uint32_t weights[4];
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
+                for (int n = 0; n < 2; ++n)
 #pragma unroll
-                    for (int n = 0; n < 2; ++n)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) s[mt][n][e] *= scale;
-                    if (!plain) {
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const bool holds = (bit[mt][e] & u.mask) != 0;
-                            int64_t fresh = 0;
-                            int token = 0, count = 0;
-                            if (holds && u.limit >= 0) {
-                                const RowId id = row_id(a, row0 + warp_row0 + mt * 16 + row_in_tile + 8 * e);
-                                const int64_t bk = static_cast<int64_t>(b) * a.beams + beam0 + id.beam;
-                                token = id.token;
-                                count = new_count(a, bk);
-                                fresh = (bk * a.N + token) * a.N;
-                            }
-#pragma unroll
-                            for (int n = 0; n < 2; ++n)
-#pragma unroll
-                                for (int x = 0; x < 2; ++x) {
-                                    bool sees = holds;
-                                    if (holds && u.limit >= 0) {
-                                        const int pos = u.start + ((key0 + n * 8 + pair * 2 + x) & (c.page - 1));
-                                        const int j = pos - u.limit;  
-                                        if (j >= 0) sees = j < count && (a.mask ? a.mask[fresh + j] != 0 : j <= token);
-                                    }
-                                    if (!sees) s[mt][n][2 * e + x] = -INFINITY;
-                                }
-                        }
-                    }
-                    // One online-softmax step of the warp's 16 positions.
+                    for (int e = 0; e < 4; ++e) s[n][e] *= scale;
+                if (!plain) {
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        float now = fmaxf(fmaxf(s[mt][0][2 * e], s[mt][0][2 * e + 1]), fmaxf(s[mt][1][2 * e], s[mt][1][2 * e + 1]));
-                        now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, 1));
-                        now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, 2));
-                        now = fmaxf(now, top[mt][e]);
-                        const float ref = now == -INFINITY ? 0.0f : now;
-                        const float keep = exp2_fast(top[mt][e] - ref);
-                        if (__any_sync(0xffffffffu, now != top[mt][e])) {
-#pragma unroll
-                            for (int n = 0; n < kSteps * 2; ++n) {
-                                acc[mt][n][2 * e] *= keep;
-                                acc[mt][n][2 * e + 1] *= keep;
-                            }
+                        const bool holds = (bit[e] & u.mask) != 0;
+                        int64_t fresh = 0;
+                        int token = 0, count = 0;
+                        if (holds && u.limit >= 0) {
+                            const RowId id = row_id(a, row0 + warp_row0 + row_in_tile + 8 * e);
+                            const int64_t bk = static_cast<int64_t>(b) * a.beams + beam0 + id.beam;
+                            token = id.token;
+                            count = new_count(a, bk);
+                            fresh = (bk * a.N + token) * a.N;
                         }
-                        top[mt][e] = now;
-                        float w[4];
 #pragma unroll
                         for (int n = 0; n < 2; ++n)
 #pragma unroll
-                            for (int x = 0; x < 2; ++x) w[2 * n + x] = exp2_fast(s[mt][n][2 * e + x] - ref);
-                        sum[mt][e] = sum[mt][e] * keep + ((w[0] + w[1]) + (w[2] + w[3]));
-                        weights[mt][e] = Pack<T>::pair(w[0], w[1]);
-                        weights[mt][2 + e] = Pack<T>::pair(w[2], w[3]);
+                            for (int x = 0; x < 2; ++x) {
+                                bool sees = holds;
+                                if (holds && u.limit >= 0) {
+                                    const int pos = u.start + ((key0 + n * 8 + pair * 2 + x) & (c.page - 1));
+                                    const int j = pos - u.limit;
+                                    if (j >= 0) sees = j < count && (a.mask ? a.mask[fresh + j] != 0 : j <= token);
+                                }
+                                if (!sees) s[n][2 * e + x] = -INFINITY;
+                            }
                     }
+                }
+                // One online-softmax step of the warp's 16 positions.
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float now = fmaxf(fmaxf(s[0][2 * e], s[0][2 * e + 1]), fmaxf(s[1][2 * e], s[1][2 * e + 1]));
+                    now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, 1));
+                    now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, 2));
+                    now = fmaxf(now, top[e]);
+                    const float ref = now == -INFINITY ? 0.0f : now;
+                    const float keep = exp2_fast(top[e] - ref);
+                    if (__any_sync(0xffffffffu, now != top[e])) {
+#pragma unroll
+                        for (int n = 0; n < kSteps * 2; ++n) {
+                            acc[n][2 * e] *= keep;
+                            acc[n][2 * e + 1] *= keep;
+                        }
+                    }
+                    top[e] = now;
+                    float w[4];
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) w[2 * n + x] = exp2_fast(s[n][2 * e + x] - ref);
+                    sum[e] = sum[e] * keep + ((w[0] + w[1]) + (w[2] + w[3]));
+                    weights[e] = Pack<T>::pair(w[0], w[1]);
+                    weights[2 + e] = Pack<T>::pair(w[2], w[3]);
                 }
 #pragma unroll
                 for (int n = 0; n < kSteps; ++n) {
                     uint32_t vf[4];
                     const int row = key0 + (lane & 15), chunk = 2 * n + (lane >> 4);
                     ldmatrix4_trans(vf, keys + S::kHalf + (chunk >> 3) * (kTileKeys * 128) + swizzled(row, chunk & 7));
-#pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) {
-                        mma<T>(acc[mt][2 * n], weights[mt], vf[0], vf[1]);
-                        mma<T>(acc[mt][2 * n + 1], weights[mt], vf[2], vf[3]);
-                    }
+                    mma<T>(acc[2 * n], weights, vf[0], vf[1]);
+                    mma<T>(acc[2 * n + 1], weights, vf[2], vf[3]);
                 }
             }
             __syncwarp();
@@ -321,17 +307,15 @@ attend_mma_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant
         // Join the warps: the rows' maxima and sums, then the outputs at the common maximum, through
         // four buffers in two rounds (the upper warps of a half's set, then the lower ones).
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                float l = sum[mt][e];
-                l += __shfl_xor_sync(0xffffffffu, l, 1);
-                l += __shfl_xor_sync(0xffffffffu, l, 2);
-                if (pair == 0) {
-                    ctl.top[warp][mt * 16 + row_in_tile + 8 * e] = top[mt][e];
-                    ctl.sum[warp][mt * 16 + row_in_tile + 8 * e] = l;
-                }
+        for (int e = 0; e < 2; ++e) {
+            float l = sum[e];
+            l += __shfl_xor_sync(0xffffffffu, l, 1);
+            l += __shfl_xor_sync(0xffffffffu, l, 2);
+            if (pair == 0) {
+                ctl.top[warp][row_in_tile + 8 * e] = top[e];
+                ctl.sum[warp][row_in_tile + 8 * e] = l;
             }
+        }
         named_sync(1, kComputeThreads);
         constexpr int kSet = WR == 1 ? kComputeWarps : kComputeWarps / 2;  // warps with the same rows
         const int set0 = WR == 1 ? 0 : half * kSet, rank = warp - set0;
@@ -347,44 +331,38 @@ attend_mma_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant
         }
         named_sync(1, kComputeThreads);
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int e = 0; e < 2; ++e) {
+            const float m = ctl.row_top[warp_row0 + row_in_tile + 8 * e];
+            const float factor = exp2_fast(top[e] - (m == -INFINITY ? 0.0f : m));
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const float m = ctl.row_top[warp_row0 + mt * 16 + row_in_tile + 8 * e];
-                const float factor = exp2_fast(top[mt][e] - (m == -INFINITY ? 0.0f : m));
-#pragma unroll
-                for (int n = 0; n < kSteps * 2; ++n) {
-                    acc[mt][n][2 * e] *= factor;
-                    acc[mt][n][2 * e + 1] *= factor;
-                }
+            for (int n = 0; n < kSteps * 2; ++n) {
+                acc[n][2 * e] *= factor;
+                acc[n][2 * e + 1] *= factor;
             }
+        }
         constexpr int kBuffers = kSet / 2;  // a set's; kBuffers * WR == 4
         float* mine = join + ((WR == 1 ? 0 : half * kBuffers) + rank % kBuffers) * (kHalfRows * DP);
-        auto spot = [&](int mt, int n, int e) {
-            const int r = mt * 16 + row_in_tile + 8 * e;
+        auto spot = [&](int n, int e) {
+            const int r = row_in_tile + 8 * e;
             return mine + r * DP + ((n * 8 + pair * 2) ^ ((r & 7) << 3));
         };
         if (rank >= kBuffers) {
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
+            for (int n = 0; n < kSteps * 2; ++n)
 #pragma unroll
-                for (int n = 0; n < kSteps * 2; ++n)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e)
-                        *reinterpret_cast<float2*>(spot(mt, n, e)) = make_float2(acc[mt][n][2 * e], acc[mt][n][2 * e + 1]);
+                for (int e = 0; e < 2; ++e)
+                    *reinterpret_cast<float2*>(spot(n, e)) = make_float2(acc[n][2 * e], acc[n][2 * e + 1]);
         }
         named_sync(1, kComputeThreads);
         if (rank < kBuffers) {
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
+            for (int n = 0; n < kSteps * 2; ++n)
 #pragma unroll
-                for (int n = 0; n < kSteps * 2; ++n)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        float2* at = reinterpret_cast<float2*>(spot(mt, n, e));
-                        const float2 o = *at;
-                        *at = make_float2(acc[mt][n][2 * e] + o.x, acc[mt][n][2 * e + 1] + o.y);
-                    }
+                for (int e = 0; e < 2; ++e) {
+                    float2* at = reinterpret_cast<float2*>(spot(n, e));
+                    const float2 o = *at;
+                    *at = make_float2(acc[n][2 * e] + o.x, acc[n][2 * e + 1] + o.y);
+                }
         }
         named_sync(1, kComputeThreads);
         // Four values at a time: to the output, or to this CTA's part of a divided segment.
@@ -441,39 +419,26 @@ attend_mma_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant
     }
 }
 
-template <class T, int DP, int MT, int WR>
+template <class T, int WR>
 cudaError_t launch_shape(const CacheView& c, const CUtensorMap& map, const AttendParams& a, int sm_count,
                          cudaStream_t stream) {
-    using S = Shape<T, DP, MT, WR>;
-    auto* kernel = attend_mma_kernel<T, DP, MT, WR>;
+    using S = Shape<WR>;
+    auto* kernel = attend_mma_kernel<T, WR>;
     static std::atomic<uint64_t> ready{0};  // a bit a device
     const cudaError_t e = allow_shared(kernel, S::kBytes, ready);
     if (e != cudaSuccess) return e;
     return launch_after(kernel, sm_count, kThreads, S::kBytes, stream, map, c, a);
 }
 
-// Rows of a block: as many as a group has, up to 64 (32 for heads above 128), in one of three
-// shapes. Fewer rows than a shape holds cost products with zeros, not bytes.
-template <class T, int DP>
-cudaError_t launch_width(const CacheView& c, const CUtensorMap& map, const AttendParams& a, int sm_count,
-                         cudaStream_t stream) {
-    const int beams = a.beams < kGroupBeams ? a.beams : kGroupBeams;
-    const int64_t rows = static_cast<int64_t>(beams) * a.N * a.G;
-    if (rows <= 16) return launch_shape<T, DP, 1, 1>(c, map, a, sm_count, stream);
-    if constexpr (DP > 128) {
-        return launch_shape<T, DP, 1, 2>(c, map, a, sm_count, stream);
-    } else {
-        if (rows <= 32) return launch_shape<T, DP, 2, 1>(c, map, a, sm_count, stream);
-        return launch_shape<T, DP, 2, 2>(c, map, a, sm_count, stream);
-    }
-}
-
+// Rows of a block: 16, or 32 where a group has more. Fewer rows than that cost products with zeros, not
+// bytes.
 template <class T>
 cudaError_t launch_typed(const CacheView& c, const CUtensorMap& map, const AttendParams& a, int sm_count,
                          cudaStream_t stream) {
-    if (c.D <= 64) return launch_width<T, 64>(c, map, a, sm_count, stream);
-    if (c.D <= 128) return launch_width<T, 128>(c, map, a, sm_count, stream);
-    return launch_width<T, 256>(c, map, a, sm_count, stream);
+    const int beams = a.beams < kGroupBeams ? a.beams : kGroupBeams;
+    const int64_t rows = static_cast<int64_t>(beams) * a.N * a.G;
+    if (rows <= 16) return launch_shape<T, 1>(c, map, a, sm_count, stream);
+    return launch_shape<T, 2>(c, map, a, sm_count, stream);
 }
 
 }  // namespace
@@ -501,7 +466,7 @@ bool page_map(const CacheView& c, int dtype, CUtensorMap* map) {
 
 int64_t attend_mma_workspace(const CacheView&, const AttendParams&, int sm_count) {
     // A counter for each CTA (8192 bytes), then two partial results for each.
-    return 8192 + static_cast<int64_t>(2) * sm_count * Shape<__half, 128, 2, 2>::kOut * 4;
+    return 8192 + static_cast<int64_t>(2) * sm_count * Shape<2>::kOut * 4;
 }
 
 cudaError_t launch_attend_mma(const CacheView& c, int dtype, const AttendParams& a, int sm_count, cudaStream_t stream) {
