@@ -296,10 +296,10 @@ attend_f32_kernel(const __grid_constant__ CacheView c, const __grid_constant__ A
             }
         }
         if (whole) continue;
-        __threadfence();
         __syncthreads();
         const Span span = span_of(work, p);
         if (tid == 0) {
+            __threadfence();  // of all the threads' stores, which the barrier put before this
             const int before = atomicAdd(counters + span.c0, 1);
             ctl.last = before == span.c1 - span.c0;
             if (ctl.last) counters[span.c0] = 0;

@@ -797,10 +797,10 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
             }
         }
         if (whole) continue;
-        __threadfence();
         named_sync(1, kSoftThreads);
         const Span span = span_of(work, p);
         if (tid == 0) {
+            __threadfence();  // of all the threads' stores, which the barrier put before this
             const int before = atomicAdd(counters + span.c0, 1);
             ctl.last = before == span.c1 - span.c0;
             if (ctl.last) counters[span.c0] = 0;

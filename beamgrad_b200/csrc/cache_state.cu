@@ -35,6 +35,22 @@ __device__ __forceinline__ void raise(const CacheView& c, int bit) { atomicOr(c.
 // The last CTA of fork_meta_kernel: ranks of the wishes, free pages for them, the copy list.
 __device__ void hand_out(const CacheView& c, int* sums) {
     const int S = c.B * c.K, tid = threadIdx.x;
+    // The first references are on their way while the wishes are counted.
+    auto zeros_at = [&](int at) {  // a bit each
+        unsigned zero = 0;
+        if (at + 16 <= c.P) {
+            int4 v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = __ldcg(reinterpret_cast<const int4*>(c.references + at) + i);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                zero |= ((v[i].x == 0) | (v[i].y == 0) << 1 | (v[i].z == 0) << 2 | (v[i].w == 0) << 3) << (4 * i);
+        } else {
+            for (int i = 0; i < 16 && at + i < c.P; ++i) zero |= (__ldcg(c.references + at + i) == 0) << i;
+        }
+        return zero;
+    };
+    unsigned zero = zeros_at(tid * 16);
     int wanted = 0;
     for (int base = 0; base < S; base += kMetaThreads) {
         const int s = base + tid;
@@ -47,22 +63,11 @@ __device__ void hand_out(const CacheView& c, int* sums) {
     // Zeros of the references, 16 a thread and round.
     int found = 0;
     for (int base = 0; base < c.P && found < wanted; base += kMetaThreads * 16) {
-        const int at = base + tid * 16;
-        unsigned zero = 0;
-        if (at + 16 <= c.P) {
-            int4 v[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = __ldcg(reinterpret_cast<const int4*>(c.references + at) + i);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                zero |= ((v[i].x == 0) | (v[i].y == 0) << 1 | (v[i].z == 0) << 2 | (v[i].w == 0) << 3) << (4 * i);
-        } else {
-            for (int i = 0; i < 16 && at + i < c.P; ++i) zero |= (__ldcg(c.references + at + i) == 0) << i;
-        }
+        if (base > 0) zero = zeros_at(base + tid * 16);
         int total;
         int rank = found + block_scan(__popc(zero), sums, &total);
         for (; zero != 0 && rank < wanted; zero &= zero - 1, ++rank) {
-            const int p = at + __ffs(zero) - 1;
+            const int p = base + tid * 16 + __ffs(zero) - 1;
             c.free_list[rank] = p;
             c.references[p] = 1;
         }
@@ -108,58 +113,57 @@ __global__ void __launch_bounds__(kMetaThreads) fork_meta_kernel(CacheView c, Fo
     const int64_t slot0 = static_cast<int64_t>(b) * K;
     grid_wait();   // what ran before may have written the parents
     grid_release();
+    const int width = K * M <= kStageInts ? M : (kStageInts / K > 1 ? kStageInts / K : 1);
+    int32_t* table = c.table + slot0 * M;
+    auto load_stage = [&](int base, int cols) {
+        for (int i = tid; i < K * cols; i += kMetaThreads) {
+            const int r = i / cols;
+            stage[r * width + i - r * cols] = table[static_cast<int64_t>(r) * M + base + i - r * cols];
+        }
+    };
+    // All that is read is asked for at once.
     for (int k = tid; k < K; k += kMetaThreads) {
         int64_t w = a.written ? a.written[slot0 + k] : a.written_all;
-        if (w < 0) {
-            raise(c, DBS_CUDA_CACHE_STATUS_INDEX);
-            w = 0;
-        }
-        int64_t n = c.lengths[slot0 + k] + w;
+        int64_t m = a.room ? a.room[slot0 + k] : a.room_all;
+        const int old = c.lengths[slot0 + k], p = a.parents ? a.parents[slot0 + k] : k;
+        if (w < 0 || (p >= 0 && m < 0) || p >= K) raise(c, DBS_CUDA_CACHE_STATUS_INDEX);
+        if (w < 0) w = 0;
         const int64_t most = static_cast<int64_t>(M) << log2;
+        int64_t n = old + w;
         if (n > most) {
             raise(c, DBS_CUDA_CACHE_STATUS_CAPACITY);
             n = most;
         }
         length[k] = static_cast<int32_t>(n < 0 ? 0 : n);
+        src[k] = p < 0 || p >= K ? -1 : p;
+        need[k] = static_cast<int>(m < 0 ? 0 : m);  // the room, until the lengths are known
         children[k] = 0;
         first[k] = INT_MAX;
         want[k] = 0;
         want_at[k] = INT_MAX;
+        copied[k] = -1;
     }
+    load_stage(0, M < width ? M : width);
     __syncthreads();
     for (int k = tid; k < K; k += kMetaThreads) {
-        int p = a.parents ? a.parents[slot0 + k] : k;
-        if (p >= K) {
-            raise(c, DBS_CUDA_CACHE_STATUS_INDEX);
-            p = -1;
-        }
-        src[k] = p < 0 ? -1 : p;
+        const int p = src[k];
         int columns = 0;
         if (p >= 0) {
             atomicAdd(&children[p], 1);
             atomicMin(&first[p], k);
-            int64_t m = a.room ? a.room[slot0 + k] : a.room_all;
-            if (m < 0) {
-                raise(c, DBS_CUDA_CACHE_STATUS_INDEX);
-                m = 0;
-            }
-            const int64_t n = (length[p] + m + c.page - 1) >> log2;
+            const int64_t n = (static_cast<int64_t>(length[p]) + need[k] + c.page - 1) >> log2;
             if (n > M) raise(c, DBS_CUDA_CACHE_STATUS_CAPACITY);
             columns = static_cast<int>(n > M ? M : n);
         }
         need[k] = columns;
-        copied[k] = -1;
     }
     __syncthreads();
-    const int width = K * M <= kStageInts ? M : (kStageInts / K > 1 ? kStageInts / K : 1);
-    int32_t* table = c.table + slot0 * M;
     for (int base = 0; base < M; base += width) {
         const int cols = M - base < width ? M - base : width;
-        for (int i = tid; i < K * cols; i += kMetaThreads) {
-            const int r = i / cols;
-            stage[r * width + i - r * cols] = table[static_cast<int64_t>(r) * M + base + i - r * cols];
+        if (base > 0) {
+            load_stage(base, cols);
+            __syncthreads();
         }
-        __syncthreads();
         for (int i = tid; i < K * cols; i += kMetaThreads) {
             const int r = i / cols, at = i - r * cols, col = base + at;
             const int old = stage[r * width + at];
