@@ -206,7 +206,10 @@ __global__ void __launch_bounds__(kMetaThreads) fork_meta_kernel(CacheView c, Fo
 }
 
 // The units of a group of beams, from its final table rows (column order, then first beam).
-// resolve: entries of -2 take their slot's new pages first.
+// resolve: entries of -2 take their slot's new pages first. A warp takes a column at a time, a lane a
+// beam: the lanes with one page find each other in one instruction.
+constexpr int kPlanPitch = kCopyThreads + 1;  // of a beam's staged columns: a column's lie in different banks
+
 __device__ void write_plan(const CacheView& c, int group, bool resolve, int* sums, int32_t* shared) {
     const int b = group / c.groups, k0 = (group - b * c.groups) * kGroupBeams;
     const int n = c.K - k0 < kGroupBeams ? c.K - k0 : kGroupBeams;
@@ -216,8 +219,9 @@ __device__ void write_plan(const CacheView& c, int group, bool resolve, int* sum
     int32_t* length = shared;                   // [32]
     int32_t* rank = shared + kGroupBeams;       // [32] rank of the first new page
     int32_t* from = shared + 2 * kGroupBeams;   // [32] its column
-    int32_t* stage = shared + 3 * kGroupBeams;  // [n, blockDim.x]
-    const int tid = threadIdx.x, threads = blockDim.x;
+    int32_t* place = shared + 3 * kGroupBeams;  // [columns] units of each, then the first one's number
+    int32_t* stage = place + kCopyThreads;      // [n][kPlanPitch]
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid < n) {
         length[tid] = c.lengths[slot0 + tid];
         rank[tid] = resolve ? c.want_rank[slot0 + tid] : 0;
@@ -226,63 +230,56 @@ __device__ void write_plan(const CacheView& c, int group, bool resolve, int* sum
     const int handed = resolve ? c.words[kWordFree] : 0;
     __syncthreads();
     int count = 0;
-    for (int base = 0; base < c.M; base += threads) {
-        const int col = base + tid;
-        int mine = 0;
-        bool shared_tail = false;
-        if (col < c.M) {
-            const int end = (col + 1) << c.page_log2;
-            uint32_t seen = 0;
-            for (int k = 0; k < n; ++k) {
-                int e = table[static_cast<int64_t>(k) * c.M + col];
-                if (resolve && e == -2) {
-                    const int at = rank[k] + col - from[k];
-                    e = at < handed ? c.free_list[at] : -1;
-                    table[static_cast<int64_t>(k) * c.M + col] = e;
-                }
-                stage[k * threads + tid] = e;
+    for (int base = 0; base < c.M; base += kCopyThreads) {
+        const int cols = c.M - base < kCopyThreads ? c.M - base : kCopyThreads;
+        for (int i = tid; i < n * cols; i += kCopyThreads) {
+            const int k = i / cols, at = i - k * cols, col = base + at;
+            int e = table[static_cast<int64_t>(k) * c.M + col];
+            if (resolve && e == -2) {
+                const int new_page = rank[k] + col - from[k];
+                e = new_page < handed ? c.free_list[new_page] : -1;
+                table[static_cast<int64_t>(k) * c.M + col] = e;
             }
-            for (int k = 0; k < n; ++k) {
-                const int e = stage[k * threads + tid];
-                if (e < 0 || (seen >> k & 1)) continue;
-                ++mine;
-                bool complete = true;
-                uint32_t holders = 0;
-                for (int j = k; j < n; ++j)
-                    if (stage[j * threads + tid] == e) {
-                        holders |= 1u << j;
-                        complete &= end <= length[j];
-                    }
-                seen |= holders;
-                shared_tail |= !complete && (holders & (holders - 1)) != 0;
-            }
+            stage[k * kPlanPitch + at] = e;
         }
+        __syncthreads();
+        // Lanes without a page get numbers that no other lane has.
+        auto holders_of = [&](int at, int* page) {
+            const int e = lane < n ? stage[lane * kPlanPitch + at] : -1;
+            *page = e;
+            return __match_any_sync(0xffffffffu, e >= 0 ? e : -1 - lane);
+        };
+        for (int at = warp; at < cols; at += kCopyThreads / 32) {
+            int e;
+            const unsigned holders = holders_of(at, &e);
+            const unsigned firsts = __ballot_sync(0xffffffffu, e >= 0 && __ffs(holders) - 1 == lane);
+            if (lane == 0) place[at] = __popc(firsts);
+        }
+        __syncthreads();
         int total;
-        int at = count + block_scan(mine, sums, &total);
-        if (mine > 0) {
-            const int end = (col + 1) << c.page_log2;
-            uint32_t seen = 0;
-            for (int k = 0; k < n; ++k) {
-                const int e = stage[k * threads + tid];
-                if (e < 0 || (seen >> k & 1)) continue;
-                bool complete = true;
-                uint32_t holders = 0;
-                for (int j = k; j < n; ++j)
-                    if (stage[j * threads + tid] == e) {
-                        holders |= 1u << j;
-                        complete &= end <= length[j];
-                    }
-                seen |= holders;
-                units[at++] = CacheUnit{e, col << c.page_log2, holders, complete ? -1 : length[k]};
+        const int at_first = count + block_scan(tid < cols ? place[tid] : 0, sums, &total);
+        if (tid < cols) place[tid] = at_first;
+        __syncthreads();
+        for (int at = warp; at < cols; at += kCopyThreads / 32) {
+            int e;
+            const unsigned holders = holders_of(at, &e);
+            const int end = (base + at + 1) << c.page_log2;
+            const unsigned whole = __ballot_sync(0xffffffffu, lane < n && end <= length[lane]);
+            const bool first = e >= 0 && __ffs(holders) - 1 == lane, complete = (holders & ~whole) == 0;
+            const unsigned firsts = __ballot_sync(0xffffffffu, first);
+            if (first) {
+                units[place[at] + __popc(firsts & ((1u << lane) - 1))] =
+                    CacheUnit{e, (base + at) << c.page_log2, holders, complete ? -1 : length[lane]};
+                if (!complete && (holders & (holders - 1)) != 0) raise(c, DBS_CUDA_CACHE_STATUS_SHARED);
             }
         }
-        if (shared_tail) raise(c, DBS_CUDA_CACHE_STATUS_SHARED);
         count += total;
+        __syncthreads();
     }
     if (tid == 0) c.unit_count[group] = count;
 }
 
-constexpr size_t plan_smem() { return (3 * kGroupBeams + kGroupBeams * kCopyThreads) * sizeof(int32_t); }
+constexpr size_t plan_smem() { return (3 * kGroupBeams + kCopyThreads + kGroupBeams * kPlanPitch) * sizeof(int32_t); }
 
 // After fork_meta_kernel: the plan and the new pages of the table (one CTA a group), and the
 // copies of incomplete pages (the other CTAs; a warp takes the rows of one layer, kind and head,
