@@ -8,7 +8,7 @@ namespace dbsb {
 
 namespace {
 
-constexpr int kAppendThreads = 128;
+constexpr int kAppendThreads = 256;
 
 // Keys and values of the new tokens into their pages, 16 bytes a thread. A value that is not
 // finite raises the cache's second status word: the attention then keeps masked values out of its
@@ -54,13 +54,7 @@ template <class T>
 cudaError_t launch_append(const CacheView& c, const AttendParams& a, int sm_count, cudaStream_t stream) {
     if (a.k == nullptr) return cudaSuccess;
     const int64_t items = static_cast<int64_t>(c.B) * a.beams * a.N * c.H * (c.D / Pack<T>::n);
-    // Two small CTAs an SM at the most: their registers fit beside those of the attention's CTA, which
-    // else waits for a place (4 us of 100 on the SMs that this kernel has).
-    const int64_t want = (items + kAppendThreads - 1) / kAppendThreads, cap = 2 * sm_count;
-    // The same split of the SM's memory as the attention's: it would wait for the SM to change it.
-    static std::atomic<uint64_t> ready{0};
-    const cudaError_t e = prefer_shared(append_kernel<T>, ready);
-    if (e != cudaSuccess) return e;
+    const int64_t want = (items + kAppendThreads - 1) / kAppendThreads, cap = 8 * sm_count;
     return launch_after(append_kernel<T>, static_cast<unsigned>(want < cap ? want : cap), kAppendThreads, 0, stream, c, a);
 }
 

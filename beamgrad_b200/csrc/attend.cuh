@@ -213,35 +213,38 @@ __device__ __forceinline__ GroupWork group_work(const CacheView& c, const Attend
     return w;
 }
 
-// All threads of the block; sums: 34 ints, found: a WorkSplit in shared memory. The host has
+// All threads of the block; sums: 35 ints, found: a WorkSplit in shared memory. The host has
 // checked that the tiles of all segments are counted in 31 bits.
 template <int kRows>
 __device__ WorkSplit split_work(const CacheView& c, const AttendParams& a, int tile_units, int min_tiles, int* sums,
                                 WorkSplit* found) {
     const int groups = c.B * c.groups, tid = threadIdx.x, threads = blockDim.x;
-    auto tiles_of = [&](int g, int* segments) {
-        *segments = 0;
+    auto tiles_of = [&](int g, int* longest) {
+        *longest = 0;
         if (g >= groups) return 0;
         const GroupWork w = group_work<kRows>(c, a, g, tile_units);
-        *segments = w.blocks * c.H;
-        return w.tiles * *segments;
+        if (w.blocks > 0) *longest = w.tiles;
+        return w.tiles * w.blocks * c.H;
     };
     // One round where a thread a group is enough; its count and place are kept for below.
-    int total = 0, mine = 0, at = 0, segments = 0;
+    int total = 0, mine = 0, at = 0;
     if (tid == 0) sums[33] = 0;
     for (int base = 0; base < groups; base += threads) {
         int sum, s;
         mine = tiles_of(base + tid, &s);
         at = total + block_scan(mine, sums, &sum);
         total += sum;
-        s = __reduce_add_sync(0xffffffffu, s);
-        if ((tid & 31) == 0 && s > 0) atomicAdd(sums + 33, s);
+        s = __reduce_max_sync(0xffffffffu, s);
+        if ((tid & 31) == 0 && s > 0) atomicMax(sums + 33, s);
     }
     __syncthreads();
-    segments = sums[33];
-    // A segment in more than 32 parts costs more to join than its parts save.
+    // A segment in more than 32 parts would cost more to join than its parts save: the longest one is 32
+    // CTAs' work at the most (and so lies in 34 of them: kMaxParts).
     int64_t ctas = total / min_tiles;
-    if (ctas > static_cast<int64_t>(segments) * 32) ctas = static_cast<int64_t>(segments) * 32;
+    if (total > 0) {
+        const int64_t cap = static_cast<int64_t>(total) * 32 / sums[33];
+        if (ctas > cap) ctas = cap;
+    }
     if (ctas > gridDim.x) ctas = gridDim.x;
     if (ctas < 1) ctas = 1;
     WorkSplit w;
@@ -371,19 +374,28 @@ __device__ __forceinline__ void load_queries(const CacheView& c, const AttendPar
 }
 
 // The parts of a divided segment to the output, in their order, so that the result does not depend
-// on which CTA comes last. A part: kRows x DP sums (kByColumn: four columns of all rows together, else
-// row by row), the rows' references (base 2), their weights' sums. scratch: 16 * kRows bytes of shared memory. All kThreads threads of named barrier 1.
-template <class T, int kRows, int DP, int kThreads, bool kByColumn>
-__device__ __forceinline__ void join_parts(const CacheView& c, const AttendParams& a, const Piece& p, Span span, int b,
+// on which CTA comes last. A part: kRows x DP sums (four columns of all rows together), the rows'
+// references (base 2), their weights' sums. scratch: join_scratch() bytes of shared memory. All
+// kThreads threads of named barrier 1.
+//
+// The last CTA joins alone, so that its latency is the call's: the parts' shares go through shared
+// memory once, and the values are read in flat order, where one index gives row and place (indexes kept
+// an item each cost the loop before it 40 registers a thread: 64 beams over 4096 in 79 us for 71). One
+// sequence of 14000 positions, 32 parts: 42 us; with shares found again for each value 56 us.
+constexpr int kMaxParts = 34;  // of a segment (split_work)
+constexpr int join_scratch(int rows) { return rows * (12 + 4 * kMaxParts); }
+
+template <class T, int kRows, int DP, int kThreads>
+__device__ __forceinline__ void join_parts(const CacheView& c, const AttendParams& a, Piece p, Span span, int b,
                                            int beam0, int row0, int rows, const float* parts, void* scratch, int tid) {
-    constexpr int kOut = kRows * (DP + 2), kVecs = DP / 4;
+    constexpr int kOut = kRows * (DP + 2);
     const int n_parts = span.c1 - span.c0 + 1;
     // A CTA's second part is the one that begins a segment.
     auto part_of = [&](int i) { return parts + static_cast<int64_t>(2 * (span.c0 + i) + (i == 0)) * kOut; };
     int64_t* places = static_cast<int64_t*>(scratch);
-    float* refs = reinterpret_cast<float*>(places + kRows);
-    float* factors = refs + kRows;  // 1 / sum; -1 for rows that are not shown
-    // The rows' common references and sums: eight lanes a row, each for every eighth part.
+    float* shown_rows = reinterpret_cast<float*>(places + kRows);  // 1; 0 for rows that are not shown
+    float* factors = shown_rows + kRows;                           // [part][row]: the part's share over the sum
+    // Eight lanes a row, each for every eighth part.
 #pragma unroll 1
     for (int r0 = 0; r0 < rows; r0 += kThreads / 8) {
         const int r = r0 + tid / 8, lane = tid % 8;
@@ -399,7 +411,11 @@ __device__ __forceinline__ void join_parts(const CacheView& c, const AttendParam
                 pl[k] = there ? __ldcg(part_of(j) + kRows * DP + kRows + r) : 0.0f;
             }
 #pragma unroll
-            for (int k = 0; k < 4; ++k) now = fmaxf(now, pm[k]);
+            for (int k = 0; k < 4; ++k) {
+                const int j = j0 + lane + 8 * k;
+                if (j < n_parts && r < rows) factors[j * kRows + r] = pm[k];
+                now = fmaxf(now, pm[k]);
+            }
 #pragma unroll
             for (int d = 4; d > 0; d >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, d));
             const float ref = now == -INFINITY ? 0.0f : now;
@@ -410,60 +426,63 @@ __device__ __forceinline__ void join_parts(const CacheView& c, const AttendParam
         }
 #pragma unroll
         for (int d = 4; d > 0; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
-        if (r < rows && lane == 0) {
+        if (r >= rows) continue;
+        const float ref = m == -INFINITY ? 0.0f : m, inverse = l > 0.0f ? 1.0f / l : l;
+#pragma unroll 1
+        for (int j = lane; j < n_parts; j += 8) {
+            float& f = factors[j * kRows + r];  // this lane's own
+            f = exp2_fast(f - ref) * inverse;
+        }
+        if (lane == 0) {
             const RowId id = row_id(a, row0 + r);
             const int64_t bk = static_cast<int64_t>(b) * a.beams + beam0 + id.beam;
             const bool shown = id.token < new_count(a, bk);
             const int64_t at = (bk * a.N + id.token) * a.Hq + p.head * a.G + id.head;
             places[r] = at;
-            refs[r] = m == -INFINITY ? 0.0f : m;
-            factors[r] = shown ? (l > 0.0f ? 1.0f / l : l) : -1.0f;
+            shown_rows[r] = shown ? 1.0f : 0.0f;
             if (a.lse != nullptr) a.lse[at] = shown && l != 0.0f ? (m + log2f(l)) * kLn2 : -INFINITY;
         }
     }
     __syncwarp();
     asm volatile("barrier.sync 1, %0;" ::"r"(kThreads) : "memory");
     // Four values of four items from four parts (two, with 512 threads' registers) in flight.
-    constexpr int kEach = 4, kPartsAtOnce = kThreads > 256 ? 2 : 4;
-    const int items = (kByColumn ? kRows : rows) * kVecs;
-    auto row_of = [](int i) { return kByColumn ? i % kRows : i / kVecs; };
+    constexpr int kEach = 4, kAtOnce = kThreads > 256 ? 2 : 4;
+    const int items = kRows * (c.D / 4);
 #pragma unroll 1
     for (int i0 = tid; i0 < items; i0 += kEach * kThreads) {
         float4 o[kEach];
 #pragma unroll
         for (int e = 0; e < kEach; ++e) o[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 1
-        for (int j0 = 0; j0 < n_parts; j0 += kPartsAtOnce) {
-            float4 v[kPartsAtOnce][kEach];
-            float w[kPartsAtOnce][kEach];
+        for (int j0 = 0; j0 < n_parts; j0 += kAtOnce) {
+            float4 v[kAtOnce][kEach];
 #pragma unroll
-            for (int k = 0; k < kPartsAtOnce; ++k) {
+            for (int k = 0; k < kAtOnce; ++k) {
                 const float* x = part_of(j0 + k < n_parts ? j0 + k : j0);
 #pragma unroll
                 for (int e = 0; e < kEach; ++e) {
-                    const int i = i0 + e * kThreads, r = row_of(i);
-                    const bool there = i < items && r < rows && j0 + k < n_parts;
-                    v[k][e] = there ? __ldcg(reinterpret_cast<const float4*>(x + i * 4)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    w[k][e] = there ? __ldcg(x + kRows * DP + r) - refs[r] : 0.0f;
+                    const int i = i0 + e * kThreads;
+                    v[k][e] = i < items && i % kRows < rows ? __ldcg(reinterpret_cast<const float4*>(x) + i) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                 }
             }
 #pragma unroll
-            for (int k = 0; k < kPartsAtOnce; ++k)
+            for (int k = 0; k < kAtOnce; ++k) {
+                if (j0 + k >= n_parts) break;
 #pragma unroll
                 for (int e = 0; e < kEach; ++e) {
-                    const float f = exp2_fast(w[k][e]);
+                    const int r = (i0 + e * kThreads) % kRows;
+                    const float f = factors[(j0 + k) * kRows + (r < rows ? r : 0)];
                     o[e].x = fmaf(v[k][e].x, f, o[e].x), o[e].y = fmaf(v[k][e].y, f, o[e].y);
                     o[e].z = fmaf(v[k][e].z, f, o[e].z), o[e].w = fmaf(v[k][e].w, f, o[e].w);
                 }
+            }
         }
 #pragma unroll
         for (int e = 0; e < kEach; ++e) {
-            const int i = i0 + e * kThreads, r = row_of(i), vec = kByColumn ? i / kRows : i % kVecs;
-            if (i >= items || r >= rows || vec * 4 >= c.D) continue;
-            const float f = factors[r];
-            float4 y = make_float4(o[e].x * f, o[e].y * f, o[e].z * f, o[e].w * f);
-            if (f == -1.0f) y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            store4(static_cast<T*>(a.out) + places[r] * c.D + vec * 4, y);
+            const int i = i0 + e * kThreads, r = i % kRows;
+            if (i >= items || r >= rows) continue;
+            if (shown_rows[r] == 0.0f) o[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            store4(static_cast<T*>(a.out) + places[r] * c.D + i / kRows * 4, o[e]);
         }
     }
 }
@@ -514,25 +533,17 @@ __device__ __forceinline__ void tma_load(uint32_t to, const CUtensorMap* map, in
         : "memory");
 }
 
-// Sets a kernel's attribute once a device. ready: a bit for each that has it.
+// Dynamic shared memory of a kernel, allowed once a device. ready: a bit for each that has it.
 template <class Kernel>
-cudaError_t set_once(Kernel* kernel, cudaFuncAttribute attribute, int value, std::atomic<uint64_t>& ready) {
+cudaError_t allow_shared(Kernel* kernel, int bytes, std::atomic<uint64_t>& ready) {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     const uint64_t bit = uint64_t{1} << (dev & 63);
     if (dev < 64 && (ready.load(std::memory_order_acquire) & bit) != 0) return cudaSuccess;
-    e = cudaFuncSetAttribute(kernel, attribute, value);
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e == cudaSuccess && dev < 64) ready.fetch_or(bit, std::memory_order_release);
     return e;
-}
-template <class Kernel>
-cudaError_t allow_shared(Kernel* kernel, int bytes, std::atomic<uint64_t>& ready) {
-    return set_once(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes, ready);
-}
-template <class Kernel>
-cudaError_t prefer_shared(Kernel* kernel, std::atomic<uint64_t>& ready) {
-    return set_once(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared, ready);
 }
 
 // The tensor map of the pages as [rows, head_dim], boxes of one page by 64 elements, swizzled so

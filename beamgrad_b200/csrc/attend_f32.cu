@@ -38,7 +38,7 @@ struct Shape {
 };
 
 struct Control {
-    int sums[34];
+    int sums[35];
     WorkSplit split;
     CacheUnit unit[2][4];
     int64_t row_at[2][64];  // of the tile's positions: the row's element among the pages of a layer's keys
@@ -279,7 +279,7 @@ attend_f32_kernel(const __grid_constant__ CacheView c, const __grid_constant__ A
                 if (col >= vecs) break;
                 const float4 o = acc[j][r];
                 if (!whole) {
-                    *reinterpret_cast<float4*>(out_part + (o_row + 2 * r) * DP + col * 4) = o;
+                    *reinterpret_cast<float4*>(out_part + (col * S::kRows + o_row + 2 * r) * 4) = o;
                 } else {
                     reinterpret_cast<float4*>(static_cast<float*>(a.out) + place * c.D)[col] =
                         shown ? make_float4(o.x * inverse, o.y * inverse, o.z * inverse, o.w * inverse)
@@ -307,14 +307,14 @@ attend_f32_kernel(const __grid_constant__ CacheView c, const __grid_constant__ A
         __syncthreads();
         if (!ctl.last) continue;
         __threadfence();
-        join_parts<float, S::kRows, DP, kThreads, false>(c, a, p, span, b, beam0, row0, rows, parts, query, tid);
+        join_parts<float, S::kRows, DP, kThreads>(c, a, p, span, b, beam0, row0, rows, parts, smem, tid);
     }
 }
 
 template <int DP, int ROWS>
 cudaError_t launch_shape(const CacheView& c, const AttendParams& a, int sm_count, cudaStream_t stream) {
     using S = Shape<DP, ROWS>;
-    static_assert(S::kBytes <= 224 * 1024);
+    static_assert(S::kBytes <= 224 * 1024 && join_scratch(ROWS) <= S::kBytes);
     auto* kernel = attend_f32_kernel<DP, ROWS>;
     static std::atomic<uint64_t> ready{0};  // a bit a device
     const cudaError_t e = allow_shared(kernel, S::kBytes, ready);

@@ -35,6 +35,7 @@ struct Shape {
     static constexpr int kStages = 128 * 1024 / (2 * kHalf);
     static constexpr int kQuery = kRows * DP * 2;
     static constexpr int kJoin = 4 * 16 * DP * 4;
+    static_assert(join_scratch(kRows) <= kJoin);
     static constexpr int kOut = kRows * (DP + 2);  // floats of a partial result
     static constexpr int kBytes = 1024 + kStages * 2 * kHalf + kQuery + kJoin;
 };
@@ -68,7 +69,7 @@ __device__ __forceinline__ void mma<__nv_bfloat16>(float (&d)[4], const uint32_t
 struct Control {
     uint64_t full[kMaxStages], empty[kMaxStages];
     CacheUnit unit[kMaxStages][4];
-    int sums[34];
+    int sums[35];
     WorkSplit split;
     float top[kComputeWarps][16], sum[kComputeWarps][16];  // each compute warp's row statistics
     float row_top[32], row_sum[32];
@@ -396,7 +397,7 @@ attend_mma_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant
             if (whole) {
                 put(r, vec, o, m, l);
             } else {
-                *reinterpret_cast<float4*>(part + r * DP + vec * 4) = o;
+                *reinterpret_cast<float4*>(part + (vec * S::kRows + r) * 4) = o;
                 if (vec == 0) {
                     part[S::kRows * DP + r] = m;
                     part[S::kRows * DP + S::kRows + r] = l;
@@ -415,7 +416,7 @@ attend_mma_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant
         named_sync(1, kComputeThreads);
         if (!ctl.last) continue;
         __threadfence();
-        join_parts<T, S::kRows, DP, kComputeThreads, false>(c, a, p, span, b, beam0, row0, rows, parts, join, tid);
+        join_parts<T, S::kRows, DP, kComputeThreads>(c, a, p, span, b, beam0, row0, rows, parts, join, tid);
     }
 }
 

@@ -36,7 +36,7 @@ struct Control {
     uint64_t full[kMaxSlots], empty[kMaxSlots];
     uint64_t queries, scores[2], weights[2], output[2];
     WorkSplit split;
-    int sums[34];
+    int sums[35];
     uint32_t tmem;
     int last;
     union {
@@ -59,8 +59,9 @@ struct Shape {
     static constexpr int kCopyWarp = kSoftThreads / 32, kIssueWarp = kCopyWarp + 1;
     static constexpr int kBlocks = DP / 64;
     static constexpr int kSlot = kTileKeys * DP * 2;
-    // The queries; at the end of a segment NQ = 1 joins its copies there, 256 x 32 floats.
-    static constexpr int kQuery = NQ * 128 * DP * 2 > 32768 ? NQ * 128 * DP * 2 : 32768;
+    // The queries; at the end of a segment copies (256 x 32 floats) and parts are joined there.
+    static constexpr int kLeast = join_scratch(kRows) > 32768 ? (join_scratch(kRows) + 1023) / 1024 * 1024 : 32768;
+    static constexpr int kQuery = NQ * 128 * DP * 2 > kLeast ? NQ * 128 * DP * 2 : kLeast;
     static constexpr int kFit = (227 * 1024 - static_cast<int>(sizeof(Control)) - kQuery) / kSlot;
     static constexpr int kSlots = kFit < kMaxSlots ? kFit : kMaxSlots;
     static constexpr int kOut = kRows * (DP + 2);  // floats of a partial result
@@ -808,7 +809,7 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
         named_sync(1, kSoftThreads);
         if (!ctl.last) continue;
         __threadfence();
-        join_parts<T, S::kRows, DP, kSoftThreads, true>(c, a, p, span, b, beam0, row0, rows, parts, query, tid);
+        join_parts<T, S::kRows, DP, kSoftThreads>(c, a, p, span, b, beam0, row0, rows, parts, query, tid);
     }
     fence_before();
     named_sync(2, kSoftThreads + 32);
