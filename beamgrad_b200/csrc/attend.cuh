@@ -185,7 +185,7 @@ __device__ __forceinline__ void attend_all_rows(const CacheView& c, const Attend
 // (rows in (beam, token, head of the key head's group) order) and one key head; its tiles are the
 // group's units, a few at a time. All tiles of all segments form one line that is cut into equal
 // parts, one a CTA, so that every SM reads the same amount whatever the lengths are. A segment
-// that a cut divides is joined by the CTA that finishes its part last.
+// that a cut divides is joined by the CTA that finishes its part last, or by a kernel of its own.
 // ---------------------------------------------------------------------------
 struct WorkSplit {
     int64_t total;   // tiles
@@ -213,11 +213,11 @@ __device__ __forceinline__ GroupWork group_work(const CacheView& c, const Attend
     return w;
 }
 
-// All threads of the block; sums: 35 ints, found: a WorkSplit in shared memory. The host has
-// checked that the tiles of all segments are counted in 31 bits.
+// The share of CTA `cta` of `grid`. All threads of the block; sums: 35 ints, found: a WorkSplit in shared
+// memory. The host has checked that the tiles of all segments are counted in 31 bits.
 template <int kRows>
 __device__ WorkSplit split_work(const CacheView& c, const AttendParams& a, int tile_units, int min_tiles, int* sums,
-                                WorkSplit* found) {
+                                WorkSplit* found, int cta, int grid) {
     const int groups = c.B * c.groups, tid = threadIdx.x, threads = blockDim.x;
     auto tiles_of = [&](int g, int* longest) {
         *longest = 0;
@@ -245,16 +245,16 @@ __device__ WorkSplit split_work(const CacheView& c, const AttendParams& a, int t
         const int64_t cap = static_cast<int64_t>(total) * 32 / sums[33];
         if (ctas > cap) ctas = cap;
     }
-    if (ctas > gridDim.x) ctas = gridDim.x;
+    if (ctas > grid) ctas = grid;
     if (ctas < 1) ctas = 1;
     WorkSplit w;
     w.total = total;
     w.ctas = static_cast<int>(ctas);
-    w.lo = static_cast<int64_t>(total) * blockIdx.x / ctas;
-    w.hi = static_cast<int64_t>(total) * (blockIdx.x + 1) / ctas;
+    w.lo = static_cast<int64_t>(total) * cta / ctas;
+    w.hi = static_cast<int64_t>(total) * (cta + 1) / ctas;
     w.group = 0;
     w.base = 0;
-    if (static_cast<int64_t>(blockIdx.x) >= ctas) {
+    if (cta >= ctas) {
         w.lo = w.hi = 0;
         return w;
     }
@@ -374,27 +374,29 @@ __device__ __forceinline__ void load_queries(const CacheView& c, const AttendPar
 }
 
 // The parts of a divided segment to the output, in their order, so that the result does not depend
-// on which CTA comes last. A part: kRows x DP sums (four columns of all rows together), the rows'
-// references (base 2), their weights' sums. scratch: join_scratch() bytes of shared memory. All
-// kThreads threads of named barrier 1.
+// on which CTA comes last: its kJoin rows from `first` on. A part: kRows x DP sums (four columns of all
+// rows together), the rows' references (base 2), their weights' sums. scratch: join_scratch(kJoin) bytes
+// of shared memory. All kThreads threads of named barrier 1.
 //
 // The last CTA joins alone, so that its latency is the call's: the parts' shares go through shared
 // memory once, and the values are read in flat order, where one index gives row and place (indexes kept
-// an item each cost the loop before it 40 registers a thread: 64 beams over 4096 in 79 us for 71). One
-// sequence of 14000 positions, 32 parts: 42 us; with shares found again for each value 56 us.
+// an item each cost the loop before it 40 registers a thread: 64 beams over 4096 in 79 us for 71).
 constexpr int kMaxParts = 34;  // of a segment (split_work)
 constexpr int join_scratch(int rows) { return rows * (12 + 4 * kMaxParts); }
 
-template <class T, int kRows, int DP, int kThreads>
+template <class T, int kRows, int DP, int kThreads, int kJoin = kRows, int kEach = 4, int kAtOnce = (kThreads > 256 ? 2 : 4)>
 __device__ __forceinline__ void join_parts(const CacheView& c, const AttendParams& a, Piece p, Span span, int b,
-                                           int beam0, int row0, int rows, const float* parts, void* scratch, int tid) {
+                                           int beam0, int row0, int rows, const float* parts, void* scratch, int tid,
+                                           int first = 0) {
     constexpr int kOut = kRows * (DP + 2);
+    rows = rows - first < kJoin ? rows - first : kJoin;
+    row0 += first;
     const int n_parts = span.c1 - span.c0 + 1;
     // A CTA's second part is the one that begins a segment.
     auto part_of = [&](int i) { return parts + static_cast<int64_t>(2 * (span.c0 + i) + (i == 0)) * kOut; };
     int64_t* places = static_cast<int64_t*>(scratch);
-    float* shown_rows = reinterpret_cast<float*>(places + kRows);  // 1; 0 for rows that are not shown
-    float* factors = shown_rows + kRows;                           // [part][row]: the part's share over the sum
+    float* shown_rows = reinterpret_cast<float*>(places + kJoin);  // 1; 0 for rows that are not shown
+    float* factors = shown_rows + kJoin;                           // [part][row]: the part's share over the sum
     // Eight lanes a row, each for every eighth part.
 #pragma unroll 1
     for (int r0 = 0; r0 < rows; r0 += kThreads / 8) {
@@ -407,13 +409,13 @@ __device__ __forceinline__ void join_parts(const CacheView& c, const AttendParam
             for (int k = 0; k < 4; ++k) {
                 const int j = j0 + lane + 8 * k;
                 const bool there = j < n_parts && r < rows;
-                pm[k] = there ? __ldcg(part_of(j) + kRows * DP + r) : -INFINITY;
-                pl[k] = there ? __ldcg(part_of(j) + kRows * DP + kRows + r) : 0.0f;
+                pm[k] = there ? __ldcg(part_of(j) + kRows * DP + first + r) : -INFINITY;
+                pl[k] = there ? __ldcg(part_of(j) + kRows * DP + kRows + first + r) : 0.0f;
             }
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const int j = j0 + lane + 8 * k;
-                if (j < n_parts && r < rows) factors[j * kRows + r] = pm[k];
+                if (j < n_parts && r < rows) factors[j * kJoin + r] = pm[k];
                 now = fmaxf(now, pm[k]);
             }
 #pragma unroll
@@ -430,7 +432,7 @@ __device__ __forceinline__ void join_parts(const CacheView& c, const AttendParam
         const float ref = m == -INFINITY ? 0.0f : m, inverse = l > 0.0f ? 1.0f / l : l;
 #pragma unroll 1
         for (int j = lane; j < n_parts; j += 8) {
-            float& f = factors[j * kRows + r];  // this lane's own
+            float& f = factors[j * kJoin + r];  // this lane's own
             f = exp2_fast(f - ref) * inverse;
         }
         if (lane == 0) {
@@ -445,9 +447,8 @@ __device__ __forceinline__ void join_parts(const CacheView& c, const AttendParam
     }
     __syncwarp();
     asm volatile("barrier.sync 1, %0;" ::"r"(kThreads) : "memory");
-    // Four values of four items from four parts (two, with 512 threads' registers) in flight.
-    constexpr int kEach = 4, kAtOnce = kThreads > 256 ? 2 : 4;
-    const int items = kRows * (c.D / 4);
+    // Four values of kEach items from kAtOnce parts in flight.
+    const int items = kJoin * (c.D / 4);
 #pragma unroll 1
     for (int i0 = tid; i0 < items; i0 += kEach * kThreads) {
         float4 o[kEach];
@@ -462,7 +463,7 @@ __device__ __forceinline__ void join_parts(const CacheView& c, const AttendParam
 #pragma unroll
                 for (int e = 0; e < kEach; ++e) {
                     const int i = i0 + e * kThreads;
-                    v[k][e] = i < items && i % kRows < rows ? __ldcg(reinterpret_cast<const float4*>(x) + i) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    v[k][e] = i < items && i % kJoin < rows ? __ldcg(reinterpret_cast<const float4*>(x) + i / kJoin * kRows + first + i % kJoin) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                 }
             }
 #pragma unroll
@@ -470,8 +471,8 @@ __device__ __forceinline__ void join_parts(const CacheView& c, const AttendParam
                 if (j0 + k >= n_parts) break;
 #pragma unroll
                 for (int e = 0; e < kEach; ++e) {
-                    const int r = (i0 + e * kThreads) % kRows;
-                    const float f = factors[(j0 + k) * kRows + (r < rows ? r : 0)];
+                    const int r = (i0 + e * kThreads) % kJoin;
+                    const float f = factors[(j0 + k) * kJoin + (r < rows ? r : 0)];
                     o[e].x = fmaf(v[k][e].x, f, o[e].x), o[e].y = fmaf(v[k][e].y, f, o[e].y);
                     o[e].z = fmaf(v[k][e].z, f, o[e].z), o[e].w = fmaf(v[k][e].w, f, o[e].w);
                 }
@@ -479,10 +480,10 @@ __device__ __forceinline__ void join_parts(const CacheView& c, const AttendParam
         }
 #pragma unroll
         for (int e = 0; e < kEach; ++e) {
-            const int i = i0 + e * kThreads, r = i % kRows;
+            const int i = i0 + e * kThreads, r = i % kJoin;
             if (i >= items || r >= rows) continue;
             if (shown_rows[r] == 0.0f) o[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            store4(static_cast<T*>(a.out) + places[r] * c.D + i / kRows * 4, o[e]);
+            store4(static_cast<T*>(a.out) + places[r] * c.D + i / kJoin * 4, o[e]);
         }
     }
 }

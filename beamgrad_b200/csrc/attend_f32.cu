@@ -65,7 +65,7 @@ attend_f32_kernel(const __grid_constant__ CacheView c, const __grid_constant__ A
     const int tile_units = S::kKeys >> c.page_log2 > 0 ? S::kKeys >> c.page_log2 : 1;
     const int page_tiles = c.page > S::kKeys ? c.page / S::kKeys : 1;  // tiles of a page (64 by tiles of 32)
 
-    const WorkSplit work = split_work<S::kRows>(c, a, tile_units, 1, ctl.sums, &ctl.split);
+    const WorkSplit work = split_work<S::kRows>(c, a, tile_units, 1, ctl.sums, &ctl.split, blockIdx.x, gridDim.x);
     grid_wait();
     grid_release();
     if (__ldcg(c.status + 1) != 0) {

@@ -59,9 +59,11 @@ struct Shape {
     static constexpr int kCopyWarp = kSoftThreads / 32, kIssueWarp = kCopyWarp + 1;
     static constexpr int kBlocks = DP / 64;
     static constexpr int kSlot = kTileKeys * DP * 2;
+    // Divided segments are joined here, or by attend_join_kernel.
+    static constexpr bool kJoined = COPIES > 1;
     // The queries; at the end of a segment copies (256 x 32 floats) and parts are joined there.
-    static constexpr int kLeast = join_scratch(kRows) > 32768 ? (join_scratch(kRows) + 1023) / 1024 * 1024 : 32768;
-    static constexpr int kQuery = NQ * 128 * DP * 2 > kLeast ? NQ * 128 * DP * 2 : kLeast;
+    static constexpr int kQuery = NQ * 128 * DP * 2 > 32768 ? NQ * 128 * DP * 2 : 32768;
+    static_assert(!kJoined || join_scratch(kRows) <= kQuery);
     static constexpr int kFit = (227 * 1024 - static_cast<int>(sizeof(Control)) - kQuery) / kSlot;
     static constexpr int kSlots = kFit < kMaxSlots ? kFit : kMaxSlots;
     static constexpr int kOut = kRows * (DP + 2);  // floats of a partial result
@@ -235,7 +237,7 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
     // that is not complete, the others before they look whether a value was not finite.
     if (a.k == nullptr) grid_wait();
     grid_release();
-    const WorkSplit work = split_work<S::kRows>(c, a, tile_units, kMinTiles, ctl.sums, &ctl.split);
+    const WorkSplit work = split_work<S::kRows>(c, a, tile_units, kMinTiles, ctl.sums, &ctl.split, blockIdx.x, gridDim.x);
     if (work.lo >= work.hi) {
         grid_wait();
         if (__ldcg(c.status + 1) != 0 && warp < kSoftThreads / 32)
@@ -655,7 +657,7 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
         // together).
         const bool whole = p.t0 == 0 && p.t1 == p.tiles;
         float* parts = static_cast<float*>(a.workspace) + 2048;
-        int32_t* counters = static_cast<int32_t*>(a.workspace);
+        [[maybe_unused]] int32_t* counters = static_cast<int32_t*>(a.workspace);
         float* part = parts + static_cast<int64_t>(2 * blockIdx.x + (p.t0 == 0)) * S::kOut;
         float m = top == -INFINITY ? top : top * scale, l = sum;  // base-2 maximum, sum
         const bool holds_rows = (my_row & ~31) < rows && (NQ == 1 || began);  // of the warp
@@ -797,23 +799,61 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
                 part[S::kRows * DP + S::kRows + my_row] = l;
             }
         }
-        if (whole) continue;
-        named_sync(1, kSoftThreads);
-        const Span span = span_of(work, p);
-        if (tid == 0) {
-            __threadfence();  // of all the threads' stores, which the barrier put before this
-            const int before = atomicAdd(counters + span.c0, 1);
-            ctl.last = before == span.c1 - span.c0;
-            if (ctl.last) counters[span.c0] = 0;
+        if constexpr (S::kJoined) {
+            if (whole) continue;
+            named_sync(1, kSoftThreads);
+            const Span span = span_of(work, p);
+            if (tid == 0) {
+                __threadfence();  // of all the threads' stores, which the barrier put before this
+                const int before = atomicAdd(counters + span.c0, 1);
+                ctl.last = before == span.c1 - span.c0;
+                if (ctl.last) counters[span.c0] = 0;
+            }
+            named_sync(1, kSoftThreads);
+            if (!ctl.last) continue;
+            __threadfence();
+            join_parts<T, S::kRows, DP, kSoftThreads>(c, a, p, span, b, beam0, row0, rows, parts, query, tid);
         }
-        named_sync(1, kSoftThreads);
-        if (!ctl.last) continue;
-        __threadfence();
-        join_parts<T, S::kRows, DP, kSoftThreads>(c, a, p, span, b, beam0, row0, rows, parts, query, tid);
     }
     fence_before();
     named_sync(2, kSoftThreads + 32);
     if (odd) attend_all_rows<T>(c, a, reinterpret_cast<float*>(query), warp, kSoftThreads / 32);
+}
+
+// Joins the divided segments of blocks of 128 rows and more, a quarter of a block a CTA, and a segment by
+// the CTAs numbered after the one that has its first tile. The last of a segment's CTAs alone would read
+// parts of 64 or 128 KB: 8 sequences of 32 beams over 4060 took 88 us, 6 beams' drafts of 18 over 1222
+// 41.5 us, with this kernel 82.7 and 35.3; only where all CTAs join while others still work it costs a
+// little (16 drafted trees of 64 over 8192: 342 us, now 347). Smaller blocks' parts are joined within
+// less time than a kernel takes to start.
+constexpr int kJoinThreads = 256;
+
+template <class T, int kRows, int DP>
+__global__ void __launch_bounds__(kJoinThreads, 4)
+attend_join_kernel(const __grid_constant__ CacheView c, const __grid_constant__ AttendParams a, int ctas) {
+    constexpr int kJoin = kRows / 4;
+    __shared__ __align__(16) uint8_t scratch[join_scratch(kJoin)];
+    __shared__ int sums[35];
+    __shared__ WorkSplit found;
+    grid_release();
+    const int cta = blockIdx.x / 4, first = blockIdx.x % 4 * kJoin, tile_units = kTileKeys >> c.page_log2;
+    const WorkSplit work = split_work<kRows>(c, a, tile_units, kMinTiles, sums, &found, cta, ctas);
+    Piece p{};
+    bool divided = false;  // a segment begins among this CTA's tiles and ends past them
+    if (work.lo < work.hi) {
+        int group = work.group;
+        int64_t base = work.base;
+        p = piece_at<kRows>(c, a, work, work.hi - 1, group, base, tile_units);
+        divided = p.first >= work.lo && p.first + p.tiles > work.hi;
+    }
+    const int row0 = p.block * kRows, rows = p.rows - row0 < kRows ? p.rows - row0 : kRows;
+    grid_wait();
+    // (After a value that was not finite the outputs are complete.)
+    if (!divided || first >= rows || __ldcg(c.status + 1) != 0) return;
+    const Span span{cta, cta_of(work, p.first + p.tiles - 1)};
+    const int b = p.group / c.groups, beam0 = (p.group - b * c.groups) * kGroupBeams;
+    join_parts<T, kRows, DP, kJoinThreads, kJoin, 2, 4>(c, a, p, span, b, beam0, row0, rows,
+                                                        static_cast<const float*>(a.workspace) + 2048, scratch, threadIdx.x, first);
 }
 
 template <class T, int DP, int NQ, int COPIES>
@@ -823,9 +863,12 @@ cudaError_t launch_shape(const CacheView& c, const CUtensorMap& map, const Atten
     static_assert(S::kBytes <= 227 * 1024 && S::kSlots >= 4);
     auto* kernel = attend_tc_kernel<T, DP, NQ, COPIES>;
     static std::atomic<uint64_t> ready{0};  // a bit a device
-    const cudaError_t e = allow_shared(kernel, S::kBytes, ready);
-    if (e != cudaSuccess) return e;
-    return launch_after(kernel, sm_count, S::kThreads, S::kBytes, stream, map, c, a);
+    cudaError_t e = allow_shared(kernel, S::kBytes, ready);
+    if (e == cudaSuccess) e = launch_after(kernel, sm_count, S::kThreads, S::kBytes, stream, map, c, a);
+    if constexpr (!S::kJoined) {
+        if (e == cudaSuccess) e = launch_after(attend_join_kernel<T, S::kRows, DP>, 4 * sm_count, kJoinThreads, 0, stream, c, a, sm_count);
+    }
+    return e;
 }
 
 template <class T, int DP>
