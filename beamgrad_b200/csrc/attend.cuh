@@ -380,7 +380,7 @@ __device__ __forceinline__ void load_queries(const CacheView& c, const AttendPar
 //
 // The last CTA joins alone, so that its latency is the call's: the parts' shares go through shared
 // memory once, and the values are read in flat order, where one index gives row and place (indexes kept
-// an item each cost the loop before it 40 registers a thread: 64 beams over 4096 in 79 us for 71).
+// an item each cost the loop before it its registers: 64 sequences of 8 beams over 576 in 79 us for 71).
 constexpr int kMaxParts = 34;  // of a segment (split_work)
 constexpr int join_scratch(int rows) { return rows * (12 + 4 * kMaxParts); }
 

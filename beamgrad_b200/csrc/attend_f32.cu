@@ -311,10 +311,13 @@ attend_f32_kernel(const __grid_constant__ CacheView c, const __grid_constant__ A
     }
 }
 
+// Floats of the largest partial result.
+constexpr int kMostOut = Shape<128, 64>::kOut > Shape<256, 32>::kOut ? Shape<128, 64>::kOut : Shape<256, 32>::kOut;
+
 template <int DP, int ROWS>
 cudaError_t launch_shape(const CacheView& c, const AttendParams& a, int sm_count, cudaStream_t stream) {
     using S = Shape<DP, ROWS>;
-    static_assert(S::kBytes <= 224 * 1024 && join_scratch(ROWS) <= S::kBytes);
+    static_assert(S::kBytes <= 224 * 1024 && join_scratch(ROWS) <= S::kBytes && S::kOut <= kMostOut);
     auto* kernel = attend_f32_kernel<DP, ROWS>;
     static std::atomic<uint64_t> ready{0};  // a bit a device
     const cudaError_t e = allow_shared(kernel, S::kBytes, ready);
@@ -338,7 +341,7 @@ cudaError_t launch_width(const CacheView& c, const AttendParams& a, int sm_count
 
 int64_t attend_f32_workspace(const CacheView&, const AttendParams&, int sm_count) {
     // A counter for each CTA (8192 bytes), then two partial results for each.
-    return 8192 + static_cast<int64_t>(2) * sm_count * Shape<256, 32>::kOut * 4;
+    return 8192 + static_cast<int64_t>(2) * sm_count * kMostOut * 4;
 }
 
 cudaError_t launch_attend_f32(const CacheView& c, const AttendParams& a, int sm_count, cudaStream_t stream) {

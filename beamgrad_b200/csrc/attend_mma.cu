@@ -424,6 +424,7 @@ template <class T, int WR>
 cudaError_t launch_shape(const CacheView& c, const CUtensorMap& map, const AttendParams& a, int sm_count,
                          cudaStream_t stream) {
     using S = Shape<WR>;
+    static_assert(S::kOut <= Shape<2>::kOut);
     auto* kernel = attend_mma_kernel<T, WR>;
     static std::atomic<uint64_t> ready{0};  // a bit a device
     const cudaError_t e = allow_shared(kernel, S::kBytes, ready);

@@ -824,7 +824,7 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
 // the CTAs numbered after the one that has its first tile. The last of a segment's CTAs alone would read
 // parts of 64 or 128 KB: 8 sequences of 32 beams over 4060 took 88 us, 6 beams' drafts of 18 over 1222
 // 41.5 us, with this kernel 82.7 and 35.3; only where all CTAs join while others still work it costs a
-// little (16 drafted trees of 64 over 8192: 342 us, now 347). Smaller blocks' parts are joined within
+// little (16 drafted trees of 64 over 8064: 342 us, now 347). Smaller blocks' parts are joined within
 // less time than a kernel takes to start.
 constexpr int kJoinThreads = 256;
 
@@ -860,7 +860,7 @@ template <class T, int DP, int NQ, int COPIES>
 cudaError_t launch_shape(const CacheView& c, const CUtensorMap& map, const AttendParams& a, int sm_count,
                          cudaStream_t stream) {
     using S = Shape<DP, NQ, COPIES>;
-    static_assert(S::kBytes <= 227 * 1024 && S::kSlots >= 4);
+    static_assert(S::kBytes <= 227 * 1024 && S::kSlots >= 4 && S::kOut <= Shape<128, 2, 1>::kOut);
     auto* kernel = attend_tc_kernel<T, DP, NQ, COPIES>;
     static std::atomic<uint64_t> ready{0};  // a bit a device
     cudaError_t e = allow_shared(kernel, S::kBytes, ready);

@@ -527,6 +527,24 @@ def test_infinite_scores():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("N, dim", [(1, 128), (16, 64), (31, 256), (40, 64), (64, 128), (72, 200), (130, 128), (300, 64)])
+def test_divided_segments_stay_in_their_workspace(N, dim, dtype):
+    # 1800 pages by heads: every CTA has parts of segments, and the last one's lie last in the workspace.
+    cache = random_cache(1, 1, np.full((1, 1), 14400), N, layers=1, heads=8, dim=dim, page=64, dtype=dtype, seed=N)
+    q, k, v = tensors(cache, N, 1, N)
+    cache.attend(0, q[:, :, :1], k[:, :, :1], v[:, :, :1])
+    (stream, workspace), = cache._workspaces.items()
+    behind = 4 << 20
+    guarded = torch.zeros(workspace.numel() + behind, dtype=torch.uint8, device="cuda")
+    guarded[-behind:] = 0x5A
+    cache._workspaces[stream] = guarded[:-behind]
+    check_attend(cache, 0, q, k, v)
+    assert cache._workspaces[stream].data_ptr() == guarded.data_ptr()
+    assert bool((guarded[-behind:] == 0x5A).all())
+
+
+@pytest.mark.gpu
 def test_strides_streams_and_fewer_beams():
     B, K, N, H, G, D = 2, 4, 3, 2, 3, 64
     cache = random_cache(B, K, np.full((B, K), 37), N, heads=H, dtype=torch.float16, seed=4)
