@@ -107,27 +107,43 @@ attend_f32_kernel(const __grid_constant__ CacheView c, const __grid_constant__ A
             if (r < rows && v < vecs) q = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + ctl.query_at[r]) + v);
             *reinterpret_cast<float4*>(query + r * S::kPitch + v * 4) = q;
         }
+        // The first tile from t on that a beam of the block sees: beams of one group that draft many tokens
+        // fill a block each, and the others' own pages are not theirs (5 x 17 beams of 62 tokens over 72: 974 us, so 191).
+        const int first_beam = row0 / (a.N * a.G), beams = (row0 + rows - 1) / (a.N * a.G) - first_beam + 1;
+        const uint32_t seen = (beams < 32 ? (1u << beams) - 1 : 0xffffffffu) << first_beam;
+        const bool sees_all = beams * a.N * a.G == p.rows;
+        auto next_seen = [&](int t) {
+            if (sees_all) return t;
+            for (; t < n_tiles; t += 32) {
+                const int at = t + lane, unit = (p.t0 + at / page_tiles) * tile_units;
+                bool any = false;
+                for (int i = unit; at < n_tiles && i < unit + tile_units && i < p.units; ++i) any |= (__ldg(&units[i].mask) & seen) != 0;
+                const uint32_t found = __ballot_sync(0xffffffffu, any);
+                if (found != 0) return t + __ffs(found) - 1;
+            }
+            return n_tiles;
+        };
         // Where the rows of tile t lie: kKeys positions of its units' pages; past the last unit page 0,
         // whatever finite values lie there meet weights of zero.
-        auto find = [&](int t) {
+        auto find = [&](int t, int slot) {
             if (tid >= S::kKeys || t >= n_tiles) return;
             const int first = (p.t0 + t / page_tiles) * tile_units, offset = t % page_tiles * S::kKeys;
             const int unit = first + (tid >> c.page_log2);
             int4 v = make_int4(0, 0, 0, -1);  // no beam holds it
             if (unit < p.units) v = __ldg(reinterpret_cast<const int4*>(units + unit));
-            ctl.row_at[t & 1][tid] = (((static_cast<int64_t>(v.x) * c.H + p.head) << c.page_log2) + ((tid + offset) & (c.page - 1))) * c.D;
+            ctl.row_at[slot][tid] = (((static_cast<int64_t>(v.x) * c.H + p.head) << c.page_log2) + ((tid + offset) & (c.page - 1))) * c.D;
             if ((tid & (c.page - 1)) == 0)
-                ctl.unit[t & 1][tid >> c.page_log2] = CacheUnit{v.x, v.y + offset, static_cast<uint32_t>(v.z), v.w};
+                ctl.unit[slot][tid >> c.page_log2] = CacheUnit{v.x, v.y + offset, static_cast<uint32_t>(v.z), v.w};
         };
-        auto fetch = [&](int t) {
+        auto fetch = [&](int slot) {
             constexpr int kChunks = DP / 4, kAtOnce = kThreads / kChunks;
-            float* stage = stages + (t & 1) * S::kStage;
+            float* stage = stages + slot * S::kStage;
             const int v = tid % kChunks, first = tid / kChunks;
             if (v < vecs) {
 #pragma unroll
                 for (int j = 0; j < S::kKeys / kAtOnce; ++j) {
                     const int key = first + j * kAtOnce;
-                    const float* from = pages + ctl.row_at[t & 1][key] + v * 4;
+                    const float* from = pages + ctl.row_at[slot][key] + v * 4;
                     copy16(stage + key * S::kPitch + v * 4, from);
                     copy16(stage + (S::kKeys + key) * S::kPitch + v * 4, from + kind_step);
                 }
@@ -149,20 +165,21 @@ attend_f32_kernel(const __grid_constant__ CacheView c, const __grid_constant__ A
 #pragma unroll
             for (int r = 0; r < kOwn; ++r) acc[j][r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 
-        find(0);
+        int now_t = next_seen(0), next_t = next_seen(now_t + 1);
+        find(now_t, 0);
         __syncthreads();
-        fetch(0);
-        find(1);
+        if (now_t < n_tiles) fetch(0);
+        find(next_t, 1);
         __syncthreads();
-        for (int t = 0; t < n_tiles; ++t) {
-            if (t + 1 < n_tiles) {
-                fetch(t + 1);
+        for (int slot = 0; now_t < n_tiles; slot ^= 1) {
+            if (next_t < n_tiles) {
+                fetch(slot ^ 1);
                 asm volatile("cp.async.wait_group 1;" ::: "memory");
             } else {
                 asm volatile("cp.async.wait_group 0;" ::: "memory");
             }
             __syncthreads();
-            const float* keys = stages + (t & 1) * S::kStage;
+            const float* keys = stages + slot * S::kStage;
             const float* values = keys + S::kKeys * S::kPitch;
             {
                 float s[4][4];
@@ -198,7 +215,7 @@ attend_f32_kernel(const __grid_constant__ CacheView c, const __grid_constant__ A
                     float v = scores[w_row * S::kScorePitch + key];
 #pragma unroll
                     for (int i = 1; i < S::kSplit; ++i) v += scores[i * S::kScores + w_row * S::kScorePitch + key];
-                    const CacheUnit u = ctl.unit[t & 1][key >> c.page_log2];
+                    const CacheUnit u = ctl.unit[slot][key >> c.page_log2];
                     bool sees = (u.mask & bit) != 0;
                     const int j = u.start + (key & (c.page - 1)) - u.limit;
                     if (sees && u.limit >= 0 && j >= 0) sees = j < count && (fresh ? fresh[j] != 0 : j <= id.token);
@@ -249,7 +266,9 @@ attend_f32_kernel(const __grid_constant__ CacheView c, const __grid_constant__ A
                     }
                 }
             }
-            find(t + 2);  // (tile t's places and units were last read before the last barrier but one)
+            now_t = next_t;
+            next_t = next_seen(now_t + 1);
+            find(next_t, slot);  // (this tile's places and units were last read before the last barrier but one)
             __syncthreads();
         }
         // To the output, or to this CTA's part of a divided segment.

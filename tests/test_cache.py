@@ -439,6 +439,9 @@ ATTEND = [  # B, K, length, N, heads, group, dim, page, tree
     (1, 1, 31, 17, 2, 2, 72, 16, True),
     (1, 2, 100, 3, 1, 2, 256, 32, True),
     (1, 4, 70, 1, 1, 16, 200, 16, False),
+    (2, 5, 100, 20, 2, 4, 64, 16, True),   # blocks of rows that hold a beam and a part of others
+    (1, 3, 530, 70, 1, 2, 128, 32, True),  # a beam fills more than a block
+    (1, 32, 40, 33, 1, 4, 64, 16, False),
 ]
 
 
