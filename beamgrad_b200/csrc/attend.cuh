@@ -346,6 +346,53 @@ __device__ __forceinline__ RowId row_id(const AttendParams& a, int r) {
     return id;
 }
 
+// The tiles of a piece that a beam of its row block holds a page of: beams that draft many tokens fill
+// blocks of their own, and the other beams' pages are nothing to those. All lanes of a warp together.
+struct SeenTiles {
+    const CacheUnit* units;  // the piece's first
+    uint32_t beams;          // of the block; 0: all that the group has
+    int count, step, parts;  // units: of the group from there on, a tile's; a unit's tiles if it fills several
+    int tiles, window;       // of the piece; the first of the 32 that `bits` tells of
+    uint32_t bits;
+
+    __device__ __forceinline__ void look() {
+        const int at = window + static_cast<int>(threadIdx.x & 31), unit = at / parts * step;
+        bool any = false;
+#pragma unroll 1
+        for (int i = unit; at < tiles && i < unit + step && i < count; ++i) any |= (__ldg(&units[i].mask) & beams) != 0;
+        bits = __ballot_sync(0xffffffffu, any);
+    }
+    // The first such tile from t on, or `tiles`; t never falls.
+    __device__ __forceinline__ int next(int t) {
+        if (beams == 0) return t;
+        if (window >= tiles) return tiles;
+        uint32_t rest = t - window < 32 ? bits & (0xffffffffu << (t - window)) : 0u;
+        while (rest == 0) {
+            window += 32;
+            if (window >= tiles) return tiles;
+            look();
+            rest = bits;
+        }
+        return window + __ffs(rest) - 1;
+    }
+};
+template <int kRows>
+__device__ __forceinline__ SeenTiles seen_tiles(const CacheView& c, const AttendParams& a, const Piece& p, int tile_units, int parts) {
+    const int row0 = p.block * kRows, rows = p.rows - row0 < kRows ? p.rows - row0 : kRows, per = a.N * a.G;
+    const int first = row0 / per, beams = (row0 + rows - 1) / per - first + 1;
+    SeenTiles s;
+    s.units = c.units + static_cast<int64_t>(p.group) * c.unit_cap + p.t0 * tile_units;
+    s.beams = beams * per == p.rows ? 0u : (beams < 32 ? (1u << beams) - 1 : 0xffffffffu) << first;
+    s.count = p.units - p.t0 * tile_units;
+    s.step = tile_units;
+    s.parts = parts;
+    s.tiles = (p.t1 - p.t0) * parts;
+    s.window = 0;
+    s.bits = 0;
+    if (s.beams != 0) s.look();
+    return s;
+}
+
 // The queries of a row block by kThreads threads, eight loads in flight each. at: the rows' places
 // in q, in shared memory; put(row, chunk, value) gets 16 bytes of every row of the block, zeros past
 // its end and past the head.

@@ -107,22 +107,7 @@ attend_f32_kernel(const __grid_constant__ CacheView c, const __grid_constant__ A
             if (r < rows && v < vecs) q = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + ctl.query_at[r]) + v);
             *reinterpret_cast<float4*>(query + r * S::kPitch + v * 4) = q;
         }
-        // The first tile from t on that a beam of the block sees: beams of one group that draft many tokens
-        // fill a block each, and the others' own pages are not theirs (5 x 17 beams of 62 tokens over 72: 974 us, so 191).
-        const int first_beam = row0 / (a.N * a.G), beams = (row0 + rows - 1) / (a.N * a.G) - first_beam + 1;
-        const uint32_t seen = (beams < 32 ? (1u << beams) - 1 : 0xffffffffu) << first_beam;
-        const bool sees_all = beams * a.N * a.G == p.rows;
-        auto next_seen = [&](int t) {
-            if (sees_all) return t;
-            for (; t < n_tiles; t += 32) {
-                const int at = t + lane, unit = (p.t0 + at / page_tiles) * tile_units;
-                bool any = false;
-                for (int i = unit; at < n_tiles && i < unit + tile_units && i < p.units; ++i) any |= (__ldg(&units[i].mask) & seen) != 0;
-                const uint32_t found = __ballot_sync(0xffffffffu, any);
-                if (found != 0) return t + __ffs(found) - 1;
-            }
-            return n_tiles;
-        };
+        SeenTiles seen = seen_tiles<S::kRows>(c, a, p, tile_units, page_tiles);
         // Where the rows of tile t lie: kKeys positions of its units' pages; past the last unit page 0,
         // whatever finite values lie there meet weights of zero.
         auto find = [&](int t, int slot) {
@@ -165,7 +150,8 @@ attend_f32_kernel(const __grid_constant__ CacheView c, const __grid_constant__ A
 #pragma unroll
             for (int r = 0; r < kOwn; ++r) acc[j][r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 
-        int now_t = next_seen(0), next_t = next_seen(now_t + 1);
+        // (5 x 17 beams of 62 tokens over 72: 974 us with every tile for every block, so 191.)
+        int now_t = seen.next(0), next_t = seen.next(now_t + 1);
         find(now_t, 0);
         __syncthreads();
         if (now_t < n_tiles) fetch(0);
@@ -267,7 +253,7 @@ attend_f32_kernel(const __grid_constant__ CacheView c, const __grid_constant__ A
                 }
             }
             now_t = next_t;
-            next_t = next_seen(now_t + 1);
+            next_t = seen.next(now_t + 1);
             find(next_t, slot);  // (this tile's places and units were last read before the last barrier but one)
             __syncthreads();
         }

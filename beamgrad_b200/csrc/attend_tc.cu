@@ -73,6 +73,12 @@ struct Shape {
 // ---- tcgen05 ----
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+// The first tile that is taken; a piece without any takes one all the same.
+__device__ __forceinline__ int first_tile(SeenTiles& seen) {
+    const int t = seen.next(0);
+    return t < seen.tiles ? t : 0;
+}
+
 // One lane of the (converged) warp. Products are issued by the elected lane of a warp that runs its
 // loop as a whole: with a loop for one lane alone, every operand of every product takes a detour to
 // the warp's uniform registers (8 products took 750 cycles to issue instead of 512).
@@ -205,7 +211,7 @@ __device__ __forceinline__ void exp2_pair(Pair x2, float& a, float& b) {
     b = __uint_as_float(__float_as_uint(q) + (__float_as_uint(v) << 23));
 }
 
-template <class T, int DP, int NQ, int COPIES>
+template <class T, int DP, int NQ, int COPIES, bool SKIP>
 __global__ void __launch_bounds__(Shape<DP, NQ, COPIES>::kThreads, 1)
 attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ CacheView c,
                  const __grid_constant__ AttendParams a) {
@@ -275,16 +281,25 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
                     return t < n_tiles && which < tile_units && i < p.units ? __ldg(reinterpret_cast<const int4*>(units + i))
                                                                             : make_int4(0, 0, 0, -1);
                 };
-                int4 next = unit_of(0);
+                int t = 0, after = 1;
+                SeenTiles seen;
+                if constexpr (SKIP) {
+                    seen = seen_tiles<S::kRows>(c, a, p, tile_units, 1);
+                    t = first_tile(seen);
+                    after = seen.next(t + 1);
+                }
+                int4 next = unit_of(t);
 #pragma unroll 1
-                for (int t = 0; t < n_tiles; ++t) {
+                while (t < n_tiles) {
                     const int page = next.x;
                     if (!waited && __any_sync(0xffffffffu, next.w >= 0)) {
                         grid_wait();
                         asm volatile("fence.proxy.async;" ::: "memory");
                         waited = true;
                     }
-                    next = unit_of(t + 1);
+                    next = unit_of(after);
+                    t = after++;
+                    if constexpr (SKIP) after = seen.next(after);
 #pragma unroll 1
                     for (int kind = 0; kind < 2; ++kind, ++used) {
                         const int slot = used % S::kSlots;
@@ -314,7 +329,15 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
             };
             for (int64_t cur = work.lo; cur < work.hi;) {
                 const Piece p = piece_at<S::kRows>(c, a, work, cur, group, base, tile_units);
-                const int n = p.t1 - p.t0;
+                int n = p.t1 - p.t0;
+                cur += n;
+                if constexpr (SKIP) {
+                    SeenTiles seen = seen_tiles<S::kRows>(c, a, p, tile_units, 1);
+                    if (seen.beams != 0) {
+                        n = 0;
+                        for (int t = first_tile(seen); t < seen.tiles; t = seen.next(t + 1)) ++n;
+                    }
+                }
                 barrier_wait(smem_address(&ctl.queries), query_phase, c.status);
                 query_phase ^= 1;
                 fence_after();
@@ -363,7 +386,6 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
                     if (j + streams < jobs) scores(j + streams);
                 }
                 used += 2 * n;
-                cur += n;
             }
             named_sync(2, kSoftThreads + 32);  // every read of tensor memory is over
             asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
@@ -447,7 +469,12 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
 
         float top = -INFINITY, sum = 0.0f;  // the reference (a score) and the weights' sum
         const bool active = NQ == 1 || rows > stream * 128;
-        const int first = NQ == 2 ? 0 : stream, step = NQ == 2 ? 1 : 2;
+        SeenTiles seen;
+        int first = NQ == 2 ? 0 : stream;
+        if constexpr (SKIP) {
+            seen = seen_tiles<S::kRows>(c, a, p, tile_units, 1);
+            first = first_tile(seen);
+        }
         bool began = false;
         if (active) {
             // Tiles from the first on whose units are all complete and held by every row of the warp.
@@ -482,7 +509,7 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
                 return u;
             };
 #pragma unroll 1
-            for (int t = first; t < n_tiles; t += step) {
+            for (int t = first; t < n_tiles; t = SKIP ? seen.next(t + 1) : t + (NQ == 2 ? 1 : 2)) {
                 CacheUnit u{-1, 0, 0, -1};
                 bool none = need == 0, plain = true;
                 if (t >= plain_tiles) {
@@ -856,12 +883,12 @@ attend_join_kernel(const __grid_constant__ CacheView c, const __grid_constant__ 
                                                         static_cast<const float*>(a.workspace) + 2048, scratch, threadIdx.x, first);
 }
 
-template <class T, int DP, int NQ, int COPIES>
+template <class T, int DP, int NQ, int COPIES, bool SKIP>
 cudaError_t launch_shape(const CacheView& c, const CUtensorMap& map, const AttendParams& a, int sm_count,
                          cudaStream_t stream) {
     using S = Shape<DP, NQ, COPIES>;
     static_assert(S::kBytes <= 227 * 1024 && S::kSlots >= 4 && S::kOut <= Shape<128, 2, 1>::kOut);
-    auto* kernel = attend_tc_kernel<T, DP, NQ, COPIES>;
+    auto* kernel = attend_tc_kernel<T, DP, NQ, COPIES, SKIP>;
     static std::atomic<uint64_t> ready{0};  // a bit a device
     cudaError_t e = allow_shared(kernel, S::kBytes, ready);
     if (e == cudaSuccess) e = launch_after(kernel, sm_count, S::kThreads, S::kBytes, stream, map, c, a);
@@ -876,10 +903,14 @@ cudaError_t launch_width(const CacheView& c, const CUtensorMap& map, const Atten
                          cudaStream_t stream) {
     const int beams = a.beams < kGroupBeams ? a.beams : kGroupBeams;
     const int64_t rows = static_cast<int64_t>(beams) * a.N * a.G;
-    if (rows <= 32) return launch_shape<T, DP, 1, 4>(c, map, a, sm_count, stream);
-    if (rows <= 64) return launch_shape<T, DP, 1, 2>(c, map, a, sm_count, stream);
-    if (rows <= 128) return launch_shape<T, DP, 1, 1>(c, map, a, sm_count, stream);
-    return launch_shape<T, DP, 2, 1>(c, map, a, sm_count, stream);
+    if (rows <= 32) return launch_shape<T, DP, 1, 4, false>(c, map, a, sm_count, stream);
+    if (rows <= 64) return launch_shape<T, DP, 1, 2, false>(c, map, a, sm_count, stream);
+    if (rows <= 128) return launch_shape<T, DP, 1, 1, false>(c, map, a, sm_count, stream);
+    // Several blocks of several beams: a block passes over the tiles of which its beams hold nothing (17 beams
+    // of 62 tokens over 72: 92 us, so 75). Where every block has all beams that costs registers for nothing
+    // (16 drafted trees: 347 us, so 360).
+    if (rows > 256 && beams > 1) return launch_shape<T, DP, 2, 1, true>(c, map, a, sm_count, stream);
+    return launch_shape<T, DP, 2, 1, false>(c, map, a, sm_count, stream);
 }
 
 template <class T>
