@@ -191,40 +191,54 @@ struct WorkSplit {
     int64_t total;   // tiles
     int ctas;        // CTAs that take part
     int64_t lo, hi;  // this CTA's tiles
-    int group;       // group that tile lo lies in
+    int group;       // block of a group that tile lo lies in
     int64_t base;    // its first tile
 };
 
+// One row block of a group. The line has the first blocks of all groups, then the second ones and so on.
 struct GroupWork {
-    int units, tiles, blocks, rows;  // blocks: row blocks
+    int group, block;
+    int units, tiles, rows;  // of the group
+    bool there;              // the group has such a block
 };
 
 template <int kRows>
-__device__ __forceinline__ GroupWork group_work(const CacheView& c, const AttendParams& a, int g, int tile_units) {
-    const int first = (g % c.groups) * kGroupBeams;
+__device__ __forceinline__ int row_blocks(const CacheView& c, const AttendParams& a) {
+    const int beams = a.beams < kGroupBeams ? a.beams : kGroupBeams;
+    return (beams * a.N * a.G + kRows - 1) / kRows;
+}
+
+// kMany: a group may have more rows than a block.
+template <int kRows, bool kMany>
+__device__ __forceinline__ GroupWork group_work(const CacheView& c, const AttendParams& a, int i, int tile_units) {
+    const int groups = c.B * c.groups;
+    GroupWork w;
+    w.block = kMany && i >= groups ? i / groups : 0;
+    w.group = i - w.block * groups;
+    const int first = (w.group % c.groups) * kGroupBeams;
     int beams = a.beams - first;
     beams = beams < 0 ? 0 : (beams > kGroupBeams ? kGroupBeams : beams);
-    GroupWork w;
-    w.units = c.unit_count[g];
+    w.units = c.unit_count[w.group];
     w.tiles = (w.units + tile_units - 1) / tile_units;
     if (w.tiles < 1) w.tiles = 1;  // rows without a page are written too
     w.rows = beams * a.N * a.G;
-    w.blocks = (w.rows + kRows - 1) / kRows;
+    w.there = w.rows > w.block * kRows;
     return w;
 }
 
 // The share of CTA `cta` of `grid`. All threads of the block; sums: 35 ints, found: a WorkSplit in shared
 // memory. The host has checked that the tiles of all segments are counted in 31 bits.
-template <int kRows>
+template <int kRows, bool kMany>
 __device__ WorkSplit split_work(const CacheView& c, const AttendParams& a, int tile_units, int min_tiles, int* sums,
                                 WorkSplit* found, int cta, int grid) {
-    const int groups = c.B * c.groups, tid = threadIdx.x, threads = blockDim.x;
+    const int blocks = kMany ? row_blocks<kRows>(c, a) : 1, groups = c.B * c.groups * blocks, tid = threadIdx.x, threads = blockDim.x;
     auto tiles_of = [&](int g, int* longest) {
         *longest = 0;
         if (g >= groups) return 0;
-        const GroupWork w = group_work<kRows>(c, a, g, tile_units);
-        if (w.blocks > 0) *longest = w.tiles;
-        return w.tiles * w.blocks * c.H;
+        const GroupWork w = group_work<kRows, kMany>(c, a, g, tile_units);
+        if (!w.there) return 0;
+        *longest = w.tiles;
+        return w.tiles * c.H;
     };
     // One round where a thread a group is enough; its count and place are kept for below.
     int total = 0, mine = 0, at = 0;
@@ -246,6 +260,10 @@ __device__ WorkSplit split_work(const CacheView& c, const AttendParams& a, int t
         if (ctas > cap) ctas = cap;
     }
     if (ctas > grid) ctas = grid;
+    // CTAs with the same tiles for different row blocks take them at the same time, so that keys and
+    // values come from memory once for all blocks (16 drafted trees, two blocks each: 1.07 GB where the second
+    // block followed the first, 340 us; so 325).
+    if (kMany && blocks <= 8 && ctas >= 16 * blocks) ctas -= ctas % blocks;
     if (ctas < 1) ctas = 1;
     WorkSplit w;
     w.total = total;
@@ -309,26 +327,28 @@ __device__ __forceinline__ Span span_of(const WorkSplit& w, const Piece& p) {
 }
 
 // The piece at tile `cur` of the line; advances group and base to it.
-template <int kRows>
+template <int kRows, bool kMany>
 __device__ __forceinline__ Piece piece_at(const CacheView& c, const AttendParams& a, const WorkSplit& w, int64_t cur,
                                           int& group, int64_t& base, int tile_units) {
-    GroupWork g = group_work<kRows>(c, a, group, tile_units);
-    while (cur >= base + static_cast<int64_t>(g.tiles) * g.blocks * c.H) {
-        base += static_cast<int64_t>(g.tiles) * g.blocks * c.H;
-        g = group_work<kRows>(c, a, ++group, tile_units);
+    GroupWork g = group_work<kRows, kMany>(c, a, group, tile_units);
+    while (true) {
+        const int64_t size = g.there ? static_cast<int64_t>(g.tiles) * c.H : 0;
+        if (cur < base + size) break;
+        base += size;
+        g = group_work<kRows, kMany>(c, a, ++group, tile_units);
     }
-    const int off = static_cast<int>(cur - base), seg = off / g.tiles;
+    const int off = static_cast<int>(cur - base);
     Piece p;
-    p.group = group;
-    p.block = seg / c.H;
-    p.head = seg - p.block * c.H;
-    p.t0 = off - seg * g.tiles;
+    p.group = g.group;
+    p.block = g.block;
+    p.head = off / g.tiles;
+    p.t0 = off - p.head * g.tiles;
     const int64_t left = w.hi - cur;
     p.t1 = left < g.tiles - p.t0 ? p.t0 + static_cast<int>(left) : g.tiles;
     p.tiles = g.tiles;
     p.units = g.units;
     p.rows = g.rows;
-    p.first = base + static_cast<int64_t>(seg) * g.tiles;
+    p.first = base + static_cast<int64_t>(p.head) * g.tiles;
     return p;
 }
 

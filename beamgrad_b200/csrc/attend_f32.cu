@@ -35,6 +35,7 @@ struct Shape {
     static constexpr int kCols = DP / 128;
     static constexpr int kBytes = (2 * kStage + kSplit * kScores + kRows * kPitch) * 4;
     static constexpr int kOut = kRows * (DP + 2);
+    static constexpr bool kMany = kRows == 64 || (DP > 128 && kRows == 32);  // the most that a block has
 };
 
 struct Control {
@@ -65,7 +66,7 @@ attend_f32_kernel(const __grid_constant__ CacheView c, const __grid_constant__ A
     const int tile_units = S::kKeys >> c.page_log2 > 0 ? S::kKeys >> c.page_log2 : 1;
     const int page_tiles = c.page > S::kKeys ? c.page / S::kKeys : 1;  // tiles of a page (64 by tiles of 32)
 
-    const WorkSplit work = split_work<S::kRows>(c, a, tile_units, 1, ctl.sums, &ctl.split, blockIdx.x, gridDim.x);
+    const WorkSplit work = split_work<S::kRows, S::kMany>(c, a, tile_units, 1, ctl.sums, &ctl.split, blockIdx.x, gridDim.x);
     grid_wait();
     grid_release();
     if (__ldcg(c.status + 1) != 0) {
@@ -88,7 +89,7 @@ attend_f32_kernel(const __grid_constant__ CacheView c, const __grid_constant__ A
     const float* pages = static_cast<const float*>(c.pages) + static_cast<int64_t>(a.layer) * 2 * kind_step;
 
     for (int64_t cur = work.lo; cur < work.hi;) {
-        const Piece p = piece_at<S::kRows>(c, a, work, cur, group, base, tile_units);
+        const Piece p = piece_at<S::kRows, S::kMany>(c, a, work, cur, group, base, tile_units);
         const int n_tiles = (p.t1 - p.t0) * page_tiles;
         cur += p.t1 - p.t0;
         const int b = p.group / c.groups, beam0 = (p.group - b * c.groups) * kGroupBeams;

@@ -103,7 +103,7 @@ attend_mma_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     // The plan was complete before the new tokens' copy began; only the pages have to be waited for.
-    const WorkSplit work = split_work<S::kRows>(c, a, tile_units, 1, ctl.sums, &ctl.split, blockIdx.x, gridDim.x);
+    const WorkSplit work = split_work<S::kRows, (WR == 2)>(c, a, tile_units, 1, ctl.sums, &ctl.split, blockIdx.x, gridDim.x);
     __syncthreads();
     grid_wait();
     grid_release();
@@ -121,7 +121,7 @@ attend_mma_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant
         if (warp > kComputeWarps) return;
         asm volatile("fence.proxy.async;" ::: "memory");
         for (int64_t cur = work.lo; cur < work.hi;) {
-            const Piece p = piece_at<S::kRows>(c, a, work, cur, group, base, tile_units);
+            const Piece p = piece_at<S::kRows, (WR == 2)>(c, a, work, cur, group, base, tile_units);
             const CacheUnit* units = c.units + static_cast<int64_t>(p.group) * c.unit_cap;
             auto fetch = [&](int t) {
                 CacheUnit u{-1, 0, 0, -1};
@@ -169,7 +169,7 @@ attend_mma_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant
     const float scale = a.scale * kLog2e;
     const uint32_t query_at = smem_address(query) + (WR == 2 ? half * kHalfRows * DP * 2 : 0);
     for (int64_t cur = work.lo; cur < work.hi;) {
-        const Piece p = piece_at<S::kRows>(c, a, work, cur, group, base, tile_units);
+        const Piece p = piece_at<S::kRows, (WR == 2)>(c, a, work, cur, group, base, tile_units);
         const int b = p.group / c.groups, beam0 = (p.group - b * c.groups) * kGroupBeams;
         const int row0 = p.block * S::kRows;
         // The queries: [row][DP], 128-byte blocks swizzled by row.

@@ -243,7 +243,7 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
     // that is not complete, the others before they look whether a value was not finite.
     if (a.k == nullptr) grid_wait();
     grid_release();
-    const WorkSplit work = split_work<S::kRows>(c, a, tile_units, kMinTiles, ctl.sums, &ctl.split, blockIdx.x, gridDim.x);
+    const WorkSplit work = split_work<S::kRows, (NQ == 2)>(c, a, tile_units, kMinTiles, ctl.sums, &ctl.split, blockIdx.x, gridDim.x);
     if (work.lo >= work.hi) {
         grid_wait();
         if (__ldcg(c.status + 1) != 0 && warp < kSoftThreads / 32)
@@ -270,7 +270,7 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
         if (warp == kCopyWarp) {
             bool waited = false;
             for (int64_t cur = work.lo; cur < work.hi;) {
-                const Piece p = piece_at<S::kRows>(c, a, work, cur, group, base, tile_units);
+                const Piece p = piece_at<S::kRows, (NQ == 2)>(c, a, work, cur, group, base, tile_units);
                 const CacheUnit* units = c.units + static_cast<int64_t>(p.group) * c.unit_cap;
                 const int n_tiles = p.t1 - p.t0;
                 // The page of this lane's copy; past the last unit, page 0: whatever finite values lie
@@ -328,7 +328,7 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
                 fence_after();
             };
             for (int64_t cur = work.lo; cur < work.hi;) {
-                const Piece p = piece_at<S::kRows>(c, a, work, cur, group, base, tile_units);
+                const Piece p = piece_at<S::kRows, (NQ == 2)>(c, a, work, cur, group, base, tile_units);
                 int n = p.t1 - p.t0;
                 cur += n;
                 if constexpr (SKIP) {
@@ -433,7 +433,7 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
                                       (((chunk & 7) ^ (in & 7)) << 4)) = v;
         }
     };
-    Piece p = piece_at<S::kRows>(c, a, work, work.lo, group, base, tile_units), next_piece = p;
+    Piece p = piece_at<S::kRows, (NQ == 2)>(c, a, work, work.lo, group, base, tile_units), next_piece = p;
     fetch_ahead(p);
     for (int64_t cur = work.lo; cur < work.hi; p = next_piece) {
         const int n_tiles = p.t1 - p.t0;
@@ -663,7 +663,7 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
             }
         }
         if (cur < work.hi) {
-            next_piece = piece_at<S::kRows>(c, a, work, cur, group, base, tile_units);
+            next_piece = piece_at<S::kRows, (NQ == 2)>(c, a, work, cur, group, base, tile_units);
             fetch_ahead(next_piece);
         }
         if (!odd_known) {
@@ -864,13 +864,13 @@ attend_join_kernel(const __grid_constant__ CacheView c, const __grid_constant__ 
     __shared__ WorkSplit found;
     grid_release();
     const int cta = blockIdx.x / 4, first = blockIdx.x % 4 * kJoin, tile_units = kTileKeys >> c.page_log2;
-    const WorkSplit work = split_work<kRows>(c, a, tile_units, kMinTiles, sums, &found, cta, ctas);
+    const WorkSplit work = split_work<kRows, (kRows > 128)>(c, a, tile_units, kMinTiles, sums, &found, cta, ctas);
     Piece p{};
     bool divided = false;  // a segment begins among this CTA's tiles and ends past them
     if (work.lo < work.hi) {
         int group = work.group;
         int64_t base = work.base;
-        p = piece_at<kRows>(c, a, work, work.hi - 1, group, base, tile_units);
+        p = piece_at<kRows, (kRows > 128)>(c, a, work, work.hi - 1, group, base, tile_units);
         divided = p.first >= work.lo && p.first + p.tiles > work.hi;
     }
     const int row0 = p.block * kRows, rows = p.rows - row0 < kRows ? p.rows - row0 : kRows;
