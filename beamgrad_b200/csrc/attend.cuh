@@ -261,8 +261,8 @@ __device__ WorkSplit split_work(const CacheView& c, const AttendParams& a, int t
     }
     if (ctas > grid) ctas = grid;
     // CTAs with the same tiles for different row blocks take them at the same time, so that keys and
-    // values come from memory once for all blocks (16 drafted trees, two blocks each: 1.07 GB where the second
-    // block followed the first, 340 us; so 325).
+    // values come from memory once for all blocks (16 drafted trees, two blocks each: 1.07 GB read where the
+    // second block followed the first, 0.55 GB so; 346 us and 326).
     if (kMany && blocks <= 8 && ctas >= 16 * blocks) ctas -= ctas % blocks;
     if (ctas < 1) ctas = 1;
     WorkSplit w;

@@ -9,8 +9,9 @@
 // shared-memory reads of 16 bytes for 64 multiply-adds take 8 (12) passes of the banks: rows are
 // padded by 16 bytes, and rows of one read lie next to each other. At 32 rows of 128 the multiply-adds
 // take 4096 cycles a tile and SM, at 16 rows the bytes bound it (2800 cycles). 64 rows have 16 warps,
-// which hide each other's reads (165 rows over 14421: 335 us, with blocks of 32 and 8 warps 373); with
-// fewer rows 8 warps of larger tiles do better (32 rows over 16000: 184 us against 214).
+// which hide each other's reads (165 rows over 14421: 331 us, with blocks of 32 and 8 warps 373; with
+// the join as it is now 318); with fewer rows 8 warps of larger tiles do better (32 rows over 16000: 184 us
+// against 214, now 179: 39 % of the multiply-add pipe).
 #include "attend.cuh"
 
 namespace dbsb {

@@ -847,23 +847,22 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
     if (odd) attend_all_rows<T>(c, a, reinterpret_cast<float*>(query), warp, kSoftThreads / 32);
 }
 
-// Joins the divided segments of blocks of 128 rows and more, a quarter of a block a CTA, and a segment by
+// Joins the divided segments of blocks of 128 rows and more, an eighth of a block a CTA, and a segment by
 // the CTAs numbered after the one that has its first tile. The last of a segment's CTAs alone would read
 // parts of 64 or 128 KB: 8 sequences of 32 beams over 4060 took 88 us, 6 beams' drafts of 18 over 1222
-// 41.5 us, with this kernel 82.7 and 35.3; only where all CTAs join while others still work it costs a
-// little (16 drafted trees of 64 over 8064: 342 us, now 347). Smaller blocks' parts are joined within
-// less time than a kernel takes to start.
-constexpr int kJoinThreads = 256;
+// 41.5 us; with this kernel 74 and 34 (84 and 36 with four CTAs a segment). Smaller blocks' parts are
+// joined within less time than a kernel takes to start.
+constexpr int kJoinThreads = 256, kJoinCtas = 8;  // of a segment
 
 template <class T, int kRows, int DP>
 __global__ void __launch_bounds__(kJoinThreads, 4)
 attend_join_kernel(const __grid_constant__ CacheView c, const __grid_constant__ AttendParams a, int ctas) {
-    constexpr int kJoin = kRows / 4;
+    constexpr int kJoin = kRows / kJoinCtas;
     __shared__ __align__(16) uint8_t scratch[join_scratch(kJoin)];
     __shared__ int sums[35];
     __shared__ WorkSplit found;
     grid_release();
-    const int cta = blockIdx.x / 4, first = blockIdx.x % 4 * kJoin, tile_units = kTileKeys >> c.page_log2;
+    const int cta = blockIdx.x / kJoinCtas, first = blockIdx.x % kJoinCtas * kJoin, tile_units = kTileKeys >> c.page_log2;
     const WorkSplit work = split_work<kRows, (kRows > 128)>(c, a, tile_units, kMinTiles, sums, &found, cta, ctas);
     Piece p{};
     bool divided = false;  // a segment begins among this CTA's tiles and ends past them
@@ -874,9 +873,12 @@ attend_join_kernel(const __grid_constant__ CacheView c, const __grid_constant__ 
         divided = p.first >= work.lo && p.first + p.tiles > work.hi;
     }
     const int row0 = p.block * kRows, rows = p.rows - row0 < kRows ? p.rows - row0 : kRows;
+    // Those with nothing to do make room; the first one stays, so that this grid ends after the attention.
+    divided = divided && first < rows;
+    if (!divided && blockIdx.x != 0) return;
     grid_wait();
     // (After a value that was not finite the outputs are complete.)
-    if (!divided || first >= rows || __ldcg(c.status + 1) != 0) return;
+    if (!divided || __ldcg(c.status + 1) != 0) return;
     const Span span{cta, cta_of(work, p.first + p.tiles - 1)};
     const int b = p.group / c.groups, beam0 = (p.group - b * c.groups) * kGroupBeams;
     join_parts<T, kRows, DP, kJoinThreads, kJoin, 2, 4>(c, a, p, span, b, beam0, row0, rows,
@@ -893,7 +895,7 @@ cudaError_t launch_shape(const CacheView& c, const CUtensorMap& map, const Atten
     cudaError_t e = allow_shared(kernel, S::kBytes, ready);
     if (e == cudaSuccess) e = launch_after(kernel, sm_count, S::kThreads, S::kBytes, stream, map, c, a);
     if constexpr (!S::kJoined) {
-        if (e == cudaSuccess) e = launch_after(attend_join_kernel<T, S::kRows, DP>, 4 * sm_count, kJoinThreads, 0, stream, c, a, sm_count);
+        if (e == cudaSuccess) e = launch_after(attend_join_kernel<T, S::kRows, DP>, kJoinCtas * sm_count, kJoinThreads, 0, stream, c, a, sm_count);
     }
     return e;
 }
