@@ -571,6 +571,38 @@ def test_strides_streams_and_fewer_beams():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype, N, group", [(torch.bfloat16, 1, 4), (torch.float16, 12, 8), (torch.float32, 5, 3)])
+def test_a_step_in_a_cuda_graph(dtype, N, group):
+    B, K = 2, 4
+    graphed, plain = (random_cache(B, K, np.full((B, K), 700), N, dtype=dtype, seed=6) for _ in range(2))
+    inputs = [tensors(graphed, N, group, 40 + i) for i in range(4)]
+    parents = [torch.randint(0, K, (B, K), device="cuda", dtype=torch.int32) for _ in range(4)]
+    static, static_parents = [x.clone() for x in inputs[0]], parents[0].clone()
+
+    def step(cache, q, k, v, by):
+        outs = [cache.attend(layer, q, k, v) for layer in range(2)]
+        cache.fork(by, written=1, room=N)
+        return outs
+
+    step(graphed, *static, static_parents)  # not in the graph: shapes are checked once
+    step(plain, *inputs[0], parents[0])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(graphed, *static, static_parents)
+    for i in range(1, 4):
+        for x, y in zip(static, inputs[i]):
+            x.copy_(y)
+        static_parents.copy_(parents[i])
+        graph.replay()
+        want = step(plain, *inputs[i], parents[i])
+        for x, y in zip(got, want):
+            assert torch.equal(x, y)
+        assert torch.equal(graphed.table, plain.table) and torch.equal(graphed.lengths, plain.lengths)
+    graphed.check()
+
+
+@pytest.mark.gpu
 def test_attend_refusals():
     cache = PagedCache(2, 3, 64, num_layers=2, num_kv_heads=2, head_dim=64, page_size=16)
     q, k, v = tensors(cache, 2, 2, 0)
