@@ -67,13 +67,12 @@ attend_f32_kernel(const __grid_constant__ CacheView c, const __grid_constant__ A
     const int tile_units = S::kKeys >> c.page_log2 > 0 ? S::kKeys >> c.page_log2 : 1;
     const int page_tiles = c.page > S::kKeys ? c.page / S::kKeys : 1;  // tiles of a page (64 by tiles of 32)
 
-    const WorkSplit work = split_work<S::kRows, S::kMany>(c, a, tile_units, 1, ctl.sums, &ctl.split, blockIdx.x, gridDim.x);
-    grid_wait();
+    // This kernel may run while the new tokens are still being written. Plan, lengths, queries and complete
+    // pages were there before that began; the first copy from a page that is not complete waits for it.
+    if (a.k == nullptr) grid_wait();
     grid_release();
-    if (__ldcg(c.status + 1) != 0) {
-        attend_all_rows<float>(c, a, smem, warp, kThreads / 32);
-        return;
-    }
+    const WorkSplit work = split_work<S::kRows, S::kMany>(c, a, tile_units, 1, ctl.sums, &ctl.split, blockIdx.x, gridDim.x);
+    bool waited = a.k == nullptr, odd = false, odd_known = false;  // odd: a value that is not finite was met, now or before
     int group = work.group;
     int64_t base = work.base;
     const float scale = a.scale * kLog2e;
@@ -126,6 +125,11 @@ attend_f32_kernel(const __grid_constant__ CacheView c, const __grid_constant__ A
             constexpr int kChunks = DP / 4, kAtOnce = kThreads / kChunks;
             float* stage = stages + slot * S::kStage;
             const int v = tid % kChunks, first = tid / kChunks;
+            for (int i = 0; !waited && i < tile_units; ++i) {
+                if (ctl.unit[slot][i].limit < 0) continue;
+                grid_wait();
+                waited = true;
+            }
             if (v < vecs) {
 #pragma unroll
                 for (int j = 0; j < S::kKeys / kAtOnce; ++j) {
@@ -259,6 +263,12 @@ attend_f32_kernel(const __grid_constant__ CacheView c, const __grid_constant__ A
             find(next_t, slot);  // (this tile's places and units were last read before the last barrier but one)
             __syncthreads();
         }
+        if (!odd_known) {
+            grid_wait();
+            odd = __ldcg(c.status + 1) != 0;
+            odd_known = true;
+        }
+        if (odd) break;
         // To the output, or to this CTA's part of a divided segment.
 #pragma unroll
         for (int m = kPerRow / 2; m > 0; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
@@ -315,6 +325,15 @@ attend_f32_kernel(const __grid_constant__ CacheView c, const __grid_constant__ A
         if (!ctl.last) continue;
         __threadfence();
         join_parts<float, S::kRows, DP, kThreads>(c, a, p, span, b, beam0, row0, rows, parts, smem, tid);
+    }
+    if (!odd_known) {  // (a CTA without tiles)
+        grid_wait();
+        odd = __ldcg(c.status + 1) != 0;
+    }
+    // Weights of zero would not keep such a value out of the sums. All CTAs see that.
+    if (odd) {
+        __syncthreads();
+        attend_all_rows<float>(c, a, smem, warp, kThreads / 32);
     }
 }
 
