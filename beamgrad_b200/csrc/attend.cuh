@@ -229,7 +229,7 @@ __device__ __forceinline__ GroupWork group_work(const CacheView& c, const Attend
 // The share of CTA `cta` of `grid`. All threads of the block; sums: 35 ints, found: a WorkSplit in shared
 // memory. The host has checked that the tiles of all segments are counted in 31 bits.
 template <int kRows, bool kMany>
-__device__ WorkSplit split_work(const CacheView& c, const AttendParams& a, int tile_units, int min_tiles, int* sums,
+__device__ WorkSplit split_work(const CacheView& c, const AttendParams& a, int tile_units, int min_tiles, int spare, int* sums,
                                 WorkSplit* found, int cta, int grid) {
     const int blocks = kMany ? row_blocks<kRows>(c, a) : 1, groups = c.B * c.groups * blocks, tid = threadIdx.x, threads = blockDim.x;
     auto tiles_of = [&](int g, int* longest) {
@@ -242,14 +242,18 @@ __device__ WorkSplit split_work(const CacheView& c, const AttendParams& a, int t
     };
     // One round where a thread a group is enough; its count and place are kept for below.
     int total = 0, mine = 0, at = 0;
-    if (tid == 0) sums[33] = 0;
+    if (tid == 0) sums[33] = sums[34] = 0;
     for (int base = 0; base < groups; base += threads) {
         int sum, s;
         mine = tiles_of(base + tid, &s);
         at = total + block_scan(mine, sums, &sum);
         total += sum;
         s = __reduce_max_sync(0xffffffffu, s);
-        if ((tid & 31) == 0 && s > 0) atomicMax(sums + 33, s);
+        const int there = __popc(__ballot_sync(0xffffffffu, mine > 0));
+        if ((tid & 31) == 0 && s > 0) {
+            atomicMax(sums + 33, s);
+            atomicAdd(sums + 34, there * c.H);
+        }
     }
     __syncthreads();
     // A segment in more than 32 parts would cost more to join than its parts save: the longest one is 32
@@ -260,6 +264,10 @@ __device__ WorkSplit split_work(const CacheView& c, const AttendParams& a, int t
         if (ctas > cap) ctas = cap;
     }
     if (ctas > grid) ctas = grid;
+    // As many CTAs a segment as a whole number, if that makes a CTA's share longer by `spare` tiles at most:
+    // the shares then begin and end with segments of one length, and a second piece takes a CTA longer.
+    const int64_t segments = sums[34], fit = segments > 0 ? ctas / segments * segments : 0;
+    if (fit > 0 && total * (ctas - fit) <= spare * ctas * fit) ctas = fit;
     // CTAs with the same tiles for different row blocks take them at the same time, so that keys and
     // values come from memory once for all blocks (16 drafted trees, two blocks each: 1.07 GB read where the
     // second block followed the first, 0.55 GB so; 346 us and 326).

@@ -104,7 +104,7 @@ attend_mma_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant
     }
     // The plan was complete before the new tokens' copy began; only the pages have to be waited for.
     if (a.k == nullptr) grid_wait();
-    const WorkSplit work = split_work<S::kRows, (WR == 2)>(c, a, tile_units, 1, ctl.sums, &ctl.split, blockIdx.x, gridDim.x);
+    const WorkSplit work = split_work<S::kRows, (WR == 2)>(c, a, tile_units, 1, 0, ctl.sums, &ctl.split, blockIdx.x, gridDim.x);
     __syncthreads();
     grid_wait();
     grid_release();

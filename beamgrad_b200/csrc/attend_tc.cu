@@ -30,6 +30,9 @@ namespace {
 constexpr int kTileKeys = 128;
 constexpr int kMaxSlots = 12;
 constexpr int kMinTiles = 2;     // tiles of a CTA at least: a join costs about as much as two
+// A tile more for whole segments: a second piece costs a CTA more (2 x 3 beams' drafts of 18 over 1222: 34 us,
+// so 30; 4 beams' drafts of 21 over 211: 32 us, so 25). Two more are too many (32 beams over 4060: 75 us, 78).
+constexpr int kSpareTiles = 1;
 constexpr float kRaise = 8.0f;  // log2 of the growth that a reference tolerates
 
 struct Control {
@@ -243,7 +246,7 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
     // that is not complete, the others before they look whether a value was not finite.
     if (a.k == nullptr) grid_wait();
     grid_release();
-    const WorkSplit work = split_work<S::kRows, (NQ == 2)>(c, a, tile_units, kMinTiles, ctl.sums, &ctl.split, blockIdx.x, gridDim.x);
+    const WorkSplit work = split_work<S::kRows, (NQ == 2)>(c, a, tile_units, kMinTiles, kSpareTiles, ctl.sums, &ctl.split, blockIdx.x, gridDim.x);
     if (work.lo >= work.hi) {
         grid_wait();
         if (__ldcg(c.status + 1) != 0 && warp < kSoftThreads / 32)
@@ -863,7 +866,7 @@ attend_join_kernel(const __grid_constant__ CacheView c, const __grid_constant__ 
     __shared__ WorkSplit found;
     grid_release();
     const int cta = blockIdx.x / kJoinCtas, first = blockIdx.x % kJoinCtas * kJoin, tile_units = kTileKeys >> c.page_log2;
-    const WorkSplit work = split_work<kRows, (kRows > 128)>(c, a, tile_units, kMinTiles, sums, &found, cta, ctas);
+    const WorkSplit work = split_work<kRows, (kRows > 128)>(c, a, tile_units, kMinTiles, kSpareTiles, sums, &found, cta, ctas);
     Piece p{};
     bool divided = false;  // a segment begins among this CTA's tiles and ends past them
     if (work.lo < work.hi) {
