@@ -912,7 +912,7 @@ cudaError_t launch_width(const CacheView& c, const CUtensorMap& map, const Atten
     if (rows <= 64) return launch_shape<T, DP, 1, 2, false>(c, map, a, sm_count, stream);
     if (rows <= 128) return launch_shape<T, DP, 1, 1, false>(c, map, a, sm_count, stream);
     // Several blocks of several beams: a block passes over the tiles of which its beams hold nothing (17 beams
-    // of 62 tokens over 72: 92 us, so 75). Where every block has all beams that costs registers for nothing
+    // of 62 tokens over 72: 92 us, so 81). Where every block has all beams that costs registers for nothing
     // (16 drafted trees: 347 us, so 360).
     if (rows > 256 && beams > 1) return launch_shape<T, DP, 2, 1, true>(c, map, a, sm_count, stream);
     return launch_shape<T, DP, 2, 1, false>(c, map, a, sm_count, stream);
