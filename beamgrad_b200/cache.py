@@ -124,9 +124,19 @@ class PagedCache:
         c.pages, c.table, c.lengths = pages.data_ptr(), table.data_ptr(), lengths.data_ptr()
         c.references, c.plan, c.status = references.data_ptr(), self._plan.data_ptr(), self._status.data_ptr()
         self._ref = C.byref(c)
-        self._workspaces = {}  # stream -> zero-initialised workspace
+        # One workspace a cache (its calls are ordered), made here: made by the first call, it would be cleared
+        # by the CUDA graph that happens to capture that call, and by no other. Only its counters have to be zero.
+        self._workspaces = {self.device.index: self._new_workspace()}
         self._calls = {}       # shapes and layouts of attend's arguments -> _Call
         self._float = torch.empty(0, dtype=torch.float32, device=self.device)
+
+    def _new_workspace(self) -> torch.Tensor:
+        a = A.AttendArgs(beams=1, new_tokens=1, query_heads=self.num_kv_heads, scale=1.0)
+        with _on(self.device):
+            size = max(0, self.lib.dbs_cuda_cache_attend_workspace_size(self._ref, C.byref(a)))  # (refused: no attend)
+        workspace = torch.empty(size, dtype=torch.uint8, device=self.device)
+        workspace[: A.CACHE_WORKSPACE_ZEROED].zero_()
+        return workspace
 
     # -- state ----------------------------------------------------------------------------
     def reset(self) -> None:
@@ -261,9 +271,7 @@ class PagedCache:
         a.scale = call.scale if scale is None else scale
         with _on(self.device):
             stream = self._stream()
-            workspace = self._workspaces.get(stream)
-            if workspace is None or workspace.numel() < call.workspace:
-                workspace = self._workspaces[stream] = torch.zeros(call.workspace, dtype=torch.uint8, device=self.device)
+            workspace = self._workspaces[self.device.index]
             a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel()
             status = self.lib.dbs_cuda_cache_attend(self._ref, call.ref, stream)
         if status:
@@ -296,8 +304,7 @@ class PagedCache:
             a.k_strides[:] = k.stride()[:4]
             a.v_strides[:] = v.stride()[:4]
         a.beams, a.new_tokens, a.query_heads, a.scale = beams, N, heads, 1.0
-        call.workspace = self.lib.dbs_cuda_cache_attend_workspace_size(self._ref, call.ref)
-        if call.workspace < 0:
+        if self.lib.dbs_cuda_cache_attend_workspace_size(self._ref, call.ref) < 0:
             raise ValueError("the engine rejects these attention sizes")
         return call
 
@@ -339,7 +346,7 @@ def _ptr(x: torch.Tensor | None) -> int | None:
 class _Call:
     """What attend keeps of arguments of one shape and layout."""
 
-    __slots__ = ("args", "ref", "shape", "mask_shape", "scale", "copies", "workspace")
+    __slots__ = ("args", "ref", "shape", "mask_shape", "scale", "copies")
 
 
 class _Here:

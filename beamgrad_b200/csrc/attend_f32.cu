@@ -279,7 +279,7 @@ attend_f32_kernel(const __grid_constant__ CacheView c, const __grid_constant__ A
         }
         __syncthreads();
         const bool whole = p.t0 == 0 && p.t1 == p.tiles;
-        float* parts = static_cast<float*>(a.workspace) + 2048;
+        float* parts = static_cast<float*>(a.workspace) + DBS_CUDA_CACHE_WORKSPACE_ZEROED / 4;
         int32_t* counters = static_cast<int32_t*>(a.workspace);
         float* out_part = parts + static_cast<int64_t>(2 * blockIdx.x + (p.t0 == 0)) * S::kOut;
 #pragma unroll
@@ -367,8 +367,8 @@ cudaError_t launch_width(const CacheView& c, const AttendParams& a, int sm_count
 }  // namespace
 
 int64_t attend_f32_workspace(const CacheView&, const AttendParams&, int sm_count) {
-    // A counter for each CTA (8192 bytes), then two partial results for each.
-    return 8192 + static_cast<int64_t>(2) * sm_count * kMostOut * 4;
+    // A counter for each CTA first, then two partial results for each.
+    return DBS_CUDA_CACHE_WORKSPACE_ZEROED + static_cast<int64_t>(2) * sm_count * kMostOut * 4;
 }
 
 cudaError_t launch_attend_f32(const CacheView& c, const AttendParams& a, int sm_count, cudaStream_t stream) {

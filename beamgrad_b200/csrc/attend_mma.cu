@@ -381,7 +381,7 @@ attend_mma_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant
             reinterpret_cast<uint2*>(static_cast<T*>(a.out) + row * c.D)[vec] = packed;
             if (vec == 0 && a.lse != nullptr) a.lse[row] = live && l != 0.0f ? (m + log2f(l)) * kLn2 : -INFINITY;
         };
-        float* parts = static_cast<float*>(a.workspace) + 2048;
+        float* parts = static_cast<float*>(a.workspace) + DBS_CUDA_CACHE_WORKSPACE_ZEROED / 4;
         int32_t* counters = static_cast<int32_t*>(a.workspace);
         float* part = parts + static_cast<int64_t>(2 * blockIdx.x + (p.t0 == 0)) * S::kOut;
         for (int i = tid; i < rows * vecs; i += kComputeThreads) {
@@ -468,8 +468,8 @@ bool page_map(const CacheView& c, int dtype, CUtensorMap* map) {
 }
 
 int64_t attend_mma_workspace(const CacheView&, const AttendParams&, int sm_count) {
-    // A counter for each CTA (8192 bytes), then two partial results for each.
-    return 8192 + static_cast<int64_t>(2) * sm_count * Shape<2>::kOut * 4;
+    // A counter for each CTA first, then two partial results for each.
+    return DBS_CUDA_CACHE_WORKSPACE_ZEROED + static_cast<int64_t>(2) * sm_count * Shape<2>::kOut * 4;
 }
 
 cudaError_t launch_attend_mma(const CacheView& c, int dtype, const AttendParams& a, int sm_count, cudaStream_t stream) {

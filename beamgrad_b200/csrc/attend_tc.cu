@@ -686,7 +686,7 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
         // To the output, or to this CTA's part of a divided segment (of which four columns of all rows lie
         // together).
         const bool whole = p.t0 == 0 && p.t1 == p.tiles;
-        float* parts = static_cast<float*>(a.workspace) + 2048;
+        float* parts = static_cast<float*>(a.workspace) + DBS_CUDA_CACHE_WORKSPACE_ZEROED / 4;
         [[maybe_unused]] int32_t* counters = static_cast<int32_t*>(a.workspace);
         float* part = parts + static_cast<int64_t>(2 * blockIdx.x + (p.t0 == 0)) * S::kOut;
         float m = top == -INFINITY ? top : top * scale, l = sum;  // base-2 maximum, sum
@@ -885,7 +885,7 @@ attend_join_kernel(const __grid_constant__ CacheView c, const __grid_constant__ 
     const Span span{cta, cta_of(work, p.first + p.tiles - 1)};
     const int b = p.group / c.groups, beam0 = (p.group - b * c.groups) * kGroupBeams;
     join_parts<T, kRows, DP, kJoinThreads, kJoin, 2, 4>(c, a, p, span, b, beam0, row0, rows,
-                                                        static_cast<const float*>(a.workspace) + 2048, scratch, threadIdx.x, first);
+                                                        static_cast<const float*>(a.workspace) + DBS_CUDA_CACHE_WORKSPACE_ZEROED / 4, scratch, threadIdx.x, first);
 }
 
 template <class T, int DP, int NQ, int COPIES, bool SKIP>
@@ -927,8 +927,8 @@ cudaError_t launch_typed(const CacheView& c, const CUtensorMap& map, const Atten
 }  // namespace
 
 int64_t attend_tc_workspace(const CacheView&, const AttendParams&, int sm_count) {
-    // A counter for each CTA (8192 bytes), then two partial results for each.
-    return 8192 + static_cast<int64_t>(2) * sm_count * Shape<128, 2, 1>::kOut * 4;
+    // A counter for each CTA first, then two partial results for each.
+    return DBS_CUDA_CACHE_WORKSPACE_ZEROED + static_cast<int64_t>(2) * sm_count * Shape<128, 2, 1>::kOut * 4;
 }
 
 cudaError_t launch_attend_tc(const CacheView& c, int dtype, const AttendParams& a, int sm_count, cudaStream_t stream) {

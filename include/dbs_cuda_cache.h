@@ -20,6 +20,7 @@ extern "C" {
 #endif
 
 #define DBS_CUDA_CACHE_MAX_HEAD_DIM 256
+#define DBS_CUDA_CACHE_WORKSPACE_ZEROED 8192 /* bytes at the front of a workspace that the caller zeroes once */
 /* Bits of the status word. */
 #define DBS_CUDA_CACHE_STATUS_POOL 1     /* the pool ran out of pages: some columns have none */
 #define DBS_CUDA_CACHE_STATUS_CAPACITY 2 /* a beam was to grow past max_pages columns */
@@ -118,11 +119,13 @@ typedef struct DBSCudaAttendArgs {
     const int32_t* counts;
     void* out;
     float* lse;
-    void* workspace; /* dbs_cuda_cache_attend_workspace_size() bytes, 256-byte aligned, zeroed once */
+    void* workspace; /* dbs_cuda_cache_attend_workspace_size() bytes, 256-byte aligned; the first
+                        DBS_CUDA_CACHE_WORKSPACE_ZEROED of them (counters, 0 between calls) zeroed once */
     int64_t workspace_bytes;
 } DBSCudaAttendArgs;
 
-/* Workspace of an attend call of these sizes; negative when they are refused. */
+/* Workspace of an attend call of these sizes (of one cache: the same for all); negative when they
+ * are refused. One workspace serves all calls on a cache, which are ordered. */
 DBS_CUDA_EXPORT int64_t dbs_cuda_cache_attend_workspace_size(const DBSCudaCache* cache, const DBSCudaAttendArgs* args);
 
 DBS_CUDA_EXPORT int dbs_cuda_cache_attend(const DBSCudaCache* cache, const DBSCudaAttendArgs* args, void* stream);

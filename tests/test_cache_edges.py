@@ -1,0 +1,54 @@
+# SPDX-License-Identifier: MIT
+"""The paged beam cache at the edges of its contract: graphs, adopted state, refused paths, values and
+weights at the ends of their ranges. Models and bounds are those of test_cache.py."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from test_cache import random_cache, tensors
+
+
+# -- the workspace ----------------------------------------------------------------------
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype, dim", [(torch.bfloat16, 64), (torch.float32, 64), (torch.float16, 200)])
+def test_graphs_of_one_cache_replay_in_any_order(dtype, dim):
+    """Two graphs of one cache, the second replayed first, in memory that an earlier graph left full of
+    ones and zeros: what divided segments are joined by cannot come from either graph."""
+    cache = random_cache(1, 4, np.full((1, 4), 900), 1, layers=1, dim=dim, dtype=dtype, seed=6)
+    inputs = [tensors(cache, 1, 4, seed) for seed in (1, 2)]
+    want = [cache.attend(0, *x) for x in inputs]
+    pool = torch.cuda.graph_pool_handle()
+    graphs = [torch.cuda.CUDAGraph() for _ in range(3)]
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graphs[0], pool=pool):
+        used = torch.full((64 << 20,), 0x5A, dtype=torch.uint8, device="cuda")
+    graphs[0].replay()
+    torch.cuda.synchronize()
+    del used
+    got = []
+    for graph, x in zip(graphs[1:], inputs):
+        with torch.cuda.graph(graph, pool=pool):
+            got.append(cache.attend(0, *x))
+    for i in (1, 0, 1):
+        graphs[1 + i].replay()
+        assert torch.equal(got[i], want[i])
+
+
+@pytest.mark.gpu
+def test_a_cache_has_one_workspace_from_the_start():
+    cache = random_cache(1, 2, np.full((1, 2), 40), 1, layers=1)
+    x = tensors(cache, 1, 2, 0)
+    before = torch.cuda.memory_allocated()
+    want = cache.attend(0, *x)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = cache.attend(0, *x)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want)
+    assert torch.cuda.memory_allocated() - before < 1 << 20  # the outputs
