@@ -188,25 +188,27 @@ __device__ __forceinline__ float max3(float a, float b, float c) {  // NaN if on
     return d;
 }
 // 2^x of a pair on the multiply-add pipe, which has room while the special-function unit (16 a cycle
-// and SM) is what the weights of 128 x 128 scores wait for. x = n + f with n = floor(x): 2^f by a
-// polynomial of degree 5 (least relative error on [0, 1], 1.6e-7 as evaluated), n added to its
-// exponent. x is at most kRaise; at -126 and below the result is a denormal (the polynomial is just
-// below 1 at 0), which the sum takes as 0.
+// and SM) is what the weights of 128 x 128 scores wait for. x = n + f with n = floor(x) (Cody and Waite's
+// reduction): 2^f by a polynomial of degree 5 that is 1 at 0 (least relative error on [0, 1] of those,
+// 8.2e-8; 1.4e-7 as evaluated, and never below 1), n added to its exponent. x is at most kRaise. At -127
+// and below, and so for a masked score, the result is 0 in every bit: anything else, however small, would
+// round to a weight in bfloat16, whose least normal number times a value of 1e38 counts. Between -127 and
+// -126 it is a denormal, which the sum takes as 0.
 __device__ __forceinline__ void exp2_pair(Pair x2, float& a, float& b) {
     float x, y;
     unpair(x2, x, y);
-    x2 = pair_of(fmaxf(x, -126.0f), fmaxf(y, -126.0f));
+    x2 = pair_of(fmaxf(x, -127.0f), fmaxf(y, -127.0f));
     const Pair shift = pair_of(12582912.0f, 12582912.0f);  // 1.5 * 2^23: n in the low bits
     Pair t, n, f;
     asm("add.rm.f32x2 %0, %1, %2;" : "=l"(t) : "l"(x2), "l"(shift));
     asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(n) : "l"(t), "l"(shift));
     asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(f) : "l"(x2), "l"(n));
     auto both = [](float c) { return pair_of(c, c); };
-    Pair r = pair_fma(both(0.0018775766948238015f), f, both(0.00898933969438076f));
-    r = pair_fma(r, f, both(0.05582631751894951f));
-    r = pair_fma(r, f, both(0.24015361070632935f));
-    r = pair_fma(r, f, both(0.6931530833244324f));
-    r = pair_fma(r, f, both(0.9999999403953552f));
+    Pair r = pair_fma(both(0.0018671300495043397f), f, both(0.009017030708491802f));
+    r = pair_fma(r, f, both(0.05579991638660431f));
+    r = pair_fma(r, f, both(0.24016445875167847f));
+    r = pair_fma(r, f, both(0.6931512951850891f));
+    r = pair_fma(r, f, both(1.0f));
     float p, q, u, v;
     unpair(r, p, q);
     unpair(t, u, v);

@@ -8,7 +8,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_cache import random_cache, tensors
+from test_cache import DTYPES, check_attend, draft_tree, random_cache, tensors
 
 
 # -- the workspace ----------------------------------------------------------------------
@@ -52,3 +52,22 @@ def test_a_cache_has_one_workspace_from_the_start():
     torch.cuda.current_stream().wait_stream(side)
     assert torch.equal(got, want)
     assert torch.cuda.memory_allocated() - before < 1 << 20  # the outputs
+
+
+# -- weights at the ends of their range -------------------------------------------------
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("K, N, group, dim", [(1, 20, 1, 64), (1, 16, 4, 64), (1, 20, 4, 128), (1, 70, 2, 64), (3, 70, 2, 64), (1, 20, 2, 200)])
+def test_hidden_values_at_the_end_of_their_type(K, N, group, dim, dtype):
+    """A weight of zero is zero: a hidden value of the type's largest magnitude shows in no output. The
+    drafted tokens that nobody sees, and the rows of the pool that nobody holds, are such values."""
+    cache = random_cache(1, K, np.full((1, K), 150), N, layers=1, heads=1, dim=dim, dtype=dtype, seed=2)
+    big = torch.finfo(dtype).max
+    cache.pages[0, 1, cache.references == 0] = big
+    q, k, v = tensors(cache, N, group, 3)
+    v[:, :, 1::2] = big
+    mask = draft_tree(1, K, N, np.random.RandomState(1))
+    mask[..., 1::2] = False
+    check_attend(cache, 0, q, k, v, mask)
