@@ -35,7 +35,7 @@ _current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice
 _STATUS = (
     (A.CACHE_STATUS_POOL, "the pool ran out of pages"),
     (A.CACHE_STATUS_CAPACITY, "a beam outgrew the table (max_length)"),
-    (A.CACHE_STATUS_INDEX, "a parent, a count, a page or a path entry was out of range"),
+    (A.CACHE_STATUS_INDEX, "a parent, a count, a page, a length or a path entry was out of range"),
     (A.CACHE_STATUS_SHARED, "an incomplete page is shared by several beams"),
     (A.CACHE_STATUS_TIMEOUT, "a bounded wait inside a kernel gave up"),
 )
@@ -148,7 +148,9 @@ class PagedCache:
         self._recount(0)
 
     def refresh(self) -> None:
-        """Recounts the references and the plan after a caller wrote the state, and notes whether the pool's values hold infinities or NaN (reads all of them)."""
+        """Recounts the references and the plan after a caller wrote the state, and notes whether the
+        pool's values hold infinities or NaN (reads all of them). Pages and lengths out of range are
+        brought into it, which :meth:`check` reports."""
         self._recount(1)
 
     def _recount(self, values: int) -> None:

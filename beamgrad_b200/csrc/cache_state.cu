@@ -475,7 +475,18 @@ __global__ void __launch_bounds__(kCopyThreads) compact_move_kernel(CacheView c)
     }
 }
 
+// Table entries and lengths that are out of range never reach an index: the entries become -1, the lengths the
+// nearest one that the table has room for.
 __global__ void refresh_count_kernel(CacheView c) {
+    const int64_t slots = static_cast<int64_t>(c.B) * c.K;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < slots;
+         i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+        const int n = c.lengths[i], most = c.M << c.page_log2;
+        if (n < 0 || n > most) {
+            raise(c, DBS_CUDA_CACHE_STATUS_INDEX);
+            c.lengths[i] = n < 0 ? 0 : most;
+        }
+    }
     const int64_t entries = static_cast<int64_t>(c.B) * c.K * c.M;
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < entries;
          i += static_cast<int64_t>(gridDim.x) * blockDim.x) {

@@ -24,7 +24,7 @@ extern "C" {
 /* Bits of the status word. */
 #define DBS_CUDA_CACHE_STATUS_POOL 1     /* the pool ran out of pages: some columns have none */
 #define DBS_CUDA_CACHE_STATUS_CAPACITY 2 /* a beam was to grow past max_pages columns */
-#define DBS_CUDA_CACHE_STATUS_INDEX 4    /* a parent, count or path entry was out of range */
+#define DBS_CUDA_CACHE_STATUS_INDEX 4    /* a parent, count, path entry, table entry or length was out of range */
 #define DBS_CUDA_CACHE_STATUS_SHARED 8   /* a page that is not complete has several holders */
 #define DBS_CUDA_CACHE_STATUS_TIMEOUT 16 /* a bounded wait inside a kernel gave up */
 
@@ -65,7 +65,8 @@ typedef struct DBSCudaCache {
 /* Bytes of the plan array; negative when the sizes are refused. */
 DBS_CUDA_EXPORT int64_t dbs_cuda_cache_plan_bytes(const DBSCudaCache* cache);
 
-/* References and plan from table and lengths, after the caller wrote those. With values set,
+/* References and plan from table and lengths, after the caller wrote those. Entries out of range become
+ * -1 and lengths outside [0, max_pages * page_size] the nearer end, with the INDEX bit. With values set,
  * also status[1] from the values of the whole pool, after the caller wrote pages. */
 DBS_CUDA_EXPORT int dbs_cuda_cache_refresh(const DBSCudaCache* cache, int values, void* stream);
 

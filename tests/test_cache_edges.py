@@ -8,7 +8,8 @@ import numpy as np
 import pytest
 import torch
 
-from test_cache import DTYPES, check_attend, draft_tree, random_cache, tensors
+from beamgrad_b200.cache import PagedCache
+from test_cache import DTYPES, Model, check_attend, draft_tree, random_cache, tensors
 
 
 # -- the workspace ----------------------------------------------------------------------
@@ -71,3 +72,30 @@ def test_hidden_values_at_the_end_of_their_type(K, N, group, dim, dtype):
     mask = draft_tree(1, K, N, np.random.RandomState(1))
     mask[..., 1::2] = False
     check_attend(cache, 0, q, k, v, mask)
+
+
+# -- adopted state ----------------------------------------------------------------------
+
+
+def adopt(table, lengths, pages=12, page=16, dtype=torch.float32):
+    put = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    pool = torch.randn((2, 2, pages, 1, page, 64), device="cuda").to(dtype)
+    return PagedCache.from_tensors(pool, put(table), put(lengths))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_adopted_lengths_out_of_range(dtype):
+    """Lengths below 0 and above the table are brought into range and reported; nothing is read or written
+    outside the pages of the table."""
+    held = [[[0, 1, 2], [3, 4, 5]], [[6, 7, 8], [9, 10, 11]]]
+    for lengths in ([[-1, 20], [-(2**31), 5]], [[49, 20], [2**31 - 1, 48]], [[-17, 2**30], [7, -3]]):
+        cache = adopt(held, lengths, dtype=dtype)
+        with pytest.raises(RuntimeError, match="length"):
+            cache.check()
+        assert cache.lengths.cpu().tolist() == [[min(max(n, 0), 48) for n in row] for row in lengths]
+        Model(cache).check_plan(cache)
+        q, k, v = tensors(cache, 2, 2, 1)
+        check_attend(cache, 0, q, k, v)
+    cache = adopt(held, [[0, 48], [16, 47]], dtype=dtype)
+    cache.check()
