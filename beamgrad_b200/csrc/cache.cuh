@@ -43,7 +43,7 @@ struct CacheView {
     int32_t* unit_count;  // [B * groups]
     CacheUnit* units;     // [B * groups, unit_cap]
     int32_t* want_count;  // [S] pages a slot asks for
-    int32_t* want_first;  // [S] the first column it asks for
+    int32_t* want_first;  // [S] the first column it asks for, or -1 (cache_state.cu)
     int32_t* want_rank;   // [S] rank of its first new page
     int32_t* copy_from;   // [S] page whose rows the slot copies, or -1
     int32_t* copy_rows;   // [S]

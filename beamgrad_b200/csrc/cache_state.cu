@@ -95,7 +95,9 @@ __device__ void hand_out(const CacheView& c, int* sums) {
     }
 }
 
-// One CTA an example. Entries that ask for a new page become -2 until cache_finish_kernel.
+// One CTA an example. Entries that ask for a new page become -2 until cache_finish_kernel, which finds a slot's
+// new pages by the columns from the first such one on. Where pages that the slot keeps lie between them (a table
+// that a caller wrote), its first column is noted as -1 and the entries are -2 less their number.
 __global__ void __launch_bounds__(kMetaThreads) fork_meta_kernel(CacheView c, ForkArgs a) {
     extern __shared__ int32_t smem[];
     __shared__ int sums[33];
@@ -188,6 +190,20 @@ __global__ void __launch_bounds__(kMetaThreads) fork_meta_kernel(CacheView c, Fo
         }
         __syncthreads();
     }
+    for (int r = tid >> 5; r < K; r += kMetaThreads / 32) {
+        const int from = want_at[r], to = need[r], lane = tid & 31;
+        if (want[r] == 0 || want[r] == to - from) continue;
+        int32_t* row = table + static_cast<int64_t>(r) * M;
+        int before = 0;
+        for (int base = from; base < to; base += 32) {
+            const bool asks = base + lane < to && row[base + lane] == -2;
+            const unsigned all = __ballot_sync(0xffffffffu, asks);
+            if (asks) row[base + lane] = -2 - (before + __popc(all & ((1u << lane) - 1)));
+            before += __popc(all);
+        }
+        if (lane == 0) want_at[r] = -1;
+    }
+    __syncthreads();
     for (int s = tid; s < K; s += kMetaThreads) {
         const int p = src[s];
         c.lengths[slot0 + s] = p >= 0 ? length[p] : 0;
@@ -206,7 +222,7 @@ __global__ void __launch_bounds__(kMetaThreads) fork_meta_kernel(CacheView c, Fo
 }
 
 // The units of a group of beams, from its final table rows (column order, then first beam).
-// resolve: entries of -2 take their slot's new pages first. A warp takes a column at a time, a lane a
+// resolve: entries below -1 take their slot's new pages first. A warp takes a column at a time, a lane a
 // beam: the lanes with one page find each other in one instruction.
 constexpr int kPlanPitch = kCopyThreads + 1;  // of a beam's staged columns: a column's lie in different banks
 
@@ -218,7 +234,7 @@ __device__ void write_plan(const CacheView& c, int group, bool resolve, int* sum
     CacheUnit* units = c.units + static_cast<int64_t>(group) * c.unit_cap;
     int32_t* length = shared;                   // [32]
     int32_t* rank = shared + kGroupBeams;       // [32] rank of the first new page
-    int32_t* from = shared + 2 * kGroupBeams;   // [32] its column
+    int32_t* from = shared + 2 * kGroupBeams;   // [32] its column, or -1
     int32_t* place = shared + 3 * kGroupBeams;  // [columns] units of each, then the first one's number
     int32_t* stage = place + kCopyThreads;      // [n][kPlanPitch]
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -235,8 +251,8 @@ __device__ void write_plan(const CacheView& c, int group, bool resolve, int* sum
         for (int i = tid; i < n * cols; i += kCopyThreads) {
             const int k = i / cols, at = i - k * cols, col = base + at;
             int e = table[static_cast<int64_t>(k) * c.M + col];
-            if (resolve && e == -2) {
-                const int new_page = rank[k] + col - from[k];
+            if (resolve && e < -1) {
+                const int new_page = rank[k] + (from[k] < 0 ? -2 - e : col - from[k]);
                 e = new_page < handed ? c.free_list[new_page] : -1;
                 table[static_cast<int64_t>(k) * c.M + col] = e;
             }

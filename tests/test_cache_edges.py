@@ -99,3 +99,47 @@ def test_adopted_lengths_out_of_range(dtype):
         check_attend(cache, 0, q, k, v)
     cache = adopt(held, [[0, 48], [16, 47]], dtype=dtype)
     cache.check()
+
+
+HOLES = [  # table rows of one example, lengths, parents, room; pages of 16
+    ([[0, -1, 5, -1], [2, 3, -1, -1]], [3, 20], None, 61),           # a spare page behind a missing one
+    ([[0, -1, 5, -1, 7, -1], [1, -1, -1, 8, -1, 2]], [16, 0], None, 80),
+    ([[-1, 4, -1, 6], [-1, -1, 3, -1]], [20, 40], None, 30),          # committed positions without a page
+    ([[0, -1, 5, -1], [2, 3, -1, 9]], [9, 20], [1, 1], 40),           # the first child keeps them, the other copies
+    ([[0, -1, 5, -1], [2, 3, -1, 9]], [9, 20], [0, 0], 55),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", range(len(HOLES)))
+def test_adopted_tables_with_holes(case):
+    """Every missing column gets a page of its own, whatever pages lie between."""
+    rows, lengths, parents, room = HOLES[case]
+    cache = adopt([rows, [[-1] * len(rows[0])] * 2], [lengths, [0, 0]], pages=24)
+    model = Model(cache)
+    by = None if parents is None else np.array([parents, [0, 1]])
+    cache.fork(None if by is None else torch.from_numpy(by).cuda(), room=room)
+    model.fork(by, 0, room)
+    model.check(cache)
+    assert int(cache.references.max()) <= (1 if parents is None else 2)
+    cache.fork(written=1, room=room + 3)
+    model.fork(None, 1, room + 3)
+    model.check(cache)
+
+
+@pytest.mark.gpu
+def test_adopted_tables_with_holes_at_random():
+    for seed in range(12):
+        rng = np.random.RandomState(seed)
+        B, K, M, P = 3, int(rng.choice([2, 5, 33])), int(rng.choice([4, 40, 300])), 4000
+        K = min(K, P // (2 * B * M) or 1)
+        table = rng.permutation(P)[: B * K * M].reshape(B, K, M)
+        table[rng.rand(B, K, M) < 0.4] = -1
+        lengths = rng.randint(0, M * 16 // 2, (B, K))
+        cache = adopt(table.tolist(), lengths.tolist(), pages=P + B * K * M)
+        model = Model(cache)
+        parents = None if seed % 2 else rng.randint(0, K, (B, K))
+        room = M * 8 - int(rng.randint(0, 20))
+        cache.fork(None if parents is None else torch.from_numpy(parents).cuda(), room=room)
+        model.fork(parents, 0, room)
+        model.check(cache)
