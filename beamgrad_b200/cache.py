@@ -187,7 +187,9 @@ class PagedCache:
         """Accepts a path through the drafted tokens that the last :meth:`attend` calls wrote:
         tokens path[b, k, :counts[b, k]] (indices into the draft, increasing; [B, K, A] and [B, K]
         int32) become the beam's next committed tokens, the other drafted ones are dropped, and
-        there are pages for ``room`` more."""
+        there are pages for ``room`` more. Of a beam whose path does not increase, or names tokens
+        that there was no room for, nothing is accepted, and :meth:`check` raises; a beam without
+        tokens and pages stays empty."""
         if path.dim() != 3 or tuple(path.shape[:2]) != (self.batch_size, self.beam_size) or path.shape[2] < 1:
             raise ValueError(f"path must be [{self.batch_size}, {self.beam_size}, A], got {tuple(path.shape)}")
         p, n = self._int32(path, "path", None), self._int32(counts, "counts")

@@ -48,6 +48,7 @@ struct CacheView {
     int32_t* copy_from;   // [S] page whose rows the slot copies, or -1
     int32_t* copy_rows;   // [S]
     int4* copies;         // [S] {from, to, rows, slot} of the slots that copy
+    int32_t* accepted;    // [S] tokens that a commit accepts
     int32_t* free_list;   // [P] fork: free pages; compact: holes
     int32_t* move_list;   // [P] compact: pages that move, in order of their holes
     int32_t* move_to;     // [P] compact: where a page at or above the live count goes
@@ -73,7 +74,7 @@ inline int64_t cache_plan_layout(CacheView& v, void* base) {
     v.words = static_cast<int32_t*>(take(kWords * 4));
     v.unit_count = static_cast<int32_t*>(take(static_cast<int64_t>(v.B) * v.groups * 4));
     v.units = static_cast<CacheUnit*>(take(static_cast<int64_t>(v.B) * v.groups * v.unit_cap * sizeof(CacheUnit)));
-    int32_t** per_slot[] = {&v.want_count, &v.want_first, &v.want_rank, &v.copy_from, &v.copy_rows};
+    int32_t** per_slot[] = {&v.want_count, &v.want_first, &v.want_rank, &v.copy_from, &v.copy_rows, &v.accepted};
     for (int32_t** p : per_slot) *p = static_cast<int32_t*>(take(S * 4));
     v.copies = static_cast<int4*>(take(S * 16));
     int32_t** per_page[] = {&v.free_list, &v.move_list, &v.move_to};

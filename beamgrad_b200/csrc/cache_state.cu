@@ -336,10 +336,11 @@ __global__ void __launch_bounds__(kCopyThreads) cache_finish_kernel(CacheView c,
 }
 
 // Rows of an accepted path to the front of the drafted area. A CTA takes one slot and a part of its
-// layers, kinds and heads; it looks the rows' places up once. A thread owns 16 bytes of every row of
-// one layer, kind and head, and moves eight rows a round: row path[a] >= a lies at or behind every row
-// that earlier rounds wrote, and a round reads all its rows before it writes.
-constexpr int kMoveRows = 256;  // accepted rows whose places are looked up at a time
+// layers, kinds and heads. The whole path is looked at before a row moves: one that does not rise, or names a
+// token without a page, is refused as a whole (0 accepted, for the fork behind this). A thread owns 16 bytes
+// of every row of one layer, kind and head, and moves eight rows a round: row path[a] >= a lies at or behind
+// every row that earlier rounds wrote, and a round reads all its rows before it writes.
+constexpr int kMoveRows = kCopyThreads;  // accepted rows whose places are looked up at a time
 
 __global__ void __launch_bounds__(kCopyThreads) commit_move_kernel(CacheView c, const int32_t* path, int path_stride,
                                                                    const int32_t* counts, int parts) {
@@ -353,34 +354,37 @@ __global__ void __launch_bounds__(kCopyThreads) commit_move_kernel(CacheView c, 
     const int n = c.lengths[slot];
     const int32_t* row = c.table + static_cast<int64_t>(slot) * c.M;
     const int32_t* steps = path + static_cast<int64_t>(slot) * path_stride;
-    if (tid == 0) {
-        bad = 0;
-        if (count > path_stride && piece == 0) raise(c, DBS_CUDA_CACHE_STATUS_INDEX);
+    const bool empty = n <= 0 && row[0] < 0;  // no tokens, no pages: nothing of this beam was drafted
+    if (tid == 0) bad = !empty && (count < 0 || count > path_stride);
+    if (empty || count > path_stride) count = 0;
+    __syncthreads();
+    // The move of entry a; (all threads with a bad one store 1).
+    auto look = [&](int a) {
+        const int from = steps[a], before = a > 0 ? steps[a - 1] : -1;
+        const int64_t at = static_cast<int64_t>(n) + from, to = static_cast<int64_t>(n) + a;
+        int p = -1, q = -1;
+        if (from > before && from >= a && (at >> c.page_log2) < c.M) p = row[at >> c.page_log2], q = row[to >> c.page_log2];
+        if (p < 0 || q < 0) bad = 1;
+        if (p < 0 || q < 0 || from == a) return make_int2(-1, -1);
+        return make_int2(p * c.H * c.page + static_cast<int>(at & (c.page - 1)), q * c.H * c.page + static_cast<int>(to & (c.page - 1)));
+    };
+    for (int a = tid; a < count; a += kMoveRows) {
+        const int2 m = look(a);
+        if (a < kMoveRows) moves[a] = m;
     }
-    if (count > path_stride) count = path_stride;
+    __syncthreads();
+    const bool refused = bad != 0;
+    if (tid == 0 && piece == 0) {
+        c.accepted[slot] = refused ? 0 : count;
+        if (refused) raise(c, DBS_CUDA_CACHE_STATUS_INDEX);
+    }
+    if (refused) return;
     const int items = c.L * 2 * c.H * row_vecs;
     for (int base = 0; base < count; base += kMoveRows) {
-        __syncthreads();
-        const int a = base + tid;
-        if (a < count) {
-            const int from = steps[a];
-            const bool rises = from > (a > 0 ? steps[a - 1] : -1);
-            if (!rises) bad = 1;  // (all such threads store 1)
-            int2 m = make_int2(-1, -1);
-            const int64_t at = static_cast<int64_t>(n) + from, to = static_cast<int64_t>(n) + a;
-            if (rises && from != a && (at >> c.page_log2) < c.M && (to >> c.page_log2) < c.M) {
-                const int p = row[at >> c.page_log2], q = row[to >> c.page_log2];
-                if (p >= 0 && q >= 0) {
-                    m.x = p * c.H * c.page + static_cast<int>(at & (c.page - 1));
-                    m.y = q * c.H * c.page + static_cast<int>(to & (c.page - 1));
-                }
-            }
-            moves[tid] = m;
-        }
-        __syncthreads();
-        if (bad) {  // not increasing: the rows are left as they are
-            if (tid == 0 && piece == 0) raise(c, DBS_CUDA_CACHE_STATUS_INDEX);
-            return;
+        if (base > 0) {
+            __syncthreads();
+            if (base + tid < count) moves[tid] = look(base + tid);
+            __syncthreads();
         }
         const int rows = count - base < kMoveRows ? count - base : kMoveRows;
         for (int i = piece * kCopyThreads + tid; i < items; i += parts * kCopyThreads) {
@@ -578,7 +582,7 @@ cudaError_t launch_cache_commit(const CacheView& c, const int32_t* path, int pat
     const cudaError_t e = launch_after(commit_move_kernel, static_cast<unsigned>(slots * parts), kCopyThreads, 0, stream, c,
                                        path, path_stride, counts, static_cast<int>(parts));
     if (e != cudaSuccess) return e;
-    return launch_cache_fork(c, nullptr, counts, 0, nullptr, room_all, sm_count, stream);
+    return launch_cache_fork(c, nullptr, c.accepted, 0, nullptr, room_all, sm_count, stream);
 }
 
 cudaError_t launch_cache_compact(const CacheView& c, int sm_count, cudaStream_t stream) {

@@ -84,7 +84,9 @@ DBS_CUDA_EXPORT int dbs_cuda_cache_fork(const DBSCudaCache* cache, const int32_t
 /* Accepts a path of the drafted tokens: row lengths + path[b, k, a] moves to row
  * lengths + a for a < counts[b, k], in every layer (path [B, K, path_stride] int32,
  * strictly increasing within the count); then dbs_cuda_cache_fork with no parents,
- * written = counts and room_all. */
+ * written = counts and room_all. Of a beam whose count is not in [0, path_stride], whose path
+ * does not rise or names a token without a page nothing is accepted or moved (the INDEX bit);
+ * a beam without tokens and pages stays empty, whatever its count. */
 DBS_CUDA_EXPORT int dbs_cuda_cache_commit(const DBSCudaCache* cache, const int32_t* path, int32_t path_stride,
                                           const int32_t* counts, int32_t room_all, void* stream);
 

@@ -143,3 +143,51 @@ def test_adopted_tables_with_holes_at_random():
         cache.fork(None if parents is None else torch.from_numpy(parents).cuda(), room=room)
         model.fork(parents, 0, room)
         model.check(cache)
+
+
+# -- paths that are refused -------------------------------------------------------------
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["falls late", "repeats", "below zero", "count above the width", "negative count", "no page", "no column"])
+def test_a_refused_path_leaves_its_beam_alone(kind):
+    cache = PagedCache(1, 4, 640, num_layers=2, num_kv_heads=1, head_dim=8, page_size=16, dtype=torch.float32)
+    cache.pages.normal_()
+    cache.fork(room=40)
+    cache.fork(torch.tensor([[0, 1, 2, -1]], device="cuda"), written=37, room=400)  # the last beam is empty
+    model = Model(cache)
+    path = np.tile(np.arange(300) + 2, (1, 4, 1))
+    counts = np.array([[3, 5, 300, 4]])
+    path[0, 0, 1:] += 1
+    good = counts.copy()
+    good[0, 1], good[0, 3] = 0, 0
+    if kind == "falls late":
+        path[0, 1, 280], counts[0, 1] = path[0, 1, 279] - 1, 300
+    elif kind == "repeats":
+        path[0, 1, 3] = path[0, 1, 2]
+    elif kind == "below zero":
+        path[0, 1, 0] = -1
+    elif kind == "count above the width":
+        counts[0, 1] = 301
+    elif kind == "negative count":
+        counts[0, 1] = -2
+    elif kind == "no page":
+        path[0, 1, 4] = 450
+    else:
+        path[0, 1, 4] = 2**31 - 1
+    dev = lambda x: torch.from_numpy(x.astype(np.int32)).cuda()  # noqa: E731
+    cache.commit(dev(path), dev(counts), room=7)
+    model.commit(path, good, 7)
+    # The empty beam has no tokens and gets room like the others.
+    model.check(cache)
+    with pytest.raises(RuntimeError, match="path entry"):
+        cache.check()
+
+
+@pytest.mark.gpu
+def test_an_empty_beam_accepts_nothing_without_an_error():
+    cache = PagedCache(1, 2, 64, num_layers=1, num_kv_heads=1, head_dim=8, page_size=16, dtype=torch.float32)
+    cache.fork(torch.tensor([[0, -1]], device="cuda"), room=6)
+    cache.commit(torch.tensor([[[0, 2], [0, 1]]], device="cuda"), torch.tensor([[2, 2]], device="cuda"))
+    assert cache.lengths.cpu().tolist() == [[2, 0]]
+    cache.check()
