@@ -13,7 +13,9 @@
 // the end of a segment.
 //
 // Scores are taken in base 2: scale * log2(e) is applied to the 32-bit product. Weights are
-// rounded to the input type for the second product, as the values are; their sum is taken before.
+// rounded to the input type for the second product, as the values are; their sum is taken before. In float16
+// they are 2^15 at the most instead of 1 (kLift), since below 2^-14 its steps are no longer relative; the
+// statistics carry that.
 #include "attend.cuh"
 
 namespace dbsb {
@@ -26,6 +28,7 @@ constexpr int kComputeWarps = 8;
 constexpr int kComputeThreads = kComputeWarps * 32;
 constexpr int kThreads = kComputeThreads + 128;  // and the producer's warpgroup, of which one warp works
 constexpr int kMaxStages = 8;
+template <class T> constexpr float kLift = std::is_same_v<T, __half> ? 15.0f : 0.0f;  // log2 of the largest weight
 
 template <int WR>
 struct Shape {
@@ -283,11 +286,12 @@ attend_mma_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant
                         }
                     }
                     top[e] = now;
+                    const float low = ref - kLift<T>;
                     float w[4];
 #pragma unroll
                     for (int n = 0; n < 2; ++n)
 #pragma unroll
-                        for (int x = 0; x < 2; ++x) w[2 * n + x] = exp2_fast(s[n][2 * e + x] - ref);
+                        for (int x = 0; x < 2; ++x) w[2 * n + x] = exp2_fast(s[n][2 * e + x] - low);
                     sum[e] = sum[e] * keep + ((w[0] + w[1]) + (w[2] + w[3]));
                     weights[e] = Pack<T>::pair(w[0], w[1]);
                     weights[2 + e] = Pack<T>::pair(w[2], w[3]);
@@ -328,7 +332,7 @@ attend_mma_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant
             const float ref = m == -INFINITY ? 0.0f : m;
             float l = 0.0f;
             for (int i = 0; i < kSet; ++i) l += ctl.sum[from + i][r] * exp2_fast(ctl.top[from + i][r] - ref);
-            ctl.row_top[tid] = m;
+            ctl.row_top[tid] = m;  // (without kLift, as the warps' own)
             ctl.row_sum[tid] = l;
         }
         named_sync(1, kComputeThreads);
@@ -394,7 +398,7 @@ attend_mma_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant
                                                                   ((vec * 4) ^ ((in_set & 7) << 3)));
                 o.x += x.x, o.y += x.y, o.z += x.z, o.w += x.w;
             }
-            const float m = ctl.row_top[r], l = ctl.row_sum[r];
+            const float m = ctl.row_top[r] - kLift<T>, l = ctl.row_sum[r];
             if (whole) {
                 put(r, vec, o, m, l);
             } else {

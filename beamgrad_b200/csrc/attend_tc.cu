@@ -19,7 +19,7 @@
 //
 // A row's reference for the exponentials is raised only when its maximum has grown by more than
 // 2^8: until then the weights stay below 2^8 and the sums within 32 bits, and O in tensor memory
-// is left alone. Weights are rounded to the input type, as the values are; their sum is taken
+// is left alone (in float16 all of them are 2^7 higher: kLift). Weights are rounded to the input type, as the values are; their sum is taken
 // before. All statistics are 32 bits.
 #include "attend.cuh"
 
@@ -34,6 +34,10 @@ constexpr int kMinTiles = 2;     // tiles of a CTA at least: a join costs about 
 // so 30; 4 beams' drafts of 21 over 211: 32 us, so 25). Two more are too many (32 beams over 4060: 75 us, 78).
 constexpr int kSpareTiles = 1;
 constexpr float kRaise = 8.0f;  // log2 of the growth that a reference tolerates
+// log2 of what all weights of a row are multiplied by. In float16 a weight below 2^-14 is a denormal with steps
+// of 2^-24: 2^7 on top of the 2^8 that a reference tolerates uses the range up to 2^15. The statistics say so
+// (a reference lower by as much), and the division at the end takes it out.
+template <class T> constexpr float kLift = std::is_same_v<T, __half> ? 7.0f : 0.0f;
 
 struct Control {
     uint64_t full[kMaxSlots], empty[kMaxSlots];
@@ -190,7 +194,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {  // NaN if on
 // 2^x of a pair on the multiply-add pipe, which has room while the special-function unit (16 a cycle
 // and SM) is what the weights of 128 x 128 scores wait for. x = n + f with n = floor(x) (Cody and Waite's
 // reduction): 2^f by a polynomial of degree 5 that is 1 at 0 (least relative error on [0, 1] of those,
-// 8.2e-8; 1.4e-7 as evaluated, and never below 1), n added to its exponent. x is at most kRaise. At -127
+// 8.2e-8; 1.4e-7 as evaluated, and never below 1), n added to its exponent. x is at most kRaise + kLift. At -127
 // and below, and so for a masked score, the result is 0 in every bit: anything else, however small, would
 // round to a weight in bfloat16, whose least normal number times a value of 1e38 counts. Between -127 and
 // -126 it is a denormal, which the sum takes as 0.
@@ -605,7 +609,8 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
                 }
                 // Nothing seen yet: any reference gives weights of 0. A maximum that is inf or NaN gives NaN.
                 const float ref = top == -INFINITY ? 0.0f : (top < INFINITY ? top * scale : NAN);
-                const Pair scale2 = pair_of(scale, scale), ref2 = pair_of(-ref, -ref);
+                const float lift = kLift<T> - ref;
+                const Pair scale2 = pair_of(scale, scale), ref2 = pair_of(lift, lift);
                 Pair part[2] = {pair_of(0.0f, 0.0f), pair_of(0.0f, 0.0f)};
 #pragma unroll
                 for (int i = 0; i < kChunks; ++i) {
@@ -691,7 +696,7 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
         float* parts = static_cast<float*>(a.workspace) + DBS_CUDA_CACHE_WORKSPACE_ZEROED / 4;
         [[maybe_unused]] int32_t* counters = static_cast<int32_t*>(a.workspace);
         float* part = parts + static_cast<int64_t>(2 * blockIdx.x + (p.t0 == 0)) * S::kOut;
-        float m = top == -INFINITY ? top : top * scale, l = sum;  // base-2 maximum, sum
+        float m = top == -INFINITY ? top : top * scale - kLift<T>, l = sum;  // base-2 reference, sum
         const bool holds_rows = (my_row & ~31) < rows && (NQ == 1 || began);  // of the warp
         if constexpr (kHalves == 2) {
             named_sync(1, kSoftThreads);  // (query_at shares the space)

@@ -74,6 +74,50 @@ def test_hidden_values_at_the_end_of_their_type(K, N, group, dim, dtype):
     check_attend(cache, 0, q, k, v, mask)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 200])
+@pytest.mark.parametrize("N", [1, 40, 100, 200])
+def test_small_weights_in_float16(N, dim):
+    """1744 keys of weight 2^-25.5 beside 256 of weight 1 whose values are 0: all of the output comes from
+    weights that float16 holds as 0 or as one step, where the largest is 1. With the largest at 2^7 a step of
+    2^-24 rounds them by 2^-25 at the most, 2^-32 of the largest: a share of 2^-6.5 of each. The sums and the
+    exponentials add 2^-19, the output's rounding 2^-11."""
+    B, H, T, low = 20, 8, 2000, -25.5
+    cache = random_cache(B, 1, np.full((B, 1), T), N, layers=1, heads=H, dim=dim, page=16, dtype=torch.float16, seed=1)
+    cache.pages.zero_()
+    others = cache.table[:, 0, 16 : T // 16].long().reshape(-1)
+    cache.pages[0, 0, others, :, :, 0] = low
+    cache.pages[0, 1, others] = 32768.0
+    cache.refresh()
+    q = torch.zeros((B, 1, N, H, dim), device="cuda", dtype=torch.float16)
+    k, v = q.clone(), q.clone()
+    q[..., 0], k[..., 0] = 1, -200  # the new tokens weigh nothing
+    out, lse = cache.attend(0, q, k, v, scale=float(np.log(2.0)), return_lse=True)
+    want = 32768 * (T - 256) * 2.0**low / 256
+    assert float((out.double() / want - 1).abs().max()) <= 2.0**-6.5 + 2.0**-11 + 2.0**-19
+    assert float((lse.double() - np.log(256 + (T - 256) * 2.0**low)).abs().max()) <= 2.0**-19 + 2.0**-21 * 6
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("N, dim", [(1, 64), (40, 64), (100, 128), (200, 64), (1, 200), (40, 200)])
+def test_scores_that_rise_within_a_row(N, dim, dtype):
+    """Every row's maximum rises from tile to tile, by less and by more than the references tolerate, with
+    values near the end of float16: weights and sums stay within their types."""
+    T = 1500
+    cache = random_cache(2, 1, np.full((2, 1), T), N, layers=1, heads=2, dim=dim, page=16, dtype=dtype, seed=3)
+    place = torch.arange(T, device="cuda")
+    pages = cache.table[:, 0].long()[:, place // 16], place % 16
+    q, k, v = tensors(cache, N, 1, 9)
+    for rise in (0.05, 0.2):  # of a score in base 2, a position
+        cache.pages[0, 0, pages[0], :, pages[1], 0] = (place * rise).to(dtype)[None, :, None]
+        cache.pages[0, 1].mul_(30000 / cache.pages[0, 1].abs().max())
+        cache.refresh()
+        for x in (q, k, v):
+            x[..., 0] = 1
+        check_attend(cache, 0, q, k, v, scale=float(np.log(2.0)))
+
+
 # -- adopted state ----------------------------------------------------------------------
 
 
