@@ -250,6 +250,7 @@ class AttendArgs(C.Structure):
 
 CACHE_STATUS_POOL, CACHE_STATUS_CAPACITY, CACHE_STATUS_INDEX = 1, 2, 4
 CACHE_STATUS_SHARED, CACHE_STATUS_TIMEOUT = 8, 16
+CACHE_VALUES_ALL, CACHE_VALUES_IF_SET = 1, 2
 CACHE_WORKSPACE_ZEROED = 8192  # DBS_CUDA_CACHE_WORKSPACE_ZEROED
 
 MAX_POOL = 1024  # DBS_CUDA_B200_MAX_POOL

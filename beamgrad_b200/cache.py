@@ -140,18 +140,19 @@ class PagedCache:
 
     # -- state ----------------------------------------------------------------------------
     def reset(self) -> None:
-        """An empty cache: no tokens, no pages. Device-side fills only."""
+        """An empty cache: no tokens, no pages, no errors, and no values in the pool that are not finite.
+        On the device alone, without a host synchronisation."""
         self.table.fill_(-1)
         self.lengths.zero_()
         self.references.zero_()
         self._status[:1].zero_()
-        self._recount(0)
+        self._recount(A.CACHE_VALUES_IF_SET)
 
     def refresh(self) -> None:
         """Recounts the references and the plan after a caller wrote the state, and notes whether the
-        pool's values hold infinities or NaN (reads all of them). Pages and lengths out of range are
-        brought into it, which :meth:`check` reports."""
-        self._recount(1)
+        pool's values hold infinities or NaN (reads all of them; those in pages that no beam holds
+        become 0). Pages and lengths out of range are brought into it, which :meth:`check` reports."""
+        self._recount(A.CACHE_VALUES_ALL)
 
     def _recount(self, values: int) -> None:
         with _on(self.device):
@@ -208,6 +209,13 @@ class PagedCache:
         bits = int(self._status[0])
         if bits:
             raise RuntimeError("paged cache: " + "; ".join(text for bit, text in _STATUS if bits & bit))
+
+    @property
+    def has_nonfinite(self) -> bool:
+        """Whether a value that is not finite was written since the last :meth:`reset` or
+        :meth:`refresh` (a host sync). While it is so, :meth:`attend` takes every row for itself, right
+        but many times slower; when the beams with such values are gone, :meth:`refresh` ends that."""
+        return bool(self._status[1])
 
     # -- attention ------------------------------------------------------------------------
     def attend(self, layer: int, q: torch.Tensor, k: torch.Tensor | None = None, v: torch.Tensor | None = None, *,

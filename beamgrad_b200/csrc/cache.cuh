@@ -60,6 +60,7 @@ constexpr int kWordCopies = 1;   // entries of copies
 constexpr int kWordFree = 2;     // entries of free_list that were handed out
 constexpr int kWordLive = 3;     // compact: pages in use
 constexpr int kWordMoves = 4;    // compact: entries of move_list
+constexpr int kWordOdd = 5;     // refresh: a page that is held has a value that is not finite
 constexpr int kWords = 64;
 
 inline int64_t cache_plan_layout(CacheView& v, void* base) {
@@ -154,7 +155,7 @@ cudaError_t launch_cache_fork(const CacheView& c, const int32_t* parents, const 
 cudaError_t launch_cache_commit(const CacheView& c, const int32_t* path, int path_stride, const int32_t* counts,
                                 int room_all, int sm_count, cudaStream_t stream);
 cudaError_t launch_cache_compact(const CacheView& c, int sm_count, cudaStream_t stream);
-cudaError_t launch_cache_refresh(const CacheView& c, int dtype, bool values, int sm_count, cudaStream_t stream);
+cudaError_t launch_cache_refresh(const CacheView& c, int dtype, int values, int sm_count, cudaStream_t stream);
 int64_t attend_workspace(const CacheView& c, const AttendParams& a, int sm_count);
 cudaError_t launch_attend(const CacheView& c, int dtype, const AttendParams& a, int sm_count, cudaStream_t stream);
 

@@ -122,9 +122,9 @@ DBS_CUDA_EXPORT int64_t dbs_cuda_cache_plan_bytes(const DBSCudaCache* cache) {
 
 DBS_CUDA_EXPORT int dbs_cuda_cache_refresh(const DBSCudaCache* cache, int values, void* stream_ptr) {
     CacheView v;
-    if (!open(cache, v)) return DBS_CUDA_STATUS_INVALID_ARGUMENT;
+    if (!open(cache, v) || values < 0 || values > DBS_CUDA_CACHE_VALUES_IF_SET) return DBS_CUDA_STATUS_INVALID_ARGUMENT;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
-    return finish(launch_cache_refresh(v, cache->data_type, values != 0, sm_count(), stream), stream);
+    return finish(launch_cache_refresh(v, cache->data_type, values, sm_count(), stream), stream);
 }
 
 DBS_CUDA_EXPORT int dbs_cuda_cache_fork(const DBSCudaCache* cache, const int32_t* parents, const int32_t* written,

@@ -526,20 +526,34 @@ __global__ void __launch_bounds__(kCopyThreads) refresh_plan_kernel(CacheView c)
     write_plan(c, blockIdx.x, false, sums, smem);
 }
 
-// Whether the values of the pool hold one that is not finite (exponent bits all set).
-__global__ void refresh_values_kernel(CacheView c, uint32_t exponent_lo, uint32_t exponent_hi) {
-    const int64_t vecs = static_cast<int64_t>(c.P) * c.H * c.page * c.D * c.elem / 16;  // of a layer and kind
+// Whether the values of the pool hold one that is not finite (exponent bits all set). In pages that nobody
+// holds such values mean nothing and become 0: the pages may be handed out again. if_set: only where
+// status[1] says that there may be some.
+__global__ void refresh_values_kernel(CacheView c, uint32_t exponent_lo, uint32_t exponent_hi, bool if_set) {
+    if (if_set && c.status[1] == 0) return;
+    const int64_t each = static_cast<int64_t>(c.H) * c.page * c.D * c.elem / 16, vecs = c.P * each;  // of a page; of a layer and kind
     bool odd = false;
     for (int layer = 0; layer < c.L; ++layer) {
-        const uint4* x = static_cast<const uint4*>(c.pages) + (2 * layer + 1) * vecs;
+        uint4* x = static_cast<uint4*>(c.pages) + (2 * layer + 1) * vecs;
         for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < vecs;
              i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
             const uint4 v = x[i];
-            for (uint32_t w : {v.x, v.y, v.z, v.w})
-                odd |= (w & exponent_lo) == exponent_lo || (w & exponent_hi) == exponent_hi;
+            uint32_t w[4] = {v.x, v.y, v.z, v.w};
+            bool here = false;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const bool lo = (w[j] & exponent_lo) == exponent_lo, hi = (w[j] & exponent_hi) == exponent_hi;
+                here |= lo || hi;
+                if (exponent_lo == exponent_hi ? lo : lo && hi) w[j] = 0;  // float32: one element
+                else if (lo) w[j] &= 0xffff0000u;
+                else if (hi) w[j] &= 0x0000ffffu;
+            }
+            if (!here) continue;
+            if (c.references[i / each] == 0) x[i] = make_uint4(w[0], w[1], w[2], w[3]);
+            else odd = true;
         }
     }
-    if (odd) c.status[1] = 1;
+    if (odd) c.words[kWordOdd] = 1;
 }
 
 size_t meta_smem(const CacheView& c) {
@@ -592,18 +606,20 @@ cudaError_t launch_cache_compact(const CacheView& c, int sm_count, cudaStream_t 
     return launch_after(compact_move_kernel, copy_blocks(most, sm_count), kCopyThreads, 0, stream, c);
 }
 
-cudaError_t launch_cache_refresh(const CacheView& c, int dtype, bool values, int sm_count, cudaStream_t stream) {
+cudaError_t launch_cache_refresh(const CacheView& c, int dtype, int values, int sm_count, cudaStream_t stream) {
     cudaError_t e = cudaMemsetAsync(c.references, 0, static_cast<size_t>(c.P) * 4, stream);
     if (e != cudaSuccess) return e;
     const int64_t entries = static_cast<int64_t>(c.B) * c.K * c.M;
     refresh_count_kernel<<<copy_blocks((entries + 255) / 256, sm_count), 256, 0, stream>>>(c);
     refresh_plan_kernel<<<c.B * c.groups, kCopyThreads, plan_smem(), stream>>>(c);
-    if (values) {
-        e = cudaMemsetAsync(c.status + 1, 0, 4, stream);
+    if (values != 0) {
+        e = cudaMemsetAsync(c.words + kWordOdd, 0, 4, stream);
         if (e != cudaSuccess) return e;
         const uint32_t exponent = dtype == DBS_CUDA_DTYPE_F16 ? 0x7c00u : 0x7f80u;
         const uint32_t lo = dtype == DBS_CUDA_DTYPE_F32 ? exponent << 16 : exponent;
-        refresh_values_kernel<<<sm_count * 8, 256, 0, stream>>>(c, lo, exponent << 16);
+        refresh_values_kernel<<<sm_count * 8, 256, 0, stream>>>(c, lo, exponent << 16, values == DBS_CUDA_CACHE_VALUES_IF_SET);
+        e = cudaMemcpyAsync(c.status + 1, c.words + kWordOdd, 4, cudaMemcpyDeviceToDevice, stream);
+        if (e != cudaSuccess) return e;
     }
     return cudaGetLastError();
 }

@@ -28,6 +28,10 @@ extern "C" {
 #define DBS_CUDA_CACHE_STATUS_SHARED 8   /* a page that is not complete has several holders */
 #define DBS_CUDA_CACHE_STATUS_TIMEOUT 16 /* a bounded wait inside a kernel gave up */
 
+/* What dbs_cuda_cache_refresh does about the pool's values. */
+#define DBS_CUDA_CACHE_VALUES_ALL 1
+#define DBS_CUDA_CACHE_VALUES_IF_SET 2
+
 /* The cache of one search: batch_size examples of beam_size beams. A beam's
  * token at position p lies in row p % page_size of page table[b, k, p / page_size],
  * for every layer and head. The caller owns all arrays:
@@ -38,7 +42,8 @@ extern "C" {
  *   references  [num_pages] int32: table entries that name the page
  *   plan        dbs_cuda_cache_plan_bytes() bytes, 256-byte aligned, zeroed once
  *   status      2 int32, zeroed once: the bits above (sticky); 1 once a value that
- *               is not finite was written
+ *               is not finite was written, until dbs_cuda_cache_refresh finds none:
+ *               attention then takes every row for itself, right but many times slower
  * A page at or behind a beam's last incomplete page belongs to that beam alone;
  * complete pages may be shared. page_size is 16, 32 or 64, head_dim a multiple of
  * 8 up to 256. */
@@ -66,8 +71,10 @@ typedef struct DBSCudaCache {
 DBS_CUDA_EXPORT int64_t dbs_cuda_cache_plan_bytes(const DBSCudaCache* cache);
 
 /* References and plan from table and lengths, after the caller wrote those. Entries out of range become
- * -1 and lengths outside [0, max_pages * page_size] the nearer end, with the INDEX bit. With values set,
- * also status[1] from the values of the whole pool, after the caller wrote pages. */
+ * -1 and lengths outside [0, max_pages * page_size] the nearer end, with the INDEX bit. values: 0, or
+ * DBS_CUDA_CACHE_VALUES_ALL: also status[1] from the values of the whole pool, after the caller wrote
+ * pages (values that are not finite in pages without a holder become 0, in others they set it), or
+ * DBS_CUDA_CACHE_VALUES_IF_SET: the same where status[1] is set, nothing where it is not. */
 DBS_CUDA_EXPORT int dbs_cuda_cache_refresh(const DBSCudaCache* cache, int values, void* stream);
 
 /* One step of the beams. First written_s tokens after each beam's committed ones become

@@ -9,7 +9,7 @@ import pytest
 import torch
 
 from beamgrad_b200.cache import PagedCache
-from test_cache import DTYPES, Model, check_attend, draft_tree, random_cache, tensors
+from test_cache import DTYPES, Model, attend_exact, check_attend, draft_tree, random_cache, tensors
 
 
 # -- the workspace ----------------------------------------------------------------------
@@ -116,6 +116,55 @@ def test_scores_that_rise_within_a_row(N, dim, dtype):
         for x in (q, k, v):
             x[..., 0] = 1
         check_attend(cache, 0, q, k, v, scale=float(np.log(2.0)))
+
+
+# -- values that are not finite ---------------------------------------------------------
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_cache_recovers_from_values_that_are_not_finite(dtype):
+    """They are forgotten with the beam that held them (refresh) and with everything else (reset); the rest of
+    the pool is left as it was."""
+    B, K, N, G = 1, 3, 2, 4
+    cache = random_cache(B, K, np.full((B, K), 60), N, layers=2, heads=1, dtype=dtype, seed=8)
+    q, k, v = tensors(cache, N, G, 2)
+    assert not cache.has_nonfinite
+    bad = v.clone()
+    bad[0, 1, 0, 0, :8] = torch.tensor([np.inf, 1, -np.inf, np.nan, 2, 3, np.nan, np.nan])
+    cache.attend(1, q, k, bad)
+    assert cache.has_nonfinite
+    cache.refresh()
+    assert cache.has_nonfinite  # beam 1 holds them
+    cache.fork(torch.tensor([[0, 0, 2]], device="cuda"), room=N)
+    assert cache.has_nonfinite
+    before = cache.pages.clone()
+    cache.refresh()
+    assert not cache.has_nonfinite
+    assert torch.equal(cache.pages, torch.where(torch.isfinite(before), before, 0))
+    check_attend(cache, 1, q, k, v)
+    cache.attend(1, q, k, bad)
+    before = cache.pages.clone()
+    assert cache.has_nonfinite
+    cache.reset()
+    assert not cache.has_nonfinite and cache.lengths.sum() == 0
+    assert torch.equal(cache.pages, torch.where(torch.isfinite(before), before, 0))
+    cache.check()
+    cache.reserve(N)
+    check_attend(cache, 1, q, k, v)
+    # A pool that was never written may hold anything where nobody looks.
+    pages = torch.full((1, 2, 6, 1, 16, 64), float("nan"), device="cuda").to(dtype)
+    pages[:, :, 2] = 1
+    adopted = PagedCache.from_tensors(pages, torch.tensor([[[2, -1]]], dtype=torch.int32, device="cuda"),
+                                      torch.tensor([[16]], dtype=torch.int32, device="cuda"))
+    assert not adopted.has_nonfinite
+    q, k, v = tensors(adopted, 1, 1, 3)
+    adopted.reserve(1)
+    before = adopted.pages[0].cpu()  # (check_attend compares the pages too, whose keys are still NaN)
+    out, lse = adopted.attend(0, q, k, v, return_lse=True)
+    want, z, bound, z_bound = attend_exact(before, adopted.table.cpu(), adopted.lengths.cpu(), q.cpu(), k.cpu(), v.cpu(), None, None, 0.125)
+    assert bool(((out.cpu().double() - want).abs().amax(-1) <= bound).all())
+    assert bool(((lse.cpu().double() - z).abs() <= z_bound).all())
 
 
 # -- adopted state ----------------------------------------------------------------------
