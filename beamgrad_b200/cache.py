@@ -32,6 +32,7 @@ _DTYPES = {torch.float32: A.DTYPE_F32, torch.float16: A.DTYPE_F16, torch.bfloat1
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 _current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+_MOST_CALLS = 256  # shapes and layouts that a cache remembers
 _STATUS = (
     (A.CACHE_STATUS_POOL, "the pool ran out of pages"),
     (A.CACHE_STATUS_CAPACITY, "a beam outgrew the table (max_length)"),
@@ -248,7 +249,10 @@ class PagedCache:
             v.shape, v.stride(), v.dtype, v.device)
         call = self._calls.get(key)
         if call is None:
-            call = self._calls[key] = self._check_shapes(q, k, v)
+            call = self._check_shapes(q, k, v)
+            if len(self._calls) >= _MOST_CALLS:  # prompts of many lengths: begin again
+                self._calls.clear()
+            self._calls[key] = call
         if not 0 <= layer < self.num_layers:
             raise ValueError(f"layer {layer} is not one of {self.num_layers}")
         a, shape = call.args, call.shape

@@ -4,10 +4,15 @@ weights at the ends of their ranges. Models and bounds are those of test_cache.p
 
 from __future__ import annotations
 
+import ctypes as C
+import math
+
 import numpy as np
 import pytest
 import torch
 
+from beamgrad_b200 import _abi as A
+from beamgrad_b200 import cache as cache_module
 from beamgrad_b200.cache import PagedCache
 from test_cache import DTYPES, Model, attend_exact, check_attend, draft_tree, random_cache, tensors
 
@@ -284,3 +289,46 @@ def test_an_empty_beam_accepts_nothing_without_an_error():
     cache.commit(torch.tensor([[[0, 2], [0, 1]]], device="cuda"), torch.tensor([[2, 2]], device="cuda"))
     assert cache.lengths.cpu().tolist() == [[2, 0]]
     cache.check()
+
+
+# -- the host side ----------------------------------------------------------------------
+
+
+class _Library:
+    """The engine's library with its launches of attend handed to the test."""
+
+    def __init__(self, launch):
+        self.real, self.launch = A.load(), launch
+
+    def __getattr__(self, name):
+        return getattr(self.real, name)
+
+    def dbs_cuda_cache_attend(self, cache, args, stream):
+        self.launch(args._obj)
+        return 0
+
+
+def host_cache(monkeypatch, launch=lambda args: None, **sizes) -> PagedCache:
+    """A cache of host memory: everything that attend does before a launch, without a device."""
+    monkeypatch.setattr(cache_module, "_on", lambda device: cache_module._HERE)
+    monkeypatch.setattr(cache_module, "_raw_stream", lambda index: 0)
+    z = lambda *shape: torch.zeros(shape, dtype=torch.int32)  # noqa: E731
+    cache = PagedCache.__new__(PagedCache)
+    pages = torch.zeros((1, 2, 8, 1, 16, 64), dtype=torch.float16)
+    cache._describe(tuple(pages.shape), (1, 2, 4), pages.dtype)
+    cache._adopt(pages, z(1, 2, 4), z(1, 2), z(8))
+    cache.lib = _Library(launch)
+    return cache
+
+
+def host_inputs(N, heads=1, shape=(1, 2)):
+    return [torch.zeros((*shape, N, heads, 64), dtype=torch.float16) for _ in range(3)]
+
+
+def test_what_attend_remembers_is_bounded(monkeypatch):
+    seen = []
+    cache = host_cache(monkeypatch, lambda a: seen.append(a.new_tokens))
+    for N in range(1, 1001):
+        cache.attend(0, *host_inputs(N))
+        assert len(cache._calls) <= 256
+    assert seen == list(range(1, 1001))
