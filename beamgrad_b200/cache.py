@@ -16,7 +16,8 @@ pool instead:
 
 All of it runs on the device without a host synchronisation, so a decode loop can be captured in a
 CUDA graph. Errors that only the device sees (the pool ran out of pages, a parent out of range) are
-sticky bits that :meth:`PagedCache.check` raises. There is no CPU path and no backward pass.
+sticky bits that :meth:`PagedCache.check` raises. There is no CPU path and no derivative: inputs that ask
+for one, backward or forward, are refused.
 """
 
 from __future__ import annotations
@@ -25,6 +26,7 @@ import ctypes as C
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from beamgrad_b200 import _abi as A
 
@@ -243,6 +245,8 @@ class PagedCache:
             raise ValueError("k and v are given together or not at all")
         if torch.is_grad_enabled() and (q.requires_grad or k is not None and (k.requires_grad or v.requires_grad)):
             raise RuntimeError("attend has no backward pass: call it under torch.no_grad()")
+        if forward_ad._current_level >= 0 and any(x is not None and forward_ad.unpack_dual(x).tangent is not None for x in (q, k, v)):
+            raise RuntimeError("attend has no forward-mode derivative: call it on the primals")
         # Arguments of one shape and layout are checked and written down once.
         key = (q.shape, q.stride(), q.dtype, q.device, mask is None) if k is None else (
             q.shape, q.stride(), q.dtype, q.device, mask is None, k.shape, k.stride(), k.dtype, k.device,

@@ -10,6 +10,7 @@ import math
 import numpy as np
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from beamgrad_b200 import _abi as A
 from beamgrad_b200 import cache as cache_module
@@ -332,3 +333,18 @@ def test_what_attend_remembers_is_bounded(monkeypatch):
         cache.attend(0, *host_inputs(N))
         assert len(cache._calls) <= 256
     assert seen == list(range(1, 1001))
+
+
+def test_tangents_are_refused(monkeypatch):
+    seen = []
+    cache = host_cache(monkeypatch, seen.append)
+    inputs = host_inputs(2)
+    with forward_ad.dual_level(), torch.no_grad():
+        for i in range(3):
+            dual = [forward_ad.make_dual(x, torch.ones_like(x)) if i == j else x for j, x in enumerate(inputs)]
+            with pytest.raises(RuntimeError, match="derivative"):
+                cache.attend(0, *dual)
+        assert not seen
+        cache.attend(0, *inputs)
+        cache.attend(0, inputs[0])
+    assert len(seen) == 2
