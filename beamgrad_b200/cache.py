@@ -24,6 +24,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import threading
 
 import torch
 from torch.autograd import forward_ad
@@ -130,7 +131,8 @@ class PagedCache:
         # One workspace a cache (its calls are ordered), made here: made by the first call, it would be cleared
         # by the CUDA graph that happens to capture that call, and by no other. Only its counters have to be zero.
         self._workspaces = {self.device.index: self._new_workspace()}
-        self._calls = {}       # shapes and layouts of attend's arguments -> _Call
+        self._calls = {}  # shapes and layouts of attend's arguments -> _Call
+        self._lock = threading.Lock()
         self._float = torch.empty(0, dtype=torch.float32, device=self.device)
 
     def _new_workspace(self) -> torch.Tensor:
@@ -259,6 +261,13 @@ class PagedCache:
             self._calls[key] = call
         if not 0 <= layer < self.num_layers:
             raise ValueError(f"layer {layer} is not one of {self.num_layers}")
+        with self._lock:  # the structure of arguments is the shape's, not the call's
+            out, lse, status = self._launch_attend(call, layer, q, k, v, mask, counts, scale, return_lse, out)
+        if status:
+            A.check(status, "cache_attend")
+        return (out, lse) if return_lse else out
+
+    def _launch_attend(self, call, layer, q, k, v, mask, counts, scale, return_lse, out):
         a, shape = call.args, call.shape
         if call.copies or (q.data_ptr() | (0 if k is None else k.data_ptr() | v.data_ptr())) % 16:
             q, k, v = self._rows(q), None if k is None else self._rows(k), None if v is None else self._rows(v)
@@ -282,6 +291,7 @@ class PagedCache:
         elif out.shape != shape or out.dtype != self.dtype or out.device != self.device or not out.is_contiguous():
             raise ValueError(f"out must be a contiguous {self.dtype} {tuple(shape)} tensor on {self.device}")
         a.out = out.data_ptr()
+        lse = None
         if return_lse:
             lse = self._float.new_empty(shape[:4])
             a.lse = lse.data_ptr()
@@ -294,9 +304,7 @@ class PagedCache:
             workspace = self._workspaces[self.device.index]
             a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel()
             status = self.lib.dbs_cuda_cache_attend(self._ref, call.ref, stream)
-        if status:
-            A.check(status, "cache_attend")
-        return (out, lse) if return_lse else out
+        return out, lse, status
 
     def _check_shapes(self, q, k, v) -> "_Call":
         if q.dim() != 5:

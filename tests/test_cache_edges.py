@@ -6,6 +6,8 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import threading
+import time
 
 import numpy as np
 import pytest
@@ -348,3 +350,29 @@ def test_tangents_are_refused(monkeypatch):
         cache.attend(0, *inputs)
         cache.attend(0, inputs[0])
     assert len(seen) == 2
+
+
+def test_two_threads_do_not_mix_their_arguments(monkeypatch):
+    wrong, calls = [], []
+
+    def launch(a):
+        at = a.q, a.k, a.v, a.out, a.lse
+        time.sleep(0.002)  # another thread may run
+        wrong.extend(x for x in zip(at, (a.q, a.k, a.v, a.out, a.lse)) if x[0] != x[1])
+        calls.append(at[:4])
+
+    cache = host_cache(monkeypatch, launch)
+    args = [host_inputs(2) for _ in range(2)]
+    outs = [torch.zeros_like(x[0]) for x in args]
+
+    def work(i):
+        for _ in range(20):
+            cache.attend(0, *args[i], out=outs[i], return_lse=True)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong and len(calls) == 40
+    assert set(calls) == {(*(x.data_ptr() for x in args[i]), outs[i].data_ptr()) for i in range(2)}
