@@ -35,6 +35,7 @@ _DTYPES = {torch.float32: A.DTYPE_F32, torch.float16: A.DTYPE_F16, torch.bfloat1
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 _current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+_INT_MAX = (1 << 31) - 1
 _MOST_CALLS = 256  # shapes and layouts that a cache remembers
 _STATUS = (
     (A.CACHE_STATUS_POOL, "the pool ran out of pages"),
@@ -355,14 +356,16 @@ class PagedCache:
             shape = self.lengths.shape
         if x.device != self.device or x.dtype not in (torch.int32, torch.int64) or shape and x.shape != shape:
             raise ValueError(f"{name} must be an integer {tuple(shape or ())} tensor on {self.device}")
-        return x if x.dtype == torch.int32 and x.is_contiguous() else x.to(torch.int32).contiguous()
+        if x.dtype == torch.int64:  # what 32 bits do not hold stays out of range
+            x = x.clamp(-1, _INT_MAX).to(torch.int32)
+        return x.contiguous()
 
     def _per_beam(self, x: int | torch.Tensor, name: str) -> tuple:
         return (self._int32(x, name), 0) if isinstance(x, torch.Tensor) else (None, _number(x, name))
 
 
 def _number(x: int, name: str) -> int:
-    if not 0 <= x < 1 << 31:
+    if not 0 <= x <= _INT_MAX:
         raise ValueError(f"{name} must not be negative, got {x}")
     return int(x)
 

@@ -376,3 +376,28 @@ def test_two_threads_do_not_mix_their_arguments(monkeypatch):
         t.join()
     assert not wrong and len(calls) == 40
     assert set(calls) == {(*(x.data_ptr() for x in args[i]), outs[i].data_ptr()) for i in range(2)}
+
+
+def test_indexes_that_32_bits_do_not_hold(monkeypatch):
+    cache = host_cache(monkeypatch)
+    x = torch.tensor([[2**32, 2**31 + 1]])
+    assert cache._int32(x, "parents").tolist() == [[2**31 - 1] * 2]
+    assert cache._int32(-x, "parents").tolist() == [[-1, -1]]
+    x = torch.tensor([[3, -1]])
+    assert cache._int32(x, "parents").tolist() == [[3, -1]] and cache._int32(x, "parents").dtype == torch.int32
+    y = x.int()
+    assert cache._int32(y, "parents") is y
+
+
+@pytest.mark.gpu
+def test_parents_that_32_bits_do_not_hold_are_out_of_range():
+    cache = PagedCache(1, 2, 64, num_layers=1, num_kv_heads=1, head_dim=8, page_size=16, dtype=torch.float32)
+    cache.fork(torch.tensor([[0, 2**32]], device="cuda"))
+    with pytest.raises(RuntimeError, match="out of range"):
+        cache.check()
+    cache.reset()
+    cache.reserve(4)
+    cache.commit(torch.tensor([[[0], [2**32]]], device="cuda"), torch.tensor([[1, 1]], device="cuda"))
+    with pytest.raises(RuntimeError, match="out of range"):
+        cache.check()
+    assert cache.lengths.cpu().tolist() == [[1, 0]]
