@@ -131,6 +131,7 @@ DBS_CUDA_EXPORT int dbs_cuda_cache_fork(const DBSCudaCache* cache, const int32_t
                                         int32_t written_all, const int32_t* room, int32_t room_all, void* stream_ptr) {
     CacheView v;
     if (!open(cache, v) || written_all < 0 || room_all < 0) return DBS_CUDA_STATUS_INVALID_ARGUMENT;
+    if (!aligned(parents, 4) || !aligned(written, 4) || !aligned(room, 4)) return DBS_CUDA_STATUS_INVALID_ARGUMENT;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
     return finish(launch_cache_fork(v, parents, written, written_all, room, room_all, sm_count(), stream), stream);
 }
@@ -139,6 +140,7 @@ DBS_CUDA_EXPORT int dbs_cuda_cache_commit(const DBSCudaCache* cache, const int32
                                           const int32_t* counts, int32_t room_all, void* stream_ptr) {
     CacheView v;
     if (!open(cache, v) || !path || path_stride < 1 || !counts || room_all < 0) return DBS_CUDA_STATUS_INVALID_ARGUMENT;
+    if (!aligned(path, 4) || !aligned(counts, 4)) return DBS_CUDA_STATUS_INVALID_ARGUMENT;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
     return finish(launch_cache_commit(v, path, path_stride, counts, room_all, sm_count(), stream), stream);
 }
@@ -165,6 +167,7 @@ DBS_CUDA_EXPORT int dbs_cuda_cache_attend(const DBSCudaCache* cache, const DBSCu
     const DBSCudaAttendArgs& a = *args;
     if (!a.q || !aligned(a.q, 16) || !a.out || !aligned(a.out, 16)) return DBS_CUDA_STATUS_INVALID_ARGUMENT;
     if ((a.k == nullptr) != (a.v == nullptr) || !aligned(a.k, 16) || !aligned(a.v, 16)) return DBS_CUDA_STATUS_INVALID_ARGUMENT;
+    if (!aligned(a.counts, 4) || !aligned(a.lse, 4)) return DBS_CUDA_STATUS_INVALID_ARGUMENT;
     const int step = 16 / v.elem;  // rows of q, k and v are read 16 bytes at a time
     for (int i = 0; i < 4; ++i) {
         p.qs[i] = a.q_strides[i], p.ks[i] = a.k_strides[i], p.vs[i] = a.v_strides[i];

@@ -401,3 +401,23 @@ def test_parents_that_32_bits_do_not_hold_are_out_of_range():
     with pytest.raises(RuntimeError, match="out of range"):
         cache.check()
     assert cache.lengths.cpu().tolist() == [[1, 0]]
+
+
+def test_misaligned_arrays_are_refused_before_a_launch():
+    """Checked where a launch could not follow: no device here, and on one every call below is refused."""
+    lib, base = A.load(), 1 << 20  # addresses that nothing reads
+    c = A.Cache(batch_size=1, beam_size=2, max_pages=4, num_pages=8, num_layers=1, num_heads=1, head_dim=64, page_size=16,
+                data_type=A.DTYPE_F16, pages=base, table=base, lengths=base, references=base, plan=base, status=base)
+    c.plan_bytes = lib.dbs_cuda_cache_plan_bytes(C.byref(c))
+    ref = C.byref(c)
+    for off in (1, 2, 3):
+        for at in range(3):
+            x = [base + off if i == at else base for i in range(3)]
+            assert lib.dbs_cuda_cache_fork(ref, x[0], x[1], 0, x[2], 0, None) == A.STATUS_INVALID_ARGUMENT
+        for x in ((base + off, base), (base, base + off)):
+            assert lib.dbs_cuda_cache_commit(ref, x[0], 2, x[1], 0, None) == A.STATUS_INVALID_ARGUMENT
+        for name in ("lse", "counts"):
+            a = A.AttendArgs(beams=2, new_tokens=1, query_heads=1, scale=1.0, q=base, out=base, workspace=base)
+            a.workspace_bytes = lib.dbs_cuda_cache_attend_workspace_size(ref, C.byref(a))
+            setattr(a, name, base + off)
+            assert lib.dbs_cuda_cache_attend(ref, C.byref(a), None) == A.STATUS_INVALID_ARGUMENT
