@@ -24,6 +24,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import operator
 import threading
 
 import torch
@@ -365,9 +366,10 @@ class PagedCache:
 
 
 def _number(x: int, name: str) -> int:
+    x = operator.index(x)  # 1.5 tokens are a TypeError
     if not 0 <= x <= _INT_MAX:
         raise ValueError(f"{name} must not be negative, got {x}")
-    return int(x)
+    return x
 
 
 def _ptr(x: torch.Tensor | None) -> int | None:

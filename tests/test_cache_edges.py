@@ -421,3 +421,12 @@ def test_misaligned_arrays_are_refused_before_a_launch():
             a.workspace_bytes = lib.dbs_cuda_cache_attend_workspace_size(ref, C.byref(a))
             setattr(a, name, base + off)
             assert lib.dbs_cuda_cache_attend(ref, C.byref(a), None) == A.STATUS_INVALID_ARGUMENT
+
+
+def test_numbers_of_tokens_are_whole(monkeypatch):
+    cache = host_cache(monkeypatch)
+    for call in (lambda: cache.fork(written=0.5), lambda: cache.fork(room=1.5), lambda: cache.reserve(0.9),
+                 lambda: cache.commit(torch.zeros((1, 2, 1), dtype=torch.int32), torch.zeros((1, 2), dtype=torch.int32), room=0.5)):
+        with pytest.raises(TypeError):
+            call()
+    assert cache_module._number(np.int64(3), "room") == 3
