@@ -109,6 +109,8 @@ class PagedCache:
         return self
 
     def _describe(self, pages: tuple, table: tuple, dtype: torch.dtype) -> None:
+        if max(*pages, *table) > _INT_MAX:  # (the structure's fields would wrap)
+            raise ValueError("sizes must fit into 31 bits")
         self.lib = A.load()
         c = self._cache = A.Cache()
         c.num_layers, _, c.num_pages, c.num_heads, c.page_size, c.head_dim = pages

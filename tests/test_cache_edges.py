@@ -430,3 +430,11 @@ def test_numbers_of_tokens_are_whole(monkeypatch):
         with pytest.raises(TypeError):
             call()
     assert cache_module._number(np.int64(3), "room") == 3
+
+
+def test_sizes_that_32_bits_do_not_hold():
+    sizes = dict(num_layers=1, num_kv_heads=1, head_dim=64, num_pages=4, page_size=16, device="cuda:0")
+    for args, change in (((1, 1, (2**32 + 2) * 16), {}), ((2**32 + 1, 1, 64), {}), ((1, 1, 64), dict(num_pages=2**32 + 4)),
+                         ((1, 1, 64), dict(head_dim=2**32 + 64))):
+        with pytest.raises(ValueError):
+            PagedCache(*args, **(sizes | change))
