@@ -60,6 +60,13 @@ cudaError_t launch_append(const CacheView& c, const AttendParams& a, int sm_coun
 
 }  // namespace
 
+bool attend_counts_tiles(const CacheView& c, const AttendParams& a) {
+    const BlockShape shape = c.elem == 4 ? attend_f32_shape(c, a) : (c.D <= 128 ? attend_tc_shape(c, a) : attend_mma_shape(c, a));
+    const int tile_units = shape.keys > c.page ? shape.keys / c.page : 1;
+    const int64_t blocks = (group_rows(a) + shape.rows - 1) / shape.rows, tiles = (c.unit_cap + tile_units - 1) / tile_units;
+    return static_cast<double>(tiles) * blocks * c.H * c.B * c.groups < INT_MAX;
+}
+
 int64_t attend_workspace(const CacheView& c, const AttendParams& a, int sm_count) {
     if (c.elem == 4) return attend_f32_workspace(c, a, sm_count);
     return c.D <= 128 ? attend_tc_workspace(c, a, sm_count) : attend_mma_workspace(c, a, sm_count);

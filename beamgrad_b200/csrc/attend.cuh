@@ -626,6 +626,18 @@ cudaError_t allow_shared(Kernel* kernel, int bytes, std::atomic<uint64_t>& ready
 // that eight rows of 128 bytes cover all banks. False: the driver refused it.
 bool page_map(const CacheView& c, int dtype, CUtensorMap* map);
 
+// Query rows of a block and positions of a tile, of the kernel that a call takes.
+struct BlockShape {
+    int rows, keys;
+};
+// Query rows of a group of beams at the most.
+inline int64_t group_rows(const AttendParams& a) {
+    return static_cast<int64_t>(a.beams < kGroupBeams ? a.beams : kGroupBeams) * a.N * a.G;
+}
+BlockShape attend_f32_shape(const CacheView& c, const AttendParams& a);
+BlockShape attend_tc_shape(const CacheView& c, const AttendParams& a);
+BlockShape attend_mma_shape(const CacheView& c, const AttendParams& a);
+
 int64_t attend_f32_workspace(const CacheView& c, const AttendParams& a, int sm_count);
 cudaError_t launch_attend_f32(const CacheView& c, const AttendParams& a, int sm_count, cudaStream_t stream);
 int64_t attend_tc_workspace(const CacheView& c, const AttendParams& a, int sm_count);

@@ -352,19 +352,24 @@ cudaError_t launch_shape(const CacheView& c, const AttendParams& a, int sm_count
     return launch_after(kernel, sm_count, S::kThreads, S::kBytes, stream, c, a);
 }
 
-// Rows of a block: as many as a group has, up to 64 (32 for heads above 128, which leave no room for
-// more). Rows past the group's cost multiply-adds with zeros.
 template <int DP>
 cudaError_t launch_width(const CacheView& c, const AttendParams& a, int sm_count, cudaStream_t stream) {
-    const int beams = a.beams < kGroupBeams ? a.beams : kGroupBeams;
-    const int64_t rows = static_cast<int64_t>(beams) * a.N * a.G;
-    if (rows <= 16) return launch_shape<DP, 16>(c, a, sm_count, stream);
+    const int rows = attend_f32_shape(c, a).rows;
+    if (rows == 16) return launch_shape<DP, 16>(c, a, sm_count, stream);
     if constexpr (DP <= 128)
-        if (rows > 32) return launch_shape<DP, 64>(c, a, sm_count, stream);
+        if (rows == 64) return launch_shape<DP, 64>(c, a, sm_count, stream);
     return launch_shape<DP, 32>(c, a, sm_count, stream);
 }
 
 }  // namespace
+
+// As many rows as a group has, up to 64 (32 for heads above 128, which leave no room for more). Rows past the
+// group's cost multiply-adds with zeros.
+BlockShape attend_f32_shape(const CacheView& c, const AttendParams& a) {
+    const int64_t rows = group_rows(a);
+    if (c.D > 128) return {rows <= 16 ? 16 : 32, Shape<256, 32>::kKeys};
+    return {rows <= 16 ? 16 : (rows <= 32 ? 32 : 64), Shape<128, 64>::kKeys};
+}
 
 int64_t attend_f32_workspace(const CacheView&, const AttendParams&, int sm_count) {
     // A counter for each CTA first, then two partial results for each.

@@ -437,18 +437,17 @@ cudaError_t launch_shape(const CacheView& c, const CUtensorMap& map, const Atten
     return launch_after(kernel, sm_count, kThreads, S::kBytes, stream, map, c, a);
 }
 
-// Rows of a block: 16, or 32 where a group has more. Fewer rows than that cost products with zeros, not
-// bytes.
 template <class T>
 cudaError_t launch_typed(const CacheView& c, const CUtensorMap& map, const AttendParams& a, int sm_count,
                          cudaStream_t stream) {
-    const int beams = a.beams < kGroupBeams ? a.beams : kGroupBeams;
-    const int64_t rows = static_cast<int64_t>(beams) * a.N * a.G;
-    if (rows <= 16) return launch_shape<T, 1>(c, map, a, sm_count, stream);
+    if (attend_mma_shape(c, a).rows == 16) return launch_shape<T, 1>(c, map, a, sm_count, stream);
     return launch_shape<T, 2>(c, map, a, sm_count, stream);
 }
 
 }  // namespace
+
+// 16 rows, or 32 where a group has more. Fewer rows than that cost products with zeros, not bytes.
+BlockShape attend_mma_shape(const CacheView&, const AttendParams& a) { return {group_rows(a) <= 16 ? 16 : 32, kTileKeys}; }
 
 bool page_map(const CacheView& c, int dtype, CUtensorMap* map) {
     using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,

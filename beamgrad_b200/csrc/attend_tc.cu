@@ -913,15 +913,14 @@ cudaError_t launch_shape(const CacheView& c, const CUtensorMap& map, const Atten
 template <class T, int DP>
 cudaError_t launch_width(const CacheView& c, const CUtensorMap& map, const AttendParams& a, int sm_count,
                          cudaStream_t stream) {
-    const int beams = a.beams < kGroupBeams ? a.beams : kGroupBeams;
-    const int64_t rows = static_cast<int64_t>(beams) * a.N * a.G;
-    if (rows <= 32) return launch_shape<T, DP, 1, 4, false>(c, map, a, sm_count, stream);
-    if (rows <= 64) return launch_shape<T, DP, 1, 2, false>(c, map, a, sm_count, stream);
-    if (rows <= 128) return launch_shape<T, DP, 1, 1, false>(c, map, a, sm_count, stream);
+    const int rows = attend_tc_shape(c, a).rows;
+    if (rows == 32) return launch_shape<T, DP, 1, 4, false>(c, map, a, sm_count, stream);
+    if (rows == 64) return launch_shape<T, DP, 1, 2, false>(c, map, a, sm_count, stream);
+    if (rows == 128) return launch_shape<T, DP, 1, 1, false>(c, map, a, sm_count, stream);
     // Several blocks of several beams: a block passes over the tiles of which its beams hold nothing (17 beams
     // of 62 tokens over 72: 92 us, so 81). Where every block has all beams that costs registers for nothing
     // (16 drafted trees: 347 us, so 360).
-    if (rows > 256 && beams > 1) return launch_shape<T, DP, 2, 1, true>(c, map, a, sm_count, stream);
+    if (group_rows(a) > 256 && a.beams > 1) return launch_shape<T, DP, 2, 1, true>(c, map, a, sm_count, stream);
     return launch_shape<T, DP, 2, 1, false>(c, map, a, sm_count, stream);
 }
 
@@ -932,6 +931,11 @@ cudaError_t launch_typed(const CacheView& c, const CUtensorMap& map, const Atten
 }
 
 }  // namespace
+
+BlockShape attend_tc_shape(const CacheView&, const AttendParams& a) {
+    const int64_t rows = group_rows(a);
+    return {rows <= 32 ? 32 : (rows <= 64 ? 64 : (rows <= 128 ? 128 : 256)), kTileKeys};
+}
 
 int64_t attend_tc_workspace(const CacheView&, const AttendParams&, int sm_count) {
     // A counter for each CTA first, then two partial results for each.

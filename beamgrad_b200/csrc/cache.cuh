@@ -156,6 +156,8 @@ cudaError_t launch_cache_commit(const CacheView& c, const int32_t* path, int pat
                                 int room_all, int sm_count, cudaStream_t stream);
 cudaError_t launch_cache_compact(const CacheView& c, int sm_count, cudaStream_t stream);
 cudaError_t launch_cache_refresh(const CacheView& c, int dtype, int values, int sm_count, cudaStream_t stream);
+// Whether the tiles of all segments of a call (attend.cuh) are counted in 31 bits, were every table full.
+bool attend_counts_tiles(const CacheView& c, const AttendParams& a);
 int64_t attend_workspace(const CacheView& c, const AttendParams& a, int sm_count);
 cudaError_t launch_attend(const CacheView& c, int dtype, const AttendParams& a, int sm_count, cudaStream_t stream);
 

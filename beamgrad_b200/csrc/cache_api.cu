@@ -97,14 +97,11 @@ bool params_of(const CacheView& v, const DBSCudaAttendArgs* a, AttendParams& p) 
     const int64_t int_max = std::numeric_limits<int32_t>::max();
     const int64_t tokens = static_cast<int64_t>(v.B) * a->beams * a->new_tokens;
     if (tokens > int_max / a->query_heads) return false;
-    // The tiles of all segments (attend.cuh), at one row block for 16 rows, are counted in 31 bits.
-    const double blocks = std::ceil(static_cast<double>(std::min(a->beams, kGroupBeams)) * a->new_tokens * (a->query_heads / v.H) / 16);
-    if ((static_cast<double>(v.unit_cap) * v.page / 64 + 1) * v.B * v.groups * blocks * v.H >= int_max) return false;
     if (a->mask != nullptr && tokens > (int64_t{1} << 46) / a->new_tokens) return false;
     p = AttendParams{};
     p.layer = a->layer, p.beams = a->beams, p.N = a->new_tokens, p.Hq = a->query_heads, p.G = a->query_heads / v.H;
     p.scale = a->scale;
-    return true;
+    return attend_counts_tiles(v, p);
 }
 
 }  // namespace

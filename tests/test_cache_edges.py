@@ -438,3 +438,45 @@ def test_sizes_that_32_bits_do_not_hold():
                          ((1, 1, 64), dict(head_dim=2**32 + 64))):
         with pytest.raises(ValueError):
             PagedCache(*args, **(sizes | change))
+
+
+# -- large calls ------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("code, dim, new, most", [(A.DTYPE_BF16, 128, 4096, 65536), (A.DTYPE_F16, 64, 4096, 65536), (A.DTYPE_F32, 64, 4096, 4096),
+                                                  (A.DTYPE_BF16, 256, 1024, 2048)])
+def test_prompts_on_large_caches_are_not_refused(code, dim, new, most):
+    """What bounds a call is that its tiles are counted in 31 bits: blocks of rows by tiles of positions as the
+    kernels have them (256 by 128, 64 by 64, 32 by 64), over full tables."""
+    lib = A.load()
+    c = A.Cache(batch_size=32, beam_size=8, max_pages=1024, num_pages=32768, num_layers=1, num_heads=8, head_dim=dim,
+                page_size=32, data_type=code)
+    size = lambda N: lib.dbs_cuda_cache_attend_workspace_size(C.byref(c), C.byref(A.AttendArgs(  # noqa: E731
+        beams=1, new_tokens=N, query_heads=64, scale=1.0)))
+    assert size(1) > 0 and size(new) == size(1) and size(most) == size(1)
+    assert size(65537) < 0
+    c.batch_size, c.num_pages = 4096, 1024  # tables of 2^25 pages
+    assert size(most) < 0 and size(1) > 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_long_prompt_on_a_large_cache(dtype):
+    B, N, H, G, D = 32, 4096, 8, 8, 8
+    cache = PagedCache(B, 8, 32768, num_layers=1, num_kv_heads=H, head_dim=D, num_pages=B * N // 32 + 8, dtype=dtype)
+    room = torch.zeros((B, 8), dtype=torch.int32, device="cuda")
+    room[:, 0] = N
+    cache.reserve(room)
+    q, k, v = tensors(cache, N, G, 4, beams=1)
+    out, lse = cache.attend(0, q, k, v, return_lse=True)
+    cache.check()
+    rng = np.random.RandomState(0)
+    u = {torch.float32: 2.0**-24, torch.float16: 2.0**-11, torch.bfloat16: 2.0**-8}[dtype]
+    for b, i, h in [(0, 0, 0), (B - 1, N - 1, H * G - 1), *zip(rng.randint(0, B, 40), rng.randint(0, N, 40), rng.randint(0, H * G, 40))]:
+        keys, values = (t[b, 0, : i + 1, h // G].double() for t in (k, v))
+        s = keys @ q[b, 0, i, h].double() / math.sqrt(D)
+        z, y = torch.logsumexp(s, 0), torch.softmax(s, 0) @ values
+        e = (D + 4) * 2.0**-24 * float((keys.abs() @ q[b, 0, i, h].double().abs()).max()) / math.sqrt(D) + 2.0**-22 * float(s.abs().max())
+        bound = float(values.abs().max()) * (2 * u + 2 * e + 2.0**-19 + 2 * (i + 1) * 2.0**-24)
+        assert float((out[b, 0, i, h].double() - y).abs().max()) <= bound
+        assert float((lse[b, 0, i, h].double() - z).abs()) <= e + 2.0**-19 + (i + 1) * 2.0**-24 + 2.0**-22 * abs(float(z))
