@@ -241,8 +241,9 @@ class PagedCache:
 
         Query i sees every committed token of its beam and the new tokens j with mask[b, k, i, j]
         ([B, beams, N, N] bool: a drafted tree's ancestors; None: j <= i). ``counts`` [B, beams]
-        int32 limits the new tokens of each beam. A query that sees nothing gives zeros (and an lse
-        of -inf). ``scale`` defaults to head_dim ** -0.5.
+        int32 limits the new tokens of each beam. A query that sees nothing, or only scores of -inf,
+        gives zeros (and an lse of -inf); a score of +inf or NaN makes both NaN. ``scale`` defaults to
+        head_dim ** -0.5.
 
         Returns out [B, beams, N, query heads, head_dim], and with ``return_lse`` also the
         logsumexp of the scaled scores, [B, beams, N, query heads] float32.

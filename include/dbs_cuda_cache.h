@@ -106,7 +106,9 @@ DBS_CUDA_EXPORT int dbs_cuda_cache_compact(const DBSCudaCache* cache, void* stre
  * value are written to layer `layer` (k, v NULL: they are there already). Query i sees the
  * committed tokens and the new tokens j with mask[b, k, i, j] (bytes [B, beams, N, N];
  * NULL: j <= i); queries at or past the count, and all that sees nothing, give 0 and an lse
- * of -inf. Tokens without a page are not written and not seen.
+ * of -inf. Tokens without a page are not written and not seen. A score of -inf (or below what
+ * 32 bits hold) weighs nothing, and a row of such alone is as one that sees nothing; one of
+ * +inf or NaN makes the row's out and lse NaN.
  *   out = softmax(scale * q k^T) v,  lse = log sum exp(scale * q k^T)
  * q, out: [B, beams, N, query_heads, head_dim]; k, v: [B, beams, N, num_heads, head_dim];
  * query head h reads head h / (query_heads / num_heads). Strides are in elements, for

@@ -126,6 +126,60 @@ def test_scores_that_rise_within_a_row(N, dim, dtype):
         check_attend(cache, 0, q, k, v, scale=float(np.log(2.0)))
 
 
+# Unit roundoff: 24, 11 and 8 significant bits, rounded to the nearest.
+UNIT = {torch.float32: 2.0**-24, torch.float16: 2.0**-11, torch.bfloat16: 2.0**-8}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("N, group, dim", [(1, 1, 64), (10, 4, 64), (50, 4, 128), (70, 4, 64), (1, 2, 200), (10, 4, 200)])
+@pytest.mark.parametrize("kind", ["some", "overflow", "all", "plus", "nan"])
+def test_scores_that_are_not_finite(kind, N, group, dim, dtype):
+    """A score of -inf (of a key that holds it, or of a sum of products that 32 bits do not hold) weighs nothing, and
+    a row with such scores alone is as one that sees nothing. A score of +inf or NaN makes the row NaN, and
+    no other row. Bound as in test_cache.py, over the keys that weigh something."""
+    T, scale = 300, 1e-3 / math.sqrt(dim) if kind == "overflow" else 1 / math.sqrt(dim)
+    cache = random_cache(1, 1, np.full((1, 1), T), N, layers=1, heads=1, dim=dim, dtype=dtype, seed=4)
+    q, k, v = tensors(cache, N, group, 5)
+    q = q.abs() + 0.25
+    if kind == "overflow":
+        q = q * 1000  # (float16 has no such sums: -65504 * 1000 * 200 is far above -3e38, and weighs nothing all the same)
+    place = torch.arange(T, device="cuda")
+    pages, at = cache.table[0, 0].long()[place // 16], place % 16
+    hit = torch.zeros(T + N, dtype=torch.bool, device="cuda")
+    if kind in ("some", "overflow"):
+        hit[:T:3] = True
+        cache.pages[0, 0, pages[::3], :, at[::3]] = -torch.finfo(dtype).max
+        if kind == "some":
+            cache.pages[0, 0, pages[::3], :, at[::3], 3] = -math.inf
+    elif kind == "all":
+        hit[:] = True
+        cache.pages[0, 0, pages, :, at, 0] = -math.inf
+        k[..., 0] = -math.inf
+    else:  # the new token N // 2, seen by itself and the later ones
+        hit[T + N // 2] = True
+        k[:, :, N // 2, :, 1] = math.inf if kind == "plus" else math.nan
+    keys = torch.cat([cache.pages[0, 0, pages, 0, at], k[0, 0, :, 0]]).double()
+    values = torch.cat([cache.pages[0, 1, pages, 0, at], v[0, 0, :, 0]]).double()
+    out, lse = (x[0, 0] for x in cache.attend(0, q, k, v, scale=scale, return_lse=True))
+    cache.check()
+    for i in range(N):
+        see = torch.arange(T + N, device="cuda") <= T + i
+        if kind in ("plus", "nan") and i >= N // 2:
+            assert bool(torch.isnan(out[i]).all()) and bool(torch.isnan(lse[i]).all())
+            continue
+        see &= ~hit
+        if not bool(see.any()):
+            assert bool((out[i] == 0).all()) and bool((lse[i] == -math.inf).all())
+            continue
+        x = (q[0, 0, i].double() @ keys[see].T) * scale  # [group, T]
+        z, y = torch.logsumexp(x, 1), torch.softmax(x, 1) @ values[see]
+        e = (dim + 4) * 2.0**-24 * scale * float((q[0, 0, i].double().abs() @ keys[see].abs().T).max()) + 2.0**-22 * float(x.abs().max())
+        bound = float(values[see].abs().max()) * (2 * UNIT[dtype] + 2 * e + 2.0**-19 + 2 * (T + N) * 2.0**-24)
+        assert float((out[i].double() - y).abs().max()) <= bound
+        assert bool(((lse[i].double() - z).abs() <= e + 2.0**-19 + (T + N) * 2.0**-24 + 2.0**-22 * z.abs()).all())
+
+
 # -- values that are not finite ---------------------------------------------------------
 
 
@@ -471,7 +525,7 @@ def test_a_long_prompt_on_a_large_cache(dtype):
     out, lse = cache.attend(0, q, k, v, return_lse=True)
     cache.check()
     rng = np.random.RandomState(0)
-    u = {torch.float32: 2.0**-24, torch.float16: 2.0**-11, torch.bfloat16: 2.0**-8}[dtype]
+    u = UNIT[dtype]
     for b, i, h in [(0, 0, 0), (B - 1, N - 1, H * G - 1), *zip(rng.randint(0, B, 40), rng.randint(0, N, 40), rng.randint(0, H * G, 40))]:
         keys, values = (t[b, 0, : i + 1, h // G].double() for t in (k, v))
         s = keys @ q[b, 0, i, h].double() / math.sqrt(D)
