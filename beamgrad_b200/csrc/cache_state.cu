@@ -286,7 +286,8 @@ __device__ void write_plan(const CacheView& c, int group, bool resolve, int* sum
             if (first) {
                 units[place[at] + __popc(firsts & ((1u << lane) - 1))] =
                     CacheUnit{e, (base + at) << c.page_log2, holders, complete ? -1 : length[lane]};
-                if (!complete && (holders & (holders - 1)) != 0) raise(c, DBS_CUDA_CACHE_STATUS_SHARED);
+                // (Other holders may be beams of another group or example, or another column.)
+                if (!complete && __ldcg(c.references + e) > 1) raise(c, DBS_CUDA_CACHE_STATUS_SHARED);
             }
         }
         count += total;

@@ -25,7 +25,7 @@ extern "C" {
 #define DBS_CUDA_CACHE_STATUS_POOL 1     /* the pool ran out of pages: some columns have none */
 #define DBS_CUDA_CACHE_STATUS_CAPACITY 2 /* a beam was to grow past max_pages columns */
 #define DBS_CUDA_CACHE_STATUS_INDEX 4    /* a parent, count, path entry, table entry or length was out of range */
-#define DBS_CUDA_CACHE_STATUS_SHARED 8   /* a page that is not complete has several holders */
+#define DBS_CUDA_CACHE_STATUS_SHARED 8   /* a page that is not complete has several holders, or one twice */
 #define DBS_CUDA_CACHE_STATUS_TIMEOUT 16 /* a bounded wait inside a kernel gave up */
 
 /* What dbs_cuda_cache_refresh does about the pool's values. */

@@ -300,6 +300,34 @@ def test_adopted_tables_with_holes_at_random():
         model.check(cache)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["another beam", "another example", "another group", "another column", "complete pages", "complete for one"])
+def test_adopted_pages_that_are_shared_before_they_are_complete(kind):
+    """The next token of one holder would be a token of the other: reported, whoever the other is."""
+    B, K = (1, 34) if kind == "another group" else (2, 2)
+    table = np.arange(B * K * 3).reshape(B, K, 3)
+    lengths = np.full((B, K), 20)
+    if kind == "another beam":
+        table[0, 1, 1] = table[0, 0, 1]
+    elif kind == "another example":
+        table[1, 1, 1] = table[0, 0, 1]
+    elif kind == "another group":
+        table[0, 33, 1] = table[0, 0, 1]
+    elif kind == "another column":
+        table[0, 0, 2] = table[0, 0, 1]
+    elif kind == "complete pages":
+        table[:, :, 0] = table[0, 0, 0]
+    else:
+        lengths[1, 1], table[1, 1, 0] = 9, table[0, 0, 0]
+    cache = adopt(table.tolist(), lengths.tolist(), pages=B * K * 3)
+    Model(cache).check_plan(cache)
+    if kind == "complete pages":
+        cache.check()
+    else:
+        with pytest.raises(RuntimeError, match="shared"):
+            cache.check()
+
+
 # -- paths that are refused -------------------------------------------------------------
 
 
