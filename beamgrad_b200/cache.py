@@ -88,7 +88,8 @@ class PagedCache:
     def from_tensors(cls, pages: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor,
                      references: torch.Tensor | None = None) -> "PagedCache":
         """A cache over existing tensors (laid out as the class says, used in place).
-        ``references`` and the internal plan are computed from ``table`` and ``lengths``."""
+        ``references`` and the internal plan are computed from ``table`` and ``lengths``, as
+        :meth:`refresh` does."""
         if pages.dim() != 6 or pages.shape[1] != 2 or pages.dtype not in _DTYPES:
             raise ValueError("pages must be a float [layers, 2, num_pages, heads, page_size, head_dim] tensor")
         if table.dim() != 3 or tuple(lengths.shape) != tuple(table.shape[:2]):

@@ -17,10 +17,11 @@
 // positions, with zeros for the others: the product costs the same, and the chain from scores to
 // weights is a half (a quarter) as long. Copies and streams are joined at the end of a segment.
 //
-// A row's reference for the exponentials is raised only when its maximum has grown by more than
-// 2^8: until then the weights stay below 2^8 and the sums within 32 bits, and O in tensor memory
-// is left alone (in float16 all of them are 2^7 higher: kLift). Weights are rounded to the input type, as the values are; their sum is taken
-// before. All statistics are 32 bits.
+// Rescaling is put off, as has been published for attention on this architecture (the code is this
+// engine's own): a row's reference for the exponentials is raised only when its maximum has grown by
+// more than 2^8. Until then the weights stay below 2^8 and the sums within 32 bits, and O in tensor
+// memory is left alone (in float16 all of them are 2^7 higher: kLift). Weights are rounded to the input
+// type, as the values are; their sum is taken before. All statistics are 32 bits.
 #include "attend.cuh"
 
 namespace dbsb {
@@ -886,8 +887,8 @@ cudaError_t launch_width(const CacheView& c, const CUtensorMap& map, const Atten
     if (rows == 64) return launch_shape<T, DP, 1, 2, false>(c, map, a, sm_count, stream);
     if (rows == 128) return launch_shape<T, DP, 1, 1, false>(c, map, a, sm_count, stream);
     // Several blocks of several beams: a block passes over the tiles of which its beams hold nothing (17 beams
-    // of 62 tokens over 72: 92 us, so 81). Where every block has all beams that costs registers for nothing
-    // (16 drafted trees: 347 us, so 360).
+    // of 62 tokens over 72: 92 us, so 81, and 79 with the exponentials as they are now). Where every block has
+    // all beams that costs registers for nothing (16 drafted trees: 347 us, so 360).
     if (group_rows(a) > 256 && a.beams > 1) return launch_shape<T, DP, 2, 1, true>(c, map, a, sm_count, stream);
     return launch_shape<T, DP, 2, 1, false>(c, map, a, sm_count, stream);
 }
